@@ -8,4 +8,5 @@ __version__ = "0.1.0"
 
 from .core.errors import KernelBuildError, KernelUnavailableError, NoBackendError  # noqa: F401
 from .core.runtime import Method  # noqa: F401
-from .registry import Backend, MSDABackend, MSDAContext, msda, msda_from_offsets  # noqa: F401
+from .registry import (  # noqa: F401
+    Backend, MSDABackend, MSDAContext, cross_attention, msda, msda_from_offsets, rotary)

@@ -20,7 +20,7 @@ import warnings
 from ._build import (LIB_PATH, build_host_module, build_library, host_module_path, is_stale)
 from .core.errors import KernelBuildError, KernelUnavailableError
 
-__all__ = ["ABI_VERSION", "Shim", "host_module", "library_path", "load_library", "loaded"]
+__all__ = ["ABI_VERSION", "AttentionCall", "Shim", "host_module", "library_path", "load_library", "loaded"]
 
 ABI_VERSION = 5
 
@@ -40,6 +40,14 @@ os.register_at_fork(after_in_child=_reset_lock_in_child)
 _i64, _vp, _int = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
 
 
+class AttentionCall(ctypes.Structure):
+    """``struct msda_b200_attention`` of the C ABI."""
+
+    _fields_ = [(name, _i64) for name in ("batch", "queries", "states", "heads", "kv_heads", "head_dim")] + [
+        ("query_strides", _i64 * 3), ("key_strides", _i64 * 3), ("value_strides", _i64 * 3),
+        ("mask", _vp), ("mask_heads", _int), ("dtype", _int), ("scale", ctypes.c_float)]
+
+
 class Shim:
     """Typed handles on the exported functions of the library."""
 
@@ -50,7 +58,10 @@ class Shim:
                "msda_b200_column_sums",
                "msda_b200_column_sums_scratch_bytes",
                "msda_b200_forward_offsets", "msda_b200_backward_offsets",
-               "msda_b200_backward_static_scratch", "msda_b200_launch_geometry")
+               "msda_b200_backward_static_scratch", "msda_b200_launch_geometry",
+               "msda_b200_attention_mask_bytes", "msda_b200_attention_pack_mask",
+               "msda_b200_attention_workspace_bytes", "msda_b200_attention_forward",
+               "msda_b200_attention_backward", "msda_b200_rotary")
 
     def __init__(self, path: str):
         self.path = path
@@ -104,6 +115,25 @@ class Shim:
         self.launch_geometry.argtypes = [_i64] * 6 + [_int, _int, ctypes.POINTER(_i64),
                                          ctypes.POINTER(_int), ctypes.POINTER(_i64),
                                          ctypes.POINTER(_i64)]
+        call = ctypes.POINTER(AttentionCall)
+        self.attention_mask_bytes = self.lib.msda_b200_attention_mask_bytes
+        self.attention_mask_bytes.restype = _i64
+        self.attention_mask_bytes.argtypes = [_i64] * 4 + [_int]
+        self.attention_pack_mask = self.lib.msda_b200_attention_pack_mask
+        self.attention_pack_mask.restype = _int
+        self.attention_pack_mask.argtypes = [_vp] * 4 + [_int] + [_i64] * 4 + [_vp, _int, _vp]
+        self.attention_workspace_bytes = self.lib.msda_b200_attention_workspace_bytes
+        self.attention_workspace_bytes.restype = _i64
+        self.attention_workspace_bytes.argtypes = [call, _int]
+        self.attention_forward = self.lib.msda_b200_attention_forward
+        self.attention_forward.restype = _int
+        self.attention_forward.argtypes = [call] + [_vp] * 6 + [_i64, _int, _vp]
+        self.attention_backward = self.lib.msda_b200_attention_backward
+        self.attention_backward.restype = _int
+        self.attention_backward.argtypes = [call] + [_vp] * 10 + [_i64, _int, _vp]
+        self.rotary = self.lib.msda_b200_rotary
+        self.rotary.restype = _int
+        self.rotary.argtypes = ([_vp] * 4 + [_int, _vp] + [_i64] * 6 + [_vp, _vp] + [_int] * 4 + [_vp])
         got = self.lib.msda_b200_abi_version()
         if got != ABI_VERSION:
             raise KernelUnavailableError(
@@ -184,7 +214,9 @@ def host_module():
                          shim.workspace_bytes, shim.lib.msda_b200_last_error,
                          shim.lib.msda_b200_column_sums,
                          shim.lib.msda_b200_column_sums_scratch_bytes,
-                         shim.offsets_workspace_bytes)
+                         shim.offsets_workspace_bytes, shim.attention_mask_bytes,
+                         shim.attention_pack_mask, shim.attention_workspace_bytes,
+                         shim.attention_forward, shim.attention_backward, shim.rotary)
             module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in functions))
             _host = module
         except Exception as exc:  # noqa: BLE001 - the Python operators remain

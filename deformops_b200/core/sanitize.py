@@ -16,7 +16,7 @@ import os
 import torch
 from torch import Tensor
 
-__all__ = ["check_msda_call", "value_checks_enabled"]
+__all__ = ["check_cross_attention_call", "check_msda_call", "check_rotary_call", "value_checks_enabled"]
 
 
 def value_checks_enabled() -> bool:
@@ -120,3 +120,73 @@ def _check_level_layout(value: Tensor, spatial_shapes: Tensor, level_start_index
             f"spatial_shapes describes {running} positions but value has {value.shape[1]} on "
             "its spatial axis; the levels must tile the value tensor exactly"
         )
+
+
+def _need_float(name: str, t: Tensor) -> None:
+    if not t.is_floating_point():
+        raise ValueError(f"{name} must be a floating-point tensor, got dtype {t.dtype}")
+
+
+def _need_one_device(named: dict[str, Tensor]) -> None:
+    if len({t.device for t in named.values()}) != 1:
+        listing = ", ".join(f"{k} on {t.device}" for k, t in named.items())
+        raise ValueError(f"all operands must be on one device, got {listing}")
+
+
+def check_cross_attention_call(query: Tensor, key: Tensor, value: Tensor, key_padding_mask: Tensor | None,
+                               attention_mask: Tensor | None) -> None:
+    """Validate ``(B,Q,G,D)``, twice ``(B,S,K,D)``, ``(B,S)`` and ``(Q,S)`` / ``(B,Q,S)`` / ``(B,1|G,Q,S)``."""
+    _need_rank("query", query, (4,), "(B, Q, G, D)")
+    _need_rank("key", key, (4,), "(B, S, K, D)")
+    _need_rank("value", value, (4,), "(B, S, K, D)")
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        _need_float(name, t)
+        if t.dtype != query.dtype:
+            raise ValueError(f"{name} has dtype {t.dtype} but query has {query.dtype}; cast to a common dtype")
+    B, Q, G, D = query.shape
+    S, K = key.shape[1], key.shape[2]
+    _need_size("key", key, 0, B, "batch of query")
+    _need_size("key", key, 3, D, "head dimension of query")
+    for axis, why in enumerate(("batch", "states", "heads", "head dimension")):
+        _need_size("value", value, axis, key.shape[axis], f"{why} of key")
+    if K == 0 or G % K != 0:
+        raise ValueError(f"the {G} heads of query must be a multiple of the {K} heads of key")
+    named = {"query": query, "key": key, "value": value}
+    if key_padding_mask is not None:
+        named["key_padding_mask"] = key_padding_mask
+        _need_rank("key_padding_mask", key_padding_mask, (2,), "(B, S)")
+        _need_size("key_padding_mask", key_padding_mask, 0, B, "batch of query")
+        _need_size("key_padding_mask", key_padding_mask, 1, S, "states of key")
+    if attention_mask is not None:
+        named["attention_mask"] = attention_mask
+        _need_rank("attention_mask", attention_mask, (2, 3, 4), "(Q, S), (B, Q, S) or (B, 1 or G, Q, S)")
+        _need_size("attention_mask", attention_mask, -2, Q, "queries")
+        _need_size("attention_mask", attention_mask, -1, S, "states of key")
+        if attention_mask.dim() > 2:
+            _need_size("attention_mask", attention_mask, 0, B, "batch of query")
+        if attention_mask.dim() == 4 and attention_mask.shape[1] not in (1, G):
+            raise ValueError(f"attention_mask has {attention_mask.shape[1]} heads but 1 or {G} are required")
+    for name in ("key_padding_mask", "attention_mask"):
+        if name in named and named[name].dtype != torch.bool:
+            raise ValueError(f"{name} must be a bool tensor, true where a state may not be seen, got "
+                             f"{named[name].dtype}; masks that are added to the scores are not taken")
+    _need_one_device(named)
+
+
+def check_rotary_call(x: Tensor, positions: Tensor, sections: tuple[int, ...]) -> None:
+    """Validate ``(B,N,G,D)``, ``(B,N,A)`` or ``(N,A)``, and pairs per axis that fit into ``D``."""
+    _need_rank("x", x, (4,), "(B, N, G, D)")
+    _need_float("x", x)
+    _need_rank("positions", positions, (2, 3), "(N, A) or (B, N, A)")
+    if positions.dtype not in (torch.float32, torch.float64, torch.int32, torch.int64):
+        raise ValueError(f"positions must be float32, float64, int32 or int64, got {positions.dtype}")
+    if positions.dim() == 3:
+        _need_size("positions", positions, 0, x.shape[0], "batch of x")
+    _need_size("positions", positions, -2, x.shape[1], "tokens of x")
+    _need_size("positions", positions, -1, len(sections), "one axis per section")
+    if any(n < 0 for n in sections) or 2 * sum(sections) > x.shape[3]:
+        raise ValueError(f"sections {sections} are pairs of channels per axis: none negative, at most "
+                         f"{x.shape[3] // 2} of a head's {x.shape[3]} channels")
+    if positions.requires_grad and torch.is_grad_enabled():
+        raise ValueError("no gradient is formed for positions: detach them")
+    _need_one_device({"x": x, "positions": positions})

@@ -1,0 +1,240 @@
+// C ABI of cross attention (declared in include/msda_b200.h): argument checks and the plan of a call.
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+
+#include "../../include/msda_b200.h"
+#include "attn_common.cuh"
+
+namespace msda_b200 {
+
+AttentionSplit attention_split(int64_t ctas, int64_t tiles, int64_t ctas_at_once, int fewest_tiles) {
+    int64_t splits = 1;
+    if (ctas > 0 && ctas < ctas_at_once) splits = std::min(ctas_at_once / ctas, tiles / std::max(fewest_tiles, 1));
+    splits = std::max<int64_t>(1, splits);
+    const int64_t each = std::max<int64_t>(1, (tiles + splits - 1) / splits);
+    return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
+}
+
+namespace {
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int refuse(int status, const char *message) { return set_last_error(status, message); }
+
+int64_t mask_words(int64_t states) { return (states + kMaskTile - 1) / kMaskTile * 4; }
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// one pass of a call: its split, and the bytes that its parts take
+struct Pass {
+    AttentionSplit split;
+    int64_t bytes;
+};
+
+Pass forward_pass(const msda_b200_attention &c) {
+    const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
+    const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
+    const int64_t row_tile = rows <= 16 ? 16 : 64;
+    const AttentionSplit s = attention_split(bk * ((rows + row_tile - 1) / row_tile), (c.states + tile - 1) / tile,
+                                             148 * 4, 4);
+    return {s, s.splits > 1 ? round16(s.splits * bk * rows * 4) + s.splits * bk * rows * c.head_dim * 4 : 0};
+}
+
+Pass backward_pass(const msda_b200_attention &c, bool keys) {
+    const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
+    const int tile = c.head_dim > 64 ? 32 : 64;
+    const int64_t held = keys ? c.states : rows, walked = keys ? rows : c.states;
+    const AttentionSplit s = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);
+    return {s, s.splits > 1 ? (keys ? 2 : 1) * s.splits * bk * held * c.head_dim * 4 : 0};
+}
+
+int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
+
+int check(const msda_b200_attention *c) {
+    if (c == nullptr) return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: null call");
+    if (c->dtype != MSDA_B200_F32 && c->dtype != MSDA_B200_F16 && c->dtype != MSDA_B200_BF16)
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: dtype is not f32, f16 or bf16");
+    if (c->batch < 0 || c->queries < 0 || c->states < 0 || c->heads <= 0 || c->kv_heads <= 0 || c->head_dim <= 0)
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: sizes out of range");
+    if (c->heads % c->kv_heads != 0)
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: heads must be a multiple of kv_heads");
+    const int vec = c->dtype == MSDA_B200_F32 ? 4 : 8;
+    if (c->head_dim % vec != 0 || c->head_dim > 128)
+        return refuse(MSDA_B200_UNSUPPORTED, "attention: head_dim must be whole 16-byte vectors and at most 128");
+    constexpr int64_t kMost = (int64_t)1 << 30;
+    if (c->batch > kMost || c->heads > kMost || c->batch * c->heads > 1 << 20 || c->queries > kMost ||
+        c->states > kMost || c->queries * (c->heads / c->kv_heads) > kMost)
+        return refuse(MSDA_B200_UNSUPPORTED, "attention: more than 2^30 rows or states, or 2^20 heads of all samples");
+    if (!(c->scale > 0.f) || std::isinf(c->scale))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: scale must be positive and finite");
+    if (c->mask_heads != 0 && c->mask_heads != 1 && c->mask_heads != c->heads)
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: mask_heads must be 0, 1 or heads");
+    if (!aligned16(c->mask)) return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: misaligned mask");
+    for (const int64_t *s : {c->query_strides, c->key_strides, c->value_strides})
+        for (int i = 0; i < 3; ++i)
+            if (s[i] < 0 || s[i] % vec != 0)
+                return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: strides must be whole 16-byte vectors");
+    return MSDA_B200_OK;
+}
+
+AttentionParams params(const msda_b200_attention &c, const void *q, const void *k, const void *v) {
+    AttentionParams p{};
+    p.q = q, p.k = k, p.v = v;
+    for (int i = 0; i < 3; ++i) p.qs[i] = c.query_strides[i], p.ks[i] = c.key_strides[i], p.vs[i] = c.value_strides[i];
+    p.B = (int)c.batch, p.K = (int)c.kv_heads, p.share = (int)(c.heads / c.kv_heads), p.Q = (int)c.queries;
+    p.S = (int)c.states, p.R = p.Q * p.share, p.D = (int)c.head_dim;
+    p.scale = c.scale;
+    p.scale_log2 = c.scale * 1.4426950408889634f;
+    p.W = (int)mask_words(c.states);
+    if (c.mask != nullptr) {
+        p.key_words = static_cast<const uint32_t *>(c.mask);
+        p.key_word_heads = c.mask_heads > 1 ? p.K : 1;
+        if (c.mask_heads > 0) {
+            p.row_words = p.key_words + (int64_t)p.B * p.key_word_heads * p.W;
+            p.row_word_heads = c.mask_heads;
+        }
+    }
+    return p;
+}
+
+int status_of(cudaError_t e) {
+    return e == cudaSuccess ? MSDA_B200_OK : refuse(MSDA_B200_CUDA_ERROR, cudaGetErrorString(e));
+}
+
+}  // namespace
+
+}  // namespace msda_b200
+
+extern "C" {
+
+using namespace msda_b200;
+
+int64_t msda_b200_attention_mask_bytes(int64_t batch, int64_t queries, int64_t states, int64_t kv_heads,
+                                       int mask_heads) {
+    if (batch <= 0 || queries < 0 || states < 0 || kv_heads <= 0 || mask_heads < 0) return 0;
+    return 4 * mask_words(states) * batch * ((mask_heads > 1 ? kv_heads : 1) + mask_heads * queries);
+}
+
+int msda_b200_attention_pack_mask(const void *padding, const int64_t *padding_strides, const void *mask,
+                                  const int64_t *mask_strides, int mask_heads, int64_t batch, int64_t queries,
+                                  int64_t states, int64_t kv_heads, void *packed, int device, void *stream) {
+    if (batch < 0 || queries < 0 || states < 0 || kv_heads <= 0 || mask_heads < 0 || (mask == nullptr) != (mask_heads == 0) ||
+        (mask_heads > 1 && mask_heads % kv_heads != 0))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_pack_mask: sizes out of range");
+    if ((padding == nullptr && mask == nullptr) || (padding != nullptr && padding_strides == nullptr) ||
+        (mask != nullptr && mask_strides == nullptr) || packed == nullptr || !aligned16(packed))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_pack_mask: null or misaligned pointer");
+    if (batch > 1 << 20 || queries > 1 << 30 || states > 1 << 30 || mask_heads > 1 << 20)
+        return refuse(MSDA_B200_UNSUPPORTED, "attention_pack_mask: sizes too large");
+    if (batch == 0 || states == 0 || (mask != nullptr && queries == 0)) return MSDA_B200_OK;
+    MaskParams p{};
+    p.padding = static_cast<const uint8_t *>(padding), p.mask = static_cast<const uint8_t *>(mask);
+    for (int i = 0; i < 2 && padding != nullptr; ++i) p.ps[i] = padding_strides[i];
+    for (int i = 0; i < 4 && mask != nullptr; ++i) p.ms[i] = mask_strides[i];
+    p.B = (int)batch, p.H = mask_heads, p.KW = mask_heads > 1 ? (int)kv_heads : 1, p.Q = (int)queries;
+    p.S = (int)states, p.W = (int)mask_words(states);
+    p.key_words = static_cast<uint32_t *>(packed);
+    p.row_words = p.key_words + (int64_t)p.B * p.KW * p.W;
+    const DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return status_of(guard.err);
+    const cudaError_t e = launch_attention_mask(p, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) count_launches(mask != nullptr ? 2 : 1, 0);
+    return status_of(e);
+}
+
+int64_t msda_b200_attention_workspace_bytes(const msda_b200_attention *call, int backward) {
+    if (check(call) != MSDA_B200_OK || call->batch == 0 || call->queries == 0 || call->states == 0) return 0;
+    if (!backward) return forward_pass(*call).bytes;
+    return delta_bytes(*call) + std::max(backward_pass(*call, true).bytes, backward_pass(*call, false).bytes);
+}
+
+int msda_b200_attention_forward(const msda_b200_attention *call, const void *query, const void *key, const void *value,
+                                void *out, float *lse, void *workspace, int64_t workspace_bytes, int device,
+                                void *stream) {
+    const int st = check(call);
+    if (st != MSDA_B200_OK) return st;
+    if (call->batch == 0 || call->queries == 0) return MSDA_B200_OK;
+    if (out == nullptr || lse == nullptr || !aligned16(out) || !aligned16(lse))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_forward: null or misaligned output");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return status_of(guard.err);
+    if (call->states == 0) {        // nothing to see: zeros (and L, which no backward pass will read)
+        const int64_t n = call->batch * call->queries * call->heads * call->head_dim;
+        count_launches(0, 1);
+        return status_of(cudaMemsetAsync(out, 0, n * (call->dtype == MSDA_B200_F32 ? 4 : 2), s));
+    }
+    if (query == nullptr || key == nullptr || value == nullptr || !aligned16(query) || !aligned16(key) || !aligned16(value))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_forward: null or misaligned operand");
+    const Pass pass = forward_pass(*call);
+    if (pass.bytes > workspace_bytes || (pass.bytes > 0 && (workspace == nullptr || !aligned16(workspace))))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_forward: workspace too small or misaligned");
+    AttentionParams p = params(*call, query, key, value);
+    p.out = out, p.lse = lse;
+    p.splits = pass.split.splits, p.tiles = pass.split.tiles;
+    p.part_lse = static_cast<float *>(workspace);
+    p.part = p.part_lse + round16((int64_t)p.splits * p.B * p.K * p.R * 4) / 4;
+    cudaError_t e = launch_attention_forward_mma(p, call->dtype, s);
+    if (e == cudaSuccess && p.splits > 1) e = launch_attention_join(p, call->dtype, s);
+    if (e == cudaSuccess) count_launches(p.splits > 1 ? 2 : 1, 0);
+    return status_of(e);
+}
+
+int msda_b200_attention_backward(const msda_b200_attention *call, const void *query, const void *key, const void *value,
+                                 const void *out, const void *grad_out, const float *lse, void *grad_query,
+                                 void *grad_key, void *grad_value, void *workspace, int64_t workspace_bytes, int device,
+                                 void *stream) {
+    const int st = check(call);
+    if (st != MSDA_B200_OK) return st;
+    if (call->batch == 0) return MSDA_B200_OK;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return status_of(guard.err);
+    const int64_t e_size = call->dtype == MSDA_B200_F32 ? 4 : 2;
+    const int64_t row_bytes = call->batch * call->queries * call->heads * call->head_dim * e_size;
+    const int64_t state_bytes = call->batch * call->states * call->kv_heads * call->head_dim * e_size;
+    for (const void *x : {grad_query, grad_key, grad_value})
+        if (!aligned16(x)) return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_backward: misaligned gradient");
+    if ((row_bytes > 0 && grad_query == nullptr) || (state_bytes > 0 && (grad_key == nullptr || grad_value == nullptr)))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_backward: null gradient");
+    if (row_bytes == 0 || state_bytes == 0) {
+        cudaError_t e = cudaSuccess;
+        if (row_bytes > 0) e = cudaMemsetAsync(grad_query, 0, row_bytes, s);
+        if (e == cudaSuccess && state_bytes > 0) e = cudaMemsetAsync(grad_key, 0, state_bytes, s);
+        if (e == cudaSuccess && state_bytes > 0) e = cudaMemsetAsync(grad_value, 0, state_bytes, s);
+        if (e == cudaSuccess) count_launches(0, (row_bytes > 0) + 2 * (state_bytes > 0));
+        return status_of(e);
+    }
+    for (const void *x : {query, key, value, out, grad_out, (const void *)lse, (const void *)workspace})
+        if (x == nullptr || !aligned16(x))
+            return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_backward: null or misaligned operand");
+    const Pass keys = backward_pass(*call, true), rows = backward_pass(*call, false);
+    if (delta_bytes(*call) + std::max(keys.bytes, rows.bytes) > workspace_bytes)
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_backward: workspace too small");
+    AttentionParams p = params(*call, query, key, value);
+    p.out = const_cast<void *>(out), p.grad_out = grad_out, p.lse = const_cast<float *>(lse);
+    p.dq = grad_query, p.dk = grad_key, p.dv = grad_value;
+    p.delta = static_cast<float *>(workspace);
+    p.part = p.delta + delta_bytes(*call) / 4;
+    int launches = 3;
+    cudaError_t e = launch_attention_delta(p, call->dtype, s);
+    if (e == cudaSuccess) {
+        p.splits = keys.split.splits, p.tiles = keys.split.tiles;
+        p.part2 = p.part + (int64_t)p.splits * p.B * p.K * p.S * p.D;
+        e = launch_attention_backward_mma(p, call->dtype, true, s);
+        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part, p.dk, true, call->dtype, s);
+        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part2, p.dv, true, call->dtype, s);
+        launches += p.splits > 1 ? 2 : 0;
+    }
+    if (e == cudaSuccess) {
+        p.splits = rows.split.splits, p.tiles = rows.split.tiles;
+        e = launch_attention_backward_mma(p, call->dtype, false, s);
+        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part, p.dq, false, call->dtype, s);
+        launches += p.splits > 1 ? 1 : 0;
+    }
+    if (e == cudaSuccess) count_launches(launches, 0);
+    return status_of(e);
+}
+
+}  // extern "C"

@@ -1,0 +1,200 @@
+// Cross attention: masks to bits, rowsum(do o), and the joining of split passes.  All of them read
+// their input once and are bound by that, or by their launch.
+#include <algorithm>
+
+#include "attn_common.cuh"
+
+namespace msda_b200 {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// A warp packs 128 states of one mask row at a time, 32 consecutive bytes to a ballot.  Rows of odd
+// length leave nothing aligned to load wider, and 32 bytes are a whole sector.
+__global__ void __launch_bounds__(kThreads) attention_mask_kernel(const __grid_constant__ MaskParams p) {
+    const int lane = threadIdx.x & 31;
+    const int groups = p.W / 4;
+    const bool own_rows = p.mask != nullptr;
+    const int64_t rows = own_rows ? (int64_t)p.B * p.H * p.Q : p.B, tasks = rows * groups;
+    for (int64_t task = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); task < tasks;
+         task += (int64_t)gridDim.x * (kThreads / 32)) {
+        const int64_t row = task / groups;
+        const int group = (int)(task - row * groups);
+        int64_t b = row, at = 0;
+        if (own_rows) {
+            const int64_t bh = row / p.Q, query = row - bh * p.Q;
+            b = bh / p.H;
+            at = b * p.ms[0] + (bh - b * p.H) * p.ms[1] + query * p.ms[2];
+        }
+        uint8_t hidden[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int state = group * 128 + w * 32 + lane;
+            hidden[w] = state >= p.S;
+            if (state < p.S && own_rows) hidden[w] = __ldg(p.mask + at + state * p.ms[3]);
+            if (state < p.S && p.padding != nullptr) hidden[w] |= __ldg(p.padding + b * p.ps[0] + state * p.ps[1]);
+        }
+        uint32_t words[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) words[w] = __ballot_sync(0xffffffffu, hidden[w] == 0);
+        if (lane == 0)
+            *reinterpret_cast<uint4 *>((own_rows ? p.row_words : p.key_words) + row * p.W + group * 4) =
+                make_uint4(words[0], words[1], words[2], words[3]);
+    }
+}
+
+// key words: the or of all rows of a sample (or of the heads that share a key head)
+__global__ void __launch_bounds__(1024) attention_mask_any_kernel(const __grid_constant__ MaskParams p) {
+    __shared__ uint32_t any[32][33];
+    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int blocks = (p.W + 31) / 32;
+    const int bk = blockIdx.x / blocks, w = (blockIdx.x - bk * blocks) * 32 + lane;
+    const int64_t rows = (int64_t)(p.H / p.KW) * p.Q;              // consecutive ones
+    uint32_t found = 0;
+    if (w < p.W)
+        for (int64_t r = part; r < rows; r += 32) found |= p.row_words[(bk * rows + r) * p.W + w];
+    any[part][lane] = found;
+    __syncthreads();
+    found = __reduce_or_sync(0xffffffffu, any[lane][part]);
+    const int word = (blockIdx.x - bk * blocks) * 32 + part;
+    if (lane == 0 && word < p.W) p.key_words[(int64_t)bk * p.W + word] = found;
+}
+
+// eight lanes to a row
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr int kVec = VecTraits<T>::kVec;
+    const int lane = threadIdx.x & 7;
+    const int64_t rows = (int64_t)p.B * p.K * p.R;
+    const int64_t first = (int64_t)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3);
+    float sum = 0.f;
+    if (first < rows) {
+        const int64_t bh = first / p.R;
+        const int r = (int)(first - bh * p.R), query = r / p.share, b = (int)(bh / p.K), h = (int)(bh - (int64_t)b * p.K);
+        const int64_t at = (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
+        for (int c = lane * kVec; c < p.D; c += 8 * kVec) {
+            float2 x[kVec / 2], y[kVec / 2];
+            VecTraits<T>::unpack(ldg16(static_cast<const T *>(p.out) + at + c), x);
+            VecTraits<T>::unpack(ldg16(static_cast<const T *>(p.grad_out) + at + c), y);
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) sum += x[i].x * y[i].x + x[i].y * y[i].y;
+        }
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0 && first < rows) p.delta[first] = sum;
+}
+
+// o = sum of 2^(L_i - L) o_i, a thread to four channels of a row
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+    const int lanes = p.D / 4;
+    const int64_t rows = (int64_t)p.B * p.K * p.R;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t row = i / lanes;
+    const int c = (int)(i - row * lanes) * 4;
+    if (row >= rows) return;
+    float top = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * rows + row]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float w = fast_exp2(p.part_lse[s * rows + row] - base);
+        const float4 x = *reinterpret_cast<const float4 *>(p.part + (s * rows + row) * p.D + c);
+        sum += w;
+        o.x += w * x.x, o.y += w * x.y, o.z += w * x.z, o.w += w * x.w;
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t bh = row / p.R;
+    const int r = (int)(row - bh * p.R), query = r / p.share, b = (int)(bh / p.K), h = (int)(bh - (int64_t)b * p.K);
+    T *to = static_cast<T *>(p.out) +
+            (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D + c;
+    to[0] = VecTraits<T>::from_float(o.x * inverse);
+    to[1] = VecTraits<T>::from_float(o.y * inverse);
+    to[2] = VecTraits<T>::from_float(o.z * inverse);
+    to[3] = VecTraits<T>::from_float(o.w * inverse);
+    if (c == 0) p.lse[row] = sum == 0.f ? INFINITY : base + log2f(sum);
+}
+
+// gradients: the parts' sum, in the order of the parts
+template <typename T, bool KEYS>
+__global__ void __launch_bounds__(kThreads) attention_sum_kernel(const __grid_constant__ AttentionParams p,
+                                                                 const float *part, T *out) {
+    const int lanes = p.D / 4, X = KEYS ? p.S : p.R;
+    const int64_t rows = (int64_t)p.B * p.K * X;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t row = i / lanes;
+    const int c = (int)(i - row * lanes) * 4;
+    if (row >= rows) return;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float4 x = *reinterpret_cast<const float4 *>(part + (s * rows + row) * p.D + c);
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    }
+    const int64_t bh = row / X;
+    const int x = (int)(row - bh * X), b = (int)(bh / p.K), h = (int)(bh - (int64_t)b * p.K), query = x / p.share;
+    T *to = out + (KEYS ? (((int64_t)b * p.S + x) * p.K + h) * p.D
+                        : (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (x - query * p.share)) * p.D) + c;
+    to[0] = VecTraits<T>::from_float(sum.x);
+    to[1] = VecTraits<T>::from_float(sum.y);
+    to[2] = VecTraits<T>::from_float(sum.z);
+    to[3] = VecTraits<T>::from_float(sum.w);
+}
+
+unsigned blocks_for(int64_t threads) {
+    return (unsigned)((threads + kThreads - 1) / kThreads);
+}
+
+template <typename T>
+cudaError_t sum_typed(const AttentionParams &p, const float *part, void *out, bool keys, cudaStream_t stream) {
+    const unsigned grid = blocks_for((int64_t)p.B * p.K * (keys ? p.S : p.R) * (p.D / 4));
+    if (keys)
+        attention_sum_kernel<T, true><<<grid, kThreads, 0, stream>>>(p, part, static_cast<T *>(out));
+    else
+        attention_sum_kernel<T, false><<<grid, kThreads, 0, stream>>>(p, part, static_cast<T *>(out));
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t join_typed(const AttentionParams &p, cudaStream_t stream) {
+    attention_join_kernel<T><<<blocks_for((int64_t)p.B * p.K * p.R * (p.D / 4)), kThreads, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t delta_typed(const AttentionParams &p, cudaStream_t stream) {
+    attention_delta_kernel<T><<<blocks_for((int64_t)p.B * p.K * p.R * 8), kThreads, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream) {
+    const int64_t tasks = (p.mask != nullptr ? (int64_t)p.B * p.H * p.Q : p.B) * (p.W / 4);
+    const int64_t grid = std::min<int64_t>((tasks + kThreads / 32 - 1) / (kThreads / 32), 148 * 64);
+    attention_mask_kernel<<<(unsigned)grid, kThreads, 0, stream>>>(p);
+    if (p.mask != nullptr)
+        attention_mask_any_kernel<<<(unsigned)(p.B * p.KW * ((p.W + 31) / 32)), 1024, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream) {
+    return dtype == 0 ? delta_typed<float>(p, stream)
+           : dtype == 1 ? delta_typed<__half>(p, stream) : delta_typed<__nv_bfloat16>(p, stream);
+}
+cudaError_t launch_attention_join(const AttentionParams &p, int dtype, cudaStream_t stream) {
+    return dtype == 0 ? join_typed<float>(p, stream)
+           : dtype == 1 ? join_typed<__half>(p, stream) : join_typed<__nv_bfloat16>(p, stream);
+}
+cudaError_t launch_attention_sum(const AttentionParams &p, const float *part, void *out, bool keys, int dtype,
+                                 cudaStream_t stream) {
+    return dtype == 0 ? sum_typed<float>(p, part, out, keys, stream)
+           : dtype == 1 ? sum_typed<__half>(p, part, out, keys, stream)
+                        : sum_typed<__nv_bfloat16>(p, part, out, keys, stream);
+}
+
+}  // namespace msda_b200

@@ -1,0 +1,101 @@
+// Cross attention: what its kernels share.
+//
+// A call has B samples, K key heads and `share` query heads for each of them.  All queries that meet
+// one (sample, key head) are the rows r = query * share + head of one matrix of R = Q * share rows,
+// so that shared heads fill the same tiles and their gradients meet without atomics.
+//
+//   s = scale * q k^T      p = exp(s - max) / sum over the states that the row may see
+//   o = p v                L = max + log(sum)      (kept, in base 2, for the backward pass)
+//   dv = p^T do   dp = do v^T   ds = p (dp - rowsum(do o))   dq = scale ds k   dk = scale ds^T q
+//
+// A row that may see nothing has o = 0, L = +inf and no gradients (exp2(x - inf) = 0).
+//
+// Masks are packed into bits by a kernel of their own (one pass over a byte mask that every head would
+// otherwise read again): bit j % 32 of word j / 32 is set where state j may be seen; words behind the
+// last state are 0.  `key_words` holds for every state whether any row may see it: the rows of k and v
+// of states that nobody sees are never used, whatever they hold.
+#pragma once
+
+#include "msda_common.cuh"
+
+namespace msda_b200 {
+
+constexpr int kMaskTile = 128;     // states per group of four mask words; mask rows are whole groups
+
+struct AttentionParams {
+    const void *q, *k, *v;
+    const void *grad_out;                  // backward only, (B, Q, G * D) like `out`
+    int64_t qs[3], ks[3], vs[3];           // strides of (sample, token, head) in elements
+    int B, K, share, Q, S, R, D;
+    float scale, scale_log2;               // scale * log2(e)
+    const uint32_t *key_words;             // (B, key_word_heads, W) or null: every state may be seen
+    const uint32_t *row_words;             // (B, row_word_heads, Q, W) or null: rows see what key_words has
+    int key_word_heads, row_word_heads, W;
+    void *out;                             // (B, Q, G * D)
+    float *lse;                            // (B, K, R), log2 of the sum of exp2
+    float *delta;                          // (B, K, R), rowsum(do o); backward only
+    void *dq, *dk, *dv;                    // contiguous (B, Q, G, D), (B, S, K, D)
+    // work over the long axis is split into `splits` stretches of `tiles` tiles; with more than one,
+    // partial results go to part (splits, B, K, rows, D) and part_lse (splits, B, K, rows)
+    float *part, *part2, *part_lse;
+    int splits, tiles;
+};
+
+// ---- which states a tile of 32 * N of them may use --------------------------------------------------
+__device__ __forceinline__ const uint32_t *key_words_of(const AttentionParams &p, int b, int h) {
+    if (p.key_words == nullptr) return nullptr;
+    return p.key_words + ((int64_t)b * p.key_word_heads + (p.key_word_heads > 1 ? h : 0)) * p.W;
+}
+
+// word `w` of the states of a (sample, head): those that exist where there is no mask
+__device__ __forceinline__ uint32_t key_word(const uint32_t *words, int S, int w) {
+    if (words != nullptr) return __ldg(words + w);
+    const int left = S - 32 * w;
+    return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
+}
+
+// the mask words of packed row r, or null where rows have none of their own
+__device__ __forceinline__ const uint32_t *row_words_of(const AttentionParams &p, int b, int h, int r) {
+    if (p.row_words == nullptr) return nullptr;
+    const int query = r / p.share;
+    const int64_t head = p.row_word_heads > 1 ? (int64_t)h * p.share + (r - query * p.share) : 0;
+    return p.row_words + (((int64_t)b * p.row_word_heads + head) * p.Q + query) * p.W;
+}
+
+// element offset of packed row r of sample b, key head h in a (B, Q, G, D) tensor of these strides
+__device__ __forceinline__ int64_t row_offset(const int64_t (&s)[3], int share, int b, int h, int r) {
+    const int query = share == 1 ? r : r / share;
+    const int head = h * share + (r - query * share);
+    return b * s[0] + query * s[1] + head * s[2];
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- host side ------------------------------------------------------------------------------------
+cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream);
+cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
+
+cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream);
+// parts of a split pass to the result: outputs and sums (forward), or the sum of gradients
+cudaError_t launch_attention_join(const AttentionParams &p, int dtype, cudaStream_t stream);
+cudaError_t launch_attention_sum(const AttentionParams &p, const float *part, void *out, bool keys, int dtype,
+                                 cudaStream_t stream);
+struct MaskParams {
+    const uint8_t *padding, *mask;        // true: not to be seen; either may be null
+    int64_t ps[2], ms[4];                 // strides of (sample, state), (sample, head, query, state)
+    int B, H, KW, Q, S, W;                // H heads of the mask (0: none), KW heads of the key words
+    uint32_t *key_words, *row_words;
+};
+cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream);
+
+// how a pass over `tiles` tiles of the long axis is split, given the CTAs that one stretch has
+struct AttentionSplit {
+    int splits, tiles;      // stretches, tiles of each
+};
+AttentionSplit attention_split(int64_t ctas, int64_t tiles, int64_t ctas_at_once, int fewest_tiles);
+
+}  // namespace msda_b200

@@ -1,0 +1,620 @@
+// Cross attention with warp-level matrix instructions: every type, every size.
+//
+// Forward: one pass over the states with the running maximum and sum of the softmax, scores and
+// weights in registers.  Backward: one kernel template in two forms.  "keys" holds 64 states and
+// walks the rows (dk, dv), the other holds 64 rows and walks the states (dq); the weights are formed
+// again in both, so that every gradient is summed by one warp in a fixed order: no atomics, the same
+// bits on every run.
+//
+// float32 operands go through the tensor cores as two terms of tf32 (x = hi + lo, 11 bits each);
+// lo * hi + hi * lo + hi * hi leaves 2^-21 of a product, sums are float32.  16-bit operands take
+// m16n8k16; the weights, and ds, are rounded to the type there (half a step each, the step of the
+// result's own rounding) and everything else stays float32.
+//
+// Where the states are many and the rows few, the states are split over CTAs and the parts joined
+// (attn_join.cu).
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.cuh"
+
+namespace msda_b200 {
+
+namespace {
+
+constexpr int kThreads = 128;      // four warps
+
+__device__ __forceinline__ uint32_t smem_address(const void *p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+__device__ __forceinline__ void cp_async16(void *to, const void *from, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_address(to)), "l"(from),
+                 "r"(valid ? 16 : 0));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// rows of a tile in shared memory are DP elements and 16 bytes apart, so that eight rows (ldmatrix),
+// and 8 x 4 or 4 x 8 single floats, fall on distinct banks
+template <typename T, int DP>
+constexpr int kPitch = DP + 16 / sizeof(T);
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_address(p)));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_address(p)));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && std::is_same_v<T, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+
+__device__ __forceinline__ void mma_tf32x3(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4],
+                                           const uint32_t (&bh)[2], const uint32_t (&bl)[2]) {
+    mma_tf32(c, al, bh);
+    mma_tf32(c, ah, bl);
+    mma_tf32(c, ah, bh);
+}
+
+// acc (16 x 8N) = A B^T: A the warp's 16 rows, B 8N rows, DP columns each
+template <typename T, int DP, int N>
+__device__ __forceinline__ void product_nt(float (&acc)[N][4], const T *a, const T *b) {
+    constexpr int P = kPitch<T, DP>;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    if constexpr (sizeof(T) == 2) {
+        const T *pa = a + (lane & 15) * P + (lane >> 4) * 8;
+        const T *pb = b + ((lane >> 4) * 8 + (lane & 7)) * P + ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int k = 0; k < DP; k += 16) {
+            uint32_t fa[4];
+            ldmatrix4(fa, pa + k);
+#pragma unroll
+            for (int n = 0; n < N; n += 2) {
+                uint32_t fb[4];
+                ldmatrix4(fb, pb + n * 8 * P + k);
+                mma16<T>(acc[n], fa, fb[0], fb[1]);
+                mma16<T>(acc[n + 1], fa, fb[2], fb[3]);
+            }
+        }
+    } else {
+#pragma unroll 4
+        for (int k = 0; k < DP; k += 8) {
+            uint32_t ah[4], al[4];
+            split_tf32(a[g * P + k + t], ah[0], al[0]);
+            split_tf32(a[(g + 8) * P + k + t], ah[1], al[1]);
+            split_tf32(a[g * P + k + t + 4], ah[2], al[2]);
+            split_tf32(a[(g + 8) * P + k + t + 4], ah[3], al[3]);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                uint32_t bh[2], bl[2];
+                split_tf32(b[(n * 8 + g) * P + k + t], bh[0], bl[0]);
+                split_tf32(b[(n * 8 + g) * P + k + t + 4], bh[1], bl[1]);
+                mma_tf32x3(acc[n], ah, al, bh, bl);
+            }
+        }
+    }
+}
+
+// acc (16 x DP) += W B: W 16 x 8N in accumulator layout, B 8N rows of DP columns
+template <typename T, int DP, int N>
+__device__ __forceinline__ void add_product_nn(float (&acc)[DP / 8][4], const float (&w)[N][4], const T *b) {
+    constexpr int P = kPitch<T, DP>;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if constexpr (sizeof(T) == 2) {
+        const T *pb = b + (lane & 15) * P + (lane >> 4) * 8;
+#pragma unroll
+        for (int n = 0; n < N; n += 2) {
+            const uint32_t fa[4] = {VecTraits<T>::pack2(make_float2(w[n][0], w[n][1])),
+                                    VecTraits<T>::pack2(make_float2(w[n][2], w[n][3])),
+                                    VecTraits<T>::pack2(make_float2(w[n + 1][0], w[n + 1][1])),
+                                    VecTraits<T>::pack2(make_float2(w[n + 1][2], w[n + 1][3]))};
+#pragma unroll
+            for (int d = 0; d < DP / 8; d += 2) {
+                uint32_t fb[4];
+                ldmatrix4_trans(fb, pb + n * 8 * P + d * 8);
+                mma16<T>(acc[d], fa, fb[0], fb[1]);
+                mma16<T>(acc[d + 1], fa, fb[2], fb[3]);
+            }
+        }
+    } else {
+        // the product's k runs over rows in any order: position t is row 2t, position t + 4 row 2t + 1,
+        // which is where the accumulator layout has them
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            uint32_t ah[4], al[4];
+            split_tf32(w[n][0], ah[0], al[0]);
+            split_tf32(w[n][2], ah[1], al[1]);
+            split_tf32(w[n][1], ah[2], al[2]);
+            split_tf32(w[n][3], ah[3], al[3]);
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d) {
+                uint32_t bh[2], bl[2];
+                split_tf32(b[(n * 8 + 2 * t) * P + d * 8 + g], bh[0], bl[0]);
+                split_tf32(b[(n * 8 + 2 * t + 1) * P + d * 8 + g], bh[1], bl[1]);
+                mma_tf32x3(acc[d], ah, al, bh, bl);
+            }
+        }
+    }
+}
+
+// The same with sums kept apart for float32: a matrix instruction cuts its sum off where it should round,
+// always towards zero, which over the thousands of instructions of a long axis adds up (17 821 states: 1.6e-5 of
+// the result, against 1e-6 so).  A tile's product starts from zero and is added with rounding; with KEEP the rows
+// of acc are scaled first, as the running maximum asks.
+template <typename T, int DP, int N, bool KEEP>
+__device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float (&w)[N][4], const T *b,
+                                           const float (&keep)[2]) {
+    if constexpr (sizeof(T) == 4) {
+        float tile[DP / 8][4];
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) tile[d][0] = tile[d][1] = tile[d][2] = tile[d][3] = 0.f;
+        add_product_nn<T, DP, N>(tile, w, b);
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                acc[d][e] = KEEP ? fmaf(acc[d][e], keep[e >> 1], tile[d][e]) : acc[d][e] + tile[d][e];
+    } else {
+        if constexpr (KEEP)
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[d][e] *= keep[e >> 1];
+        add_product_nn<T, DP, N>(acc, w, b);
+    }
+}
+
+// rows first .. first + ROWS of k or v to shared memory; rows that nobody may see become zeros
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void load_states(T *to, const T *base, int64_t stride, int first, int S, int D,
+                                            const uint32_t *words) {
+    constexpr int kVec = 16 / sizeof(T), kChunks = DP / kVec;
+    for (int i = threadIdx.x; i < ROWS * kChunks; i += kThreads) {
+        const int row = i / kChunks, chunk = i - row * kChunks, state = first + row;
+        const bool valid = chunk * kVec < D && ((key_word(words, S, state >> 5) >> (state & 31)) & 1);
+        cp_async16(to + row * kPitch<T, DP> + chunk * kVec, valid ? base + state * stride + chunk * kVec : base, valid);
+    }
+}
+
+// packed rows first .. first + ROWS of a (B, Q, G, D) tensor
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void load_rows(T *to, const T *base, const int64_t (&strides)[3], const AttentionParams &p,
+                                          int b, int h, int first) {
+    constexpr int kVec = 16 / sizeof(T), kChunks = DP / kVec;
+    for (int i = threadIdx.x; i < ROWS * kChunks; i += kThreads) {
+        const int row = i / kChunks, chunk = i - row * kChunks, r = first + row;
+        const bool valid = chunk * kVec < p.D && r < p.R;
+        cp_async16(to + row * kPitch<T, DP> + chunk * kVec,
+                   valid ? base + row_offset(strides, p.share, b, h, r) + chunk * kVec : base, valid);
+    }
+}
+
+template <typename T, int DP>
+constexpr int kTile = sizeof(T) == 4 && DP == 128 ? 32 : 64;      // rows of a walked tile
+
+// the first tile of `tiles` (each WORDS mask words) from t on in which some state may be seen
+template <int WORDS>
+__device__ __forceinline__ int next_tile(const uint32_t *words, int S, int t, int end) {
+    if (words == nullptr) return t;
+    for (; t < end; ++t) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) any |= 32 * (t * WORDS + i) < S ? __ldg(words + t * WORDS + i) : 0;
+        if (any) return t;
+    }
+    return end;
+}
+
+// WR warps side by side over 16 rows each, the other way 4 / WR warps over parts of every tile
+template <typename T, int DP, int WR>
+__global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr int BN = kTile<T, DP>, KG = 4 / WR, N = BN / KG / 8, ROWS = 16 * WR, P = kPitch<T, DP>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    T *const sq = reinterpret_cast<T *>(smem);
+    T *const sk = sq + ROWS * P;                       // two stages of k and v
+    T *const sv = sk + 2 * BN * P;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int wr = warp % WR, wk = warp / WR;
+
+    const int row_tiles = (p.R + ROWS - 1) / ROWS;
+    int64_t i = blockIdx.x;
+    const int first = (int)(i % row_tiles) * ROWS;
+    i /= row_tiles;
+    const int part = (int)(i % p.splits);
+    const int64_t bh = i / p.splits;
+    const int b = (int)(bh / p.K), h = (int)(bh % p.K);
+    const T *k = static_cast<const T *>(p.k) + b * p.ks[0] + h * p.ks[2];
+    const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + h * p.vs[2];
+    const uint32_t *words = key_words_of(p, b, h);
+    const int all_tiles = (p.S + BN - 1) / BN;
+    const int end = min(all_tiles, (part + 1) * p.tiles);
+
+    int tile = next_tile<BN / 32>(words, p.S, part * p.tiles, end);
+    load_rows<T, DP, ROWS>(sq, static_cast<const T *>(p.q), p.qs, p, b, h, first);
+    if (tile < end) {
+        load_states<T, DP, BN>(sk, k, p.ks[1], tile * BN, p.S, p.D, words);
+        load_states<T, DP, BN>(sv, v, p.vs[1], tile * BN, p.S, p.D, words);
+    }
+    cp_async_commit();
+
+    float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    const int r0 = first + wr * 16 + g;
+    const uint32_t *rw[2] = {r0 < p.R ? row_words_of(p, b, h, r0) : nullptr,
+                             r0 + 8 < p.R ? row_words_of(p, b, h, r0 + 8) : nullptr};
+
+    for (int stage = 0; tile < end; stage ^= 1) {
+        const int next = next_tile<BN / 32>(words, p.S, tile + 1, end);
+        if (next < end) {
+            load_states<T, DP, BN>(sk + (stage ^ 1) * BN * P, k, p.ks[1], next * BN, p.S, p.D, words);
+            load_states<T, DP, BN>(sv + (stage ^ 1) * BN * P, v, p.vs[1], next * BN, p.S, p.D, words);
+        }
+        cp_async_commit();
+        cp_async_wait<1>();
+        __syncthreads();
+
+        float s[N][4];
+        product_nt<T, DP, N>(s, sq + wr * 16 * P, sk + (stage * BN + wk * N * 8) * P);
+        float top[2] = {m[0], m[1]}, keep[2];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int state = tile * BN + (wk * N + n) * 8;
+            const uint32_t common = key_word(words, p.S, state >> 5);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t bits = (rw[half] != nullptr ? __ldg(rw[half] + (state >> 5)) : common) >> ((state & 31) + 2 * t);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float &x = s[n][2 * half + e];
+                    x = (bits >> e) & 1 ? x * p.scale_log2 : -INFINITY;
+                    top[half] = fmaxf(top[half], x);
+                }
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
+            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
+            const float base = top[half] == -INFINITY ? 0.f : top[half];     // nothing seen so far
+            keep[half] = fast_exp2(m[half] - base);
+            m[half] = top[half];
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[n][2 * half + e] = fast_exp2(s[n][2 * half + e] - base);
+                    sum += s[n][2 * half + e];
+                }
+            l[half] = l[half] * keep[half] + sum;
+        }
+        product_nn<T, DP, N, true>(o, s, sv + (stage * BN + wk * N * 8) * P, keep);
+        __syncthreads();
+        tile = next;
+    }
+    cp_async_wait<0>();
+
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+    }
+    if constexpr (KG > 1) {
+        // the warps' parts meet in the first warp of each row group
+        __syncthreads();
+        float *const sm = reinterpret_cast<float *>(smem);            // (4, 16) maxima, sums, then (4, 16, DP)
+        float *const sl = sm + 64, *const so = sl + 64;
+        if (t == 0) {
+            sm[warp * 16 + g] = m[0], sm[warp * 16 + g + 8] = m[1];
+            sl[warp * 16 + g] = l[0], sl[warp * 16 + g + 8] = l[1];
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                so[(warp * 16 + g + 8 * (e >> 1)) * DP + d * 8 + 2 * t + (e & 1)] = o[d][e];
+        __syncthreads();
+        if (wk != 0) return;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int row = g + 8 * half;
+            float top = m[half];
+            for (int w = 1; w < KG; ++w) top = fmaxf(top, sm[(w * WR + wr) * 16 + row]);
+            const float base = top == -INFINITY ? 0.f : top;
+            l[half] *= fast_exp2(m[half] - base);
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) o[d][2 * half + e] *= fast_exp2(m[half] - base);
+            for (int w = 1; w < KG; ++w) {
+                const int from = (w * WR + wr) * 16 + row;
+                const float keep = fast_exp2(sm[from] - base);
+                l[half] += keep * sl[from];
+#pragma unroll
+                for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        o[d][2 * half + e] += keep * so[from * DP + d * 8 + 2 * t + e];
+            }
+            m[half] = top;
+        }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = r0 + 8 * half;
+        if (r >= p.R) continue;
+        const float inverse = l[half] > 0.f || l[half] != l[half] ? 1.f / l[half] : 0.f;
+        // (a part that saw nothing has no weight when the parts are joined)
+        const float lse = l[half] == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m[half] + log2f(l[half]);
+        const int64_t at = bh * p.R + r;
+        if (p.splits > 1) {
+            float *to = p.part + (part * (int64_t)p.B * p.K * p.R + at) * p.D;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+                if (d * 8 + 2 * t < p.D)
+                    *reinterpret_cast<float2 *>(to + d * 8 + 2 * t) =
+                        make_float2(o[d][2 * half] * inverse, o[d][2 * half + 1] * inverse);
+            if (t == 0) p.part_lse[part * (int64_t)p.B * p.K * p.R + at] = lse;
+        } else {
+            const int query = r / p.share;
+            T *to = static_cast<T *>(p.out) +
+                    (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+                if (d * 8 + 2 * t < p.D) {
+                    to[d * 8 + 2 * t] = VecTraits<T>::from_float(o[d][2 * half] * inverse);
+                    to[d * 8 + 2 * t + 1] = VecTraits<T>::from_float(o[d][2 * half + 1] * inverse);
+                }
+            if (t == 0) p.lse[at] = lse;
+        }
+    }
+}
+
+// KEYS: holds 64 states, walks the rows, sums dv = p^T do and dk = ds^T q.  Otherwise holds 64 rows,
+// walks the states and sums dq = ds k.
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr int BX = 64, BN = DP == 128 ? 32 : 64, N = BN / 8, P = kPitch<T, DP>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    T *const x0 = reinterpret_cast<T *>(smem);         // k or q
+    T *const x1 = x0 + BX * P;                         // v or do
+    T *const y0 = x1 + BX * P;                         // two stages: q or k
+    T *const y1 = y0 + 2 * BN * P;                     // do or v
+    float *const s_lse = reinterpret_cast<float *>(y1 + 2 * BN * P);      // two stages of BN, KEYS only
+    float *const s_delta = s_lse + 2 * BN;
+    uint32_t *const s_words = reinterpret_cast<uint32_t *>(s_delta + 2 * BN);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+
+    const int x_tiles = ((KEYS ? p.S : p.R) + BX - 1) / BX;
+    int64_t i = blockIdx.x;
+    const int first = (int)(i % x_tiles) * BX;
+    i /= x_tiles;
+    const int part = (int)(i % p.splits);
+    const int64_t bh = i / p.splits;
+    const int b = (int)(bh / p.K), h = (int)(bh % p.K);
+    const T *k = static_cast<const T *>(p.k) + b * p.ks[0] + h * p.ks[2];
+    const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + h * p.vs[2];
+    const int64_t gs[3] = {(int64_t)p.Q * p.K * p.share * p.D, (int64_t)p.K * p.share * p.D, p.D};
+    const uint32_t *words = key_words_of(p, b, h);
+    const int all_tiles = ((KEYS ? p.R : p.S) + BN - 1) / BN;
+    int end = min(all_tiles, (part + 1) * p.tiles);
+    if (KEYS && next_tile<BX / 32>(words, p.S, first / BX, first / BX + 1) != first / BX) end = 0;   // nobody sees them
+
+    auto skip = [&](int tile) { return KEYS ? tile : next_tile<BN / 32>(words, p.S, tile, end); };
+    auto load = [&](int tile, int stage) {
+        if constexpr (KEYS) {
+            load_rows<T, DP, BN>(y0 + stage * BN * P, static_cast<const T *>(p.q), p.qs, p, b, h, tile * BN);
+            load_rows<T, DP, BN>(y1 + stage * BN * P, static_cast<const T *>(p.grad_out), gs, p, b, h, tile * BN);
+            for (int c = threadIdx.x; c < BN; c += kThreads) {
+                const int r = tile * BN + c;
+                s_lse[stage * BN + c] = r < p.R ? p.lse[bh * p.R + r] : INFINITY;
+                s_delta[stage * BN + c] = r < p.R ? p.delta[bh * p.R + r] : 0.f;
+                if (p.row_words != nullptr)
+#pragma unroll
+                    for (int w = 0; w < BX / 32; ++w)
+                        s_words[(stage * BN + c) * (BX / 32) + w] =
+                            r < p.R ? __ldg(row_words_of(p, b, h, r) + first / 32 + w) : 0;
+            }
+        } else {
+            load_states<T, DP, BN>(y0 + stage * BN * P, k, p.ks[1], tile * BN, p.S, p.D, words);
+            load_states<T, DP, BN>(y1 + stage * BN * P, v, p.vs[1], tile * BN, p.S, p.D, words);
+        }
+    };
+
+    int tile = skip(part * p.tiles);
+    if constexpr (KEYS) {
+        load_states<T, DP, BX>(x0, k, p.ks[1], first, p.S, p.D, words);
+        load_states<T, DP, BX>(x1, v, p.vs[1], first, p.S, p.D, words);
+    } else {
+        load_rows<T, DP, BX>(x0, static_cast<const T *>(p.q), p.qs, p, b, h, first);
+        load_rows<T, DP, BX>(x1, static_cast<const T *>(p.grad_out), gs, p, b, h, first);
+    }
+    if (tile < end) load(tile, 0);
+    cp_async_commit();
+
+    const int x_row = first + warp * 16 + g;           // and x_row + 8
+    float lse[2] = {INFINITY, INFINITY}, delta[2] = {0.f, 0.f};
+    const uint32_t *rw[2] = {nullptr, nullptr};
+    bool seen[2] = {false, false};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = x_row + 8 * half;
+        if constexpr (KEYS) {
+            seen[half] = (key_word(words, p.S, r >> 5) >> (r & 31)) & 1;
+        } else if (r < p.R) {
+            lse[half] = p.lse[bh * p.R + r];
+            delta[half] = p.delta[bh * p.R + r];
+            rw[half] = row_words_of(p, b, h, r);
+        }
+    }
+
+    float a0[KEYS ? DP / 8 : 1][4], a1[DP / 8][4];
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) {
+        if constexpr (KEYS) a0[d][0] = a0[d][1] = a0[d][2] = a0[d][3] = 0.f;
+        a1[d][0] = a1[d][1] = a1[d][2] = a1[d][3] = 0.f;
+    }
+
+    for (int stage = 0; tile < end; stage ^= 1) {
+        const int next = skip(tile + 1);
+        if (next < end) load(next, stage ^ 1);
+        cp_async_commit();
+        cp_async_wait<1>();
+        __syncthreads();
+
+        float s[N][4], ds[N][4];
+        product_nt<T, DP, N>(s, x0 + warp * 16 * P, y0 + stage * BN * P);
+        product_nt<T, DP, N>(ds, x1 + warp * 16 * P, y1 + stage * BN * P);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int col = n * 8 + 2 * t + e, j = 2 * half + e;
+                    bool may;
+                    float row_lse, row_delta;
+                    if constexpr (KEYS) {
+                        const int c = stage * BN + col, key = warp * 16 + g + 8 * half;
+                        may = p.row_words != nullptr ? (s_words[c * (BX / 32) + (key >> 5)] >> (key & 31)) & 1 : seen[half];
+                        row_lse = s_lse[c], row_delta = s_delta[c];
+                    } else {
+                        const int state = tile * BN + col;
+                        may = ((rw[half] != nullptr ? __ldg(rw[half] + (state >> 5)) : key_word(words, p.S, state >> 5)) >>
+                               (state & 31)) & 1;
+                        row_lse = lse[half], row_delta = delta[half];
+                    }
+                    s[n][j] = may ? fast_exp2(s[n][j] * p.scale_log2 - row_lse) : 0.f;
+                    ds[n][j] = may ? s[n][j] * (ds[n][j] - row_delta) : 0.f;
+                }
+        if constexpr (KEYS) product_nn<T, DP, N, false>(a0, s, y1 + stage * BN * P, delta);
+        product_nn<T, DP, N, false>(a1, ds, y0 + stage * BN * P, delta);
+        __syncthreads();
+        tile = next;
+    }
+    cp_async_wait<0>();
+
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int x = x_row + 8 * half;
+        if (x >= (KEYS ? p.S : p.R)) continue;
+        const int64_t rows = (int64_t)p.B * p.K * (KEYS ? p.S : p.R);
+        const int64_t at = bh * (KEYS ? p.S : p.R) + x;
+        const int query = x / p.share;
+        const int64_t final_at = KEYS ? (((int64_t)b * p.S + x) * p.K + h) * p.D
+                                      : (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (x - query * p.share)) * p.D;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+            const int c = d * 8 + 2 * t;
+            if (c >= p.D) continue;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float grad = a1[d][2 * half + e] * p.scale;
+                if (p.splits > 1) {
+                    p.part[(part * rows + at) * p.D + c + e] = grad;
+                    if constexpr (KEYS) p.part2[(part * rows + at) * p.D + c + e] = a0[d][2 * half + e];
+                } else {
+                    static_cast<T *>(KEYS ? p.dk : p.dq)[final_at + c + e] = VecTraits<T>::from_float(grad);
+                    if constexpr (KEYS)
+                        static_cast<T *>(p.dv)[final_at + c + e] = VecTraits<T>::from_float(a0[d][2 * half + e]);
+                }
+            }
+        }
+    }
+}
+
+// more than 48 KB have to be asked for; once per kernel and device, since a capture may not be told
+template <typename Kernel>
+cudaError_t launch(Kernel kernel, int64_t grid, size_t smem, cudaStream_t stream, const AttentionParams &p) {
+    if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)grid, kThreads, smem, stream>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T, int DP, int WR>
+cudaError_t forward(const AttentionParams &p, cudaStream_t stream) {
+    constexpr int rows = 16 * WR;
+    constexpr size_t tiles = (size_t)(rows + 4 * kTile<T, DP>) * kPitch<T, DP> * sizeof(T);
+    constexpr size_t join = (128 + 64 * DP) * sizeof(float);
+    const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + rows - 1) / rows);
+    return launch(attention_forward_mma_kernel<T, DP, WR>, grid, WR < 4 ? std::max(tiles, join) : tiles, stream, p);
+}
+
+template <typename T, int DP, bool KEYS>
+cudaError_t backward(const AttentionParams &p, cudaStream_t stream) {
+    constexpr int BN = DP == 128 ? 32 : 64;
+    constexpr size_t smem = (size_t)(128 + 4 * BN) * kPitch<T, DP> * sizeof(T) + 4 * BN * sizeof(float) +
+                            (size_t)2 * BN * 2 * sizeof(uint32_t);
+    const int64_t grid = (int64_t)p.B * p.K * p.splits * (((KEYS ? p.S : p.R) + 63) / 64);
+    return launch(attention_backward_mma_kernel<T, DP, KEYS>, grid, smem, stream, p);
+}
+
+template <typename T, int DP>
+cudaError_t forward_rows(const AttentionParams &p, cudaStream_t stream) {
+    return p.R <= 16 ? forward<T, DP, 1>(p, stream) : forward<T, DP, 4>(p, stream);
+}
+template <typename T, int DP>
+cudaError_t backward_side(const AttentionParams &p, bool keys, cudaStream_t stream) {
+    return keys ? backward<T, DP, true>(p, stream) : backward<T, DP, false>(p, stream);
+}
+
+template <typename T>
+cudaError_t forward_typed(const AttentionParams &p, cudaStream_t stream) {
+    return p.D <= 32 ? forward_rows<T, 32>(p, stream)
+           : p.D <= 64 ? forward_rows<T, 64>(p, stream) : forward_rows<T, 128>(p, stream);
+}
+template <typename T>
+cudaError_t backward_typed(const AttentionParams &p, bool keys, cudaStream_t stream) {
+    return p.D <= 32 ? backward_side<T, 32>(p, keys, stream)
+           : p.D <= 64 ? backward_side<T, 64>(p, keys, stream) : backward_side<T, 128>(p, keys, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream) {
+    return dtype == 0 ? forward_typed<float>(p, stream)
+           : dtype == 1 ? forward_typed<__half>(p, stream) : forward_typed<__nv_bfloat16>(p, stream);
+}
+
+cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream) {
+    return dtype == 0 ? backward_typed<float>(p, keys, stream)
+           : dtype == 1 ? backward_typed<__half>(p, keys, stream) : backward_typed<__nv_bfloat16>(p, keys, stream);
+}
+
+}  // namespace msda_b200

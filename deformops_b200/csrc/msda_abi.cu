@@ -107,23 +107,7 @@ int plan(msda_b200::Params &p, int64_t B, int64_t S, int64_t G, int64_t D, int64
     return MSDA_B200_OK;
 }
 
-// Makes `device` current for the duration of a call and restores the previous one.
-struct DeviceGuard {
-    int prev = -1;
-    bool switched = false;
-    cudaError_t err = cudaSuccess;
-    explicit DeviceGuard(int device) {
-        if (device < 0) return;
-        err = cudaGetDevice(&prev);
-        if (err == cudaSuccess && prev != device) {
-            err = cudaSetDevice(device);
-            switched = (err == cudaSuccess);
-        }
-    }
-    ~DeviceGuard() {
-        if (switched) cudaSetDevice(prev);
-    }
-};
+using msda_b200::DeviceGuard;
 
 int cuda_fail(cudaError_t e, const char *what) {
     return fail(MSDA_B200_CUDA_ERROR, "%s: %s (%s)", what, cudaGetErrorName(e),

@@ -753,4 +753,22 @@ int set_last_error(int status, const char *message);
 // adds to what msda_b200_launches() reports; defined there too
 void count_launches(int kernels, int memsets);
 
+// Makes `device` current for the duration of a call and restores the previous one.
+struct DeviceGuard {
+    int prev = -1;
+    bool switched = false;
+    cudaError_t err = cudaSuccess;
+    explicit DeviceGuard(int device) {
+        if (device < 0) return;
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != device) {
+            err = cudaSetDevice(device);
+            switched = (err == cudaSuccess);
+        }
+    }
+    ~DeviceGuard() {
+        if (switched) cudaSetDevice(prev);
+    }
+};
+
 }  // namespace msda_b200

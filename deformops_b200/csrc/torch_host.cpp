@@ -35,7 +35,10 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
+#include <string>
+#include <utility>
 
 #include "../../include/msda_b200.h"
 
@@ -54,6 +57,12 @@ struct Abi {
     decltype(&msda_b200_column_sums) column_sums = nullptr;
     decltype(&msda_b200_column_sums_scratch_bytes) column_sums_scratch_bytes = nullptr;
     decltype(&msda_b200_backward_offsets_workspace_bytes) offsets_workspace_bytes = nullptr;
+    decltype(&msda_b200_attention_mask_bytes) attention_mask_bytes = nullptr;
+    decltype(&msda_b200_attention_pack_mask) attention_pack_mask = nullptr;
+    decltype(&msda_b200_attention_workspace_bytes) attention_workspace_bytes = nullptr;
+    decltype(&msda_b200_attention_forward) attention_forward = nullptr;
+    decltype(&msda_b200_attention_backward) attention_backward = nullptr;
+    decltype(&msda_b200_rotary) rotary = nullptr;
 } abi;
 
 // One call: the operands as the kernels take them.  `ref` is undefined when `points` holds
@@ -170,6 +179,15 @@ variable_list run_backward(const Call &c, const Tensor &grad_in) {
     return {grad_value, grad_points, grad_attn};
 }
 
+// what a backward pass returns cannot be differentiated again
+variable_list once_only(variable_list out, const Tensor &grad) {
+    if (!at::GradMode::is_enabled() || !grad.requires_grad()) return out;
+    for (Tensor &t : out) t.requires_grad_(true);
+    torch::autograd::DelayedError once(
+        "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)out.size());
+    return once.apply(std::move(out));
+}
+
 // The autograd formula; differentiable once, like the Python one.
 template <bool SOFTMAX>
 struct MsdaFunction : torch::autograd::Function<MsdaFunction<SOFTMAX>> {
@@ -191,13 +209,7 @@ struct MsdaFunction : torch::autograd::Function<MsdaFunction<SOFTMAX>> {
             out = run_backward(
                 Call(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], SOFTMAX), grads[0]);
         }
-        if (at::GradMode::is_enabled() && grads[0].requires_grad()) {
-            for (Tensor &t : out) t.requires_grad_(true);
-            torch::autograd::DelayedError once(
-                "trying to differentiate twice a function that was marked with @once_differentiable",
-                (int64_t)out.size());
-            out = once.apply(std::move(out));
-        }
+        out = once_only(std::move(out), grads[0]);
         return {out[0], Tensor(), Tensor(), Tensor(), out[1], out[2]};
     }
 };
@@ -251,6 +263,188 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
             if (ctx->needs_input_grad(2 + 2 * i)) out[2 + 2 * i] = bias_gradient(g);
         }
         if (out[0].defined()) out[0] = out[0].view(x.sizes());
+        return out;
+    }
+};
+
+// ---- cross attention and rotary positions ---------------------------------------------------------
+void set_strides(const Tensor &t, int64_t (&to)[3]) {
+    // an axis of one element may have any stride; it is never taken
+    for (int i = 0; i < 3; ++i) to[i] = t.size(i) <= 1 ? 0 : t.stride(i);
+}
+
+// as the kernels read it: dense last axis, everything else in whole 16-byte vectors
+Tensor readable(const Tensor &t) {
+    const int64_t vec = 16 / (int64_t)t.element_size();
+    int64_t strides[3];
+    set_strides(t, strides);
+    bool fine = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    for (const int64_t s : strides) fine = fine && s >= 0 && s % vec == 0;
+    return fine ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+msda_b200_attention attention_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &packed,
+                                   int64_t mask_heads, double scale) {
+    msda_b200_attention c{};
+    c.batch = q.size(0), c.queries = q.size(1), c.states = k.size(1), c.heads = q.size(2), c.kv_heads = k.size(2);
+    c.head_dim = q.size(3);
+    set_strides(q, c.query_strides), set_strides(k, c.key_strides), set_strides(v, c.value_strides);
+    c.mask = packed.defined() ? packed.const_data_ptr() : nullptr;
+    c.mask_heads = (int)mask_heads;
+    c.dtype = dtype_code(q.scalar_type());
+    c.scale = (float)scale;
+    return c;
+}
+
+Tensor attention_workspace(const msda_b200_attention &c, bool backward, const at::Device &device) {
+    const int64_t nbytes = abi.attention_workspace_bytes(&c, backward);
+    return nbytes > 0 ? empty({nbytes}, at::kByte, device) : Tensor();
+}
+
+Tensor pack_mask(const Tensor &q, const Tensor &k, const Tensor &padding, const Tensor &mask, int64_t heads) {
+    if (!padding.defined() && !mask.defined()) return Tensor();
+    const at::Device device = q.device();
+    Tensor packed = empty({abi.attention_mask_bytes(q.size(0), q.size(1), k.size(1), k.size(2), (int)heads)}, at::kByte, device);
+    int64_t ps[2] = {0, 0}, ms[4] = {0, 0, 0, 0};
+    if (padding.defined()) ps[0] = padding.stride(0), ps[1] = padding.stride(1);
+    if (mask.defined()) {
+        const int64_t dim = mask.dim();
+        ms[2] = mask.stride(dim - 2), ms[3] = mask.stride(dim - 1);
+        if (dim > 2) ms[0] = mask.stride(0);
+        if (dim == 4) ms[1] = mask.stride(1);
+    }
+    check_status(abi.attention_pack_mask(padding.defined() ? padding.const_data_ptr() : nullptr, ps,
+                                         mask.defined() ? mask.const_data_ptr() : nullptr, ms, (int)heads, q.size(0),
+                                         q.size(1), k.size(1), k.size(2), packed.mutable_data_ptr(), device.index(),
+                                         c10::cuda::getCurrentCUDAStream(device.index()).stream()),
+                 "msda_b200_attention_pack_mask");
+    return packed;
+}
+
+// (out, lse)
+std::pair<Tensor, Tensor> run_attention(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, const Tensor &packed,
+                                        int64_t mask_heads, double scale) {
+    const at::Device device = q_in.device();
+    const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
+    const msda_b200_attention c = attention_call(q, k, v, packed, mask_heads, scale);
+    Tensor out = empty({c.batch, c.queries, c.heads * c.head_dim}, q.scalar_type(), device);
+    Tensor lse = empty({c.batch, c.kv_heads, c.queries, c.heads / c.kv_heads}, at::kFloat, device);
+    const Tensor workspace = attention_workspace(c, false, device);
+    check_status(abi.attention_forward(&c, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
+                                       out.mutable_data_ptr(), static_cast<float *>(lse.mutable_data_ptr()),
+                                       workspace.defined() ? workspace.mutable_data_ptr() : nullptr,
+                                       workspace.defined() ? workspace.numel() : 0, device.index(),
+                                       c10::cuda::getCurrentCUDAStream(device.index()).stream()),
+                 "msda_b200_attention_forward");
+    return {out, lse};
+}
+
+variable_list run_attention_backward(const variable_list &saved, const Tensor &grad_in, int64_t mask_heads, double scale) {
+    RECORD_FUNCTION("deformops_b200::cross_attention_backward", std::vector<c10::IValue>());
+    const at::Device device = saved[0].device();
+    const c10::cuda::CUDAGuard on_device(device);
+    const Tensor q = readable(saved[0]), k = readable(saved[1]), v = readable(saved[2]);
+    const Tensor &packed = saved[3], out = aligned(saved[4]), &lse = saved[5];
+    const Tensor grad_out = aligned(grad_in.to(q.scalar_type()).contiguous());
+    const msda_b200_attention c = attention_call(q, k, v, packed, mask_heads, scale);
+    variable_list grads = {empty(q.sizes(), q.scalar_type(), device), empty(k.sizes(), k.scalar_type(), device),
+                           empty(v.sizes(), v.scalar_type(), device)};
+    const Tensor workspace = attention_workspace(c, true, device);
+    check_status(abi.attention_backward(&c, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
+                                        out.const_data_ptr(), grad_out.const_data_ptr(),
+                                        static_cast<const float *>(lse.const_data_ptr()), grads[0].mutable_data_ptr(),
+                                        grads[1].mutable_data_ptr(), grads[2].mutable_data_ptr(),
+                                        workspace.defined() ? workspace.mutable_data_ptr() : nullptr,
+                                        workspace.defined() ? workspace.numel() : 0, device.index(),
+                                        c10::cuda::getCurrentCUDAStream(device.index()).stream()),
+                 "msda_b200_attention_backward");
+    return grads;
+}
+
+struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v,
+                          const std::optional<Tensor> &packed, int64_t mask_heads, double scale) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const auto [out, lse] = run_attention(q, k, v, packed.value_or(Tensor()), mask_heads, scale);
+        ctx->save_for_backward({q, k, v, packed.value_or(Tensor()), out, lse});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["mask_heads"] = mask_heads;
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static variable_list backward(torch::autograd::AutogradContext *ctx, const variable_list &grads) {
+        if (!grads[0].defined()) return variable_list(6);
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list out;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out = run_attention_backward(saved, grads[0], ctx->saved_data["mask_heads"].toInt(),
+                                         ctx->saved_data["scale"].toDouble());
+        }
+        out = once_only(std::move(out), grads[0]);
+        out.resize(6);
+        return out;
+    }
+};
+
+// Frequencies and axes of the pairs, packed by registry/rotary.py: doubles, then ints.
+struct RotaryPlan {
+    const std::string &packed;
+    int64_t pairs() const { return (int64_t)(packed.size() / (sizeof(double) + sizeof(int))); }
+    const double *frequencies() const { return reinterpret_cast<const double *>(packed.data()); }
+    const int *axes() const { return reinterpret_cast<const int *>(packed.data() + pairs() * sizeof(double)); }
+};
+
+int position_code(at::ScalarType t) {
+    return t == at::kFloat    ? MSDA_B200_F32
+           : t == at::kDouble ? MSDA_B200_F64
+           : t == at::kInt    ? MSDA_B200_I32
+           : t == at::kLong   ? MSDA_B200_I64
+                              : -1;
+}
+
+Tensor run_rotary(const Tensor &x_in, const Tensor &positions, const std::string &packed, bool interleaved, bool inverse) {
+    RECORD_FUNCTION("deformops_b200::rotary_turn", std::vector<c10::IValue>());
+    const at::Device device = x_in.device();
+    const c10::cuda::CUDAGuard on_device(device);
+    const Tensor x = x_in.stride(3) == 1 ? x_in : x_in.contiguous();
+    const RotaryPlan plan{packed};
+    Tensor out = empty(x.sizes(), x.scalar_type(), device);
+    const int64_t xs[3] = {x.stride(0), x.stride(1), x.stride(2)};
+    const int64_t d = positions.dim();
+    const int64_t ps[3] = {d == 3 ? positions.stride(0) : 0, positions.stride(d - 2), positions.stride(d - 1)};
+    check_status(abi.rotary(x.const_data_ptr(), xs, positions.const_data_ptr(), ps, position_code(positions.scalar_type()),
+                            out.mutable_data_ptr(), x.size(0), x.size(1), x.size(2), x.size(3), positions.size(-1),
+                            plan.pairs(), plan.frequencies(), plan.axes(), interleaved, inverse,
+                            dtype_code(x.scalar_type()), device.index(),
+                            c10::cuda::getCurrentCUDAStream(device.index()).stream()),
+                 "msda_b200_rotary");
+    return out;
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &positions,
+                          const std::string &packed, bool interleaved, bool inverse) {
+        ctx->save_for_backward({positions});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["packed"] = packed;
+        ctx->saved_data["flags"] = (int64_t)(interleaved + 2 * inverse);
+        at::AutoDispatchBelowADInplaceOrView below;
+        return run_rotary(x, positions, packed, interleaved, inverse);
+    }
+    static variable_list backward(torch::autograd::AutogradContext *ctx, const variable_list &grads) {
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const Tensor positions = ctx->get_saved_variables()[0];
+        const std::string &packed = ctx->saved_data["packed"].toStringRef();
+        const int64_t flags = ctx->saved_data["flags"].toInt();
+        // a rotation's derivative is the rotation back, which has a derivative itself
+        if (at::GradMode::is_enabled() && grads[0].requires_grad()) {
+            out[0] = RotaryFunction::apply(grads[0], positions, packed, (flags & 1) != 0, (flags & 2) == 0);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out[0] = run_rotary(grads[0], positions, packed, (flags & 1) != 0, (flags & 2) == 0);
+        }
         return out;
     }
 };
@@ -433,12 +627,105 @@ PyObject *py_linear(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// cross_attention(query, key, value, padding | None, mask | None, scale | None) -> Tensor | None
+PyObject *py_cross_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 6, "cross_attention takes six arguments");
+    if (abi.forward == nullptr || !all_plain(args, 3) || !plain_thread_state()) Py_RETURN_NONE;
+    for (int i = 3; i < 5; ++i)
+        if (args[i] != Py_None && !THPVariable_CheckExact(args[i])) Py_RETURN_NONE;
+    const Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]);
+    const Tensor padding = args[3] == Py_None ? Tensor() : THPVariable_Unpack(args[3]);
+    const Tensor mask = args[4] == Py_None ? Tensor() : THPVariable_Unpack(args[4]);
+    const at::Device device = q.device();
+    for (const Tensor *t : {&q, &k, &v, &padding, &mask})
+        if (t->defined() && !plain_tensor(*t, device)) Py_RETURN_NONE;
+    // the conditions of check_cross_attention_call and _unsupported of the Python side
+    const int dtype = dtype_code(q.scalar_type());
+    if (!supported_device(device) || dtype < 0 || k.scalar_type() != q.scalar_type() ||
+        v.scalar_type() != q.scalar_type() || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || q.numel() == 0 ||
+        k.numel() == 0 || k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3) ||
+        q.size(2) % k.size(2) != 0 || q.size(3) > 128 || q.size(3) % (dtype == MSDA_B200_F32 ? 4 : 8) != 0)
+        Py_RETURN_NONE;
+    const int64_t B = q.size(0), Q = q.size(1), G = q.size(2), S = k.size(1);
+    if (padding.defined() && (padding.scalar_type() != at::kBool || padding.dim() != 2 || padding.size(0) != B || padding.size(1) != S))
+        Py_RETURN_NONE;
+    int64_t mask_heads = 0;
+    if (mask.defined()) {
+        const int64_t d = mask.dim();
+        if (mask.scalar_type() != at::kBool || d < 2 || d > 4 || mask.size(d - 2) != Q || mask.size(d - 1) != S ||
+            (d > 2 && mask.size(0) != B) || (d == 4 && mask.size(1) != 1 && mask.size(1) != G))
+            Py_RETURN_NONE;
+        mask_heads = d == 4 ? mask.size(1) : 1;
+    }
+    double scale = 1.0 / std::sqrt((double)q.size(3));
+    if (args[5] != Py_None) {
+        scale = PyFloat_AsDouble(args[5]);
+        if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+        if (!((float)scale > 0.f) || std::isinf((float)scale)) Py_RETURN_NONE;
+    }
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        RECORD_FUNCTION("deformops_b200::cross_attention_forward", std::vector<c10::IValue>());
+        const c10::cuda::CUDAGuard on_device(device);
+        Tensor packed;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            packed = pack_mask(q, k, padding, mask, mask_heads);
+        }
+        if (at::GradMode::is_enabled() && !c10::impl::tls_is_dispatch_key_excluded(c10::DispatchKey::AutogradCUDA) &&
+            (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+            out = AttentionFunction::apply(q, k, v, packed.defined() ? std::optional<Tensor>(packed) : std::nullopt,
+                                           mask_heads, scale);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out = run_attention(q, k, v, packed, mask_heads, scale).first;
+        }
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// rotary(x, positions, packed plan, axes, interleaved) -> Tensor | None
+PyObject *py_rotary(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(nargs == 5 && PyBytes_Check(args[2]), "rotary takes five arguments");
+    if (abi.forward == nullptr || !all_plain(args, 2) || !plain_thread_state()) Py_RETURN_NONE;
+    const Tensor &x = THPVariable_Unpack(args[0]), &positions = THPVariable_Unpack(args[1]);
+    const at::Device device = x.device();
+    for (const Tensor *t : {&x, &positions})
+        if (!plain_tensor(*t, device)) Py_RETURN_NONE;
+    const std::string packed(PyBytes_AS_STRING(args[2]), (size_t)PyBytes_GET_SIZE(args[2]));
+    const int64_t pairs = RotaryPlan{packed}.pairs(), axes = PyLong_AsLongLong(args[3]), d = positions.dim();
+    if (!supported_device(device) || dtype_code(x.scalar_type()) < 0 || x.dim() != 4 || x.numel() == 0 ||
+        position_code(positions.scalar_type()) < 0 || (d != 2 && d != 3) || positions.size(d - 2) != x.size(1) ||
+        positions.size(d - 1) != axes || axes == 0 || axes > 255 || (d == 3 && positions.size(0) != x.size(0)) || 2 * pairs > x.size(3) ||
+        pairs > 128 || (positions.requires_grad() && at::GradMode::is_enabled()))
+        Py_RETURN_NONE;
+    const bool interleaved = PyObject_IsTrue(args[4]) == 1;
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (at::GradMode::is_enabled() && x.requires_grad() &&
+            !c10::impl::tls_is_dispatch_key_excluded(c10::DispatchKey::AutogradCUDA)) {
+            out = RotaryFunction::apply(x, positions, packed, interleaved, false);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out = run_rotary(x, positions, packed, interleaved, false);
+        }
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses of the ABI functions in the order of struct Abi)
 PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(nargs == 9, "bind takes nine addresses");
-    void *p[9];
-    for (int i = 0; i < 9; ++i) {
+    constexpr int kAddresses = 15;
+    TORCH_CHECK(nargs == kAddresses, "bind takes ", kAddresses, " addresses");
+    void *p[kAddresses];
+    for (int i = 0; i < kAddresses; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
         if (p[i] == nullptr) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
@@ -453,6 +740,12 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     abi.column_sums = reinterpret_cast<decltype(abi.column_sums)>(p[6]);
     abi.column_sums_scratch_bytes = reinterpret_cast<decltype(abi.column_sums_scratch_bytes)>(p[7]);
     abi.offsets_workspace_bytes = reinterpret_cast<decltype(abi.offsets_workspace_bytes)>(p[8]);
+    abi.attention_mask_bytes = reinterpret_cast<decltype(abi.attention_mask_bytes)>(p[9]);
+    abi.attention_pack_mask = reinterpret_cast<decltype(abi.attention_pack_mask)>(p[10]);
+    abi.attention_workspace_bytes = reinterpret_cast<decltype(abi.attention_workspace_bytes)>(p[11]);
+    abi.attention_forward = reinterpret_cast<decltype(abi.attention_forward)>(p[12]);
+    abi.attention_backward = reinterpret_cast<decltype(abi.attention_backward)>(p[13]);
+    abi.rotary = reinterpret_cast<decltype(abi.rotary)>(p[14]);
     abi.forward = reinterpret_cast<decltype(abi.forward)>(p[0]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
@@ -466,6 +759,8 @@ PyCFunction as_method(F f) {
 PyMethodDef methods[] = {
     {"msda", as_method(py_msda), METH_FASTCALL, nullptr},
     {"msda_offsets", as_method(py_msda_offsets), METH_FASTCALL, nullptr},
+    {"cross_attention", as_method(py_cross_attention), METH_FASTCALL, nullptr},
+    {"rotary", as_method(py_rotary), METH_FASTCALL, nullptr},
     {"linear", as_method(py_linear<1>), METH_FASTCALL, nullptr},
     {"linear_pair", as_method(py_linear<2>), METH_FASTCALL, nullptr},
     {"bind", as_method(py_bind), METH_FASTCALL, nullptr},

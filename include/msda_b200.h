@@ -48,7 +48,8 @@ extern "C" {
  * (torch.autograd.gradcheck), as in the reference (msda_launch.cuh:54-61); simple kernels, any
  * D >= 1, no scratch, not available through the *_offsets entry points.
  */
-enum msda_b200_dtype { MSDA_B200_F32 = 0, MSDA_B200_F16 = 1, MSDA_B200_BF16 = 2, MSDA_B200_F64 = 3 };
+enum msda_b200_dtype { MSDA_B200_F32 = 0, MSDA_B200_F16 = 1, MSDA_B200_BF16 = 2, MSDA_B200_F64 = 3,
+                       MSDA_B200_I32 = 4, MSDA_B200_I64 = 5 /* positions of msda_b200_rotary only */ };
 
 enum msda_b200_status {
     MSDA_B200_OK = 0,
@@ -231,6 +232,68 @@ int msda_b200_backward_static_scratch(const void *value, const int64_t *spatial_
 int msda_b200_launch_geometry(int64_t B, int64_t G, int64_t D, int64_t Q, int64_t L, int64_t K,
                               int dtype, int apply_softmax, int64_t *grid, int *threads,
                               int64_t *smem_fwd, int64_t *smem_bwd);
+
+/*
+ * Cross attention: every query attends to all states of an encoder.
+ *     out[b,q,g,:] = sum_j p_j value[b,j,h,:],  p = softmax_j(scale * query[b,q,g,:] . key[b,j,h,:])
+ * over the states j that the mask lets query q see; h = g / (heads / kv_heads).  A query that may see
+ * nothing has zeros, and no gradients.
+ *   query (batch, queries, heads, head_dim), key and value (batch, states, kv_heads, head_dim): last
+ *   axis dense, the other strides (in elements) given, whole 16-byte vectors; pointers 16-byte
+ *   aligned.  out and grad_out (batch, queries, heads * head_dim), grad_query like a dense query,
+ *   grad_key and grad_value like a dense key.  lse (batch, kv_heads, queries, heads / kv_heads) float32: base-2
+ *   logarithm of the softmax's sum, written by the forward call for the backward one.
+ *   dtype f32, f16 or bf16; head_dim at most 128, whole 16-byte vectors; scale positive.
+ *   What key and value hold for a state that no query may see is never used (it may be NaN).
+ * All sums are formed in a fixed order: the same call gives the same bits.  No counterpart in the
+ * reference.
+ */
+typedef struct msda_b200_attention {
+    int64_t batch, queries, states, heads, kv_heads, head_dim;
+    int64_t query_strides[3], key_strides[3], value_strides[3]; /* (batch, token, head) */
+    const void *mask; /* packed by msda_b200_attention_pack_mask, or NULL: all may be seen */
+    int mask_heads;   /* as it was packed: 0 without masks of single queries, 1 or `heads` with */
+    int dtype;
+    float scale;
+} msda_b200_attention;
+
+/* Bytes of a packed mask: bits instead of bytes, and which states any query may see. */
+int64_t msda_b200_attention_mask_bytes(int64_t batch, int64_t queries, int64_t states, int64_t kv_heads, int mask_heads);
+
+/*
+ * Packs `padding` (batch, states) and `mask` (batch, mask_heads, queries, states), bytes that are not
+ * zero where a state may not be seen; either may be NULL (mask_heads is 0 without `mask`).  Strides in
+ * bytes; an axis may have stride 0.
+ */
+int msda_b200_attention_pack_mask(const void *padding, const int64_t *padding_strides, const void *mask,
+                                  const int64_t *mask_strides, int mask_heads, int64_t batch, int64_t queries,
+                                  int64_t states, int64_t kv_heads, void *packed, int device, void *stream);
+
+/* Bytes of workspace (device memory, 16-byte aligned) of the forward or the backward call; may be 0. */
+int64_t msda_b200_attention_workspace_bytes(const msda_b200_attention *call, int backward);
+
+int msda_b200_attention_forward(const msda_b200_attention *call, const void *query, const void *key, const void *value,
+                                void *out, float *lse, void *workspace, int64_t workspace_bytes, int device,
+                                void *stream);
+
+int msda_b200_attention_backward(const msda_b200_attention *call, const void *query, const void *key, const void *value,
+                                 const void *out, const void *grad_out, const float *lse, void *grad_query,
+                                 void *grad_key, void *grad_value, void *workspace, int64_t workspace_bytes, int device,
+                                 void *stream);
+
+/*
+ * Rotary positions of several axes.  Pair i of every head of x (B, N, G, D) is turned by the angle
+ * positions[b, n, axis_of_pair[i]] * frequencies[i]; `interleaved` pairs are the channels (2i, 2i + 1),
+ * others (i, i + pairs); channels from 2 * pairs on are copied.  `inverse` turns back (the backward
+ * pass).  x: last axis dense, strides of (sample, token, head) in elements; positions (B, N, axes) of
+ * f32, f64, i32 or i64 with strides of all three axes; out dense.  Any alignment of whole elements.
+ * `frequencies` and `axis_of_pair` are HOST arrays of `pairs` (at most 128) entries, read during the call.
+ * Angles are formed in 64 bits.  No counterpart in the reference.
+ */
+int msda_b200_rotary(const void *x, const int64_t *x_strides, const void *positions, const int64_t *position_strides,
+                     int position_dtype, void *out, int64_t B, int64_t N, int64_t G, int64_t D, int64_t axes,
+                     int64_t pairs, const double *frequencies, const int *axis_of_pair, int interleaved, int inverse,
+                     int dtype, int device, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,380 @@
+"""Cross attention against its formula in 64 bits, with bounds that count the roundings."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from deformops_b200 import NoBackendError
+from deformops_b200.registry import Backend, cross_attention
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def make(B, Q, S, G, K, D, dtype, seed=0, device="cuda"):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    draw = lambda *s: torch.randn(*s, generator=gen, device=device).to(dtype)  # noqa: E731
+    return draw(B, Q, G, D), draw(B, S, K, D), draw(B, S, K, D), draw(B, Q, G * D)
+
+
+def hidden_of(B, Q, S, G, padding, mask, device):
+    """(B, G, Q, S): true where a state may not be seen."""
+    hidden = torch.zeros(B, G, Q, S, dtype=torch.bool, device=device)
+    if padding is not None:
+        hidden |= padding.view(B, 1, 1, S)
+    if mask is not None:
+        hidden |= mask if mask.dim() == 4 else mask.view(-1, 1, Q, S)
+    return hidden
+
+
+def formula(q, k, v, do, padding=None, mask=None, scale=None):
+    """Outputs, gradients and how far each may be off, all (value, bound) in 64 bits.
+
+    With u half a step of the type and w = 2^-24: scores are sums of D products (float32 operands go
+    through two terms of 11 bits: 2^-21 of a product), weights and ds are rounded to the type (not for
+    float32), sums over n terms are n w off at most, and every result is rounded once.
+    """
+    B, Q, G, D = q.shape
+    S, K = k.shape[1:3]
+    dtype = q.dtype
+    u, w = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    wide = dtype == torch.float32
+    product = 2.0 ** -21 if wide else 0.0
+    inner = 0.0 if wide else u
+    scale = D ** -0.5 if scale is None else scale
+    q, k, v, do = (t.detach().double() for t in (q, k, v, do))
+    q, do = q.transpose(1, 2), do.view(B, Q, G, D).transpose(1, 2)
+    k, v = (t.transpose(1, 2).repeat_interleave(G // K, 1) for t in (k, v))
+    hidden = hidden_of(B, Q, S, G, padding, mask, q.device)
+    # what nobody may see is never used
+    unused = hidden.all(2).unsqueeze(-1)
+    shared = unused.view(B, K, G // K, S, 1).all(2).repeat_interleave(G // K, 1)
+    k, v = k.masked_fill(shared, 0.0), v.masked_fill(shared, 0.0)
+    some = ~hidden.all(-1, keepdim=True)
+    s = (q @ k.transpose(-1, -2)) * scale
+    p = torch.softmax(s.masked_fill(hidden, -1e300), -1) * some
+    p = p.masked_fill(hidden, 0.0)
+    size = (q.abs() @ k.abs().transpose(-1, -2)) * scale
+    # of a weight, relative: its score's error and those of the sum (both sides), 2^-21 for each exponential
+    # (2 ulp, and the score's own rounding at its size), S w for the sum
+    off = ((D + 4) * w + product) * size.masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+    off = 2 * (off + 2.0 ** -21) + (S + 8) * w
+    o = p @ v
+    pv = p @ v.abs()
+    eo = u * o.abs() + (off + inner + product + (S + 8) * w) * pv
+    dp = do @ v.transpose(-1, -2)
+    delta = (do * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_dp = ((D + 4) * w + product) * (do.abs() @ v.abs().transpose(-1, -2))
+    e_delta = (do.abs() * eo).sum(-1, keepdim=True) + (D + 4) * w * (do.abs() * o.abs()).sum(-1, keepdim=True)
+    e_ds = p * (e_dp + e_delta) + (off + inner + product) * ds.abs()
+    n = Q * (G // K) + 8
+    dq = ds @ k * scale
+    dk = ds.transpose(-1, -2) @ q * scale
+    dv = p.transpose(-1, -2) @ do
+    e_dq = u * dq.abs() + ((e_ds + (S + 8) * w * ds.abs()) @ k.abs()) * scale
+    e_dk = ((e_ds + n * w * ds.abs()).transpose(-1, -2) @ q.abs()) * scale
+    e_dv = ((off + inner + product + n * w) * p).transpose(-1, -2) @ do.abs()
+
+    def heads(t):
+        return t.view(B, K, G // K, S, D).sum(2).transpose(1, 2)
+
+    tiny = torch.finfo(dtype).tiny
+    dk, dv, e_dk, e_dv = map(heads, (dk, dv, e_dk, e_dv))
+    e_dk, e_dv = e_dk + u * dk.abs(), e_dv + u * dv.abs()
+    back = lambda t: t.transpose(1, 2)  # noqa: E731
+    pairs = ((back(o).reshape(B, Q, G * D), back(eo).reshape(B, Q, G * D)), (back(dq), back(e_dq)), (dk, e_dk), (dv, e_dv))
+    # (products below the smallest normal number of 16-bit types are off by its half step)
+    return [(x, 1.02 * e + tiny) for x, e in pairs]
+
+
+def check(got, want, names=("out", "grad_query", "grad_key", "grad_value")):
+    for name, x, (y, bound) in zip(names, got, want):
+        x = x.detach().double()
+        assert x.shape == y.shape, name
+        worst = ((x - y).abs() / bound).max().item() if x.numel() else 0.0
+        assert worst <= 1.0, f"{name} is {worst:.2f} of its bound off"
+
+
+def run(q, k, v, do, **options):
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    out = cross_attention(q, k, v, **options)
+    return [out, *torch.autograd.grad(out, [q, k, v], do)]
+
+
+def masks(kind, B, Q, S, G, device="cuda", seed=1):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    draw = lambda *s: torch.rand(*s, generator=gen, device=device)  # noqa: E731
+    padding = mask = None
+    if "padding" in kind:
+        padding = draw(B, S) < 0.4
+        padding[:, S // 2:] |= draw(B, 1) < 0.5
+    if "shared" in kind:
+        mask = draw(Q, S) < 0.5
+    elif "heads" in kind:
+        mask = draw(B, G, Q, S) < 0.6
+        mask[:, 0] = True                                    # a head that sees nothing
+    elif "queries" in kind:
+        mask = draw(B, Q, S) < 0.7
+        mask[:, Q // 2] = True                               # a query that sees nothing
+    if "none" in kind:
+        padding = torch.ones(B, S, dtype=torch.bool, device=device)
+    return {"key_padding_mask": padding, "attention_mask": mask}
+
+
+SIZES = [  # B, Q, S, G, K, D, masks
+    (1, 1, 1, 1, 1, 8, ""), (1, 1, 77, 8, 8, 64, ""), (3, 1, 1500, 8, 2, 128, "padding"), (2, 5, 129, 4, 4, 32, "queries"),
+    (2, 16, 64, 8, 8, 32, ""), (1, 17, 300, 6, 3, 40, "heads"), (2, 100, 1344, 8, 8, 32, "padding"),
+    (2, 100, 1000, 8, 8, 32, "queries"), (1, 300, 2311, 8, 8, 32, "padding queries"), (1, 129, 65, 4, 1, 96, "shared"),
+    (2, 1000, 16, 2, 2, 64, "heads"), (1, 257, 513, 4, 2, 128, "padding"), (2, 33, 127, 2, 2, 16, "none"),
+    (1, 640, 640, 3, 3, 64, ""), (1, 200, 130, 16, 4, 128, "queries"), (1, 2, 5000, 2, 2, 32, "padding"),
+    (5, 128, 128, 1, 1, 128, ""), (1, 70, 4099, 1, 1, 56, "padding"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_outputs_and_gradients(size, dtype):
+    B, Q, S, G, K, D, kind = size
+    q, k, v, do = make(B, Q, S, G, K, D, dtype)
+    options = masks(kind, B, Q, S, G)
+    want = formula(q, k, v, do, options["key_padding_mask"], options["attention_mask"])
+    got = run(q, k, v, do, **options)
+    assert all(t.dtype == dtype for t in got)
+    check(got, want)
+    with torch.no_grad():
+        assert torch.equal(cross_attention(q, k, v, **options), got[0])
+    again = run(q, k, v, do, **options)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))        # the same bits on every run
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("Q", [1, 20, 150])
+def test_states_that_nobody_sees_may_hold_anything(dtype, Q):
+    B, S, G, K, D = 2, 260, 4, 2, 32
+    q, k, v, do = make(B, Q, S, G, K, D, dtype)
+    padding = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+    padding[0, 100:] = True
+    padding[1, ::3] = True
+    clean = run(q, k, v, do, key_padding_mask=padding)
+    for bad in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max):
+        kb, vb = (t.masked_fill(padding.view(B, S, 1, 1), bad) for t in (k, v))
+        got = run(q, kb, vb, do, key_padding_mask=padding)
+        assert all(torch.equal(a, b) for a, b in zip(got, clean))
+        # the same through a mask of every query
+        wide = padding.view(B, 1, S).expand(B, Q, S)
+        assert all(torch.equal(a, b) for a, b in zip(run(q, kb, vb, do, attention_mask=wide), clean))
+    assert all(torch.isfinite(t).all() for t in clean)
+    assert clean[2].masked_select(padding.view(B, S, 1, 1)).eq(0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_nothing_to_see_is_zero(dtype):
+    q, k, v, do = make(2, 40, 90, 2, 2, 32, dtype)
+    hidden = torch.ones(2, 90, dtype=torch.bool, device="cuda")
+    assert all(t.eq(0).all() for t in run(q, k, v, do, key_padding_mask=hidden))
+    for shape in ((2, 0, 90), (0, 40, 90), (2, 40, 0)):
+        B, Q, S = shape
+        q, k, v, do = make(B, Q, S, 2, 2, 32, dtype)
+        got = run(q, k, v, do)
+        assert got[0].shape == (B, Q, 64) and all(t.eq(0).all() for t in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_large_scores(dtype):
+    """Scores of hundreds: the maximum moves by more than an exponential's range from tile to tile."""
+    q, k, v, do = make(1, 150, 700, 2, 2, 64, dtype)
+    k = (k * torch.linspace(0.05, 8.0, 700, device="cuda").view(1, -1, 1, 1)).to(dtype)
+    check(run(q, k, v, do, scale=0.5), formula(q, k, v, do, scale=0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("Q", [3, 130])
+def test_strides(dtype, Q):
+    B, S, G, K, D = 2, 200, 8, 4, 32
+    q, k, v, do = make(B, Q, S, G, K, D, dtype)
+    mask = masks("queries", B, Q, S, G)["attention_mask"]
+    want = run(q, k, v, do, attention_mask=mask)
+    packed = torch.stack([k, v], 2)                                    # keys and values side by side
+    heads_first = q.transpose(1, 2).contiguous().transpose(1, 2)
+    odd = torch.zeros(B, S, K, D + 1, dtype=dtype, device="cuda")
+    odd[..., :D] = k
+    shifted = torch.zeros(v.numel() + 3, dtype=dtype, device="cuda")[3:].view(v.shape).copy_(v)
+    turned = mask.transpose(1, 2).contiguous().transpose(1, 2)
+    for a, b, c, m in ((q, packed[:, :, 0], packed[:, :, 1], mask), (heads_first, odd[..., :D], v, turned),
+                       (q, k, shifted, mask.view(B, 1, Q, S).expand(B, G, Q, S))):
+        got = run(a, b, c, do, attention_mask=m)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    # broadcast states: their gradient is the sum over the samples
+    one = run(q, k[:1].expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1), do)
+    full = run(q, k[:1].repeat(B, 1, 1, 1), v[:1].repeat(B, 1, 1, 1), do)
+    assert all(torch.equal(x, y) for x, y in zip(one, full))
+    leaf = k[:1].clone().requires_grad_()
+    out = cross_attention(q, leaf.expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1))
+    (grad,) = torch.autograd.grad(out, leaf, do)
+    assert torch.allclose(grad.double(), full[2].double().sum(0, keepdim=True), atol=4 * torch.finfo(dtype).eps * full[2].abs().max().item())
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """float32, along random directions: central differences with a step of 2^-6 are off by its square."""
+    q, k, v, do = make(1, 6, 40, 4, 2, 16, torch.float32, seed=5)
+    mask = masks("queries", 1, 6, 40, 4)["attention_mask"]
+    grads = run(q, k, v, do, attention_mask=mask)[1:]
+    for i in range(3):
+        step = torch.randn_like((q, k, v)[i]) * 2.0 ** -6
+        ends = []
+        for sign in (1, -1):
+            args = [q, k, v]
+            args[i] = args[i] + sign * step
+            ends.append((cross_attention(*args, attention_mask=mask).double() * do.double()).sum().item())
+        slope = (ends[0] - ends[1]) / 2
+        # third derivatives of a softmax-weighted mean are of the first one's order here
+        assert abs(slope - (grads[i].double() * step.double()).sum().item()) < 2e-3 * step.norm().item() * grads[i].norm().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_both_call_paths_agree(dtype):
+    q, k, v, do = make(2, 70, 150, 4, 2, 32, dtype)
+    options = masks("padding queries", 2, 70, 150, 4)
+    want = run(q, k, v, do, **options)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = torch.ops.deformops_b200.cross_attention_forward(*leaves, options["key_padding_mask"], options["attention_mask"],
+                                                           32 ** -0.5)[0]
+    got = [out, *torch.autograd.grad(out, leaves, do)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(cross_attention(q, k, v, backend=Backend.CUDA, **options), want[0])
+    compiled = torch.compile(lambda *a: cross_attention(*a, **options), backend="eager", fullgraph=True)
+    assert torch.equal(compiled(q, k, v), want[0])
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed():
+    q, k, v, do = make(2, 300, 1111, 8, 8, 32, torch.bfloat16)
+    options = masks("padding queries", 2, 300, 1111, 8)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        out = cross_attention(*leaves, **options)
+        return [out, *torch.autograd.grad(out, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        for t in leaves:
+            t.mul_(0.5)
+        options["key_padding_mask"].logical_not_()
+    graph.replay()
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    sets = [make(2, 64, 2000, 4, 4, 64, torch.float16, seed=s) for s in range(2)]
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(run(*s))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    q, k, v, do = make(1, 4, 6, 2, 2, 32, torch.float16)
+    with pytest.raises(NoBackendError, match="head dimension"):
+        cross_attention(*make(1, 4, 6, 2, 2, 136, torch.float16)[:3])
+    with pytest.raises(NoBackendError, match="head dimension"):
+        cross_attention(*make(1, 4, 6, 2, 2, 12, torch.float16)[:3])
+    with pytest.raises(NoBackendError, match="float64"):
+        cross_attention(q.double(), k.double(), v.double())
+    with pytest.raises(ValueError, match="one device"):
+        cross_attention(q, k, v.cpu())
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            cross_attention(q, k, v, scale=scale)
+    leaf = q.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(cross_attention(leaf, k, v), leaf, do.clone().requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grad.sum().backward()
+
+
+@pytest.mark.parametrize("change, message", [
+    (lambda a: a.update(query=torch.zeros(2, 3, 64)), "query must have 4"),
+    (lambda a: a.update(key=torch.zeros(2, 5, 2, 16)), "head dimension of query"),
+    (lambda a: a.update(key=torch.zeros(1, 5, 2, 32)), "batch of query"),
+    (lambda a: a.update(value=torch.zeros(2, 6, 2, 32)), "states of key"),
+    (lambda a: a.update(key=torch.zeros(2, 5, 3, 32), value=torch.zeros(2, 5, 3, 32)), "multiple of the 3 heads"),
+    (lambda a: a.update(key=torch.zeros(2, 5, 2, 32).half()), "common dtype"),
+    (lambda a: a.update({n: a[n].long() for n in ("query", "key", "value")}), "floating-point"),
+    (lambda a: a.update(key_padding_mask=torch.zeros(2, 5)), "bool tensor"),
+    (lambda a: a.update(key_padding_mask=torch.zeros(2, 4, dtype=torch.bool)), "states of key"),
+    (lambda a: a.update(attention_mask=torch.zeros(2, 3, 5)), "added to the scores"),
+    (lambda a: a.update(attention_mask=torch.zeros(2, 3, 3, 5, dtype=torch.bool)), "1 or 4"),
+    (lambda a: a.update(attention_mask=torch.zeros(4, 5, dtype=torch.bool)), "queries"),
+    (lambda a: a.update(attention_mask=torch.zeros(1, 3, 5, dtype=torch.bool)), "batch of query"),
+])
+def test_refusals(change, message):
+    args = {"query": torch.zeros(2, 3, 4, 32), "key": torch.zeros(2, 5, 2, 32), "value": torch.zeros(2, 5, 2, 32),
+            "key_padding_mask": None, "attention_mask": None}
+    change(args)
+    with pytest.raises(ValueError, match=message):
+        cross_attention(args.pop("query"), args.pop("key"), args.pop("value"), **args)
+
+
+def test_refusals_without_a_gpu():
+    q, k = torch.zeros(2, 3, 4, 32), torch.zeros(2, 5, 2, 32)
+    with pytest.raises(NoBackendError, match="no CPU path"):
+        cross_attention(q, k, k)
+    with pytest.raises(NoBackendError, match="not part of this build"):
+        cross_attention(q, k, k, backend=Backend.EAGER)
+    with pytest.raises(TypeError, match="string"):
+        cross_attention(q, k, k, backend="cuda")
+
+
+def test_statuses_of_the_c_interface():
+    import ctypes
+
+    from deformops_b200._loader import AttentionCall, load_library
+
+    shim = load_library()
+    three = ctypes.c_int64 * 3
+
+    def call(**changes):
+        fields = {"batch": 1, "queries": 4, "states": 9, "heads": 4, "kv_heads": 2, "head_dim": 32,
+                  "query_strides": three(512, 128, 32), "key_strides": three(576, 64, 32),
+                  "value_strides": three(576, 64, 32), "mask": None, "mask_heads": 0, "dtype": 2, "scale": 0.1}
+        fields.update(changes)
+        c = AttentionCall(**fields)
+        return shim.attention_forward(ctypes.byref(c), *[None] * 6, 0, -1, None)
+
+    assert call() == -1 and "null" in shim.last_error()
+    assert call(dtype=3) == -1 and "dtype" in shim.last_error()
+    assert call(heads=3) == -1 and call(batch=-1) == -1 and call(scale=0.0) == -1 and call(mask_heads=3) == -1
+    assert call(head_dim=36) == -2 and call(head_dim=136) == -2 and call(states=1 << 31) == -2
+    assert call(query_strides=three(512, 127, 32)) == -1 and "strides" in shim.last_error()
+    assert call(key_strides=three(-8, 64, 32)) == -1
+    assert call(queries=0) == 0 and call(batch=0) == 0
+    assert shim.attention_forward(None, *[None] * 6, 0, -1, None) == -1
+    assert shim.attention_mask_bytes(2, 5, 129, 2, 0) == 2 * 8 * 4
+    assert shim.attention_mask_bytes(2, 5, 129, 2, 4) == 4 * 8 * 2 * (2 + 4 * 5)
