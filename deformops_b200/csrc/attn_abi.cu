@@ -30,15 +30,24 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 struct Pass {
     AttentionSplit split;
     int64_t bytes;
+    int row_tiles;       // forward: tiles of 128 rows that a CTA of the tensor-core kernel holds, 0 for the other
 };
 
 Pass forward_pass(const msda_b200_attention &c) {
     const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
-    const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
-    const int64_t row_tile = rows <= 16 ? 16 : 64;
-    const AttentionSplit s = attention_split(bk * ((rows + row_tile - 1) / row_tile), (c.states + tile - 1) / tile,
-                                             148 * 4, 4);
-    return {s, s.splits > 1 ? round16(s.splits * bk * rows * 4) + s.splits * bk * rows * c.head_dim * 4 : 0};
+    Pass pass{};
+    if (c.dtype != MSDA_B200_F32 && rows > 16) {
+        pass.row_tiles = c.head_dim > 64 ? 2 : 1;
+        const int64_t held = 128 * pass.row_tiles;
+        pass.split = attention_split(bk * ((rows + held - 1) / held), (c.states + 127) / 128, 148 * (pass.row_tiles == 1 ? 2 : 1), 2);
+    } else {
+        const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
+        const int64_t held = rows <= 16 ? 16 : 64;
+        pass.split = attention_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 148 * 4, 4);
+    }
+    const int64_t parts = pass.split.splits * bk * rows;
+    pass.bytes = pass.split.splits > 1 ? round16(parts * 4) + parts * c.head_dim * 4 : 0;
+    return pass;
 }
 
 Pass backward_pass(const msda_b200_attention &c, bool keys) {
@@ -46,7 +55,7 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
     const int tile = c.head_dim > 64 ? 32 : 64;
     const int64_t held = keys ? c.states : rows, walked = keys ? rows : c.states;
     const AttentionSplit s = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);
-    return {s, s.splits > 1 ? (keys ? 2 : 1) * s.splits * bk * held * c.head_dim * 4 : 0};
+    return {s, s.splits > 1 ? (keys ? 2 : 1) * s.splits * bk * held * c.head_dim * 4 : 0, 0};
 }
 
 int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
@@ -175,7 +184,12 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     p.splits = pass.split.splits, p.tiles = pass.split.tiles;
     p.part_lse = static_cast<float *>(workspace);
     p.part = p.part_lse + round16((int64_t)p.splits * p.B * p.K * p.R * 4) / 4;
-    cudaError_t e = launch_attention_forward_mma(p, call->dtype, s);
+    cudaError_t e = cudaErrorNotSupported;
+    if (pass.row_tiles > 0) {
+        e = launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
+        if (e == cudaErrorNotSupported) p.tiles *= 2;      // the other kernel's tiles have 64 states
+    }
+    if (e == cudaErrorNotSupported) e = launch_attention_forward_mma(p, call->dtype, s);
     if (e == cudaSuccess && p.splits > 1) e = launch_attention_join(p, call->dtype, s);
     if (e == cudaSuccess) count_launches(p.splits > 1 ? 2 : 1, 0);
     return status_of(e);

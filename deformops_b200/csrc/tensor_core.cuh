@@ -1,0 +1,162 @@
+// Blackwell's asynchronous units as the attention kernels use them: mbarriers, tiled TMA loads,
+// tcgen05 matrix instructions and tensor memory.  One CTA, no clusters.
+//
+// Operand tiles in shared memory are rows of 64 or 128 bytes, swizzled: the 16-byte chunk c of row r lies
+// at r * pitch + 16 * (c ^ x), x = r % 8 (128-byte rows) or (r / 2) % 4 (64-byte rows).  Heads of 128
+// channels are two such blocks of 64 channels behind one another.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace msda_b200 {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_address(const void *p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+// ---- mbarriers ------------------------------------------------------------------------------------
+__device__ __forceinline__ void barrier_init(uint64_t *bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(bar)) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(bar)), "r"(bytes)
+                 : "memory");
+}
+// Whether the phase of this parity ended.  Bounded: a wait that runs out (it takes some seconds, no call
+// gets there) lets its role leave, so that a mistake cannot hold the GPU.
+__device__ __forceinline__ bool barrier_wait(uint64_t *bar, uint32_t parity) {
+    const uint32_t at = smem_address(bar);
+    for (int i = 0; i < 1 << 22; ++i) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done)
+                     : "r"(at), "r"(parity)
+                     : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
+// plain stores to shared memory, before the asynchronous units read them
+__device__ __forceinline__ void fence_async_shared() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// ---- TMA ------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load(void *to, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(smem_address(to)), "l"(map), "r"(smem_address(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+}
+
+// ---- tensor memory --------------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(uint32_t *to, uint32_t columns) {       // one whole warp
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(to)), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {         // one whole warp
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of the thread's own lane
+__device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31,%32};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// loaded registers may be used from here on (the compiler has to be told: nothing else ties them to the wait)
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), 
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), 
+                   "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- matrix instructions ---------------------------------------------------------------------------
+// Shared memory descriptor: address, the two strides (all in 16 bytes), version 1, swizzle of 128 or 64
+// bytes.  Rows along the product's k ("k-major"): STRIDE is that of eight rows, LEADING is not used.  Rows
+// along the other axis: STRIDE is that of eight rows (of k), LEADING that of the next 64 (32) elements.
+template <int ROW_BYTES>
+__device__ __forceinline__ uint64_t descriptor(uint32_t at, uint32_t leading) {
+    constexpr uint64_t kSwizzle = ROW_BYTES == 128 ? 2 : 4;
+    return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)((leading & 0x3ffff) >> 4) << 16 |
+           (uint64_t)((8 * ROW_BYTES) >> 4) << 32 | (uint64_t)1 << 46 | kSwizzle << 61;
+}
+// float32 sums of two 16-bit types alike; b_rows: B's rows run along k
+__host__ __device__ constexpr uint32_t instruction(bool bf16, int m, int n, bool a_rows, bool b_rows) {
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_rows ? 1u << 15 : 0u) | (b_rows ? 1u << 16 : 0u) |
+           (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"((uint32_t)add)
+                 : "memory");
+}
+// A from tensor memory: two 16-bit elements of k to a column
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+                 "r"((uint32_t)add)
+                 : "memory");
+}
+// arrives on the barrier when everything that this thread has issued is done
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(bar))
+                 : "memory");
+}
+
+// ---- swizzled tiles ---------------------------------------------------------------------------------
+template <int DP>
+constexpr int kRowBytes = DP == 32 ? 64 : 128;
+// byte offset of the 16-byte chunk (of eight channels) `chunk` of `row`, in a tile of ROWS rows
+template <int DP, int ROWS>
+__device__ __forceinline__ int swizzled(int row, int chunk) {
+    if constexpr (DP == 32) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    const int block = chunk >> 3;
+    return block * ROWS * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+template <int N>
+__device__ __forceinline__ void registers_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+}  // namespace tc
+}  // namespace msda_b200
