@@ -1,6 +1,7 @@
 // C ABI of cross attention (declared in include/msda_b200.h): argument checks and the plan of a call.
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <cstdio>
 
 #include "../../include/msda_b200.h"
@@ -30,7 +31,7 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 struct Pass {
     AttentionSplit split;
     int64_t bytes;
-    int row_tiles;       // forward: tiles of 128 rows that a CTA of the tensor-core kernel holds, 0 for the other
+    int row_tiles;       // tiles of 128 rows that a CTA of the tensor-core kernel holds, 0 for the other
 };
 
 Pass forward_pass(const msda_b200_attention &c) {
@@ -50,12 +51,44 @@ Pass forward_pass(const msda_b200_attention &c) {
     return pass;
 }
 
+// Splits of a pass whose CTAs (148 of them) take items in turn: the number that ends soonest, where an item
+// costs its tiles and `extra` more.
+AttentionSplit even_split(int64_t items, int64_t tiles, int extra) {
+    int64_t best = 1, best_cost = INT64_MAX;
+    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(tiles / 2, 148)); ++s) {
+        const int64_t each = (tiles + s - 1) / s, cost = (items * s + 147) / 148 * (each + extra);
+        if (cost < best_cost) best = s, best_cost = cost;
+        if (items * s > 148 * 8) break;
+    }
+    const int64_t each = std::max<int64_t>(1, (tiles + best - 1) / best);
+    return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
+}
+
 Pass backward_pass(const msda_b200_attention &c, bool keys) {
-    const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
-    const int tile = c.head_dim > 64 ? 32 : 64;
+    const int64_t share = c.heads / c.kv_heads, rows = c.queries * share, bk = c.batch * c.kv_heads;
     const int64_t held = keys ? c.states : rows, walked = keys ? rows : c.states;
-    const AttentionSplit s = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);
-    return {s, s.splits > 1 ? (keys ? 2 : 1) * s.splits * bk * held * c.head_dim * 4 : 0, 0};
+    Pass pass{};
+    if (c.dtype != MSDA_B200_F32 && share <= 64) {
+        pass.row_tiles = 1;
+        const int64_t x_rows = keys ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
+        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, 6);
+    } else {
+        const int tile = c.head_dim > 64 ? 32 : 64;
+        pass.split = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);
+    }
+    pass.bytes = pass.split.splits > 1 ? (keys ? 2 : 1) * pass.split.splits * bk * held * c.head_dim * 4 : 0;
+    return pass;
+}
+
+// a pass on the tensor cores, or on the other kernel (whose tiles have 64 rows, or 32) where they cannot take it
+cudaError_t launch_backward(AttentionParams &p, const Pass &pass, int dtype, bool keys, cudaStream_t stream) {
+    p.splits = pass.split.splits, p.tiles = pass.split.tiles;
+    if (pass.row_tiles > 0) {
+        const cudaError_t e = launch_attention_backward_tc(p, dtype, keys, stream);
+        if (e != cudaErrorNotSupported) return e;
+        if (p.D > 64) p.tiles *= 2;
+    }
+    return launch_attention_backward_mma(p, dtype, keys, stream);
 }
 
 int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
@@ -234,16 +267,14 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
     int launches = 3;
     cudaError_t e = launch_attention_delta(p, call->dtype, s);
     if (e == cudaSuccess) {
-        p.splits = keys.split.splits, p.tiles = keys.split.tiles;
-        p.part2 = p.part + (int64_t)p.splits * p.B * p.K * p.S * p.D;
-        e = launch_attention_backward_mma(p, call->dtype, true, s);
+        p.part2 = p.part + (int64_t)keys.split.splits * p.B * p.K * p.S * p.D;
+        e = launch_backward(p, keys, call->dtype, true, s);
         if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part, p.dk, true, call->dtype, s);
         if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part2, p.dv, true, call->dtype, s);
         launches += p.splits > 1 ? 2 : 0;
     }
     if (e == cudaSuccess) {
-        p.splits = rows.split.splits, p.tiles = rows.split.tiles;
-        e = launch_attention_backward_mma(p, call->dtype, false, s);
+        e = launch_backward(p, rows, call->dtype, false, s);
         if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part, p.dq, false, call->dtype, s);
         launches += p.splits > 1 ? 1 : 0;
     }

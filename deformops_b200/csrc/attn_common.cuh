@@ -80,6 +80,7 @@ cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cu
 // 16-bit types; row_tiles of 128 rows to a CTA, stretches of whole 128-state tiles.  cudaErrorNotSupported (and
 // nothing launched) where k or v cannot be described to TMA.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
+cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream);

@@ -25,14 +25,6 @@ constexpr int kTileRows = 128, kTileStates = 128;
 template <int DP>
 constexpr int kStages = DP == 32 ? 4 : 2;
 
-// where a state, a head and a sample stand among the axes of a tensor map, and which sample's rows a
-// broadcast tensor has
-struct TensorMap {
-    CUtensorMap map;
-    int axis_state, axis_head, axis_batch;       // 1 .. 3
-    int one_batch, one_head;
-};
-
 template <int DP, int NQ>
 struct Shared {
     alignas(1024) unsigned char q[NQ][kTileRows * DP * 2];
@@ -59,22 +51,10 @@ __device__ __forceinline__ int next_tile(const uint32_t *words, int t, int end) 
     return end;
 }
 
-template <int DP>
-__device__ __forceinline__ void load_tile(unsigned char *to, const TensorMap &m, uint64_t *bar, int b, int h, int state) {
-    tc::barrier_expect(bar, kTileStates * DP * 2);
-    int c[4];
-#pragma unroll
-    for (int i = 1; i < 4; ++i)
-        c[i] = i == m.axis_state ? state : i == m.axis_head ? (m.one_head ? 0 : h) : (m.one_batch ? 0 : b);
-#pragma unroll
-    for (int d = 0; d < DP; d += 64)
-        tc::tma_load(to + d * kTileStates * 2, &m.map, bar, d, c[1], c[2], c[3]);
-}
-
 template <typename T, int DP, int NQ>
 __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1)
-    attention_forward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMap km,
-                                const __grid_constant__ TensorMap vm) {
+    attention_forward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap km,
+                                const __grid_constant__ tc::TensorMap vm) {
     using namespace tc;
     // columns of tensor memory of one row tile: S, P, O.  At 128 channels P takes the place of S, and the next
     // scores wait for the product that reads it.
@@ -279,9 +259,15 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1)
             for (int tile = next_tile(words, part * p.tiles, end); fine && tile < end; ++n) {
                 const int stage = n % ST, turn = n / ST;
                 if (turn > 0) fine = barrier_wait(&sm.k_free[stage], (turn - 1) & 1);
-                if (fine) load_tile<DP>(sm.k[stage], km, &sm.k_full[stage], b, h, tile * kTileStates);
+                if (fine) {
+                    barrier_expect(&sm.k_full[stage], kTileStates * DP * 2);
+                    load_rows<DP, kTileStates>(sm.k[stage], km, &sm.k_full[stage], b, h, tile * kTileStates);
+                }
                 if (fine && turn > 0) fine = barrier_wait(&sm.v_free[stage], (turn - 1) & 1);
-                if (fine) load_tile<DP>(sm.v[stage], vm, &sm.v_full[stage], b, h, tile * kTileStates);
+                if (fine) {
+                    barrier_expect(&sm.v_full[stage], kTileStates * DP * 2);
+                    load_rows<DP, kTileStates>(sm.v[stage], vm, &sm.v_full[stage], b, h, tile * kTileStates);
+                }
                 tile = next_tile(words, tile + 1, end);
             }
             // nothing may still be on its way when the CTA ends
@@ -368,66 +354,11 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1)
     }
 }
 
-// the driver's own entry, asked for once
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-    static const EncodeTiled found = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult result;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &result) != cudaSuccess ||
-            result != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return found;
-}
-
-// k or v (samples, states, heads, D) with the strides of the first three axes, as tiles of 128 states
-template <typename T, int DP>
-bool make_map(TensorMap &m, const void *base, const int64_t (&strides)[3], int B, int S, int K, int D) {
-    const EncodeTiled encode = encode_tiled();
-    if (encode == nullptr) return false;
-    struct Axis {
-        int64_t stride, size;
-        int what;
-    } axes[3] = {{strides[0], B, 0}, {strides[1], S, 1}, {strides[2], K, 2}};
-    m.one_batch = m.one_head = 0;
-    for (Axis &a : axes) {
-        if (a.stride != 0 || a.what == 1) continue;
-        (a.what == 0 ? m.one_batch : m.one_head) = 1;                 // one, or the same one for all
-        a.size = 1;
-    }
-    if (axes[1].stride == 0) {
-        if (S > 1) return false;
-        axes[1].size = 1;
-    }
-    // axes from the densest on; those of one element get a stride that fits
-    std::sort(axes, axes + 3, [](const Axis &x, const Axis &y) {
-        return (x.stride == 0) != (y.stride == 0) ? y.stride == 0 : x.stride < y.stride;
-    });
-    cuuint64_t dims[4] = {(cuuint64_t)D, 0, 0, 0}, bytes[3];
-    cuuint32_t box[4] = {(cuuint32_t)std::min(DP, 64), 1, 1, 1}, ones[4] = {1, 1, 1, 1};
-    int64_t widest = (D + 7) / 8 * 8;
-    for (int i = 0; i < 3; ++i) {
-        dims[i + 1] = (cuuint64_t)axes[i].size;
-        const int64_t stride = axes[i].stride != 0 ? axes[i].stride : widest;
-        widest = std::max(widest, stride * axes[i].size);
-        bytes[i] = (cuuint64_t)stride * 2;
-        (axes[i].what == 0 ? m.axis_batch : axes[i].what == 1 ? m.axis_state : m.axis_head) = i + 1;
-        if (axes[i].what == 1) box[i + 1] = kTileStates;
-    }
-    return encode(&m.map, std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                  const_cast<void *>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  DP == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int DP, int NQ>
 cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
-    TensorMap km, vm;
-    if (!make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, p.D) || !make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, p.D))
+    tc::TensorMap km, vm;
+    if (!tc::make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, 1, p.D, kTileStates) ||
+        !tc::make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, 1, p.D, kTileStates))
         return cudaErrorNotSupported;
     const auto kernel = attention_forward_tc_kernel<T, DP, NQ>;
     constexpr size_t smem = sizeof(Shared<DP, NQ>);

@@ -7,8 +7,12 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
 
 namespace msda_b200 {
 namespace tc {
@@ -81,6 +85,13 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(at));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
+}
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -99,6 +110,13 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), 
                    "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), 
                    "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void loaded(uint32_t (&r)[16]) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), 
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
 }
@@ -147,6 +165,80 @@ __device__ __forceinline__ int swizzled(int row, int chunk) {
     if constexpr (DP == 32) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
     const int block = chunk >> 3;
     return block * ROWS * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// ---- tensor maps -------------------------------------------------------------------------------------
+// A (sample, token, head, D) tensor in tiles of rows.  Without shared heads a row is a token of one head;
+// else the rows of a key head are its `share` query heads, token after token, and a tile has whole tokens.
+struct TensorMap {
+    CUtensorMap map;
+    int axis_token, axis_head, axis_batch;       // 1 .. 3
+    int share, one_batch, one_head;              // one_*: the same for all
+};
+
+// rows first .. of key head h; `first` is a multiple of share.  The barrier expects the bytes already.
+template <int DP, int ROWS>
+__device__ __forceinline__ void load_rows(unsigned char *to, const TensorMap &m, uint64_t *bar, int b, int h, int first) {
+    const int token = m.share == 1 ? first : first / m.share;
+    int c[4];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+        c[i] = i == m.axis_token ? token : i == m.axis_head ? (m.one_head ? 0 : h * m.share) : (m.one_batch ? 0 : b);
+#pragma unroll
+    for (int d = 0; d < DP; d += 64) tma_load(to + d * ROWS * 2, &m.map, bar, d, c[1], c[2], c[3]);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// the driver's function, asked for once
+inline EncodeTiled encode_tiled() {
+    static const EncodeTiled found = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return found;
+}
+
+// `heads` key heads of `share` heads each; false where TMA cannot describe the tensor so
+template <typename T, int DP>
+bool make_map(TensorMap &m, const void *base, const int64_t (&strides)[3], int B, int tokens, int heads, int share, int D,
+              int tile_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr || share > tile_rows) return false;
+    struct Axis {
+        int64_t stride, size;
+        int what;
+    } axes[3] = {{strides[0], B, 0}, {strides[1], tokens, 1}, {strides[2], (int64_t)heads * share, 2}};
+    if ((strides[1] == 0 && tokens > 1) || (strides[2] == 0 && share > 1)) return false;
+    m.share = share;
+    m.one_batch = strides[0] == 0, m.one_head = strides[2] == 0;
+    for (Axis &a : axes)
+        if (a.stride == 0) a.size = 1;
+    // axes from the densest on, but a tile's heads before its tokens; those of one element get a stride that fits
+    const auto rank = [&](const Axis &a) { return a.stride == 0 ? INT64_MAX : a.stride; };
+    std::stable_sort(axes, axes + 3, [&](const Axis &x, const Axis &y) { return rank(x) < rank(y); });
+    if (share > 1) std::stable_sort(axes, axes + 3, [](const Axis &x, const Axis &y) { return x.what == 2 && y.what != 2; });
+    cuuint64_t dims[4] = {(cuuint64_t)D, 0, 0, 0}, bytes[3];
+    cuuint32_t box[4] = {(cuuint32_t)std::min(DP, 64), 1, 1, 1}, ones[4] = {1, 1, 1, 1};
+    int64_t widest = (D + 7) / 8 * 8;
+    for (int i = 0; i < 3; ++i) {
+        dims[i + 1] = (cuuint64_t)axes[i].size;
+        const int64_t stride = axes[i].stride != 0 ? axes[i].stride : widest;
+        widest = std::max(widest, stride * axes[i].size);
+        bytes[i] = (cuuint64_t)stride * 2;
+        (axes[i].what == 0 ? m.axis_batch : axes[i].what == 1 ? m.axis_token : m.axis_head) = i + 1;
+        if (axes[i].what == 1) box[i + 1] = (cuuint32_t)(tile_rows / share);
+        if (axes[i].what == 2) box[i + 1] = (cuuint32_t)share;
+    }
+    return encode(&m.map, std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void *>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  DP == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int N>
