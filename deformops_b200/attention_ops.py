@@ -142,11 +142,13 @@ def _backward_cuda(query, key, value, packed, mask_heads, out, grad_output, lse,
 def _forward_meta(query, key, value, key_padding_mask, attention_mask, scale):
     B, Q, G, D = query.shape
     S, K = key.shape[1], key.shape[2]
-    words = (S + 127) // 128 * 4
-    heads = 0 if attention_mask is None else attention_mask.shape[1] if attention_mask.dim() == 4 else 1
+    # the packed mask's size as msda_b200_attention_mask_bytes has it
+    words, lists = (S + 127) // 128 * 4, (2 + (S + 63) // 64 + (S + 127) // 128 + 3) // 4 * 4
+    heads = _mask_heads(attention_mask)
     nbytes = 0
     if key_padding_mask is not None or attention_mask is not None:
-        nbytes = 4 * words * B * ((K if heads > 1 else 1) + heads * Q)
+        key_heads = K if heads > 1 else 1
+        nbytes = 4 * B * (key_heads * lists + words * (key_heads + heads * Q))
     return (query.new_empty((B, Q, G * D)), query.new_empty((B, K, Q, G // K), dtype=torch.float32),
             query.new_empty((nbytes,), dtype=torch.uint8))
 

@@ -34,23 +34,6 @@ struct Pass {
     int row_tiles;       // tiles of 128 rows that a CTA of the tensor-core kernel holds, 0 for the other
 };
 
-Pass forward_pass(const msda_b200_attention &c) {
-    const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
-    Pass pass{};
-    if (c.dtype != MSDA_B200_F32 && rows > 16) {
-        pass.row_tiles = c.head_dim > 64 ? 2 : 1;
-        const int64_t held = 128 * pass.row_tiles;
-        pass.split = attention_split(bk * ((rows + held - 1) / held), (c.states + 127) / 128, 148 * (pass.row_tiles == 1 ? 2 : 1), 2);
-    } else {
-        const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
-        const int64_t held = rows <= 16 ? 16 : 64;
-        pass.split = attention_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 148 * 4, 4);
-    }
-    const int64_t parts = pass.split.splits * bk * rows;
-    pass.bytes = pass.split.splits > 1 ? round16(parts * 4) + parts * c.head_dim * 4 : 0;
-    return pass;
-}
-
 // Splits of a pass whose CTAs (148 of them) take items in turn: the number that ends soonest, where an item
 // costs its tiles and `extra` more.
 AttentionSplit even_split(int64_t items, int64_t tiles, int extra) {
@@ -62,6 +45,26 @@ AttentionSplit even_split(int64_t items, int64_t tiles, int extra) {
     }
     const int64_t each = std::max<int64_t>(1, (tiles + best - 1) / best);
     return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
+}
+
+Pass forward_pass(const msda_b200_attention &c) {
+    const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
+    Pass pass{};
+    if (c.dtype != MSDA_B200_F32 && rows > 16) {
+        // Two tiles of rows to a CTA share its loads and take 2 where one takes 1.3 (2048 x 4096, 2 samples, 16 heads x
+        // 64: 107 us against 156), unless the second has too few rows (300 x 17 821, 4 samples, 8 heads x 32: 109
+        // against 89).
+        pass.row_tiles = 13 * ((rows + 127) / 128) > 20 * ((rows + 255) / 256) ? 2 : 1;
+        const int64_t held = 128 * pass.row_tiles, tile = c.head_dim > 64 ? 128 : 64;
+        pass.split = even_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 8);
+    } else {
+        const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
+        const int64_t held = rows <= 16 ? 16 : 64;
+        pass.split = attention_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 148 * 4, 4);
+    }
+    const int64_t parts = pass.split.splits * bk * rows;
+    pass.bytes = pass.split.splits > 1 ? round16(parts * 4) + parts * c.head_dim * 4 : 0;
+    return pass;
 }
 
 Pass backward_pass(const msda_b200_attention &c, bool keys) {
@@ -130,8 +133,9 @@ AttentionParams params(const msda_b200_attention &c, const void *q, const void *
     p.scale_log2 = c.scale * 1.4426950408889634f;
     p.W = (int)mask_words(c.states);
     if (c.mask != nullptr) {
-        p.key_words = static_cast<const uint32_t *>(c.mask);
+        p.lists = static_cast<const uint32_t *>(c.mask);
         p.key_word_heads = c.mask_heads > 1 ? p.K : 1;
+        p.key_words = p.lists + (int64_t)p.B * p.key_word_heads * list_words(p.S);
         if (c.mask_heads > 0) {
             p.row_words = p.key_words + (int64_t)p.B * p.key_word_heads * p.W;
             p.row_word_heads = c.mask_heads;
@@ -155,7 +159,8 @@ using namespace msda_b200;
 int64_t msda_b200_attention_mask_bytes(int64_t batch, int64_t queries, int64_t states, int64_t kv_heads,
                                        int mask_heads) {
     if (batch <= 0 || queries < 0 || states < 0 || kv_heads <= 0 || mask_heads < 0) return 0;
-    return 4 * mask_words(states) * batch * ((mask_heads > 1 ? kv_heads : 1) + mask_heads * queries);
+    const int64_t key_heads = mask_heads > 1 ? kv_heads : 1;
+    return 4 * batch * (key_heads * list_words(states) + mask_words(states) * (key_heads + mask_heads * queries));
 }
 
 int msda_b200_attention_pack_mask(const void *padding, const int64_t *padding_strides, const void *mask,
@@ -176,12 +181,13 @@ int msda_b200_attention_pack_mask(const void *padding, const int64_t *padding_st
     for (int i = 0; i < 4 && mask != nullptr; ++i) p.ms[i] = mask_strides[i];
     p.B = (int)batch, p.H = mask_heads, p.KW = mask_heads > 1 ? (int)kv_heads : 1, p.Q = (int)queries;
     p.S = (int)states, p.W = (int)mask_words(states);
-    p.key_words = static_cast<uint32_t *>(packed);
+    p.lists = static_cast<uint32_t *>(packed);
+    p.key_words = p.lists + (int64_t)p.B * p.KW * list_words(states);
     p.row_words = p.key_words + (int64_t)p.B * p.KW * p.W;
     const DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return status_of(guard.err);
     const cudaError_t e = launch_attention_mask(p, static_cast<cudaStream_t>(stream));
-    if (e == cudaSuccess) count_launches(mask != nullptr ? 2 : 1, 0);
+    if (e == cudaSuccess) count_launches(mask != nullptr ? 3 : 1, 0);
     return status_of(e);
 }
 
@@ -220,7 +226,7 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     cudaError_t e = cudaErrorNotSupported;
     if (pass.row_tiles > 0) {
         e = launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
-        if (e == cudaErrorNotSupported) p.tiles *= 2;      // the other kernel's tiles have 64 states
+        if (e == cudaErrorNotSupported && p.D > 64) p.tiles *= 2;      // the other kernel's tiles have 64 states
     }
     if (e == cudaErrorNotSupported) e = launch_attention_forward_mma(p, call->dtype, s);
     if (e == cudaSuccess && p.splits > 1) e = launch_attention_join(p, call->dtype, s);

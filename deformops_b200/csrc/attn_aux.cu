@@ -10,37 +10,119 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A warp packs 128 states of one mask row at a time, 32 consecutive bytes to a ballot.  Rows of odd
-// length leave nothing aligned to load wider, and 32 bytes are a whole sector.
+// Lists of a sample's tiles, by one CTA: positions by counting within warps, then over the warps.
+template <int BN>
+__device__ void list_tiles(const uint32_t *words, int S, uint32_t *count, uint32_t *list) {
+    __shared__ int warps[33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tiles = (S + BN - 1) / BN;
+    int done = 0;
+    for (int base = 0; base < tiles; base += 1024) {
+        const int tile = base + threadIdx.x;
+        uint32_t any = 0, all = 0xffffffffu;
+        if (tile < tiles)
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                const uint32_t w = words[tile * (BN / 32) + i];
+                any |= w, all &= w;
+            }
+        const uint32_t mine = __ballot_sync(0xffffffffu, any != 0);
+        if (lane == 0) warps[warp] = __popc(mine);
+        __syncthreads();
+        if (warp == 0) {
+            int n = warps[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int from = __shfl_up_sync(0xffffffffu, n, o);
+                if (lane >= o) n += from;
+            }
+            warps[lane + 1] = n;
+        }
+        __syncthreads();
+        const int before = warp == 0 ? 0 : warps[warp];
+        if (any != 0)
+            list[done + before + __popc(mine & ((1u << lane) - 1))] = (uint32_t)tile | (all == 0xffffffffu ? 0x80000000u : 0u);
+        done += warps[32];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *count = done;
+}
+__device__ void list_both(const uint32_t *words, int S, uint32_t *lists) {
+    list_tiles<64>(words, S, lists, lists + 2);
+    list_tiles<128>(words, S, lists + 1, lists + 2 + (S + 63) / 64);
+}
+
+// 32 states' bits, a lane to a state; nothing before `S`
+__device__ __forceinline__ uint32_t pack_word(const uint8_t *hidden, int64_t stride, int state, int S) {
+    return __ballot_sync(0xffffffffu, state < S && __ldg(hidden + state * stride) == 0);
+}
+
+// padding alone: a CTA to a sample packs it and lists its tiles
+__global__ void __launch_bounds__(1024) attention_padding_kernel(const __grid_constant__ MaskParams p) {
+    const int lane = threadIdx.x & 31, b = blockIdx.x;
+    const uint8_t *padding = p.padding + b * p.ps[0];
+    uint32_t *words = p.key_words + (int64_t)b * p.W;
+    for (int w = threadIdx.x >> 5; w < p.W; w += 32) {
+        const uint32_t word = pack_word(padding, p.ps[1], w * 32 + lane, p.S);
+        if (lane == 0) words[w] = word;
+    }
+    __syncthreads();
+    list_both(words, p.S, p.lists + b * list_words(p.S));
+}
+
+// A warp packs 1024 states of one mask row at a time.  Rows whose states are neighbours are read 16 bytes to a
+// lane from the last 16-byte boundary on, and the bytes that were asked for are moved into place on the way (rows
+// of odd length have no alignment); others a byte to a lane.
 __global__ void __launch_bounds__(kThreads) attention_mask_kernel(const __grid_constant__ MaskParams p) {
     const int lane = threadIdx.x & 31;
-    const int groups = p.W / 4;
-    const bool own_rows = p.mask != nullptr;
-    const int64_t rows = own_rows ? (int64_t)p.B * p.H * p.Q : p.B, tasks = rows * groups;
+    const int groups = (p.W + 31) / 32;
+    const int64_t rows = (int64_t)p.B * p.H * p.Q, tasks = rows * groups;
     for (int64_t task = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); task < tasks;
          task += (int64_t)gridDim.x * (kThreads / 32)) {
         const int64_t row = task / groups;
-        const int group = (int)(task - row * groups);
-        int64_t b = row, at = 0;
-        if (own_rows) {
-            const int64_t bh = row / p.Q, query = row - bh * p.Q;
-            b = bh / p.H;
-            at = b * p.ms[0] + (bh - b * p.H) * p.ms[1] + query * p.ms[2];
-        }
-        uint8_t hidden[4];
+        const int first = (int)(task - row * groups) * 32;                 // word
+        const int64_t bh = row / p.Q, query = row - bh * p.Q, b = bh / p.H;
+        const uint8_t *mask = p.mask + b * p.ms[0] + (bh - b * p.H) * p.ms[1] + query * p.ms[2];
+        uint32_t word = 0;
+        if (p.ms[3] == 1) {
+            // lane i: bytes of states first * 32 + 32 i .. + 31, from three aligned vectors
+            const int state = (first + lane) * 32;
+            const uintptr_t at = reinterpret_cast<uintptr_t>(mask + state);
+            const uint4 *from = reinterpret_cast<const uint4 *>(at & ~(uintptr_t)15);
+            const int off = (int)(at & 15), left = p.S - state;            // bytes that exist
+            uint32_t bits[2] = {0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const int state = group * 128 + w * 32 + lane;
-            hidden[w] = state >= p.S;
-            if (state < p.S && own_rows) hidden[w] = __ldg(p.mask + at + state * p.ms[3]);
-            if (state < p.S && p.padding != nullptr) hidden[w] |= __ldg(p.padding + b * p.ps[0] + state * p.ps[1]);
-        }
-        uint32_t words[4];
+            for (int v = 0; v < 3; ++v) {
+                // (a vector with one byte that exists is within the allocation's 16-byte granule)
+                if (left > 0 && 16 * v - off < min(left, 32)) {
+                    const uint4 x = __ldg(from + v);
+                    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                    uint32_t seen = 0;                                       // of 16 bytes
 #pragma unroll
-        for (int w = 0; w < 4; ++w) words[w] = __ballot_sync(0xffffffffu, hidden[w] == 0);
-        if (lane == 0)
-            *reinterpret_cast<uint4 *>((own_rows ? p.row_words : p.key_words) + row * p.W + group * 4) =
-                make_uint4(words[0], words[1], words[2], words[3]);
+                    for (int i = 0; i < 4; ++i)
+                        // each byte 0 or not: its lowest bit to bit 4 i + byte
+                        seen |= ((__vcmpeq4(in[i], 0) & 0x08040201u) * 0x01010101u >> 24) << (4 * i);
+                    if (v < 2)
+                        bits[0] |= seen << (16 * v);
+                    else
+                        bits[1] = seen;
+                }
+            }
+            word = __funnelshift_r(bits[0], bits[1], off);
+            if (left < 32) word = left <= 0 ? 0u : word & ((1u << left) - 1);
+        } else {
+            for (int i = 0; i < 32 && first + i < p.W; ++i) {
+                const uint32_t x = pack_word(mask, p.ms[3], (first + i) * 32 + lane, p.S);
+                if (i == lane) word = x;
+            }
+        }
+        if (p.padding != nullptr) {
+            const uint8_t *padding = p.padding + b * p.ps[0];
+            for (int i = 0; i < 32 && first + i < p.W; ++i) {
+                const uint32_t x = pack_word(padding, p.ps[1], (first + i) * 32 + lane, p.S);
+                if (i == lane) word &= x;
+            }
+        }
+        if (first + lane < p.W) p.row_words[row * p.W + first + lane] = word;
     }
 }
 
@@ -59,6 +141,10 @@ __global__ void __launch_bounds__(1024) attention_mask_any_kernel(const __grid_c
     found = __reduce_or_sync(0xffffffffu, any[lane][part]);
     const int word = (blockIdx.x - bk * blocks) * 32 + part;
     if (lane == 0 && word < p.W) p.key_words[(int64_t)bk * p.W + word] = found;
+}
+
+__global__ void __launch_bounds__(1024) attention_list_kernel(const __grid_constant__ MaskParams p) {
+    list_both(p.key_words + (int64_t)blockIdx.x * p.W, p.S, p.lists + blockIdx.x * list_words(p.S));
 }
 
 // eight lanes to a row
@@ -174,11 +260,15 @@ cudaError_t delta_typed(const AttentionParams &p, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream) {
-    const int64_t tasks = (p.mask != nullptr ? (int64_t)p.B * p.H * p.Q : p.B) * (p.W / 4);
+    if (p.mask == nullptr) {
+        attention_padding_kernel<<<(unsigned)p.B, 1024, 0, stream>>>(p);
+        return cudaGetLastError();
+    }
+    const int64_t tasks = (int64_t)p.B * p.H * p.Q * ((p.W + 31) / 32);
     const int64_t grid = std::min<int64_t>((tasks + kThreads / 32 - 1) / (kThreads / 32), 148 * 64);
     attention_mask_kernel<<<(unsigned)grid, kThreads, 0, stream>>>(p);
-    if (p.mask != nullptr)
-        attention_mask_any_kernel<<<(unsigned)(p.B * p.KW * ((p.W + 31) / 32)), 1024, 0, stream>>>(p);
+    attention_mask_any_kernel<<<(unsigned)(p.B * p.KW * ((p.W + 31) / 32)), 1024, 0, stream>>>(p);
+    attention_list_kernel<<<(unsigned)(p.B * p.KW), 1024, 0, stream>>>(p);
     return cudaGetLastError();
 }
 

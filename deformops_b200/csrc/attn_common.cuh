@@ -10,10 +10,12 @@
 //
 // A row that may see nothing has o = 0, L = +inf and no gradients (exp2(x - inf) = 0).
 //
-// Masks are packed into bits by a kernel of their own (one pass over a byte mask that every head would
+// Masks are packed into bits by kernels of their own (one pass over a byte mask that every head would
 // otherwise read again): bit j % 32 of word j / 32 is set where state j may be seen; words behind the
 // last state are 0.  `key_words` holds for every state whether any row may see it: the rows of k and v
-// of states that nobody sees are never used, whatever they hold.
+// of states that nobody sees are never used, whatever they hold.  `lists` names the tiles of 64 and of 128
+// states of which some may be seen, bit 31 set where all may: a pass over the states takes those and no
+// others, and is split over CTAs by their number.
 #pragma once
 
 #include "msda_common.cuh"
@@ -30,6 +32,7 @@ struct AttentionParams {
     float scale, scale_log2;               // scale * log2(e)
     const uint32_t *key_words;             // (B, key_word_heads, W) or null: every state may be seen
     const uint32_t *row_words;             // (B, row_word_heads, Q, W) or null: rows see what key_words has
+    const uint32_t *lists;                 // (B, key_word_heads, 2 + T64 + T128): two counts, two lists; or null
     int key_word_heads, row_word_heads, W;
     void *out;                             // (B, Q, G * D)
     float *lse;                            // (B, K, R), log2 of the sum of exp2
@@ -54,6 +57,32 @@ __device__ __forceinline__ uint32_t key_word(const uint32_t *words, int S, int w
     return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
 }
 
+// ---- the tiles of BN states that a stretch of a pass takes -----------------------------------------
+__host__ __device__ inline int64_t list_words(int64_t S) { return (2 + (S + 63) / 64 + (S + 127) / 128 + 3) / 4 * 4; }
+
+template <int BN>
+struct Tiles {
+    const uint32_t *list;        // entries from the first one on, or null: all tiles
+    int first, count, S;
+
+    __device__ __forceinline__ Tiles(const AttentionParams &p, int b, int h, int part) : list(nullptr), S(p.S) {
+        int all = (S + BN - 1) / BN;
+        if (p.lists != nullptr) {
+            const uint32_t *l = p.lists + ((int64_t)b * p.key_word_heads + (p.key_word_heads > 1 ? h : 0)) * list_words(S);
+            all = (int)__ldg(l + (BN == 128));
+            list = l + 2 + (BN == 128 ? (S + 63) / 64 : 0);
+        }
+        first = (int)((int64_t)part * all / p.splits);
+        count = (int)((int64_t)(part + 1) * all / p.splits) - first;
+        if (list != nullptr) list += first;
+    }
+    // tile n of the stretch, bit 31 set where all of its states may be seen (by somebody)
+    __device__ __forceinline__ uint32_t operator[](int n) const {
+        if (list != nullptr) return __ldg(list + n);
+        return (uint32_t)(first + n) | ((first + n + 1) * (int64_t)BN <= S ? 0x80000000u : 0u);
+    }
+};
+
 // the mask words of packed row r, or null where rows have none of their own
 __device__ __forceinline__ const uint32_t *row_words_of(const AttentionParams &p, int b, int h, int r) {
     if (p.row_words == nullptr) return nullptr;
@@ -75,9 +104,26 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
+// a * b + c of pairs, into registers of its own
+__device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)),
+          "l"(reinterpret_cast<const unsigned long long &>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
+    return r;
+}
+
 // ---- host side ------------------------------------------------------------------------------------
 cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream);
-// 16-bit types; row_tiles of 128 rows to a CTA, stretches of whole 128-state tiles.  cudaErrorNotSupported (and
+// 16-bit types; row_tiles of 128 rows to a CTA, stretches of whole tiles of 64 states (128 where D > 64).  cudaErrorNotSupported (and
 // nothing launched) where k or v cannot be described to TMA.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
@@ -92,7 +138,7 @@ struct MaskParams {
     const uint8_t *padding, *mask;        // true: not to be seen; either may be null
     int64_t ps[2], ms[4];                 // strides of (sample, state), (sample, head, query, state)
     int B, H, KW, Q, S, W;                // H heads of the mask (0: none), KW heads of the key words
-    uint32_t *key_words, *row_words;
+    uint32_t *key_words, *row_words, *lists;
 };
 cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream);
 

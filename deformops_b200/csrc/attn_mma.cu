@@ -188,11 +188,12 @@ __device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float 
             for (int e = 0; e < 4; ++e)
                 acc[d][e] = KEEP ? fmaf(acc[d][e], keep[e >> 1], tile[d][e]) : acc[d][e] + tile[d][e];
     } else {
-        if constexpr (KEEP)
+        if constexpr (KEEP) {
 #pragma unroll
             for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[d][e] *= keep[e >> 1];
+        }
         add_product_nn<T, DP, N>(acc, w, b);
     }
 }

@@ -27,7 +27,11 @@ namespace {
 constexpr int kX = 128, kY = 64;
 
 template <int DP>
-constexpr int kStages = DP == 128 ? 2 : 4;
+constexpr int kStages = DP == 128 ? 2 : 6;
+
+// warpgroups that take the tiles Y in turn: as many as tensor memory has room for
+template <int DP>
+constexpr int kGroupsOf = DP == 128 ? 2 : 3;
 
 template <int DP, bool KEYS>
 struct Shared {
@@ -37,99 +41,100 @@ struct Shared {
     alignas(16) float lse[KEYS ? ST : 1][kY];                   // of the walked rows, both with the sign turned
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
-    uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], row_full[ST], row_free[ST];
-    uint64_t s_full[2], p_full[2], acc_full, acc_free;
+    uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
+    uint64_t s_full[kGroupsOf<DP>], p_full[kGroupsOf<DP>], acc_full, acc_free;
     uint32_t tmem;
 };
 
+// What a CTA does at a time: a tile X and a stretch of tiles Y.
 struct Item {
-    int first, part, b, h, begin, end;       // of X; of Y, in tiles
+    int first, part, b, h;       // of X
     int64_t bh;
 };
 
-// x_rows, y_rows: rows that a tile takes (all of them for states; whole groups of heads for packed rows)
-template <bool KEYS>
-__device__ __forceinline__ Item item_of(const AttentionParams &p, int64_t i, int x_rows, int y_rows) {
-    const int X = KEYS ? p.S : p.R, Y = KEYS ? p.R : p.S;
-    const int x_tiles = (X + x_rows - 1) / x_rows, y_tiles = (Y + y_rows - 1) / y_rows;
+// x_rows: rows that a tile takes (all of them for states; whole groups of heads for packed rows)
+__device__ __forceinline__ Item item_of(const AttentionParams &p, int64_t i, int x_tiles, int x_rows) {
     Item t;
     t.first = (int)(i % x_tiles) * x_rows;
     i /= x_tiles;
     t.part = (int)(i % p.splits);
     t.bh = i / p.splits;
     t.b = (int)(t.bh / p.K), t.h = (int)(t.bh % p.K);
-    t.begin = t.part * p.tiles;
-    t.end = min(y_tiles, t.begin + p.tiles);
-    if constexpr (KEYS) {
-        const uint32_t *words = key_words_of(p, t.b, t.h);
-        if (words != nullptr) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(words + t.first / 32));
-            if ((w.x | w.y | w.z | w.w) == 0) t.end = t.begin;              // nobody sees these states
-        }
-    }
     return t;
 }
 
-// the first tile of 64 states from t on in which some may be seen
-__device__ __forceinline__ int next_tile(const uint32_t *words, int t, int end) {
-    if (words == nullptr) return t;
-    for (; t < end; ++t) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(words) + t);
-        if (w.x | w.y) return t;
+// the tiles Y of an item: listed tiles of states, or all of the rows
+template <bool KEYS>
+struct Walk;
+template <>
+struct Walk<false> : Tiles<kY> {
+    __device__ __forceinline__ Walk(const AttentionParams &p, const Item &t, int) : Tiles<kY>(p, t.b, t.h, t.part) {}
+};
+template <>
+struct Walk<true> {
+    int first, count;
+    __device__ __forceinline__ Walk(const AttentionParams &p, const Item &t, int y_rows) {
+        const int all = (p.R + y_rows - 1) / y_rows;
+        first = (int)((int64_t)t.part * all / p.splits);
+        count = (int)((int64_t)(t.part + 1) * all / p.splits) - first;
+        const uint32_t *words = key_words_of(p, t.b, t.h);
+        if (words != nullptr) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(words + t.first / 32));
+            if ((w.x | w.y | w.z | w.w) == 0) count = 0;                  // nobody sees these states
+        }
     }
-    return end;
-}
-
-// 64 columns of exponents or differences at a time: x = a * scale + b over pairs
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    ffma2(c, a, b);
-    return c;
-}
+    __device__ __forceinline__ uint32_t operator[](int n) const { return (uint32_t)(first + n); }
+};
 
 template <typename T, int DP, bool KEYS>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
     attention_backward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap x0m,
                                  const __grid_constant__ tc::TensorMap x1m, const __grid_constant__ tc::TensorMap y0m,
                                  const __grid_constant__ tc::TensorMap y1m, int64_t items, int x_rows, int y_rows) {
     using namespace tc;
     constexpr int ST = kStages<DP>;
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
-    constexpr uint32_t kS = 0, kT = 64, kGroup = 128, kAcc0 = 256, kAcc1 = KEYS ? 256 + DP : 256;
+    constexpr int kGroups = kGroupsOf<DP>, kLast = 4 * kGroups;
+    constexpr uint32_t kS = 0, kT = 64, kGroup = 128, kAcc0 = kGroups * 128, kAcc1 = KEYS ? kAcc0 + DP : kAcc0;
+    static_assert(kAcc1 + DP <= 512);
     extern __shared__ __align__(1024) unsigned char raw[];
     auto &sm = *reinterpret_cast<Shared<DP, KEYS> *>(raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-    if (warp == 8) tmem_alloc(&sm.tmem, 512);
+    if (warp == kLast) tmem_alloc(&sm.tmem, 512);
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
             barrier_init(&sm.x_full[s], 1), barrier_init(&sm.x_free[s], 1);
-            barrier_init(&sm.s_full[s], 1), barrier_init(&sm.p_full[s], 128);
         }
+        for (int g = 0; g < kGroups; ++g) barrier_init(&sm.s_full[g], 1), barrier_init(&sm.p_full[g], 128);
         for (int s = 0; s < ST; ++s) {
             barrier_init(&sm.y_full[s], 1), barrier_init(&sm.y_free[s], 1);
+            barrier_init(&sm.y_clean[s], 32);
             barrier_init(&sm.row_full[s], 32), barrier_init(&sm.row_free[s], 128);
         }
-        barrier_init(&sm.acc_full, 1), barrier_init(&sm.acc_free, 256);
+        barrier_init(&sm.acc_full, 1), barrier_init(&sm.acc_free, 256);      // (two groups write the sums)
     }
     if (y_rows < kY) {      // rows that no load reaches
-        for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += 384) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += kGroups * 128 + 128) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
         fence_async_shared();
     }
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sm.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    const int x_tiles = ((KEYS ? p.S : p.R) + x_rows - 1) / x_rows;
     bool fine = true;
 
-    if (warp < 8) {
-        registers_up<224>();
+    if (warp < kLast) {
+        registers_up<kGroups == 2 ? 224 : 152>();
         const int group = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t mine = tmem + group * kGroup + lanes;
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
         int n = 0, done = 0;             // tiles and items with tiles so far
         for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
-            const Item it = item_of<KEYS>(p, i, x_rows, y_rows);
+            const Item it = item_of(p, i, x_tiles, x_rows);
+            const Walk<KEYS> walk(p, it, y_rows);
             const uint32_t *words = key_words_of(p, it.b, it.h);
             const int x = it.first + row;
             const bool mine_valid = row < x_rows && x < (KEYS ? p.S : p.R);
@@ -144,30 +149,36 @@ __global__ void __launch_bounds__(384, 1)
                 my_delta = -p.delta[it.bh * p.R + x];
                 rw = row_words_of(p, it.b, it.h, x);
             }
+            const bool own_words = p.row_words != nullptr;
             const int before = n;
-            for (int tile = KEYS ? it.begin : next_tile(words, it.begin, it.end); fine && tile < it.end; ++n) {
-                const int next = KEYS ? tile + 1 : next_tile(words, tile + 1, it.end);
-                if ((n & 1) != group) {
-                    tile = next;
-                    continue;
-                }
+            if (rw == nullptr) rw = words;
+            uint32_t entry = 0;
+            uint2 see = make_uint2(0, 0);
+            // the mask of this group's next tile comes while it works on another
+            const auto fetch = [&](int at) {
+                if (at >= before + walk.count) return;
+                entry = walk[at - before];
+                if (rw != nullptr && (own_words || !(entry >> 31)))
+                    see = __ldg(reinterpret_cast<const uint2 *>(rw) + (entry & 0x7fffffff));
+            };
+            n += (group + kGroups - n % kGroups) % kGroups;
+            if constexpr (!KEYS) fetch(n);
+            for (; fine && n < before + walk.count; n += kGroups) {
                 const int stage = n % ST;
-                uint2 see = make_uint2(0, 0);
-                if constexpr (!KEYS)
-                    see = rw != nullptr ? __ldg(reinterpret_cast<const uint2 *>(rw) + tile)
-                                        : make_uint2(key_word(words, p.S, 2 * tile), key_word(words, p.S, 2 * tile + 1));
+                const uint32_t now = entry;
+                uint2 may = see;
+                if constexpr (!KEYS) fetch(n + kGroups);
                 if constexpr (KEYS) fine = barrier_wait(&sm.row_full[stage], (n / ST) & 1);
-                fine = barrier_wait(&sm.s_full[group], (n >> 1) & 1) && fine;
+                fine = barrier_wait(&sm.s_full[group], (n / kGroups) & 1) && fine;
                 if (!fine) break;
                 fence_after();
                 if (!idle) {
-                    uint32_t s[2][32], t[2][32];
+                    uint32_t s[2][32], t[32];
                     tmem_load32(s[0], mine + kS), tmem_load32(s[1], mine + kS + 32);
                     tmem_wait_load();
                     loaded(s[0]), loaded(s[1]);
-                    tmem_load32(t[0], mine + kT), tmem_load32(t[1], mine + kT + 32);
+                    tmem_load32(t, mine + kT);
                     float2 w[32];
-                    uint32_t packed[32];
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         const uint32_t *from = &s[c >> 4][(2 * c) & 31];
@@ -179,13 +190,18 @@ __global__ void __launch_bounds__(384, 1)
                         w[c + 1].x = fast_exp2(w[c + 1].x), w[c + 1].y = fast_exp2(w[c + 1].y);
                     }
                     // which of the 64 may be seen; `some` where not all of the warp's are
-                    const bool some = KEYS ? p.row_words != nullptr || !__all_sync(0xffffffffu, seen)
-                                           : !__all_sync(0xffffffffu, (see.x & see.y) == 0xffffffffu);
-                    uint32_t see0 = see.x, see1 = see.y;
+                    const bool some = KEYS ? own_words || !__all_sync(0xffffffffu, seen)
+                                      : own_words ? !__all_sync(0xffffffffu, (may.x & may.y) == 0xffffffffu) : !(now >> 31);
+                    uint32_t see0 = may.x, see1 = may.y;
                     if (some) {
+                        if constexpr (!KEYS)
+                            if (rw == nullptr) {
+                                see0 = key_word(nullptr, p.S, 2 * (now & 0x7fffffff));
+                                see1 = key_word(nullptr, p.S, 2 * (now & 0x7fffffff) + 1);
+                            }
                         if constexpr (KEYS) {
                             see0 = see1 = seen ? 0xffffffffu : 0u;
-                            if (p.row_words != nullptr) {
+                            if (own_words) {
                                 see0 = see1 = 0;
                                 const uint32_t *of = sm.words[stage][warp & 3];
 #pragma unroll
@@ -204,46 +220,54 @@ __global__ void __launch_bounds__(384, 1)
                     }
                     if constexpr (KEYS) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) packed[c] = VecTraits<T>::pack2(w[c]);
-                        tmem_store32(mine + kS, packed);
-                    }
-                    tmem_wait_load();
-                    loaded(t[0]), loaded(t[1]);
+                        for (int half = 0; half < 2; ++half) {
+                            uint32_t packed[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const uint32_t *from = &t[c >> 4][(2 * c) & 31];
-                        float4 d = make_float4(my_delta, my_delta, my_delta, my_delta);
-                        if constexpr (KEYS) d = *reinterpret_cast<const float4 *>(&sm.delta[stage][2 * c]);
-                        const float2 one = make_float2(1.f, 1.f);
-                        w[c] = fmul2(w[c], fma2(make_float2(__uint_as_float(from[0]), __uint_as_float(from[1])), one, make_float2(d.x, d.y)));
-                        w[c + 1] = fmul2(w[c + 1], fma2(make_float2(__uint_as_float(from[2]), __uint_as_float(from[3])), one, make_float2(d.z, d.w)));
-                    }
-                    if (some) {
-                        // (0 times what an unseen state's v holds)
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const uint32_t bits = c < 16 ? see0 >> (2 * c) : see1 >> (2 * c - 32);
-                            if (!(bits & 1)) w[c].x = 0.f;
-                            if (!(bits & 2)) w[c].y = 0.f;
+                            for (int c = 0; c < 16; ++c) packed[c] = VecTraits<T>::pack2(w[16 * half + c]);
+                            tmem_store16(mine + kS + 16 * half, packed);
                         }
                     }
+                    // (the first half of dS takes the place of a quarter of T that is in registers by then)
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) packed[c] = VecTraits<T>::pack2(w[c]);
-                    tmem_store32(mine + kT, packed);
+                    for (int half = 0; half < 2; ++half) {
+                        if (half == 1) tmem_load32(t, mine + kT + 32);
+                        tmem_wait_load();
+                        loaded(t);
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) {
+                            const int at = 16 * half + c;
+                            float4 d = make_float4(my_delta, my_delta, my_delta, my_delta);
+                            if constexpr (KEYS) d = *reinterpret_cast<const float4 *>(&sm.delta[stage][2 * at]);
+                            float2 x = fmul2(w[at], add2(make_float2(__uint_as_float(t[2 * c]), __uint_as_float(t[2 * c + 1])), make_float2(d.x, d.y)));
+                            float2 y = fmul2(w[at + 1], add2(make_float2(__uint_as_float(t[2 * c + 2]), __uint_as_float(t[2 * c + 3])), make_float2(d.z, d.w)));
+                            if (some) {
+                                // (0 times what an unseen state's v holds)
+                                const uint32_t bits = half == 0 ? see0 >> (2 * c) : see1 >> (2 * c);
+                                if (!(bits & 1)) x.x = 0.f;
+                                if (!(bits & 2)) x.y = 0.f;
+                                if (!(bits & 4)) y.x = 0.f;
+                                if (!(bits & 8)) y.y = 0.f;
+                            }
+                            packed[c] = VecTraits<T>::pack2(x), packed[c + 1] = VecTraits<T>::pack2(y);
+                        }
+                        tmem_store16(mine + kT + 16 * half, packed);
+                    }
                     tmem_wait_store();
                 }
                 if constexpr (KEYS) barrier_arrive(&sm.row_free[stage]);
                 fence_before();
                 barrier_arrive(&sm.p_full[group]);
-                tile = next;
             }
-            const bool some = n > before;
+            n = before + walk.count;
+            const bool some = walk.count > 0;
             if (some) {
                 fine = fine && barrier_wait(&sm.acc_full, done & 1);
                 fence_after();
                 ++done;
             }
-            // sums to memory: each group takes one of the two, or half of the one
+            // sums to memory: two of the groups take one of the two each, or half of the one
+            if (group > 1) continue;
             constexpr int kHalf = KEYS ? DP : DP / 2;
             const uint32_t acc = tmem + lanes + (KEYS ? (group == 0 ? kAcc0 : kAcc1) : kAcc1 + group * kHalf);
             const int from = KEYS ? 0 : group * kHalf;
@@ -289,13 +313,12 @@ __global__ void __launch_bounds__(384, 1)
         }
     } else {
         registers_down<56>();
-        if (warp == 8 && lane == 0) {
+        if (warp == kLast && elect_one()) {
             int n = 0, done = 0;
             for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
-                const Item it = item_of<KEYS>(p, i, x_rows, y_rows);
-                const uint32_t *words = key_words_of(p, it.b, it.h);
-                int tile = KEYS ? it.begin : next_tile(words, it.begin, it.end);
-                if (tile >= it.end) continue;
+                const Item it = item_of(p, i, x_tiles, x_rows);
+                const Walk<KEYS> walk(p, it, y_rows);
+                if (walk.count == 0) continue;
                 const int buffer = done & 1;
                 if (done > 1) fine = barrier_wait(&sm.x_free[buffer], ((done >> 1) - 1) & 1);
                 if (!fine) break;
@@ -303,14 +326,13 @@ __global__ void __launch_bounds__(384, 1)
                 load_rows<DP, kX>(sm.x[buffer][0], x0m, &sm.x_full[buffer], it.b, it.h, it.first);
                 load_rows<DP, kX>(sm.x[buffer][1], x1m, &sm.x_full[buffer], it.b, it.h, it.first);
                 ++done;
-                for (; fine && tile < it.end; ++n) {
-                    const int stage = n % ST;
+                for (int j = 0; fine && j < walk.count; ++j, ++n) {
+                    const int stage = n % ST, row = (int)(walk[j] & 0x7fffffff) * y_rows;
                     if (n >= ST) fine = barrier_wait(&sm.y_free[stage], (n / ST - 1) & 1);
                     if (!fine) break;
                     barrier_expect(&sm.y_full[stage], 2 * y_rows * DP * 2);
-                    load_rows<DP, kY>(sm.y[stage][0], y0m, &sm.y_full[stage], it.b, it.h, tile * y_rows);
-                    load_rows<DP, kY>(sm.y[stage][1], y1m, &sm.y_full[stage], it.b, it.h, tile * y_rows);
-                    tile = KEYS ? tile + 1 : next_tile(words, tile + 1, it.end);
+                    load_rows<DP, kY>(sm.y[stage][0], y0m, &sm.y_full[stage], it.b, it.h, row);
+                    load_rows<DP, kY>(sm.y[stage][1], y1m, &sm.y_full[stage], it.b, it.h, row);
                 }
             }
             if (!fine) {     // nothing may still be on its way when the CTA ends
@@ -319,13 +341,14 @@ __global__ void __launch_bounds__(384, 1)
                 for (int s = 0; s < ST; ++s)
                     if (n > s) barrier_wait(&sm.y_full[s], ((n - s + ST - 1) / ST - 1) & 1);
             }
-        } else if (warp == 10 && KEYS) {
+        } else if (warp == kLast + 2 && KEYS) {
             // what the walked rows need beside their tiles
             int n = 0;
             for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
-                const Item it = item_of<KEYS>(p, i, x_rows, y_rows);
-                for (int tile = it.begin; fine && tile < it.end; ++tile, ++n) {
-                    const int stage = n % ST;
+                const Item it = item_of(p, i, x_tiles, x_rows);
+                const Walk<KEYS> walk(p, it, y_rows);
+                for (int j = 0; fine && j < walk.count; ++j, ++n) {
+                    const int stage = n % ST, tile = (int)walk[j];
                     float lse[2], delta[2];
                     uint4 see[2];
 #pragma unroll
@@ -352,23 +375,88 @@ __global__ void __launch_bounds__(384, 1)
                     barrier_arrive(&sm.row_full[stage]);
                 }
             }
-        } else if (warp == 9) {
+        } else if (warp == kLast + 1 && elect_one()) {
             constexpr uint32_t kScores = instruction(kBf16, kX, kY, false, false);
             constexpr uint32_t kSums = instruction(kBf16, kX, DP, false, true);
             constexpr int kRow = kRowBytes<DP>;
-            // the tile whose products with P and dS are still to be issued
-            int pending = -1, pending_n = 0;
-            bool pending_first = false;
-            const uint32_t *pending_words = nullptr;
-            int n = 0, done = 0;
-            const auto issue_sums = [&](bool last) {
-                const int group = pending_n & 1, stage = pending_n % ST;
-                if (pending_first && done > 1) fine = fine && barrier_wait(&sm.acc_free, (done - 2) & 1);
-                fine = fine && barrier_wait(&sm.p_full[group], (pending_n >> 1) & 1);
-                if (!KEYS && pending_words != nullptr && fine) {
-                    // rows of k that nobody may see: their dS is 0 and its products have to be
-                    const uint2 see = __ldg(reinterpret_cast<const uint2 *>(pending_words) + pending);
-                    if ((see.x & see.y) != 0xffffffffu) {
+            constexpr uint32_t kXBytes = kX * DP * 2, kYBytes = kY * DP * 2;
+            const uint32_t x0 = descriptor(smem_address(sm.x), 16), y0 = descriptor(smem_address(sm.y), 16),
+                           z0 = descriptor(smem_address(sm.y), kY * 128);
+            // Tiles whose products with P and dS are still to be issued, one fewer than there are groups: the scores
+            // of a tile take the place of what the oldest one's products have read.
+            struct Pending {
+                int n, item;
+                bool first, last;
+            } queue[kGroups - 1];
+            int waiting = 0, n = 0, done = 0;
+            const auto issue_sums = [&] {
+                const Pending t = queue[0];
+#pragma unroll
+                for (int i = 0; i + 1 < kGroups - 1; ++i) queue[i] = queue[i + 1];
+                --waiting;
+                const int group = t.n % kGroups, stage = t.n % ST;
+                if (t.first && t.item > 0) fine = fine && barrier_wait(&sm.acc_free, (t.item - 1) & 1);
+                if (!KEYS && p.key_words != nullptr) fine = fine && barrier_wait(&sm.y_clean[stage], (t.n / ST) & 1);
+                fine = fine && barrier_wait(&sm.p_full[group], (t.n / kGroups) & 1);
+                fence_after();
+                if (fine) {
+                    const uint32_t from = tmem + group * kGroup, za = z0 + stage * (2 * kYBytes >> 4);
+                    if constexpr (KEYS) {
+#pragma unroll
+                        for (int j = 0; j < kY; j += 16)
+                            mma_ts<kRow>(tmem + kAcc0, from + kS + j / 2, za + (kYBytes + j * kRow >> 4), kSums, !t.first || j > 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kY; j += 16)
+                        mma_ts<kRow>(tmem + kAcc1, from + kT + j / 2, za + (j * kRow >> 4), kSums, !t.first || j > 0);
+                    commit(&sm.y_free[stage]);
+                    if (t.last) commit(&sm.acc_full);
+                }
+            };
+            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+                const Item it = item_of(p, i, x_tiles, x_rows);
+                const Walk<KEYS> walk(p, it, y_rows);
+                if (walk.count == 0) continue;
+                const int buffer = done & 1;
+                fine = barrier_wait(&sm.x_full[buffer], (done >> 1) & 1);
+                for (int j = 0; fine && j < walk.count; ++j, ++n) {
+                    const bool first = j == 0;
+                    const int stage = n % ST, group = n % kGroups;
+                    fine = barrier_wait(&sm.y_full[stage], (n / ST) & 1);
+                    if (fine) {
+                        const uint32_t to = tmem + group * kGroup;
+                        const uint32_t xa = x0 + buffer * (2 * kXBytes >> 4), ya = y0 + stage * (2 * kYBytes >> 4);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int d = 0; d < DP; d += 16)
+                                mma<kRow>(to + (half == 0 ? kS : kT), xa + (half * kXBytes + (d & ~63) * kX * 2 + (d & 63) * 2 >> 4),
+                                          ya + (half * kYBytes + (d & ~63) * kY * 2 + (d & 63) * 2 >> 4), kScores, d > 0);
+                        commit(&sm.s_full[group]);
+                        if (j == walk.count - 1) commit(&sm.x_free[buffer]);
+                    }
+                    if (waiting == kGroups - 1) issue_sums();
+                    const Pending t = {n, done, first, j == walk.count - 1};
+                    if (kGroups == 2 || waiting == 0) queue[0] = t; else queue[kGroups - 2] = t;
+                    ++waiting;
+                }
+                ++done;
+            }
+            while (fine && waiting > 0) issue_sums();
+        } else if (warp == kLast + 3 && !KEYS && p.key_words != nullptr) {
+            // rows of k that nobody may see: their dS is 0 and its products have to be
+            int n = 0;
+            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+                const Item it = item_of(p, i, x_tiles, x_rows);
+                const Walk<KEYS> walk(p, it, y_rows);
+                const uint32_t *words = key_words_of(p, it.b, it.h);
+                for (int j = 0; fine && j < walk.count; ++j, ++n) {
+                    const uint32_t entry = walk[j];
+                    const int stage = n % ST;
+                    // (whether their scores are formed before or after makes no difference: they are masked)
+                    fine = barrier_wait(&sm.y_full[stage], (n / ST) & 1);
+                    if (fine && !(entry >> 31)) {
+                        const uint2 see = __ldg(reinterpret_cast<const uint2 *>(words) + entry);
                         constexpr int kChunks = DP / 8;
                         for (int c = lane; c < 64 * kChunks; c += 32) {
                             const int r = c / kChunks;
@@ -376,63 +464,15 @@ __global__ void __launch_bounds__(384, 1)
                                 *reinterpret_cast<uint4 *>(sm.y[stage][0] + swizzled<DP, kY>(r, c % kChunks)) = make_uint4(0, 0, 0, 0);
                         }
                         fence_async_shared();
-                        __syncwarp();
                     }
-                }
-                fence_after();
-                if (fine && lane == 0) {
-                    const uint32_t from = tmem + group * kGroup;
-                    const uint32_t y0 = smem_address(sm.y[stage][0]), y1 = smem_address(sm.y[stage][1]);
-                    if constexpr (KEYS)
-#pragma unroll
-                        for (int j = 0; j < kY; j += 16)
-                            mma_ts(tmem + kAcc0, from + kS + j / 2, descriptor<kRow>(y1 + j * kRow, kY * 128), kSums, !pending_first || j > 0);
-#pragma unroll
-                    for (int j = 0; j < kY; j += 16)
-                        mma_ts(tmem + kAcc1, from + kT + j / 2, descriptor<kRow>(y0 + j * kRow, kY * 128), kSums, !pending_first || j > 0);
-                    commit(&sm.y_free[stage]);
-                    if (last) commit(&sm.acc_full);
-                }
-                pending = -1;
-            };
-            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
-                const Item it = item_of<KEYS>(p, i, x_rows, y_rows);
-                const uint32_t *words = key_words_of(p, it.b, it.h);
-                int tile = KEYS ? it.begin : next_tile(words, it.begin, it.end);
-                if (tile >= it.end) continue;
-                const int buffer = done & 1;
-                fine = barrier_wait(&sm.x_full[buffer], (done >> 1) & 1);
-                bool first = true;
-                for (; fine && tile < it.end; ++n) {
-                    const int next = KEYS ? tile + 1 : next_tile(words, tile + 1, it.end);
-                    const int stage = n % ST, group = n & 1;
-                    fine = barrier_wait(&sm.y_full[stage], (n / ST) & 1);
-                    fence_after();
-                    if (fine && lane == 0) {
-                        const uint32_t to = tmem + group * kGroup;
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t xa = smem_address(sm.x[buffer][half]), ya = smem_address(sm.y[stage][half]);
-#pragma unroll
-                            for (int d = 0; d < DP; d += 16)
-                                mma(to + (half == 0 ? kS : kT), descriptor<kRow>(xa + (d >> 6) * kX * 128 + (d & 63) * 2, 16),
-                                    descriptor<kRow>(ya + (d >> 6) * kY * 128 + (d & 63) * 2, 16), kScores, d > 0);
-                        }
-                        commit(&sm.s_full[group]);
-                        if (next >= it.end) commit(&sm.x_free[buffer]);
-                    }
-                    if (pending >= 0) issue_sums(first);
-                    if (first) ++done;
-                    pending = tile, pending_n = n, pending_first = first, pending_words = words;
-                    first = false;
-                    tile = next;
+                    barrier_arrive(&sm.y_clean[stage]);
                 }
             }
-            if (pending >= 0) issue_sums(true);
         }
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kLast) {
+        __syncwarp();
         fence_after();
         tmem_free(tmem, 512);
     }
@@ -456,7 +496,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     const int x_rows = KEYS ? kX : rows, y_rows = KEYS ? rows : kY;
     const int64_t items = (int64_t)p.B * p.K * p.splits * (((KEYS ? p.S : p.R) + x_rows - 1) / x_rows);
     const unsigned grid = (unsigned)std::min<int64_t>(items, 148);
-    kernel<<<grid, 384, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v, items, x_rows, y_rows);
+    kernel<<<grid, kGroupsOf<DP> * 128 + 128, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v, items, x_rows, y_rows);
     return cudaGetLastError();
 }
 

@@ -1,11 +1,16 @@
 // Cross attention forward on the fifth-generation tensor cores, 16-bit types.
 //
-// A CTA holds NQ tiles of 128 rows and walks the states 128 at a time.  One thread has TMA bring the
-// tiles of k and v, one thread issues the products, and four warps per row tile do the softmax, a
-// thread to a row: scores come from tensor memory, weights go back there as the left operand of the
-// second product, whose sums stay in tensor memory until the end.
+// A CTA holds RT tiles of 128 rows and walks tiles of BN states.  One thread has TMA bring the tiles of
+// k and v, one thread issues the products, and RT * KW groups of four warps do the softmax, a thread to
+// a row: scores come from tensor memory, weights go back there (in the scores' place) as the left
+// operand of the second product, whose sums stay in tensor memory until the end.
 //
-//   S = q k^T (tensor memory, 128 columns)   P = exp2(c S - m) (64 columns, 16-bit)   O += P v
+//   S = q k^T (BN columns)   P = exp2(c S - m) (BN / 2 columns, 16-bit)   O += P v (DP columns)
+//
+// KW groups share a row tile and take the state tiles in turn, each with a maximum, sum and O of its
+// own; at the end the parts are weighted and added.  The work is bound by latencies of a group's cycle
+// (scores, loads, exponentials, stores, product), so as many groups as tensor memory holds run at once:
+// four with BN = 64 up to 64 channels, two with BN = 128 above.
 //
 // The running maximum is only raised when a row would leave exp2's range of 2^8 above it: then the
 // row's sums in tensor memory are scaled, which is rare after the first tiles, and exact in between (a
@@ -20,74 +25,91 @@ namespace msda_b200 {
 
 namespace {
 
-constexpr int kTileRows = 128, kTileStates = 128;
+constexpr int kTileRows = 128;
 
-template <int DP>
-constexpr int kStages = DP == 32 ? 4 : 2;
+template <int DP, int RT, int KW>
+struct Shape {
+    static constexpr int BN = DP == 128 ? 128 : 64;            // states of a tile
+    static constexpr int ST = DP == 128 ? KW + 1 : 8;          // tiles of k and v in flight
+    static constexpr int kGroups = RT * KW;
+    static constexpr int kThreads = kGroups * 128 + 128;
+    static constexpr uint32_t kColumns = BN + DP;              // of tensor memory, for a group: S (and P), O
+    // what a thread may hold: all of the block's at launch, less what the last four warps need
+    static constexpr int kRegisters = kGroups == 4 ? 104 : 224, kFew = kGroups == 4 ? 64 : 56;
+    static_assert(kGroups * kColumns <= 512);
+    static_assert(ST > KW);                                    // a tile is freed KW tiles after its scores
+};
 
-template <int DP, int NQ>
+template <int DP, int RT, int KW>
 struct Shared {
-    alignas(1024) unsigned char q[NQ][kTileRows * DP * 2];
-    alignas(1024) unsigned char k[kStages<DP>][kTileStates * DP * 2];
-    alignas(1024) unsigned char v[kStages<DP>][kTileStates * DP * 2];
-    uint64_t k_full[kStages<DP>], k_free[kStages<DP>], v_full[kStages<DP>], v_free[kStages<DP>];
-    uint64_t s_full[NQ], s_free[NQ], p_full[NQ], o_full[NQ];
+    using Sh = Shape<DP, RT, KW>;
+    alignas(1024) unsigned char q[RT][kTileRows * DP * 2];
+    alignas(1024) unsigned char k[Sh::ST][Sh::BN * DP * 2];
+    alignas(1024) unsigned char v[Sh::ST][Sh::BN * DP * 2];
+    float m[Sh::kGroups][kTileRows], l[Sh::kGroups][kTileRows];
+    uint64_t full[Sh::ST], clean[Sh::ST], free[Sh::ST];        // of a stage: its k and v
+    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], o_full[Sh::kGroups];
     uint32_t tmem;
 };
 
-__device__ __forceinline__ uint4 tile_words(const uint32_t *words, int S, int tile) {
-    if (words != nullptr) return __ldg(reinterpret_cast<const uint4 *>(words) + tile);
-    return make_uint4(key_word(nullptr, S, 4 * tile), key_word(nullptr, S, 4 * tile + 1), key_word(nullptr, S, 4 * tile + 2),
-                      key_word(nullptr, S, 4 * tile + 3));
-}
-
-// the first tile from t on in which some state may be seen
-__device__ __forceinline__ int next_tile(const uint32_t *words, int t, int end) {
-    if (words == nullptr) return t;
-    for (; t < end; ++t) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(words) + t);
-        if (w.x | w.y | w.z | w.w) return t;
+// the BN / 32 mask words of a tile
+template <int N>
+struct Words {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const uint32_t *from, int tile) {
+        if constexpr (N == 4) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(from) + tile);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else {
+            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(from) + tile);
+            w[0] = x.x, w[1] = x.y;
+        }
     }
-    return end;
-}
+    __device__ __forceinline__ void existing(int S, int tile) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = key_word(nullptr, S, tile * N + i);
+    }
+    __device__ __forceinline__ bool all() const {
+        uint32_t x = w[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) x &= w[i];
+        return x == 0xffffffffu;
+    }
+};
 
-template <typename T, int DP, int NQ>
-__global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1)
+template <typename T, int DP, int RT, int KW>
+__global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
     attention_forward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap km,
                                 const __grid_constant__ tc::TensorMap vm) {
     using namespace tc;
-    // columns of tensor memory of one row tile: S, P, O.  At 128 channels P takes the place of S, and the next
-    // scores wait for the product that reads it.
-    constexpr bool kAlias = DP == 128;
-    constexpr uint32_t kS = 0, kP = kAlias ? 0 : 128, kO = kAlias ? 128 : 192, kColumns = 256;
-    constexpr int ST = kStages<DP>;
+    using Sh = Shape<DP, RT, KW>;
+    constexpr int BN = Sh::BN, NW = BN / 32, ST = Sh::ST;
+    constexpr uint32_t kO = BN;
+    constexpr int kLast = Sh::kGroups * 4;                     // first of the last four warps
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     extern __shared__ __align__(1024) unsigned char raw[];
-    auto &sm = *reinterpret_cast<Shared<DP, NQ> *>(raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto &sm = *reinterpret_cast<Shared<DP, RT, KW> *>(raw);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-    const int row_tiles = (p.R + NQ * kTileRows - 1) / (NQ * kTileRows);
+    const int row_tiles = (p.R + RT * kTileRows - 1) / (RT * kTileRows);
     int64_t i = blockIdx.x;
-    const int first = (int)(i % row_tiles) * NQ * kTileRows;
+    const int first = (int)(i % row_tiles) * RT * kTileRows;
     i /= row_tiles;
     const int part = (int)(i % p.splits);
     const int64_t bh = i / p.splits;
     const int b = (int)(bh / p.K), h = (int)(bh % p.K);
     const uint32_t *words = key_words_of(p, b, h);
-    const int end = min((p.S + kTileStates - 1) / kTileStates, (part + 1) * p.tiles);
+    const Tiles<BN> tiles(p, b, h, part);
 
-    if (warp == 4 * NQ) tmem_alloc(&sm.tmem, NQ * kColumns);
+    if (warp == kLast) tmem_alloc(&sm.tmem, 512);
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
-            barrier_init(&sm.k_full[s], 1), barrier_init(&sm.k_free[s], 1);
-            barrier_init(&sm.v_full[s], 1), barrier_init(&sm.v_free[s], 1);
+            barrier_init(&sm.full[s], 1), barrier_init(&sm.free[s], 1), barrier_init(&sm.clean[s], 32);
         }
-        for (int q = 0; q < NQ; ++q) {
-            barrier_init(&sm.s_full[q], 1), barrier_init(&sm.s_free[q], 128);
-            barrier_init(&sm.p_full[q], 128), barrier_init(&sm.o_full[q], 1);
-        }
+        for (int g = 0; g < Sh::kGroups; ++g)
+            barrier_init(&sm.s_full[g], 1), barrier_init(&sm.p_full[g], 128), barrier_init(&sm.o_full[g], 1);
     }
-    if (warp < 4 * NQ) {
+    if (warp < 4 * RT) {
         // a thread to a row of q
         const int r = first + threadIdx.x;
         const T *q = static_cast<const T *>(p.q) + (r < p.R ? row_offset(p.qs, p.share, b, h, r) : 0);
@@ -102,279 +124,282 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1)
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sm.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
     bool fine = true;
 
-    if (warp < 4 * NQ) {
-        registers_up<NQ == 1 ? 200 : 224>();
-        const int q = warp >> 2;
-        const uint32_t mine = tmem + q * kColumns + ((uint32_t)(warp & 3) << 21);
-        const int r = first + threadIdx.x;
-        const bool idle = first + (warp << 5) >= p.R;              // a whole warp behind the last row
+    if (warp < kLast) {
+        registers_up<Sh::kRegisters>();
+        const int group = warp >> 2, tile_of_rows = group % RT, way = group / RT, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const uint32_t mine = tmem + group * Sh::kColumns + lanes;
+        const int r = first + tile_of_rows * kTileRows + row;
+        const bool idle = first + tile_of_rows * kTileRows + (row & ~31) >= p.R;       // a whole warp behind the last row
         const uint32_t *rw = r < p.R ? row_words_of(p, b, h, r) : nullptr;
+        if (rw == nullptr) rw = words;
         float m = -INFINITY, l = 0.f;
         int done = 0;
-        for (int tile = next_tile(words, part * p.tiles, end); fine && tile < end; ++done) {
-            const int next = next_tile(words, tile + 1, end);
-            const uint4 see = rw != nullptr ? __ldg(reinterpret_cast<const uint4 *>(rw) + tile) : tile_words(words, p.S, tile);
-            fine = barrier_wait(&sm.s_full[q], done & 1);
+        const bool own_words = p.row_words != nullptr;
+        uint32_t entry = way < tiles.count ? tiles[way] : 0;
+        Words<NW> see{};
+        if (rw != nullptr && way < tiles.count && (own_words || !(entry >> 31))) see.load(rw, entry & 0x7fffffff);
+        for (int n = way; fine && n < tiles.count; n += KW, ++done) {
+            // the next tile's mask comes while this one is worked on
+            uint32_t entry_next = 0;
+            Words<NW> see_next{};
+            if (n + KW < tiles.count) {
+                entry_next = tiles[n + KW];
+                if (rw != nullptr && (own_words || !(entry_next >> 31))) see_next.load(rw, entry_next & 0x7fffffff);
+            }
+            fine = barrier_wait(&sm.s_full[group], done & 1);
             if (!fine) break;
             fence_after();
-            if (idle) {
-                if constexpr (!kAlias) {
-                    barrier_arrive(&sm.s_free[q]);
-                    // (not before the other warps' weights of the tile before have been counted)
-                    if (done > 0) fine = barrier_wait(&sm.o_full[q], (done - 1) & 1);
+            if (!idle) {
+                uint32_t s[NW][32];
+#pragma unroll
+                for (int j = 0; j < NW; ++j) tmem_load32(s[j], mine + 32 * j);
+                tmem_wait_load();
+#pragma unroll
+                for (int j = 0; j < NW; ++j) loaded(s[j]);
+                if (own_words ? !__all_sync(0xffffffffu, see.all()) : !(entry >> 31)) {
+                    if (rw == nullptr) see.existing(p.S, entry & 0x7fffffff);
+#pragma unroll
+                    for (int j = 0; j < NW; ++j)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see.w[j] & (1u << c))) s[j][c] = 0xff800000u;        // -inf
                 }
-                barrier_arrive(&sm.p_full[q]);
-                tile = next;
-                continue;
-            }
-            uint32_t s[4][32];
+                float top[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_load32(s[j], mine + kS + 32 * j);
-            tmem_wait_load();
+                for (int j = 0; j < 4; ++j) {
+                    constexpr int kRun = BN / 4;
+                    top[j] = __uint_as_float(s[j * kRun / 32][j * kRun % 32]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) loaded(s[j]);
-            if constexpr (!kAlias) {
-                fence_before();
-                barrier_arrive(&sm.s_free[q]);
-            }
-            if (!__all_sync(0xffffffffu, (see.x & see.y & see.z & see.w) == 0xffffffffu)) {
-                const uint32_t w[4] = {see.x, see.y, see.z, see.w};
+                    for (int c = 1; c < kRun; ++c) top[j] = fmaxf(top[j], __uint_as_float(s[(j * kRun + c) / 32][(j * kRun + c) % 32]));
+                }
+                const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+                const bool raise = best > m + 8.f || (m == -INFINITY && best > m);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float to = raise ? best : m;
+                    const float keep = to == -INFINITY ? 1.f : fast_exp2(m - to);
+                    m = to;
+                    l *= keep;
+                    if (done > 0) {        // (that the scores are there says that the product before is done)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                        for (int d = 0; d < DP; d += 16) {
+                            uint32_t o[16];
+                            tmem_load16(o, mine + kO + d);
+                            tmem_wait_load();
+                            loaded(o);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (!(w[j] & (1u << c))) s[j][c] = 0xff800000u;        // -inf
-            }
-            float top[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                top[j] = __uint_as_float(s[j][0]);
-#pragma unroll
-                for (int c = 1; c < 32; ++c) top[j] = fmaxf(top[j], __uint_as_float(s[j][c]));
-            }
-            const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-            const bool raise = best > m + 8.f || (m == -INFINITY && best > m);
-            bool waited = kAlias || done == 0;       // the product before has read P and added to O
-            if (__any_sync(0xffffffffu, raise)) {
-                const float to = raise ? best : m;
-                const float keep = to == -INFINITY ? 1.f : fast_exp2(m - to);
-                m = to;
-                l *= keep;
-                if (done > 0) {
-                    if (!waited) {
-                        fine = barrier_wait(&sm.o_full[q], (done - 1) & 1);
-                        fence_after();
-                        waited = true;
-                    }
-#pragma unroll
-                    for (int d = 0; d < DP; d += 32) {
-                        uint32_t o[32];
-                        tmem_load32(o, mine + kO + d);
-                        tmem_wait_load();
-                        loaded(o);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
-                        tmem_store32(mine + kO + d, o);
+                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * keep);
+                            tmem_store16(mine + kO + d, o);
+                        }
                     }
                 }
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-            float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
-            const float2 one = make_float2(1.f, 1.f);
+                const float base = m == -INFINITY ? 0.f : m;
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), less2 = make_float2(-base, -base);
+                float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                uint32_t w[32];
+                for (int j = 0; j < NW; ++j) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int c = 0; c < 64; c += 2) {
-                    float2 x = make_float2(-base, -base);
-                    ffma2(x, make_float2(__uint_as_float(s[j + (c >> 5)][c & 31]), __uint_as_float(s[j + (c >> 5)][(c & 31) + 1])),
-                          scale2);
-                    x.x = fast_exp2(x.x), x.y = fast_exp2(x.y);
-                    ffma2(sum[(c >> 1) & 1], x, one);
-                    w[c >> 1] = VecTraits<T>::pack2(x);
+                    for (int c = 0; c < 32; c += 2) {
+                        float2 x = fma2(make_float2(__uint_as_float(s[j][c]), __uint_as_float(s[j][c + 1])), scale2, less2);
+                        x.x = fast_exp2(x.x), x.y = fast_exp2(x.y);
+                        sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], x);
+                        w[c >> 1] = VecTraits<T>::pack2(x);
+                    }
+                    tmem_store16(mine + 16 * j, w);
                 }
-                if (!waited) {
-                    fine = barrier_wait(&sm.o_full[q], (done - 1) & 1) && fine;
-                    fence_after();
-                    waited = true;
-                }
-                tmem_store32(mine + kP + 16 * j, w);
+                l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tmem_wait_store();
             }
-            l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            tmem_wait_store();
             fence_before();
-            barrier_arrive(&sm.p_full[q]);
-            tile = next;
+            barrier_arrive(&sm.p_full[group]);
+            entry = entry_next;
+            see = see_next;
         }
-        // results: the rows of O over their sums
-        if (done > 0 && !idle) {
-            fine = barrier_wait(&sm.o_full[q], (done - 1) & 1) && fine;
+        // the groups of a row tile: every one adds a share of the columns of all
+        if (done > 0) {
+            fine = fine && barrier_wait(&sm.o_full[group], 0);
             fence_after();
         }
-        const float inverse = !fine ? NAN : l > 0.f || l != l ? 1.f / l : 0.f;
-        const float lse = l == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m + log2f(l);
+        if (!fine) l = NAN;
+        float factor[KW], lse;
+        if constexpr (KW > 1) {
+            sm.m[group][row] = m, sm.l[group][row] = l;
+            fence_before();
+            asm volatile("bar.sync 1, %0;" ::"n"(Sh::kGroups * 128) : "memory");
+            fence_after();
+            float best = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) best = fmaxf(best, sm.m[w * RT + tile_of_rows][row]);
+            const float base = best == -INFINITY ? 0.f : best;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const float lw = sm.l[w * RT + tile_of_rows][row];
+                factor[w] = lw == 0.f ? 0.f : fast_exp2(sm.m[w * RT + tile_of_rows][row] - base);
+                total += factor[w] * lw;
+            }
+#pragma unroll
+            for (int w = 0; w < KW; ++w) factor[w] = total == 0.f ? 0.f : factor[w] / total;
+            lse = total == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : best + log2f(total);
+        } else {
+            factor[0] = l == 0.f ? 0.f : 1.f / l;
+            lse = l == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m + log2f(l);
+        }
         const int64_t at = bh * p.R + r, rows = (int64_t)p.B * p.K * p.R;
         const int query = r / p.share;
         T *out = static_cast<T *>(p.out) + (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
         float *parts = p.part + (part * rows + at) * p.D;
-        if (r < p.R) (p.splits > 1 ? p.part_lse + part * rows : p.lse)[at] = lse;
+        if (r < p.R && way == 0) (p.splits > 1 ? p.part_lse + part * rows : p.lse)[at] = lse;
+        constexpr int kShare = DP / KW, kStep = kShare < 16 ? 8 : 16;
         if (!idle) {
 #pragma unroll
-            for (int d = 0; d < DP; d += 32) {
-                uint32_t o[32];
-                if (done > 0) {
-                    tmem_load32(o, mine + kO + d);
+            for (int d = 0; d < kShare; d += kStep) {
+                const int col = way * kShare + d;
+                float2 x[kStep / 2];
+#pragma unroll
+                for (int c = 0; c < kStep / 2; ++c) x[c] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    uint32_t o[kStep];
+                    const uint32_t from = tmem + (w * RT + tile_of_rows) * Sh::kColumns + lanes + kO + col;
+                    if constexpr (kStep == 16) tmem_load16(o, from); else tmem_load8(o, from);
                     tmem_wait_load();
                     loaded(o);
+                    // (a group that had no tile has never written its columns)
+                    if (factor[w] != 0.f) {
+#pragma unroll
+                        for (int c = 0; c < kStep / 2; ++c)
+                            ffma2(x[c], make_float2(__uint_as_float(o[2 * c]), __uint_as_float(o[2 * c + 1])), make_float2(factor[w], factor[w]));
+                    }
                 }
-                float2 x[16];
+                if (r >= p.R) continue;
 #pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    x[c] = done > 0 ? make_float2(__uint_as_float(o[2 * c]) * inverse, __uint_as_float(o[2 * c + 1]) * inverse)
-                                    : make_float2(0.f, 0.f);
-                if (r < p.R && p.splits > 1) {
-#pragma unroll
-                    for (int c = 0; c < 16; c += 2)
-                        if (d + 2 * c < p.D)
-                            *reinterpret_cast<float4 *>(parts + d + 2 * c) = make_float4(x[c].x, x[c].y, x[c + 1].x, x[c + 1].y);
-                } else if (r < p.R) {
-#pragma unroll
-                    for (int c = 0; c < 16; c += 4)
-                        if (d + 2 * c < p.D) {
-                            const float2 y[4] = {x[c], x[c + 1], x[c + 2], x[c + 3]};
-                            *reinterpret_cast<uint4 *>(out + d + 2 * c) = VecTraits<T>::pack(y);
-                        }
+                for (int c = 0; c < kStep / 2; c += 4) {
+                    if (col + 2 * c >= p.D) continue;
+                    if (p.splits > 1) {
+                        *reinterpret_cast<float4 *>(parts + col + 2 * c) = make_float4(x[c].x, x[c].y, x[c + 1].x, x[c + 1].y);
+                        *reinterpret_cast<float4 *>(parts + col + 2 * c + 4) = make_float4(x[c + 2].x, x[c + 2].y, x[c + 3].x, x[c + 3].y);
+                    } else {
+                        const float2 y[4] = {x[c], x[c + 1], x[c + 2], x[c + 3]};
+                        *reinterpret_cast<uint4 *>(out + col + 2 * c) = VecTraits<T>::pack(y);
+                    }
                 }
             }
         }
         fence_before();
     } else {
-        registers_down<56>();
-        if (warp == 4 * NQ && lane == 0) {
+        registers_down<Sh::kFew>();
+        if (warp == kLast && elect_one()) {
             int n = 0;
-            for (int tile = next_tile(words, part * p.tiles, end); fine && tile < end; ++n) {
-                const int stage = n % ST, turn = n / ST;
-                if (turn > 0) fine = barrier_wait(&sm.k_free[stage], (turn - 1) & 1);
-                if (fine) {
-                    barrier_expect(&sm.k_full[stage], kTileStates * DP * 2);
-                    load_rows<DP, kTileStates>(sm.k[stage], km, &sm.k_full[stage], b, h, tile * kTileStates);
-                }
-                if (fine && turn > 0) fine = barrier_wait(&sm.v_free[stage], (turn - 1) & 1);
-                if (fine) {
-                    barrier_expect(&sm.v_full[stage], kTileStates * DP * 2);
-                    load_rows<DP, kTileStates>(sm.v[stage], vm, &sm.v_full[stage], b, h, tile * kTileStates);
-                }
-                tile = next_tile(words, tile + 1, end);
+            for (; fine && n < tiles.count; ++n) {
+                const int stage = n % ST, turn = n / ST, state = (int)(tiles[n] & 0x7fffffff) * BN;
+                if (turn > 0) fine = barrier_wait(&sm.free[stage], (turn - 1) & 1);
+                if (!fine) break;
+                barrier_expect(&sm.full[stage], 2 * BN * DP * 2);
+                load_rows<DP, BN>(sm.k[stage], km, &sm.full[stage], b, h, state);
+                load_rows<DP, BN>(sm.v[stage], vm, &sm.full[stage], b, h, state);
             }
             // nothing may still be on its way when the CTA ends
-            for (int s = 0; s < ST; ++s) {
+            for (int s = 0; s < ST && !fine; ++s) {
                 const int turns = (n - s + ST - 1) / ST;
-                if (turns > 0 && !fine) barrier_wait(&sm.k_full[s], (turns - 1) & 1), barrier_wait(&sm.v_full[s], (turns - 1) & 1);
+                if (turns > 0) barrier_wait(&sm.full[s], (turns - 1) & 1);
             }
-        } else if (warp == 4 * NQ + 1) {
-            constexpr uint32_t kScores = instruction(kBf16, 128, 128, false, false);
-            constexpr uint32_t kOut = instruction(kBf16, 128, DP, false, true);
+        } else if (warp == kLast + 1 && elect_one()) {
+            constexpr uint32_t kScores = instruction(kBf16, kTileRows, BN, false, false);
+            constexpr uint32_t kOut = instruction(kBf16, kTileRows, DP, false, true);
             constexpr int kRow = kRowBytes<DP>;
-            int before = -1, n = 0;
-            // n-th tile: its scores, then the product with the weights of the tile before
-            for (int tile = next_tile(words, part * p.tiles, end); fine && (tile < end || before >= 0); ++n) {
-                const bool scores = tile < end, weights = before >= 0;
-                const int stage = n % ST, last = (n + ST - 1) % ST;
-                if (scores) fine = barrier_wait(&sm.k_full[stage], (n / ST) & 1);
-                if (weights) {
-                    fine = fine && barrier_wait(&sm.v_full[last], ((n - 1) / ST) & 1);
-                    if (words != nullptr && fine) {
-                        // rows of v that nobody may see: whatever they hold, their weight is 0 and has to stay it
-                        const uint4 see = __ldg(reinterpret_cast<const uint4 *>(words) + before);
-                        if ((see.x & see.y & see.z & see.w) != 0xffffffffu) {
-                            const uint32_t w[4] = {see.x, see.y, see.z, see.w};
-                            constexpr int kChunks = DP / 8;
+            // The n-th tile is the groups' n % KW and their n / KW-th.  Its scores take the place of the weights of
+            // their tile before, so the product with those is issued first: products are done in order.
+            const uint32_t q0 = descriptor(smem_address(sm.q), 16), k0 = descriptor(smem_address(sm.k), 16),
+                           v0 = descriptor(smem_address(sm.v), BN * 128);
+            int n = 0;
+            for (int round = 0; fine && n < tiles.count + KW; ++round) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                for (int c = lane; c < 32 * kChunks; c += 32)
-                                    if (!((w[j] >> (c / kChunks)) & 1))
-                                        *reinterpret_cast<uint4 *>(sm.v[last] + swizzled<DP, kTileStates>(32 * j + c / kChunks, c % kChunks)) =
-                                            make_uint4(0, 0, 0, 0);
-                            fence_async_shared();
-                            __syncwarp();
+                for (int w = 0; w < KW; ++w, ++n) {
+                    const bool scores = n < tiles.count, weights = n >= KW && n - KW < tiles.count;
+                    const int stage = n % ST, last = (n + ST - KW) % ST;
+                    if (scores) fine = fine && barrier_wait(&sm.full[stage], (n / ST) & 1);
+                    if (weights && words != nullptr) fine = fine && barrier_wait(&sm.clean[last], ((n - KW) / ST) & 1);
+                    const uint32_t ka = k0 + stage * (BN * DP * 2 >> 4), va = v0 + last * (BN * DP * 2 >> 4);
+#pragma unroll
+                    for (int q = 0; q < RT; ++q) {
+                        const int group = w * RT + q;
+                        const uint32_t at = tmem + group * Sh::kColumns;
+                        if (weights) {
+                            fine = fine && barrier_wait(&sm.p_full[group], (round - 1) & 1);
+                            if (!fine) break;
+                            fence_after();
+#pragma unroll
+                            for (int j = 0; j < BN; j += 16)
+                                mma_ts<kRow>(at + kO, at + j / 2, va + (j * kRow >> 4), kOut, round > 1 || j > 0);
+                            if (q == RT - 1) commit(&sm.free[last]);
+                            if (!scores) commit(&sm.o_full[group]);
+                        }
+                        if (scores && fine) {
+#pragma unroll
+                            for (int d = 0; d < DP; d += 16)
+                                mma<kRow>(at, q0 + ((q * DP + (d & ~63)) * kTileRows * 2 + (d & 63) * 2 >> 4),
+                                          ka + ((d & ~63) * BN * 2 + (d & 63) * 2 >> 4), kScores, d > 0);
+                            commit(&sm.s_full[group]);
                         }
                     }
                 }
+            }
+        } else if (warp == kLast + 2 && words != nullptr) {
+            // rows of v that nobody may see: whatever they hold, their weight is 0 and has to stay it
+            for (int n = 0; fine && n < tiles.count; ++n) {
+                const uint32_t entry = tiles[n];
+                const int stage = n % ST;
+                fine = barrier_wait(&sm.full[stage], (n / ST) & 1);
+                if (fine && !(entry >> 31)) {
+                    Words<NW> see;
+                    see.load(words, entry);
+                    constexpr int kChunks = DP / 8;
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    const uint32_t at = tmem + q * kColumns;
-                    const auto issue_scores = [&] {
-                        if (!kAlias && n > 0) fine = fine && barrier_wait(&sm.s_free[q], (n - 1) & 1);
-                        fence_after();
-                        if (fine && lane == 0) {
-                            const uint32_t qa = smem_address(sm.q[q]), ka = smem_address(sm.k[stage]);
-#pragma unroll
-                            for (int d = 0; d < DP; d += 16) {
-                                const uint32_t off = (d >> 6) * kTileRows * 128 + (d & 63) * 2;
-                                mma(at + kS, descriptor<kRow>(qa + off, 16), descriptor<kRow>(ka + off, 16), kScores, d > 0);
-                            }
-                            commit(&sm.s_full[q]);
-                            if (q == NQ - 1) commit(&sm.k_free[stage]);
-                        }
-                    };
-                    const auto issue_weights = [&] {
-                        fine = fine && barrier_wait(&sm.p_full[q], (n - 1) & 1);
-                        fence_after();
-                        if (fine && lane == 0) {
-                            const uint32_t va = smem_address(sm.v[last]);
-#pragma unroll
-                            for (int j = 0; j < kTileStates; j += 16)
-                                mma_ts(at + kO, at + kP + j / 2, descriptor<kRow>(va + j * kRow, kTileStates * 128), kOut,
-                                       n > 1 || j > 0);
-                            commit(&sm.o_full[q]);
-                            if (q == NQ - 1) commit(&sm.v_free[last]);
-                        }
-                    };
-                    if constexpr (kAlias) {
-                        if (weights) issue_weights();
-                        if (scores) issue_scores();
-                    } else {
-                        if (scores) issue_scores();
-                        if (weights) issue_weights();
-                    }
+                    for (int j = 0; j < NW; ++j)
+                        for (int c = lane; c < 32 * kChunks; c += 32)
+                            if (!((see.w[j] >> (c / kChunks)) & 1))
+                                *reinterpret_cast<uint4 *>(sm.v[stage] + swizzled<DP, BN>(32 * j + c / kChunks, c % kChunks)) =
+                                    make_uint4(0, 0, 0, 0);
+                    fence_async_shared();
                 }
-                before = scores ? tile : -1;
-                if (scores) tile = next_tile(words, tile + 1, end);
+                barrier_arrive(&sm.clean[stage]);
             }
         }
     }
     __syncthreads();
-    if (warp == 4 * NQ) {
+    if (warp == kLast) {
+        __syncwarp();
         fence_after();
-        tmem_free(tmem, NQ * kColumns);
+        tmem_free(tmem, 512);
     }
 }
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int RT, int KW>
 cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
+    using Sh = Shape<DP, RT, KW>;
     tc::TensorMap km, vm;
-    if (!tc::make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, 1, p.D, kTileStates) ||
-        !tc::make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, 1, p.D, kTileStates))
+    if (!tc::make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, 1, p.D, Sh::BN) ||
+        !tc::make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, 1, p.D, Sh::BN))
         return cudaErrorNotSupported;
-    const auto kernel = attention_forward_tc_kernel<T, DP, NQ>;
-    constexpr size_t smem = sizeof(Shared<DP, NQ>);
+    const auto kernel = attention_forward_tc_kernel<T, DP, RT, KW>;
+    constexpr size_t smem = sizeof(Shared<DP, RT, KW>);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + NQ * kTileRows - 1) / (NQ * kTileRows));
+    const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + RT * kTileRows - 1) / (RT * kTileRows));
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    kernel<<<(unsigned)grid, NQ * 128 + 128, smem, stream>>>(p, km, vm);
+    kernel<<<(unsigned)grid, Sh::kThreads, smem, stream>>>(p, km, vm);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_typed(const AttentionParams &p, int row_tiles, cudaStream_t stream) {
-    if (p.D <= 32) return row_tiles == 1 ? launch<T, 32, 1>(p, stream) : launch<T, 32, 2>(p, stream);
-    if (p.D <= 64) return row_tiles == 1 ? launch<T, 64, 1>(p, stream) : launch<T, 64, 2>(p, stream);
-    return launch<T, 128, 2>(p, stream);
+    if (p.D <= 32) return row_tiles == 1 ? launch<T, 32, 1, 4>(p, stream) : launch<T, 32, 2, 2>(p, stream);
+    if (p.D <= 64) return row_tiles == 1 ? launch<T, 64, 1, 4>(p, stream) : launch<T, 64, 2, 2>(p, stream);
+    return row_tiles == 1 ? launch<T, 128, 1, 2>(p, stream) : launch<T, 128, 2, 1>(p, stream);
 }
 
 }  // namespace

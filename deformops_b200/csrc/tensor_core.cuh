@@ -21,6 +21,13 @@ __device__ __forceinline__ uint32_t smem_address(const void *p) {
     return (uint32_t)__cvta_generic_to_shared(p);
 }
 
+// one thread of the (whole) warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t chosen;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+    return chosen != 0;
+}
+
 // ---- mbarriers ------------------------------------------------------------------------------------
 __device__ __forceinline__ void barrier_init(uint64_t *bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bar)), "r"(count) : "memory");
@@ -32,21 +39,37 @@ __device__ __forceinline__ void barrier_expect(uint64_t *bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(bar)), "r"(bytes)
                  : "memory");
 }
-// Whether the phase of this parity ended.  Bounded: a wait that runs out (it takes some seconds, no call
-// gets there) lets its role leave, so that a mistake cannot hold the GPU.
+__device__ __forceinline__ bool barrier_try(uint32_t at, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(at), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+// Whether the phase of this parity ended.  Bounded: a wait of 2^33 cycles (four seconds and more; no call gets
+// there) lets its role leave, so that a mistake cannot hold the GPU.  A phase that is over costs 48 cycles so;
+// a bounded loop from the first try on costs 170.
 __device__ __forceinline__ bool barrier_wait(uint64_t *bar, uint32_t parity) {
     const uint32_t at = smem_address(bar);
-    for (int i = 0; i < 1 << 22; ++i) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done)
-                     : "r"(at), "r"(parity)
-                     : "memory");
-        if (done) return true;
-    }
-    return false;
+    if (barrier_try(at, parity) || barrier_try(at, parity) || barrier_try(at, parity)) return true;
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .u64 begun, now;\n\tmov.u64 begun, %%clock64;\n\t"
+                 "again_%=:\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "@p bra over_%=;\n\t"
+                 "mov.u64 now, %%clock64;\n\t"
+                 "sub.u64 now, now, begun;\n\t"
+                 "setp.lt.u64 q, now, %3;\n\t"
+                 "@q bra again_%=;\n\t"
+                 "over_%=:\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(at), "r"(parity), "n"(1ll << 33)
+                 : "memory");
+    return done != 0;
 }
 
 // plain stores to shared memory, before the asynchronous units read them
@@ -92,6 +115,18 @@ __device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at));
 }
+__device__ __forceinline__ void tmem_load8(uint32_t (&r)[8], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -120,34 +155,43 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void loaded(uint32_t (&r)[8]) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- matrix instructions ---------------------------------------------------------------------------
-// Shared memory descriptor: address, the two strides (all in 16 bytes), version 1, swizzle of 128 or 64
-// bytes.  Rows along the product's k ("k-major"): STRIDE is that of eight rows, LEADING is not used.  Rows
-// along the other axis: STRIDE is that of eight rows (of k), LEADING that of the next 64 (32) elements.
+// A shared memory descriptor has the address and the two strides (all in 16 bytes), version 1 and the swizzle of
+// 128 or 64 bytes.  Rows along the product's k ("k-major"): STRIDE is that of eight rows, LEADING is not used.  Rows
+// along the other axis: STRIDE is that of eight rows (of k), LEADING that of the next 64 (32) elements.  The upper
+// half is a constant; offsets within a tile are added to the lower one.
 template <int ROW_BYTES>
-__device__ __forceinline__ uint64_t descriptor(uint32_t at, uint32_t leading) {
-    constexpr uint64_t kSwizzle = ROW_BYTES == 128 ? 2 : 4;
-    return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)((leading & 0x3ffff) >> 4) << 16 |
-           (uint64_t)((8 * ROW_BYTES) >> 4) << 32 | (uint64_t)1 << 46 | kSwizzle << 61;
-}
+constexpr uint32_t kDescriptorHigh = (8 * ROW_BYTES >> 4) | 1u << 14 | (ROW_BYTES == 128 ? 2u : 4u) << 29;
+__device__ __forceinline__ uint32_t descriptor(uint32_t at, uint32_t leading) { return at >> 4 | leading >> 4 << 16; }
 // float32 sums of two 16-bit types alike; b_rows: B's rows run along k
 __host__ __device__ constexpr uint32_t instruction(bool bf16, int m, int n, bool a_rows, bool b_rows) {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_rows ? 1u << 15 : 0u) | (b_rows ? 1u << 16 : 0u) |
            (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"((uint32_t)add)
+// Issued by one thread, which has to be one that elect_one() chose: then the compiler knows that there is one,
+// and every operand is in uniform registers (an `if (lane == 0)` costs about 100 cycles a product).
+template <int ROW_BYTES>
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+                 "r"((uint32_t)add), "n"(kDescriptorHigh<ROW_BYTES>)
                  : "memory");
 }
 // A from tensor memory: two 16-bit elements of k to a column
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-                 "r"((uint32_t)add)
+template <int ROW_BYTES>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+                 "r"((uint32_t)add), "n"(kDescriptorHigh<ROW_BYTES>)
                  : "memory");
 }
 // arrives on the barrier when everything that this thread has issued is done

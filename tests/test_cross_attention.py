@@ -130,7 +130,7 @@ SIZES = [  # B, Q, S, G, K, D, masks
     (2, 100, 1000, 8, 8, 32, "queries"), (1, 300, 2311, 8, 8, 32, "padding queries"), (1, 129, 65, 4, 1, 96, "shared"),
     (2, 1000, 16, 2, 2, 64, "heads"), (1, 257, 513, 4, 2, 128, "padding"), (2, 33, 127, 2, 2, 16, "none"),
     (1, 640, 640, 3, 3, 64, ""), (1, 200, 130, 16, 4, 128, "queries"), (1, 2, 5000, 2, 2, 32, "padding"),
-    (5, 128, 128, 1, 1, 128, ""), (1, 70, 4099, 1, 1, 56, "padding"),
+    (10, 40, 1000, 16, 16, 128, ""), (3, 130, 700, 60, 60, 128, ""), (10, 40, 1000, 16, 16, 64, ""), (5, 128, 128, 1, 1, 128, ""), (1, 70, 4099, 1, 1, 56, "padding"),
 ]
 
 
@@ -153,13 +153,15 @@ def test_outputs_and_gradients(size, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("D", [32, 128])
 @pytest.mark.parametrize("Q", [1, 20, 150])
-def test_states_that_nobody_sees_may_hold_anything(dtype, Q):
-    B, S, G, K, D = 2, 260, 4, 2, 32
+def test_states_that_nobody_sees_may_hold_anything(dtype, Q, D):
+    B, S, G, K = 2, 1900, 4, 2
     q, k, v, do = make(B, Q, S, G, K, D, dtype)
     padding = torch.zeros(B, S, dtype=torch.bool, device="cuda")
-    padding[0, 100:] = True
-    padding[1, ::3] = True
+    padding[0, 100:300] = True
+    padding[0, 1700:] = True
+    padding[1, 700::3] = True                       # whole tiles first
     clean = run(q, k, v, do, key_padding_mask=padding)
     for bad in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max):
         kb, vb = (t.masked_fill(padding.view(B, S, 1, 1), bad) for t in (k, v))
@@ -376,5 +378,6 @@ def test_statuses_of_the_c_interface():
     assert call(key_strides=three(-8, 64, 32)) == -1
     assert call(queries=0) == 0 and call(batch=0) == 0
     assert shim.attention_forward(None, *[None] * 6, 0, -1, None) == -1
-    assert shim.attention_mask_bytes(2, 5, 129, 2, 0) == 2 * 8 * 4
-    assert shim.attention_mask_bytes(2, 5, 129, 2, 4) == 4 * 8 * 2 * (2 + 4 * 5)
+    # 129 states: 8 words, lists of 3 and 2 tiles with their counts (in whole 16 bytes)
+    assert shim.attention_mask_bytes(2, 5, 129, 2, 0) == 2 * (8 + 8) * 4
+    assert shim.attention_mask_bytes(2, 5, 129, 2, 4) == 4 * 2 * (2 * 8 + 8 * (2 + 4 * 5))
