@@ -30,15 +30,16 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 // one pass of a call: its split, and the bytes that its parts take
 struct Pass {
     AttentionSplit split;
-    int64_t bytes;
+    int64_t bytes;       // parts
     int row_tiles;       // tiles of 128 rows that a CTA of the tensor-core kernel holds, 0 for the other
 };
 
 // Splits of a pass whose CTAs (148 of them) take items in turn: the number that ends soonest, where an item
-// costs its tiles and `extra` more.
-AttentionSplit even_split(int64_t items, int64_t tiles, int extra) {
-    int64_t best = 1, best_cost = INT64_MAX;
-    for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(tiles / 2, 148)); ++s) {
+// costs its tiles and `extra` more; items of at most `most` tiles.
+AttentionSplit even_split(int64_t items, int64_t tiles, int extra, int64_t most) {
+    const int64_t fewest = std::max<int64_t>(1, (tiles + most - 1) / most);
+    int64_t best = fewest, best_cost = INT64_MAX;
+    for (int64_t s = fewest; s <= std::max<int64_t>(fewest, std::min<int64_t>(tiles / 2, 148)); ++s) {
         const int64_t each = (tiles + s - 1) / s, cost = (items * s + 147) / 148 * (each + extra);
         if (cost < best_cost) best = s, best_cost = cost;
         if (items * s > 148 * 8) break;
@@ -47,16 +48,20 @@ AttentionSplit even_split(int64_t items, int64_t tiles, int extra) {
     return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
 }
 
+// Float32 sums on the tensor cores are cut off, not rounded, at every product that is added: with at most 32
+// tiles (2048 states or rows) to a part, and parts added with rounding, that stays near 2^-20.
+constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 32;
+
+bool on_tensor_cores(const msda_b200_attention &c) { return c.dtype != MSDA_B200_F32 || c.head_dim <= 64; }
+
 Pass forward_pass(const msda_b200_attention &c) {
     const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
     Pass pass{};
-    if (c.dtype != MSDA_B200_F32 && rows > 16) {
-        // Two tiles of rows to a CTA share its loads and take 2 where one takes 1.3 (2048 x 4096, 2 samples, 16 heads x
-        // 64: 107 us against 156), unless the second has too few rows (300 x 17 821, 4 samples, 8 heads x 32: 109
-        // against 89).
+    if (on_tensor_cores(c) && rows > 16) {
         pass.row_tiles = 13 * ((rows + 127) / 128) > 20 * ((rows + 255) / 256) ? 2 : 1;
         const int64_t held = 128 * pass.row_tiles, tile = c.head_dim > 64 ? 128 : 64;
-        pass.split = even_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 8);
+        pass.split = even_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 8,
+                                c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
     } else {
         const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
         const int64_t held = rows <= 16 ? 16 : 64;
@@ -71,10 +76,11 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
     const int64_t share = c.heads / c.kv_heads, rows = c.queries * share, bk = c.batch * c.kv_heads;
     const int64_t held = keys ? c.states : rows, walked = keys ? rows : c.states;
     Pass pass{};
-    if (c.dtype != MSDA_B200_F32 && share <= 64) {
+    if (on_tensor_cores(c) && share <= 64) {
         pass.row_tiles = 1;
         const int64_t x_rows = keys ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
-        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, 6);
+        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, 6,
+                                c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
     } else {
         const int tile = c.head_dim > 64 ? 32 : 64;
         pass.split = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);
@@ -94,7 +100,21 @@ cudaError_t launch_backward(AttentionParams &p, const Pass &pass, int dtype, boo
     return launch_attention_backward_mma(p, dtype, keys, stream);
 }
 
+// the terms of `tokens` x `heads` float32 rows, where a pass needs them
+int64_t term_bytes(const msda_b200_attention &c, int64_t tokens, int64_t heads) {
+    return 6 * c.batch * tokens * heads * ((c.head_dim + 7) / 8 * 8);
+}
+int64_t forward_bytes(const msda_b200_attention &c, const Pass &pass) {
+    const bool terms = c.dtype == MSDA_B200_F32 && pass.row_tiles > 0;
+    return round16(pass.bytes) + (terms ? 2 * term_bytes(c, c.states, c.kv_heads) : 0);
+}
 int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
+
+int64_t backward_bytes(const msda_b200_attention &c, const Pass &keys, const Pass &rows) {
+    const bool terms = c.dtype == MSDA_B200_F32 && keys.row_tiles > 0;
+    return delta_bytes(c) + round16(std::max(keys.bytes, rows.bytes)) +
+           (terms ? 2 * term_bytes(c, c.states, c.kv_heads) + 2 * term_bytes(c, c.queries, c.heads) : 0);
+}
 
 int check(const msda_b200_attention *c) {
     if (c == nullptr) return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: null call");
@@ -193,8 +213,8 @@ int msda_b200_attention_pack_mask(const void *padding, const int64_t *padding_st
 
 int64_t msda_b200_attention_workspace_bytes(const msda_b200_attention *call, int backward) {
     if (check(call) != MSDA_B200_OK || call->batch == 0 || call->queries == 0 || call->states == 0) return 0;
-    if (!backward) return forward_pass(*call).bytes;
-    return delta_bytes(*call) + std::max(backward_pass(*call, true).bytes, backward_pass(*call, false).bytes);
+    if (!backward) return forward_bytes(*call, forward_pass(*call));
+    return backward_bytes(*call, backward_pass(*call, true), backward_pass(*call, false));
 }
 
 int msda_b200_attention_forward(const msda_b200_attention *call, const void *query, const void *key, const void *value,
@@ -216,13 +236,17 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     if (query == nullptr || key == nullptr || value == nullptr || !aligned16(query) || !aligned16(key) || !aligned16(value))
         return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_forward: null or misaligned operand");
     const Pass pass = forward_pass(*call);
-    if (pass.bytes > workspace_bytes || (pass.bytes > 0 && (workspace == nullptr || !aligned16(workspace))))
+    const int64_t needed = forward_bytes(*call, pass);
+    if (needed > workspace_bytes || (needed > 0 && (workspace == nullptr || !aligned16(workspace))))
         return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_forward: workspace too small or misaligned");
     AttentionParams p = params(*call, query, key, value);
     p.out = out, p.lse = lse;
     p.splits = pass.split.splits, p.tiles = pass.split.tiles;
     p.part_lse = static_cast<float *>(workspace);
     p.part = p.part_lse + round16((int64_t)p.splits * p.B * p.K * p.R * 4) / 4;
+    p.k_terms = static_cast<char *>(workspace) + round16(pass.bytes);
+    p.v_terms = static_cast<char *>(p.k_terms) + term_bytes(*call, call->states, call->kv_heads);
+    const int terms = call->dtype == MSDA_B200_F32 && pass.row_tiles > 0 ? 2 : 0;
     cudaError_t e = cudaErrorNotSupported;
     if (pass.row_tiles > 0) {
         e = launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
@@ -230,7 +254,7 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     }
     if (e == cudaErrorNotSupported) e = launch_attention_forward_mma(p, call->dtype, s);
     if (e == cudaSuccess && p.splits > 1) e = launch_attention_join(p, call->dtype, s);
-    if (e == cudaSuccess) count_launches(p.splits > 1 ? 2 : 1, 0);
+    if (e == cudaSuccess) count_launches((p.splits > 1 ? 2 : 1) + terms, 0);
     return status_of(e);
 }
 
@@ -263,7 +287,7 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
         if (x == nullptr || !aligned16(x))
             return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_backward: null or misaligned operand");
     const Pass keys = backward_pass(*call, true), rows = backward_pass(*call, false);
-    if (delta_bytes(*call) + std::max(keys.bytes, rows.bytes) > workspace_bytes)
+    if (backward_bytes(*call, keys, rows) > workspace_bytes)
         return refuse(MSDA_B200_INVALID_ARGUMENT, "attention_backward: workspace too small");
     AttentionParams p = params(*call, query, key, value);
     p.out = const_cast<void *>(out), p.grad_out = grad_out, p.lse = const_cast<float *>(lse);
@@ -272,6 +296,19 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
     p.part = p.delta + delta_bytes(*call) / 4;
     int launches = 3;
     cudaError_t e = launch_attention_delta(p, call->dtype, s);
+    if (call->dtype == MSDA_B200_F32 && keys.row_tiles > 0) {
+        const int64_t gs[3] = {call->queries * call->heads * call->head_dim, call->heads * call->head_dim, call->head_dim};
+        char *terms = reinterpret_cast<char *>(p.part) + round16(std::max(keys.bytes, rows.bytes));
+        const int64_t state_terms = term_bytes(*call, call->states, call->kv_heads), row_terms = term_bytes(*call, call->queries, call->heads);
+        p.k_terms = terms, p.v_terms = terms + state_terms, p.q_terms = terms + 2 * state_terms;
+        p.g_terms = terms + 2 * state_terms + row_terms;
+        const int H = (int)call->heads;
+        if (e == cudaSuccess) e = launch_attention_terms(p.k, p.ks, p.B, p.S, p.K, p.D, p.k_terms, s);
+        if (e == cudaSuccess) e = launch_attention_terms(p.v, p.vs, p.B, p.S, p.K, p.D, p.v_terms, s);
+        if (e == cudaSuccess) e = launch_attention_terms(p.q, p.qs, p.B, p.Q, H, p.D, p.q_terms, s);
+        if (e == cudaSuccess) e = launch_attention_terms(p.grad_out, gs, p.B, p.Q, H, p.D, p.g_terms, s);
+        launches += 4;
+    }
     if (e == cudaSuccess) {
         p.part2 = p.part + (int64_t)keys.split.splits * p.B * p.K * p.S * p.D;
         e = launch_backward(p, keys, call->dtype, true, s);

@@ -147,6 +147,25 @@ __global__ void __launch_bounds__(1024) attention_list_kernel(const __grid_const
     list_both(p.key_words + (int64_t)blockIdx.x * p.W, p.S, p.lists + blockIdx.x * list_words(p.S));
 }
 
+// a thread to eight channels, zeros behind the last one
+__global__ void __launch_bounds__(kThreads) attention_terms_kernel(const float *x, int64_t s0, int64_t s1, int64_t s2, int tokens,
+                                                                   int heads, int D, int64_t rows, uint4 *terms) {
+    const int chunks = (D + 7) / 8;
+    const int64_t all = rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t row = i / chunks, token = row / heads, b = token / tokens;
+        const int c = (int)(i - row * chunks) * 8;
+        const float *from = x + b * s0 + (token - b * tokens) * s1 + (row - token * heads) * s2 + c;
+        const float4 lo = __ldg(reinterpret_cast<const float4 *>(from));
+        const float4 hi = c + 4 < D ? __ldg(reinterpret_cast<const float4 *>(from + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t t[4][3];
+        split_terms(make_float2(lo.x, lo.y), t[0]), split_terms(make_float2(lo.z, lo.w), t[1]);
+        split_terms(make_float2(hi.x, hi.y), t[2]), split_terms(make_float2(hi.z, hi.w), t[3]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) terms[k * all + i] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+    }
+}
+
 // eight lanes to a row
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_constant__ AttentionParams p) {
@@ -269,6 +288,15 @@ cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream) {
     attention_mask_kernel<<<(unsigned)grid, kThreads, 0, stream>>>(p);
     attention_mask_any_kernel<<<(unsigned)(p.B * p.KW * ((p.W + 31) / 32)), 1024, 0, stream>>>(p);
     attention_list_kernel<<<(unsigned)(p.B * p.KW), 1024, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attention_terms(const void *x, const int64_t (&strides)[3], int B, int tokens, int heads, int D, void *terms,
+                                   cudaStream_t stream) {
+    const int64_t rows = (int64_t)B * tokens * heads;
+    const int64_t grid = std::min<int64_t>((rows * ((D + 7) / 8) + kThreads - 1) / kThreads, 148 * 32);
+    attention_terms_kernel<<<(unsigned)grid, kThreads, 0, stream>>>(static_cast<const float *>(x), strides[0], strides[1], strides[2],
+                                                                     tokens, heads, D, rows, static_cast<uint4 *>(terms));
     return cudaGetLastError();
 }
 

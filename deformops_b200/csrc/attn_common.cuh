@@ -42,7 +42,25 @@ struct AttentionParams {
     // partial results go to part (splits, B, K, rows, D) and part_lse (splits, B, K, rows)
     float *part, *part2, *part_lse;
     int splits, tiles;
+    // float32 on the tensor cores: the operands' three bf16 terms, dense (3, B, tokens, heads, D8), D8 whole
+    // vectors of eight channels
+    void *q_terms, *k_terms, *v_terms, *g_terms;
 };
+
+// Float32 operands as x = x0 + x1 + x2 of bf16 (8 bits each), products x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0: what
+// is left out is 2^-24 of a product.  In the order that has the small ones first.
+constexpr int kPairs = 6;
+__host__ __device__ constexpr int left_term(int pair) { return pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0; }
+__host__ __device__ constexpr int right_term(int pair) { return pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0; }
+// (x, y) as terms, packed like the products' operands
+__device__ __forceinline__ void split_terms(float2 x, uint32_t (&t)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        t[i] = VecTraits<__nv_bfloat16>::pack2(x);
+        const float2 y = VecTraits<__nv_bfloat16>::unpack2(t[i]);
+        x.x -= y.x, x.y -= y.y;
+    }
+}
 
 // ---- which states a tile of 32 * N of them may use --------------------------------------------------
 __device__ __forceinline__ const uint32_t *key_words_of(const AttentionParams &p, int b, int h) {
@@ -123,12 +141,15 @@ __device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
 
 // ---- host side ------------------------------------------------------------------------------------
 cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream);
-// 16-bit types; row_tiles of 128 rows to a CTA, stretches of whole tiles of 64 states (128 where D > 64).  cudaErrorNotSupported (and
+// 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to a CTA, stretches of whole tiles of 64 states (128 where D > 64).  cudaErrorNotSupported (and
 // nothing launched) where k or v cannot be described to TMA.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 
+// the terms of a (B, tokens, heads, D) float32 tensor with these strides
+cudaError_t launch_attention_terms(const void *x, const int64_t (&strides)[3], int B, int tokens, int heads, int D, void *terms,
+                                   cudaStream_t stream);
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream);
 // parts of a split pass to the result: outputs and sums (forward), or the sum of gradients
 cudaError_t launch_attention_join(const AttentionParams &p, int dtype, cudaStream_t stream);

@@ -1,4 +1,5 @@
-// Cross attention backward on the fifth-generation tensor cores, 16-bit types.
+// Cross attention backward on the fifth-generation tensor cores, 16-bit types, and float32 up to 64 channels as three
+// bf16 terms of every operand (TERMS = 3: six products for one).
 //
 // One kernel template in two forms.  A CTA holds a tile X of 128 and walks tiles Y of 64:
 //
@@ -26,23 +27,33 @@ namespace {
 
 constexpr int kX = 128, kY = 64;
 
-template <int DP>
-constexpr int kStages = DP == 128 ? 2 : 6;
+template <int DP, bool KEYS, int TERMS>
+struct Shape {
+    static constexpr int ST = TERMS == 3 ? (DP == 32 ? 4 : 2) : DP == 128 ? 2 : 6;      // tiles Y in flight
+    static constexpr int XB = DP * TERMS > 128 ? 1 : 2;                                  // tiles X
+    // warpgroups that take the tiles Y in turn: as many as tensor memory has room for
+    static constexpr int kGroups = TERMS == 3 || DP == 128 ? 2 : 3;
+    static constexpr int kThreads = kGroups * 128 + 128;
+    // columns of tensor memory: of a group S and T, in whose places P and dS come (third terms need more), then the sums
+    static constexpr uint32_t kS = 0, kT = 64;
+    static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }
+    static constexpr uint32_t kGroup = TERMS == 1 ? 128 : KEYS ? 192 : 160;
+    static constexpr uint32_t kAcc0 = kGroups * kGroup, kAcc1 = KEYS ? kAcc0 + DP : kAcc0;
+    static_assert(kAcc1 + DP <= 512);
+    static_assert(ST >= kGroups);
+};
 
-// warpgroups that take the tiles Y in turn: as many as tensor memory has room for
-template <int DP>
-constexpr int kGroupsOf = DP == 128 ? 2 : 3;
-
-template <int DP, bool KEYS>
+template <int DP, bool KEYS, int TERMS>
 struct Shared {
-    static constexpr int ST = kStages<DP>;
-    alignas(1024) unsigned char x[2][2][kX * DP * 2];          // two items' X0 and X1
-    alignas(1024) unsigned char y[ST][2][kY * DP * 2];
+    using Sh = Shape<DP, KEYS, TERMS>;
+    static constexpr int ST = Sh::ST;
+    alignas(1024) unsigned char x[Sh::XB][2][TERMS][kX * DP * 2];       // of an item X0 and X1
+    alignas(1024) unsigned char y[ST][2][TERMS][kY * DP * 2];
     alignas(16) float lse[KEYS ? ST : 1][kY];                   // of the walked rows, both with the sign turned
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
     uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
-    uint64_t s_full[kGroupsOf<DP>], p_full[kGroupsOf<DP>], acc_full, acc_free;
+    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full, acc_free;
     uint32_t tmem;
 };
 
@@ -86,19 +97,21 @@ struct Walk<true> {
     __device__ __forceinline__ uint32_t operator[](int n) const { return (uint32_t)(first + n); }
 };
 
-template <typename T, int DP, bool KEYS>
-__global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
+template <typename T, int DP, bool KEYS, int TERMS>
+__global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     attention_backward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap x0m,
                                  const __grid_constant__ tc::TensorMap x1m, const __grid_constant__ tc::TensorMap y0m,
                                  const __grid_constant__ tc::TensorMap y1m, int64_t items, int x_rows, int y_rows) {
     using namespace tc;
-    constexpr int ST = kStages<DP>;
+    using Sh = Shape<DP, KEYS, TERMS>;
+    using Out = std::conditional_t<TERMS == 3, float, T>;      // of the call's tensors; T is that of the products
+    constexpr int ST = Sh::ST, XB = Sh::XB, kGroups = Sh::kGroups, kLast = 4 * kGroups;
+    constexpr int kPairsOf = TERMS == 3 ? kPairs : 1;
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
-    constexpr int kGroups = kGroupsOf<DP>, kLast = 4 * kGroups;
-    constexpr uint32_t kS = 0, kT = 64, kGroup = 128, kAcc0 = kGroups * 128, kAcc1 = KEYS ? kAcc0 + DP : kAcc0;
-    static_assert(kAcc1 + DP <= 512);
+    constexpr uint32_t kS = Sh::kS, kT = Sh::kT, kGroup = Sh::kGroup, kAcc0 = Sh::kAcc0, kAcc1 = Sh::kAcc1;
+    constexpr uint32_t kXBytes = kX * DP * 2, kYBytes = kY * DP * 2;
     extern __shared__ __align__(1024) unsigned char raw[];
-    auto &sm = *reinterpret_cast<Shared<DP, KEYS> *>(raw);
+    auto &sm = *reinterpret_cast<Shared<DP, KEYS, TERMS> *>(raw);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (warp == kLast) tmem_alloc(&sm.tmem, 512);
@@ -131,6 +144,15 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t mine = tmem + group * kGroup + lanes;
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+        const auto put = [](float2 x, uint32_t (&to)[TERMS][16], int c) {
+            if constexpr (TERMS == 3) {
+                uint32_t t[3];
+                split_terms(x, t);
+                to[0][c] = t[0], to[1][c] = t[1], to[TERMS - 1][c] = t[2];
+            } else {
+                to[0][c] = VecTraits<T>::pack2(x);
+            }
+        };
         int n = 0, done = 0;             // tiles and items with tiles so far
         for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
             const Item it = item_of(p, i, x_tiles, x_rows);
@@ -221,19 +243,25 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                     if constexpr (KEYS) {
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            uint32_t packed[16];
+                            uint32_t packed[TERMS][16];
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) packed[c] = VecTraits<T>::pack2(w[16 * half + c]);
-                            tmem_store16(mine + kS + 16 * half, packed);
+                            for (int c = 0; c < 16; ++c) put(w[16 * half + c], packed, c);
+                            tmem_store16(mine + kS + 16 * half, packed[0]);
+                            if constexpr (TERMS == 3) {
+                                tmem_store16(mine + kS + 32 + 16 * half, packed[1]);
+                                tmem_store16(mine + Sh::third(true) + 16 * half, packed[TERMS - 1]);
+                            }
                         }
                     }
-                    // (the first half of dS takes the place of a quarter of T that is in registers by then)
+                    // The first half of dS takes the place of a quarter of T that is in registers by then.  With three
+                    // terms its second one would take T's second half: that is kept back.
+                    uint32_t second[16];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         if (half == 1) tmem_load32(t, mine + kT + 32);
                         tmem_wait_load();
                         loaded(t);
-                        uint32_t packed[16];
+                        uint32_t packed[TERMS][16];
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
                             const int at = 16 * half + c;
@@ -249,9 +277,19 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                                 if (!(bits & 4)) y.x = 0.f;
                                 if (!(bits & 8)) y.y = 0.f;
                             }
-                            packed[c] = VecTraits<T>::pack2(x), packed[c + 1] = VecTraits<T>::pack2(y);
+                            put(x, packed, c), put(y, packed, c + 1);
                         }
-                        tmem_store16(mine + kT + 16 * half, packed);
+                        tmem_store16(mine + kT + 16 * half, packed[0]);
+                        if constexpr (TERMS == 3) {
+                            tmem_store16(mine + Sh::third(false) + 16 * half, packed[TERMS - 1]);
+                            if (half == 0) {
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) second[c] = packed[1][c];
+                            } else {
+                                tmem_store16(mine + kT + 32, second);
+                                tmem_store16(mine + kT + 48, packed[1]);
+                            }
+                        }
                     }
                     tmem_wait_store();
                 }
@@ -276,7 +314,7 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
             const int query = x / p.share;
             const int64_t at = KEYS ? (((int64_t)it.b * p.S + x) * p.K + it.h) * p.D
                                     : (((int64_t)it.b * p.Q + query) * p.K * p.share + it.h * p.share + (x - query * p.share)) * p.D;
-            T *out = static_cast<T *>(KEYS ? (group == 0 ? p.dv : p.dk) : p.dq) + at;
+            Out *out = static_cast<Out *>(KEYS ? (group == 0 ? p.dv : p.dk) : p.dq) + at;
             float *parts = (KEYS && group == 0 ? p.part2 : p.part) +
                            ((it.part * (int64_t)p.B * p.K + it.bh) * rows + x) * p.D;
 #pragma unroll
@@ -297,10 +335,12 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                 for (int c = 0; c < 8; c += 4) {
                     const int col = from + d + 2 * c;
                     if (col >= p.D) continue;
-                    if (p.splits > 1) {
-                        *reinterpret_cast<float4 *>(parts + col) = make_float4(y[c].x, y[c].y, y[c + 1].x, y[c + 1].y);
-                        *reinterpret_cast<float4 *>(parts + col + 4) = make_float4(y[c + 2].x, y[c + 2].y, y[c + 3].x, y[c + 3].y);
-                    } else {
+                    if (TERMS == 3 || p.splits > 1) {
+                        float *to = p.splits > 1 ? parts : reinterpret_cast<float *>(out);
+                        *reinterpret_cast<float4 *>(to + col) = make_float4(y[c].x, y[c].y, y[c + 1].x, y[c + 1].y);
+                        if (col + 4 < p.D)
+                            *reinterpret_cast<float4 *>(to + col + 4) = make_float4(y[c + 2].x, y[c + 2].y, y[c + 3].x, y[c + 3].y);
+                    } else if constexpr (TERMS == 1) {
                         const float2 z[4] = {y[c], y[c + 1], y[c + 2], y[c + 3]};
                         *reinterpret_cast<uint4 *>(out + col) = VecTraits<T>::pack(z);
                     }
@@ -319,25 +359,31 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                 const Item it = item_of(p, i, x_tiles, x_rows);
                 const Walk<KEYS> walk(p, it, y_rows);
                 if (walk.count == 0) continue;
-                const int buffer = done & 1;
-                if (done > 1) fine = barrier_wait(&sm.x_free[buffer], ((done >> 1) - 1) & 1);
+                const int buffer = done % XB;
+                if (done >= XB) fine = barrier_wait(&sm.x_free[buffer], (done / XB - 1) & 1);
                 if (!fine) break;
-                barrier_expect(&sm.x_full[buffer], 2 * x_rows * DP * 2);
-                load_rows<DP, kX>(sm.x[buffer][0], x0m, &sm.x_full[buffer], it.b, it.h, it.first);
-                load_rows<DP, kX>(sm.x[buffer][1], x1m, &sm.x_full[buffer], it.b, it.h, it.first);
+                barrier_expect(&sm.x_full[buffer], 2 * TERMS * x_rows * DP * 2);
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) {
+                    load_rows<DP, kX>(sm.x[buffer][0][k], x0m, &sm.x_full[buffer], it.b + k * p.B, it.h, it.first);
+                    load_rows<DP, kX>(sm.x[buffer][1][k], x1m, &sm.x_full[buffer], it.b + k * p.B, it.h, it.first);
+                }
                 ++done;
                 for (int j = 0; fine && j < walk.count; ++j, ++n) {
                     const int stage = n % ST, row = (int)(walk[j] & 0x7fffffff) * y_rows;
                     if (n >= ST) fine = barrier_wait(&sm.y_free[stage], (n / ST - 1) & 1);
                     if (!fine) break;
-                    barrier_expect(&sm.y_full[stage], 2 * y_rows * DP * 2);
-                    load_rows<DP, kY>(sm.y[stage][0], y0m, &sm.y_full[stage], it.b, it.h, row);
-                    load_rows<DP, kY>(sm.y[stage][1], y1m, &sm.y_full[stage], it.b, it.h, row);
+                    barrier_expect(&sm.y_full[stage], 2 * TERMS * y_rows * DP * 2);
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        load_rows<DP, kY>(sm.y[stage][0][k], y0m, &sm.y_full[stage], it.b + k * p.B, it.h, row);
+                        load_rows<DP, kY>(sm.y[stage][1][k], y1m, &sm.y_full[stage], it.b + k * p.B, it.h, row);
+                    }
                 }
             }
             if (!fine) {     // nothing may still be on its way when the CTA ends
-                for (int s = 0; s < 2; ++s)
-                    if (done > s) barrier_wait(&sm.x_full[s], ((done - s + 1) / 2 - 1) & 1);
+                for (int s = 0; s < XB; ++s)
+                    if (done > s) barrier_wait(&sm.x_full[s], ((done - s + XB - 1) / XB - 1) & 1);
                 for (int s = 0; s < ST; ++s)
                     if (n > s) barrier_wait(&sm.y_full[s], ((n - s + ST - 1) / ST - 1) & 1);
             }
@@ -379,7 +425,6 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
             constexpr uint32_t kScores = instruction(kBf16, kX, kY, false, false);
             constexpr uint32_t kSums = instruction(kBf16, kX, DP, false, true);
             constexpr int kRow = kRowBytes<DP>;
-            constexpr uint32_t kXBytes = kX * DP * 2, kYBytes = kY * DP * 2;
             const uint32_t x0 = descriptor(smem_address(sm.x), 16), y0 = descriptor(smem_address(sm.y), 16),
                            z0 = descriptor(smem_address(sm.y), kY * 128);
             // Tiles whose products with P and dS are still to be issued, one fewer than there are groups: the scores
@@ -387,7 +432,7 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
             struct Pending {
                 int n, item;
                 bool first, last;
-            } queue[kGroups - 1];
+            } queue[kGroups - 1] = {};
             int waiting = 0, n = 0, done = 0;
             const auto issue_sums = [&] {
                 const Pending t = queue[0];
@@ -400,15 +445,18 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                 fine = fine && barrier_wait(&sm.p_full[group], (t.n / kGroups) & 1);
                 fence_after();
                 if (fine) {
-                    const uint32_t from = tmem + group * kGroup, za = z0 + stage * (2 * kYBytes >> 4);
-                    if constexpr (KEYS) {
+                    const uint32_t from = tmem + group * kGroup, za = z0 + stage * (2 * TERMS * kYBytes >> 4);
 #pragma unroll
-                        for (int j = 0; j < kY; j += 16)
-                            mma_ts<kRow>(tmem + kAcc0, from + kS + j / 2, za + (kYBytes + j * kRow >> 4), kSums, !t.first || j > 0);
+                    for (int k = kPairs - kPairsOf; k < kPairs; ++k) {
+                        const bool add = !t.first || k > kPairs - kPairsOf;
+#pragma unroll
+                        for (int j = 0; j < kY; j += 16) {
+                            const uint32_t of = right_term(k) * kYBytes + j * kRow;
+                            if constexpr (KEYS)
+                                mma_ts<kRow>(tmem + kAcc0, from + (left_term(k) == 2 ? Sh::third(true) : kS + 32 * left_term(k)) + j / 2, za + (TERMS * kYBytes + of >> 4), kSums, add || j > 0);
+                            mma_ts<kRow>(tmem + kAcc1, from + (left_term(k) == 2 ? Sh::third(false) : kT + 32 * left_term(k)) + j / 2, za + (of >> 4), kSums, add || j > 0);
+                        }
                     }
-#pragma unroll
-                    for (int j = 0; j < kY; j += 16)
-                        mma_ts<kRow>(tmem + kAcc1, from + kT + j / 2, za + (j * kRow >> 4), kSums, !t.first || j > 0);
                     commit(&sm.y_free[stage]);
                     if (t.last) commit(&sm.acc_full);
                 }
@@ -417,21 +465,27 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                 const Item it = item_of(p, i, x_tiles, x_rows);
                 const Walk<KEYS> walk(p, it, y_rows);
                 if (walk.count == 0) continue;
-                const int buffer = done & 1;
-                fine = barrier_wait(&sm.x_full[buffer], (done >> 1) & 1);
+                const int buffer = done % XB;
+                fine = barrier_wait(&sm.x_full[buffer], (done / XB) & 1);
                 for (int j = 0; fine && j < walk.count; ++j, ++n) {
                     const bool first = j == 0;
                     const int stage = n % ST, group = n % kGroups;
                     fine = barrier_wait(&sm.y_full[stage], (n / ST) & 1);
                     if (fine) {
                         const uint32_t to = tmem + group * kGroup;
-                        const uint32_t xa = x0 + buffer * (2 * kXBytes >> 4), ya = y0 + stage * (2 * kYBytes >> 4);
+                        const uint32_t xa = x0 + buffer * (2 * TERMS * kXBytes >> 4), ya = y0 + stage * (2 * TERMS * kYBytes >> 4);
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
+                        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                            for (int d = 0; d < DP; d += 16)
-                                mma<kRow>(to + (half == 0 ? kS : kT), xa + (half * kXBytes + (d & ~63) * kX * 2 + (d & 63) * 2 >> 4),
-                                          ya + (half * kYBytes + (d & ~63) * kY * 2 + (d & 63) * 2 >> 4), kScores, d > 0);
+                            for (int k = kPairs - kPairsOf; k < kPairs; ++k) {
+#pragma unroll
+                                for (int d = 0; d < DP; d += 16)
+                                    mma<kRow>(to + (half == 0 ? kS : kT),
+                                              xa + ((half * TERMS + left_term(k)) * kXBytes + (d & ~63) * kX * 2 + (d & 63) * 2 >> 4),
+                                              ya + ((half * TERMS + right_term(k)) * kYBytes + (d & ~63) * kY * 2 + (d & 63) * 2 >> 4), kScores,
+                                              d > 0 || k > kPairs - kPairsOf);
+                            }
+                        }
                         commit(&sm.s_full[group]);
                         if (j == walk.count - 1) commit(&sm.x_free[buffer]);
                     }
@@ -460,8 +514,11 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
                         constexpr int kChunks = DP / 8;
                         for (int c = lane; c < 64 * kChunks; c += 32) {
                             const int r = c / kChunks;
-                            if (!(((r < 32 ? see.x : see.y) >> (r & 31)) & 1))
-                                *reinterpret_cast<uint4 *>(sm.y[stage][0] + swizzled<DP, kY>(r, c % kChunks)) = make_uint4(0, 0, 0, 0);
+                            if (!(((r < 32 ? see.x : see.y) >> (r & 31)) & 1)) {
+#pragma unroll
+                                for (int k = 0; k < TERMS; ++k)
+                                    *reinterpret_cast<uint4 *>(sm.y[stage][0][k] + swizzled<DP, kY>(r, c % kChunks)) = make_uint4(0, 0, 0, 0);
+                            }
                         }
                         fence_async_shared();
                     }
@@ -478,25 +535,37 @@ __global__ void __launch_bounds__(kGroupsOf<DP> * 128 + 128, 1)
     }
 }
 
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, bool KEYS, int TERMS = 1>
 cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
-    const int64_t gs[3] = {(int64_t)p.Q * p.K * p.share * p.D, (int64_t)p.K * p.share * p.D, p.D};
     const int row_tile = KEYS ? kY : kX, state_tile = KEYS ? kX : kY;
     tc::TensorMap q, g, k, v;
-    if (!tc::make_map<T, DP>(q, p.q, p.qs, p.B, p.Q, p.K, p.share, p.D, row_tile) ||
-        !tc::make_map<T, DP>(g, p.grad_out, gs, p.B, p.Q, p.K, p.share, p.D, row_tile) ||
-        !tc::make_map<T, DP>(k, p.k, p.ks, p.B, p.S, p.K, 1, p.D, state_tile) ||
-        !tc::make_map<T, DP>(v, p.v, p.vs, p.B, p.S, p.K, 1, p.D, state_tile))
-        return cudaErrorNotSupported;
-    const auto kernel = attention_backward_tc_kernel<T, DP, KEYS>;
-    constexpr size_t smem = sizeof(Shared<DP, KEYS>);
+    if constexpr (TERMS == 3) {
+        const int64_t D8 = (p.D + 7) / 8 * 8, heads = (int64_t)p.K * p.share;
+        const int64_t rows[3] = {p.Q * heads * D8, heads * D8, D8}, states[3] = {p.S * p.K * D8, p.K * D8, D8};
+        if (!tc::make_map<T, DP>(q, p.q_terms, rows, 3 * p.B, p.Q, p.K, p.share, (int)D8, row_tile) ||
+            !tc::make_map<T, DP>(g, p.g_terms, rows, 3 * p.B, p.Q, p.K, p.share, (int)D8, row_tile) ||
+            !tc::make_map<T, DP>(k, p.k_terms, states, 3 * p.B, p.S, p.K, 1, (int)D8, state_tile) ||
+            !tc::make_map<T, DP>(v, p.v_terms, states, 3 * p.B, p.S, p.K, 1, (int)D8, state_tile))
+            return cudaErrorNotSupported;
+    } else {
+        const int64_t gs[3] = {(int64_t)p.Q * p.K * p.share * p.D, (int64_t)p.K * p.share * p.D, p.D};
+        if (!tc::make_map<T, DP>(q, p.q, p.qs, p.B, p.Q, p.K, p.share, p.D, row_tile) ||
+            !tc::make_map<T, DP>(g, p.grad_out, gs, p.B, p.Q, p.K, p.share, p.D, row_tile) ||
+            !tc::make_map<T, DP>(k, p.k, p.ks, p.B, p.S, p.K, 1, p.D, state_tile) ||
+            !tc::make_map<T, DP>(v, p.v, p.vs, p.B, p.S, p.K, 1, p.D, state_tile))
+            return cudaErrorNotSupported;
+    }
+    const auto kernel = attention_backward_tc_kernel<T, DP, KEYS, TERMS>;
+    constexpr size_t smem = sizeof(Shared<DP, KEYS, TERMS>);
+    static_assert(smem <= 227 * 1024);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const int rows = row_tile / p.share * p.share;
     const int x_rows = KEYS ? kX : rows, y_rows = KEYS ? rows : kY;
     const int64_t items = (int64_t)p.B * p.K * p.splits * (((KEYS ? p.S : p.R) + x_rows - 1) / x_rows);
     const unsigned grid = (unsigned)std::min<int64_t>(items, 148);
-    kernel<<<grid, kGroupsOf<DP> * 128 + 128, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v, items, x_rows, y_rows);
+    kernel<<<grid, Shape<DP, KEYS, TERMS>::kThreads, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v, items,
+                                                                     x_rows, y_rows);
     return cudaGetLastError();
 }
 
@@ -507,10 +576,17 @@ cudaError_t launch_typed(const AttentionParams &p, bool keys, cudaStream_t strea
     return keys ? launch<T, 128, true>(p, stream) : launch<T, 128, false>(p, stream);
 }
 
+cudaError_t launch_float(const AttentionParams &p, bool keys, cudaStream_t stream) {
+    using T = __nv_bfloat16;
+    if (p.D <= 32) return keys ? launch<T, 32, true, 3>(p, stream) : launch<T, 32, false, 3>(p, stream);
+    return keys ? launch<T, 64, true, 3>(p, stream) : launch<T, 64, false, 3>(p, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream) {
-    return dtype == 1 ? launch_typed<__half>(p, keys, stream) : launch_typed<__nv_bfloat16>(p, keys, stream);
+    return dtype == 0 ? launch_float(p, keys, stream)
+           : dtype == 1 ? launch_typed<__half>(p, keys, stream) : launch_typed<__nv_bfloat16>(p, keys, stream);
 }
 
 }  // namespace msda_b200

@@ -1,4 +1,5 @@
-// Cross attention forward on the fifth-generation tensor cores, 16-bit types.
+// Cross attention forward on the fifth-generation tensor cores, 16-bit types, and float32 up to 64 channels as three
+// bf16 terms of every operand (TERMS = 3: six products for one).
 //
 // A CTA holds RT tiles of 128 rows and walks tiles of BN states.  One thread has TMA bring the tiles of
 // k and v, one thread issues the products, and RT * KW groups of four warps do the softmax, a thread to
@@ -27,25 +28,26 @@ namespace {
 
 constexpr int kTileRows = 128;
 
-template <int DP, int RT, int KW>
+template <int DP, int RT, int KW, int TERMS>
 struct Shape {
     static constexpr int BN = DP == 128 ? 128 : 64;            // states of a tile
-    static constexpr int ST = DP == 128 ? KW + 1 : 8;          // tiles of k and v in flight
+    static constexpr int ST = DP == 128 || DP * TERMS > 128 ? KW + 1 : TERMS == 3 ? 6 : 8;     // tiles of k and v in flight
     static constexpr int kGroups = RT * KW;
     static constexpr int kThreads = kGroups * 128 + 128;
-    static constexpr uint32_t kColumns = BN + DP;              // of tensor memory, for a group: S (and P), O
+    // columns of tensor memory of a group: S, in whose place P comes (a third term needs more), O
+    static constexpr uint32_t kWeights = BN / 2, kO = std::max<uint32_t>(BN, TERMS * kWeights), kColumns = kO + DP;
     // what a thread may hold: all of the block's at launch, less what the last four warps need
     static constexpr int kRegisters = kGroups == 4 ? 104 : 224, kFew = kGroups == 4 ? 64 : 56;
     static_assert(kGroups * kColumns <= 512);
     static_assert(ST > KW);                                    // a tile is freed KW tiles after its scores
 };
 
-template <int DP, int RT, int KW>
+template <int DP, int RT, int KW, int TERMS>
 struct Shared {
-    using Sh = Shape<DP, RT, KW>;
-    alignas(1024) unsigned char q[RT][kTileRows * DP * 2];
-    alignas(1024) unsigned char k[Sh::ST][Sh::BN * DP * 2];
-    alignas(1024) unsigned char v[Sh::ST][Sh::BN * DP * 2];
+    using Sh = Shape<DP, RT, KW, TERMS>;
+    alignas(1024) unsigned char q[RT][TERMS][kTileRows * DP * 2];
+    alignas(1024) unsigned char k[Sh::ST][TERMS][Sh::BN * DP * 2];
+    alignas(1024) unsigned char v[Sh::ST][TERMS][Sh::BN * DP * 2];
     float m[Sh::kGroups][kTileRows], l[Sh::kGroups][kTileRows];
     uint64_t full[Sh::ST], clean[Sh::ST], free[Sh::ST];        // of a stage: its k and v
     uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], o_full[Sh::kGroups];
@@ -77,18 +79,20 @@ struct Words {
     }
 };
 
-template <typename T, int DP, int RT, int KW>
-__global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
+template <typename T, int DP, int RT, int KW, int TERMS>
+__global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
     attention_forward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap km,
                                 const __grid_constant__ tc::TensorMap vm) {
     using namespace tc;
-    using Sh = Shape<DP, RT, KW>;
+    using Sh = Shape<DP, RT, KW, TERMS>;
+    using Out = std::conditional_t<TERMS == 3, float, T>;      // of the call's tensors; T is that of the products
     constexpr int BN = Sh::BN, NW = BN / 32, ST = Sh::ST;
-    constexpr uint32_t kO = BN;
+    constexpr uint32_t kO = Sh::kO, kP = Sh::kWeights;
+    constexpr int kPairsOf = TERMS == 3 ? kPairs : 1, kTile = BN * DP * 2;
     constexpr int kLast = Sh::kGroups * 4;                     // first of the last four warps
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     extern __shared__ __align__(1024) unsigned char raw[];
-    auto &sm = *reinterpret_cast<Shared<DP, RT, KW> *>(raw);
+    auto &sm = *reinterpret_cast<Shared<DP, RT, KW, TERMS> *>(raw);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     const int row_tiles = (p.R + RT * kTileRows - 1) / (RT * kTileRows);
@@ -112,12 +116,28 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
     if (warp < 4 * RT) {
         // a thread to a row of q
         const int r = first + threadIdx.x;
-        const T *q = static_cast<const T *>(p.q) + (r < p.R ? row_offset(p.qs, p.share, b, h, r) : 0);
-        unsigned char *to = sm.q[warp >> 2];
+        const Out *q = static_cast<const Out *>(p.q) + (r < p.R ? row_offset(p.qs, p.share, b, h, r) : 0);
 #pragma unroll
         for (int c = 0; c < DP / 8; ++c) {
-            const uint4 x = r < p.R && c * 8 < p.D ? ldg16(q + c * 8) : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4 *>(to + swizzled<DP, kTileRows>(threadIdx.x & 127, c)) = x;
+            uint4 x[TERMS];
+            if constexpr (TERMS == 3) {
+                const uint4 none = make_uint4(0, 0, 0, 0);
+                const uint4 f[2] = {r < p.R && c * 8 < p.D ? ldg16(q + c * 8) : none,
+                                    r < p.R && c * 8 + 4 < p.D ? ldg16(q + c * 8 + 4) : none};
+                uint32_t t[4][3];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    split_terms(make_float2(__uint_as_float(f[i].x), __uint_as_float(f[i].y)), t[2 * i]);
+                    split_terms(make_float2(__uint_as_float(f[i].z), __uint_as_float(f[i].w)), t[2 * i + 1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x[i] = make_uint4(t[0][i], t[1][i], t[2][i], t[3][i]);
+            } else {
+                x[0] = r < p.R && c * 8 < p.D ? ldg16(q + c * 8) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i)
+                *reinterpret_cast<uint4 *>(sm.q[warp >> 2][i] + swizzled<DP, kTileRows>(threadIdx.x & 127, c)) = x[i];
         }
         fence_async_shared();
     }
@@ -201,15 +221,22 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
                 float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int j = 0; j < NW; ++j) {
-                    uint32_t w[16];
+                    uint32_t w[TERMS][16];
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         float2 x = fma2(make_float2(__uint_as_float(s[j][c]), __uint_as_float(s[j][c + 1])), scale2, less2);
                         x.x = fast_exp2(x.x), x.y = fast_exp2(x.y);
                         sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], x);
-                        w[c >> 1] = VecTraits<T>::pack2(x);
+                        if constexpr (TERMS == 3) {
+                            uint32_t t[3];
+                            split_terms(x, t);
+                            w[0][c >> 1] = t[0], w[1][c >> 1] = t[1], w[TERMS - 1][c >> 1] = t[2];
+                        } else {
+                            w[0][c >> 1] = VecTraits<T>::pack2(x);
+                        }
                     }
-                    tmem_store16(mine + 16 * j, w);
+#pragma unroll
+                    for (int i = 0; i < TERMS; ++i) tmem_store16(mine + i * kP + 16 * j, w[i]);
                 }
                 l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_store();
@@ -250,7 +277,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
         }
         const int64_t at = bh * p.R + r, rows = (int64_t)p.B * p.K * p.R;
         const int query = r / p.share;
-        T *out = static_cast<T *>(p.out) + (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
+        Out *out = static_cast<Out *>(p.out) + (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
         float *parts = p.part + (part * rows + at) * p.D;
         if (r < p.R && way == 0) (p.splits > 1 ? p.part_lse + part * rows : p.lse)[at] = lse;
         constexpr int kShare = DP / KW, kStep = kShare < 16 ? 8 : 16;
@@ -279,10 +306,12 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < kStep / 2; c += 4) {
                     if (col + 2 * c >= p.D) continue;
-                    if (p.splits > 1) {
-                        *reinterpret_cast<float4 *>(parts + col + 2 * c) = make_float4(x[c].x, x[c].y, x[c + 1].x, x[c + 1].y);
-                        *reinterpret_cast<float4 *>(parts + col + 2 * c + 4) = make_float4(x[c + 2].x, x[c + 2].y, x[c + 3].x, x[c + 3].y);
-                    } else {
+                    if (TERMS == 3 || p.splits > 1) {
+                        float *to = p.splits > 1 ? parts : reinterpret_cast<float *>(out);
+                        *reinterpret_cast<float4 *>(to + col + 2 * c) = make_float4(x[c].x, x[c].y, x[c + 1].x, x[c + 1].y);
+                        if (col + 2 * c + 4 < p.D)
+                            *reinterpret_cast<float4 *>(to + col + 2 * c + 4) = make_float4(x[c + 2].x, x[c + 2].y, x[c + 3].x, x[c + 3].y);
+                    } else if constexpr (TERMS == 1) {
                         const float2 y[4] = {x[c], x[c + 1], x[c + 2], x[c + 3]};
                         *reinterpret_cast<uint4 *>(out + col + 2 * c) = VecTraits<T>::pack(y);
                     }
@@ -298,9 +327,12 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
                 const int stage = n % ST, turn = n / ST, state = (int)(tiles[n] & 0x7fffffff) * BN;
                 if (turn > 0) fine = barrier_wait(&sm.free[stage], (turn - 1) & 1);
                 if (!fine) break;
-                barrier_expect(&sm.full[stage], 2 * BN * DP * 2);
-                load_rows<DP, BN>(sm.k[stage], km, &sm.full[stage], b, h, state);
-                load_rows<DP, BN>(sm.v[stage], vm, &sm.full[stage], b, h, state);
+                barrier_expect(&sm.full[stage], 2 * TERMS * kTile);
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) {
+                    load_rows<DP, BN>(sm.k[stage][i], km, &sm.full[stage], b + i * p.B, h, state);
+                    load_rows<DP, BN>(sm.v[stage][i], vm, &sm.full[stage], b + i * p.B, h, state);
+                }
             }
             // nothing may still be on its way when the CTA ends
             for (int s = 0; s < ST && !fine; ++s) {
@@ -323,7 +355,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
                     const int stage = n % ST, last = (n + ST - KW) % ST;
                     if (scores) fine = fine && barrier_wait(&sm.full[stage], (n / ST) & 1);
                     if (weights && words != nullptr) fine = fine && barrier_wait(&sm.clean[last], ((n - KW) / ST) & 1);
-                    const uint32_t ka = k0 + stage * (BN * DP * 2 >> 4), va = v0 + last * (BN * DP * 2 >> 4);
+                    const uint32_t ka = k0 + stage * (TERMS * kTile >> 4), va = v0 + last * (TERMS * kTile >> 4);
 #pragma unroll
                     for (int q = 0; q < RT; ++q) {
                         const int group = w * RT + q;
@@ -333,16 +365,24 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
                             if (!fine) break;
                             fence_after();
 #pragma unroll
-                            for (int j = 0; j < BN; j += 16)
-                                mma_ts<kRow>(at + kO, at + j / 2, va + (j * kRow >> 4), kOut, round > 1 || j > 0);
+                            for (int i = kPairs - kPairsOf; i < kPairs; ++i) {
+#pragma unroll
+                                for (int j = 0; j < BN; j += 16)
+                                    mma_ts<kRow>(at + kO, at + left_term(i) * kP + j / 2, va + (right_term(i) * kTile + j * kRow >> 4), kOut,
+                                                 round > 1 || j > 0 || i > kPairs - kPairsOf);
+                            }
                             if (q == RT - 1) commit(&sm.free[last]);
                             if (!scores) commit(&sm.o_full[group]);
                         }
                         if (scores && fine) {
 #pragma unroll
-                            for (int d = 0; d < DP; d += 16)
-                                mma<kRow>(at, q0 + ((q * DP + (d & ~63)) * kTileRows * 2 + (d & 63) * 2 >> 4),
-                                          ka + ((d & ~63) * BN * 2 + (d & 63) * 2 >> 4), kScores, d > 0);
+                            for (int i = kPairs - kPairsOf; i < kPairs; ++i) {
+#pragma unroll
+                                for (int d = 0; d < DP; d += 16)
+                                    mma<kRow>(at, q0 + (((q * TERMS + left_term(i)) * DP + (d & ~63)) * kTileRows * 2 + (d & 63) * 2 >> 4),
+                                              ka + (right_term(i) * kTile + (d & ~63) * BN * 2 + (d & 63) * 2 >> 4), kScores,
+                                              d > 0 || i > kPairs - kPairsOf);
+                            }
                             commit(&sm.s_full[group]);
                         }
                     }
@@ -361,9 +401,12 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < NW; ++j)
                         for (int c = lane; c < 32 * kChunks; c += 32)
-                            if (!((see.w[j] >> (c / kChunks)) & 1))
-                                *reinterpret_cast<uint4 *>(sm.v[stage] + swizzled<DP, BN>(32 * j + c / kChunks, c % kChunks)) =
-                                    make_uint4(0, 0, 0, 0);
+                            if (!((see.w[j] >> (c / kChunks)) & 1)) {
+#pragma unroll
+                                for (int i = 0; i < TERMS; ++i)
+                                    *reinterpret_cast<uint4 *>(sm.v[stage][i] + swizzled<DP, BN>(32 * j + c / kChunks, c % kChunks)) =
+                                        make_uint4(0, 0, 0, 0);
+                            }
                     fence_async_shared();
                 }
                 barrier_arrive(&sm.clean[stage]);
@@ -378,15 +421,25 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW>::kThreads, 1)
     }
 }
 
-template <typename T, int DP, int RT, int KW>
+template <typename T, int DP, int RT, int KW, int TERMS = 1>
 cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
-    using Sh = Shape<DP, RT, KW>;
+    using Sh = Shape<DP, RT, KW, TERMS>;
     tc::TensorMap km, vm;
-    if (!tc::make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, 1, p.D, Sh::BN) ||
-        !tc::make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, 1, p.D, Sh::BN))
+    if constexpr (TERMS == 3) {
+        const int64_t D8 = (p.D + 7) / 8 * 8, dense[3] = {(int64_t)p.S * p.K * D8, p.K * D8, D8};
+        if (!tc::make_map<T, DP>(km, p.k_terms, dense, 3 * p.B, p.S, p.K, 1, (int)D8, Sh::BN) ||
+            !tc::make_map<T, DP>(vm, p.v_terms, dense, 3 * p.B, p.S, p.K, 1, (int)D8, Sh::BN))
+            return cudaErrorNotSupported;
+        cudaError_t e = launch_attention_terms(p.k, p.ks, p.B, p.S, p.K, p.D, p.k_terms, stream);
+        if (e == cudaSuccess) e = launch_attention_terms(p.v, p.vs, p.B, p.S, p.K, p.D, p.v_terms, stream);
+        if (e != cudaSuccess) return e;
+    } else if (!tc::make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, 1, p.D, Sh::BN) ||
+               !tc::make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, 1, p.D, Sh::BN)) {
         return cudaErrorNotSupported;
-    const auto kernel = attention_forward_tc_kernel<T, DP, RT, KW>;
-    constexpr size_t smem = sizeof(Shared<DP, RT, KW>);
+    }
+    const auto kernel = attention_forward_tc_kernel<T, DP, RT, KW, TERMS>;
+    constexpr size_t smem = sizeof(Shared<DP, RT, KW, TERMS>);
+    static_assert(smem <= 227 * 1024);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + RT * kTileRows - 1) / (RT * kTileRows));
@@ -402,10 +455,17 @@ cudaError_t launch_typed(const AttentionParams &p, int row_tiles, cudaStream_t s
     return row_tiles == 1 ? launch<T, 128, 1, 2>(p, stream) : launch<T, 128, 2, 1>(p, stream);
 }
 
+cudaError_t launch_float(const AttentionParams &p, int row_tiles, cudaStream_t stream) {
+    using T = __nv_bfloat16;
+    if (p.D <= 32) return row_tiles == 1 ? launch<T, 32, 1, 4, 3>(p, stream) : launch<T, 32, 2, 2, 3>(p, stream);
+    return row_tiles == 1 ? launch<T, 64, 1, 2, 3>(p, stream) : launch<T, 64, 2, 1, 3>(p, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream) {
-    return dtype == 1 ? launch_typed<__half>(p, row_tiles, stream) : launch_typed<__nv_bfloat16>(p, row_tiles, stream);
+    return dtype == 0 ? launch_float(p, row_tiles, stream)
+           : dtype == 1 ? launch_typed<__half>(p, row_tiles, stream) : launch_typed<__nv_bfloat16>(p, row_tiles, stream);
 }
 
 }  // namespace msda_b200
