@@ -36,7 +36,7 @@ struct Shape {
     static constexpr int kThreads = kGroups * 128 + 128;
     // columns of tensor memory: of a group S and T, in whose places P and dS come (third terms need more), then the sums
     static constexpr uint32_t kS = 0, kT = 64;
-    static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }
+    __host__ __device__ static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }
     static constexpr uint32_t kGroup = TERMS == 1 ? 128 : KEYS ? 192 : 160;
     static constexpr uint32_t kAcc0 = kGroups * kGroup, kAcc1 = KEYS ? kAcc0 + DP : kAcc0;
     static_assert(kAcc1 + DP <= 512);
@@ -53,7 +53,7 @@ struct Shared {
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
     uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
-    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full, acc_free;
+    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[4], acc_free;
     uint32_t tmem;
 };
 
@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             barrier_init(&sm.y_clean[s], 32);
             barrier_init(&sm.row_full[s], 32), barrier_init(&sm.row_free[s], 128);
         }
-        barrier_init(&sm.acc_full, 1), barrier_init(&sm.acc_free, 256);      // (two groups write the sums)
+        for (int s = 0; s < 4; ++s) barrier_init(&sm.acc_full[s], 1);
+        barrier_init(&sm.acc_free, 128);
     }
     if (y_rows < kY) {      // rows that no load reaches
         for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += kGroups * 128 + 128) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
@@ -298,51 +299,55 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 barrier_arrive(&sm.p_full[group]);
             }
             n = before + walk.count;
+            // The group that had the last tile writes the sums; its next tile is the furthest off, and the others go
+            // on with the next item.  (Four barriers in turn: a group that waits for one of them has to find the
+            // phase before over, and no more than three items are under way.)
             const bool some = walk.count > 0;
+            const int item = done;
+            if (some) ++done;
+            if (group != (some ? (n - 1) % kGroups : 0)) continue;
             if (some) {
-                fine = fine && barrier_wait(&sm.acc_full, done & 1);
+                fine = fine && barrier_wait(&sm.acc_full[item & 3], (item >> 2) & 1);
                 fence_after();
-                ++done;
             }
-            // sums to memory: two of the groups take one of the two each, or half of the one
-            if (group > 1) continue;
-            constexpr int kHalf = KEYS ? DP : DP / 2;
-            const uint32_t acc = tmem + lanes + (KEYS ? (group == 0 ? kAcc0 : kAcc1) : kAcc1 + group * kHalf);
-            const int from = KEYS ? 0 : group * kHalf;
-            const float factor = !fine ? NAN : KEYS && group == 0 ? 1.f : p.scale;
             const int rows = KEYS ? p.S : p.R;
             const int query = x / p.share;
             const int64_t at = KEYS ? (((int64_t)it.b * p.S + x) * p.K + it.h) * p.D
                                     : (((int64_t)it.b * p.Q + query) * p.K * p.share + it.h * p.share + (x - query * p.share)) * p.D;
-            Out *out = static_cast<Out *>(KEYS ? (group == 0 ? p.dv : p.dk) : p.dq) + at;
-            float *parts = (KEYS && group == 0 ? p.part2 : p.part) +
-                           ((it.part * (int64_t)p.B * p.K + it.bh) * rows + x) * p.D;
+            const int64_t part_at = ((it.part * (int64_t)p.B * p.K + it.bh) * rows + x) * p.D;
 #pragma unroll
-            for (int d = 0; d < kHalf; d += 16) {
-                uint32_t v[16];
-                if (some && !idle) {
-                    tmem_load16(v, acc + d);
-                    tmem_wait_load();
-                    loaded(v);
-                }
-                float2 y[8];
+            for (int which = KEYS ? 0 : 1; which < 2; ++which) {
+                const uint32_t acc = tmem + lanes + (which == 0 ? kAcc0 : kAcc1);
+                const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale;
+                Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
+                float *parts = (which == 0 ? p.part2 : p.part) + part_at;
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    y[c] = some ? make_float2(__uint_as_float(v[2 * c]) * factor, __uint_as_float(v[2 * c + 1]) * factor)
-                                : make_float2(0.f, 0.f);
-                if (!mine_valid) continue;
+                for (int d = 0; d < DP; d += 16) {
+                    uint32_t v[16];
+                    if (some && !idle) {
+                        tmem_load16(v, acc + d);
+                        tmem_wait_load();
+                        loaded(v);
+                    }
+                    float2 y[8];
 #pragma unroll
-                for (int c = 0; c < 8; c += 4) {
-                    const int col = from + d + 2 * c;
-                    if (col >= p.D) continue;
-                    if (TERMS == 3 || p.splits > 1) {
-                        float *to = p.splits > 1 ? parts : reinterpret_cast<float *>(out);
-                        *reinterpret_cast<float4 *>(to + col) = make_float4(y[c].x, y[c].y, y[c + 1].x, y[c + 1].y);
-                        if (col + 4 < p.D)
-                            *reinterpret_cast<float4 *>(to + col + 4) = make_float4(y[c + 2].x, y[c + 2].y, y[c + 3].x, y[c + 3].y);
-                    } else if constexpr (TERMS == 1) {
-                        const float2 z[4] = {y[c], y[c + 1], y[c + 2], y[c + 3]};
-                        *reinterpret_cast<uint4 *>(out + col) = VecTraits<T>::pack(z);
+                    for (int c = 0; c < 8; ++c)
+                        y[c] = some ? make_float2(__uint_as_float(v[2 * c]) * factor, __uint_as_float(v[2 * c + 1]) * factor)
+                                    : make_float2(0.f, 0.f);
+                    if (!mine_valid) continue;
+#pragma unroll
+                    for (int c = 0; c < 8; c += 4) {
+                        const int col = d + 2 * c;
+                        if (col >= p.D) continue;
+                        if (TERMS == 3 || p.splits > 1) {
+                            float *to = p.splits > 1 ? parts : reinterpret_cast<float *>(out);
+                            *reinterpret_cast<float4 *>(to + col) = make_float4(y[c].x, y[c].y, y[c + 1].x, y[c + 1].y);
+                            if (col + 4 < p.D)
+                                *reinterpret_cast<float4 *>(to + col + 4) = make_float4(y[c + 2].x, y[c + 2].y, y[c + 3].x, y[c + 3].y);
+                        } else if constexpr (TERMS == 1) {
+                            const float2 z[4] = {y[c], y[c + 1], y[c + 2], y[c + 3]};
+                            *reinterpret_cast<uint4 *>(out + col) = VecTraits<T>::pack(z);
+                        }
                     }
                 }
             }
@@ -458,7 +463,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         }
                     }
                     commit(&sm.y_free[stage]);
-                    if (t.last) commit(&sm.acc_full);
+                    if (t.last) commit(&sm.acc_full[t.item & 3]);
                 }
             };
             for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
