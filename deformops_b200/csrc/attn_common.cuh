@@ -90,9 +90,14 @@ struct Tiles {
             all = (int)__ldg(l + (BN == 128));
             list = l + 2 + (BN == 128 ? (S + 63) / 64 : 0);
         }
-        first = (int)((int64_t)part * all / p.splits);
-        count = (int)((int64_t)(part + 1) * all / p.splits) - first;
+        stretch(all, p.splits, part, first, count);
         if (list != nullptr) list += first;
+    }
+    // the part-th of `splits` nearly equal stretches
+    static __device__ __forceinline__ void stretch(int all, int splits, int part, int &first, int &count) {
+        const int each = all / splits, more = all - each * splits;
+        first = part * each + min(part, more);
+        count = each + (part < more);
     }
     // tile n of the stretch, bit 31 set where all of its states may be seen (by somebody)
     __device__ __forceinline__ uint32_t operator[](int n) const {

@@ -29,8 +29,8 @@ constexpr int kX = 128, kY = 64;
 
 template <int DP, bool KEYS, int TERMS>
 struct Shape {
-    static constexpr int ST = TERMS == 3 ? (DP == 32 ? 4 : 2) : DP == 128 ? 2 : 6;      // tiles Y in flight
-    static constexpr int XB = DP * TERMS > 128 ? 1 : 2;                                  // tiles X
+    static constexpr int ST = TERMS == 3 ? (DP == 32 ? 4 : 2) : DP == 128 ? 4 : 6;      // tiles Y in flight
+    static constexpr int XB = DP * TERMS > 96 ? 1 : 2;                                   // tiles X
     // warpgroups that take the tiles Y in turn: as many as tensor memory has room for
     static constexpr int kGroups = TERMS == 3 || DP == 128 ? 2 : 3;
     static constexpr int kThreads = kGroups * 128 + 128;
@@ -38,8 +38,9 @@ struct Shape {
     static constexpr uint32_t kS = 0, kT = 64;
     __host__ __device__ static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }
     static constexpr uint32_t kGroup = TERMS == 1 ? 128 : KEYS ? 192 : 160;
-    static constexpr uint32_t kAcc0 = kGroups * kGroup, kAcc1 = KEYS ? kAcc0 + DP : kAcc0;
-    static_assert(kAcc1 + DP <= 512);
+    static constexpr uint32_t kAcc = kGroups * kGroup, kSums = KEYS ? 2 * DP : DP;      // dv and dk, or dq
+    static constexpr int AB = kAcc + 2 * kSums <= 512 ? 2 : 1;                           // of as many items
+    static_assert(kAcc + AB * kSums <= 512);
     static_assert(ST >= kGroups);
 };
 
@@ -53,7 +54,7 @@ struct Shared {
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
     uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
-    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[4], acc_free;
+    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[4], acc_free[2];
     uint32_t tmem;
 };
 
@@ -64,13 +65,13 @@ struct Item {
 };
 
 // x_rows: rows that a tile takes (all of them for states; whole groups of heads for packed rows)
-__device__ __forceinline__ Item item_of(const AttentionParams &p, int64_t i, int x_tiles, int x_rows) {
+__device__ __forceinline__ Item item_of(const AttentionParams &p, unsigned i, unsigned x_tiles, int x_rows) {
     Item t;
-    t.first = (int)(i % x_tiles) * x_rows;
-    i /= x_tiles;
-    t.part = (int)(i % p.splits);
-    t.bh = i / p.splits;
-    t.b = (int)(t.bh / p.K), t.h = (int)(t.bh % p.K);
+    const unsigned j = i / x_tiles, bh = j / p.splits;
+    t.first = (int)(i - j * x_tiles) * x_rows;
+    t.part = (int)(j - bh * p.splits);
+    t.bh = bh;
+    t.b = (int)(bh / p.K), t.h = (int)(bh - t.b * p.K);
     return t;
 }
 
@@ -86,8 +87,7 @@ struct Walk<true> {
     int first, count;
     __device__ __forceinline__ Walk(const AttentionParams &p, const Item &t, int y_rows) {
         const int all = (p.R + y_rows - 1) / y_rows;
-        first = (int)((int64_t)t.part * all / p.splits);
-        count = (int)((int64_t)(t.part + 1) * all / p.splits) - first;
+        Tiles<kY>::stretch(all, p.splits, t.part, first, count);
         const uint32_t *words = key_words_of(p, t.b, t.h);
         if (words != nullptr) {
             const uint4 w = __ldg(reinterpret_cast<const uint4 *>(words + t.first / 32));
@@ -101,14 +101,15 @@ template <typename T, int DP, bool KEYS, int TERMS>
 __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     attention_backward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap x0m,
                                  const __grid_constant__ tc::TensorMap x1m, const __grid_constant__ tc::TensorMap y0m,
-                                 const __grid_constant__ tc::TensorMap y1m, int64_t items, int x_rows, int y_rows) {
+                                 const __grid_constant__ tc::TensorMap y1m, unsigned items, int x_rows, int y_rows) {
     using namespace tc;
     using Sh = Shape<DP, KEYS, TERMS>;
     using Out = std::conditional_t<TERMS == 3, float, T>;      // of the call's tensors; T is that of the products
     constexpr int ST = Sh::ST, XB = Sh::XB, kGroups = Sh::kGroups, kLast = 4 * kGroups;
     constexpr int kPairsOf = TERMS == 3 ? kPairs : 1;
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
-    constexpr uint32_t kS = Sh::kS, kT = Sh::kT, kGroup = Sh::kGroup, kAcc0 = Sh::kAcc0, kAcc1 = Sh::kAcc1;
+    constexpr int AB = Sh::AB;
+    constexpr uint32_t kS = Sh::kS, kT = Sh::kT, kGroup = Sh::kGroup;
     constexpr uint32_t kXBytes = kX * DP * 2, kYBytes = kY * DP * 2;
     extern __shared__ __align__(1024) unsigned char raw[];
     auto &sm = *reinterpret_cast<Shared<DP, KEYS, TERMS> *>(raw);
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             barrier_init(&sm.row_full[s], 32), barrier_init(&sm.row_free[s], 128);
         }
         for (int s = 0; s < 4; ++s) barrier_init(&sm.acc_full[s], 1);
-        barrier_init(&sm.acc_free, 128);
+        for (int s = 0; s < 2; ++s) barrier_init(&sm.acc_free[s], 128);
     }
     if (y_rows < kY) {      // rows that no load reaches
         for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += kGroups * 128 + 128) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-    const int x_tiles = ((KEYS ? p.S : p.R) + x_rows - 1) / x_rows;
+    const unsigned x_tiles = ((KEYS ? p.S : p.R) + x_rows - 1) / x_rows;
     bool fine = true;
 
     if (warp < kLast) {
@@ -154,8 +155,13 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 to[0][c] = VecTraits<T>::pack2(x);
             }
         };
-        int n = 0, done = 0;             // tiles and items with tiles so far
-        for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+        int before = 0, n = group;       // tiles of the items so far; this group's next one
+        Ring<ST> y;
+        Ring<4> full;                    // of items with tiles
+        Ring<AB> sums;
+        uint32_t turn = 0;               // parity of the group's tiles
+        y.next(group);
+        for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
             const Item it = item_of(p, i, x_tiles, x_rows);
             const Walk<KEYS> walk(p, it, y_rows);
             const uint32_t *words = key_words_of(p, it.b, it.h);
@@ -173,7 +179,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 rw = row_words_of(p, it.b, it.h, x);
             }
             const bool own_words = p.row_words != nullptr;
-            const int before = n;
             if (rw == nullptr) rw = words;
             uint32_t entry = 0;
             uint2 see = make_uint2(0, 0);
@@ -184,15 +189,14 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 if (rw != nullptr && (own_words || !(entry >> 31)))
                     see = __ldg(reinterpret_cast<const uint2 *>(rw) + (entry & 0x7fffffff));
             };
-            n += (group + kGroups - n % kGroups) % kGroups;
             if constexpr (!KEYS) fetch(n);
-            for (; fine && n < before + walk.count; n += kGroups) {
-                const int stage = n % ST;
+            for (; fine && n < before + walk.count; n += kGroups, y.next(kGroups), turn ^= 1) {
+                const int stage = y.at;
                 const uint32_t now = entry;
                 uint2 may = see;
                 if constexpr (!KEYS) fetch(n + kGroups);
-                if constexpr (KEYS) fine = barrier_wait(&sm.row_full[stage], (n / ST) & 1);
-                fine = barrier_wait(&sm.s_full[group], (n / kGroups) & 1) && fine;
+                if constexpr (KEYS) fine = barrier_wait(&sm.row_full[stage], y.parity);
+                fine = barrier_wait(&sm.s_full[group], turn) && fine;
                 if (!fine) break;
                 fence_after();
                 if (!idle) {
@@ -298,16 +302,17 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 fence_before();
                 barrier_arrive(&sm.p_full[group]);
             }
-            n = before + walk.count;
             // The group that had the last tile writes the sums; its next tile is the furthest off, and the others go
             // on with the next item.  (Four barriers in turn: a group that waits for one of them has to find the
             // phase before over, and no more than three items are under way.)
             const bool some = walk.count > 0;
-            const int item = done;
-            if (some) ++done;
-            if (group != (some ? (n - 1) % kGroups : 0)) continue;
+            before += walk.count;
+            const Ring<4> item = full;
+            const Ring<AB> buffer = sums;
+            if (some) full.next(), sums.next();
+            if (some ? n - kGroups != before - 1 : group != 0) continue;
             if (some) {
-                fine = fine && barrier_wait(&sm.acc_full[item & 3], (item >> 2) & 1);
+                fine = fine && barrier_wait(&sm.acc_full[item.at], item.parity);
                 fence_after();
             }
             const int rows = KEYS ? p.S : p.R;
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             const int64_t part_at = ((it.part * (int64_t)p.B * p.K + it.bh) * rows + x) * p.D;
 #pragma unroll
             for (int which = KEYS ? 0 : 1; which < 2; ++which) {
-                const uint32_t acc = tmem + lanes + (which == 0 ? kAcc0 : kAcc1);
+                const uint32_t acc = tmem + lanes + Sh::kAcc + buffer.at * Sh::kSums + (KEYS && which == 1 ? DP : 0);
                 const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale;
                 Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
                 float *parts = (which == 0 ? p.part2 : p.part) + part_at;
@@ -353,19 +358,21 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             }
             if (some) {
                 fence_before();
-                barrier_arrive(&sm.acc_free);
+                barrier_arrive(&sm.acc_free[buffer.at]);
             }
         }
     } else {
         registers_down<56>();
         if (warp == kLast && elect_one()) {
             int n = 0, done = 0;
-            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+            Ring<XB> x;
+            Ring<ST> y;
+            for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
                 const Item it = item_of(p, i, x_tiles, x_rows);
                 const Walk<KEYS> walk(p, it, y_rows);
                 if (walk.count == 0) continue;
-                const int buffer = done % XB;
-                if (done >= XB) fine = barrier_wait(&sm.x_free[buffer], (done / XB - 1) & 1);
+                const int buffer = x.at;
+                fine = barrier_wait(&sm.x_free[buffer], x.parity ^ 1);
                 if (!fine) break;
                 barrier_expect(&sm.x_full[buffer], 2 * TERMS * x_rows * DP * 2);
 #pragma unroll
@@ -373,10 +380,10 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                     load_rows<DP, kX>(sm.x[buffer][0][k], x0m, &sm.x_full[buffer], it.b + k * p.B, it.h, it.first);
                     load_rows<DP, kX>(sm.x[buffer][1][k], x1m, &sm.x_full[buffer], it.b + k * p.B, it.h, it.first);
                 }
-                ++done;
-                for (int j = 0; fine && j < walk.count; ++j, ++n) {
-                    const int stage = n % ST, row = (int)(walk[j] & 0x7fffffff) * y_rows;
-                    if (n >= ST) fine = barrier_wait(&sm.y_free[stage], (n / ST - 1) & 1);
+                ++done, x.next();
+                for (int j = 0; fine && j < walk.count; ++j, ++n, y.next()) {
+                    const int stage = y.at, row = (int)(walk[j] & 0x7fffffff) * y_rows;
+                    fine = barrier_wait(&sm.y_free[stage], y.parity ^ 1);
                     if (!fine) break;
                     barrier_expect(&sm.y_full[stage], 2 * TERMS * y_rows * DP * 2);
 #pragma unroll
@@ -394,12 +401,12 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             }
         } else if (warp == kLast + 2 && KEYS) {
             // what the walked rows need beside their tiles
-            int n = 0;
-            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+            Ring<ST> y;
+            for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
                 const Item it = item_of(p, i, x_tiles, x_rows);
                 const Walk<KEYS> walk(p, it, y_rows);
-                for (int j = 0; fine && j < walk.count; ++j, ++n) {
-                    const int stage = n % ST, tile = (int)walk[j];
+                for (int j = 0; fine && j < walk.count; ++j, y.next()) {
+                    const int stage = y.at, tile = (int)walk[j];
                     float lse[2], delta[2];
                     uint4 see[2];
 #pragma unroll
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                             see[c] = valid ? __ldg(reinterpret_cast<const uint4 *>(row_words_of(p, it.b, it.h, r) + it.first / 32))
                                            : make_uint4(0, 0, 0, 0);
                     }
-                    if (n >= ST) fine = barrier_wait(&sm.row_free[stage], (n / ST - 1) & 1);
+                    fine = barrier_wait(&sm.row_free[stage], y.parity ^ 1);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int col = lane + 32 * c;
@@ -428,29 +435,38 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             }
         } else if (warp == kLast + 1 && elect_one()) {
             constexpr uint32_t kScores = instruction(kBf16, kX, kY, false, false);
-            constexpr uint32_t kSums = instruction(kBf16, kX, DP, false, true);
+            constexpr uint32_t kGradients = instruction(kBf16, kX, DP, false, true);
             constexpr int kRow = kRowBytes<DP>;
             const uint32_t x0 = descriptor(smem_address(sm.x), 16), y0 = descriptor(smem_address(sm.y), 16),
                            z0 = descriptor(smem_address(sm.y), kY * 128);
             // Tiles whose products with P and dS are still to be issued, one fewer than there are groups: the scores
             // of a tile take the place of what the oldest one's products have read.
             struct Pending {
-                int n, item;
+                int group, acc_full;
+                uint32_t turn;
+                Ring<ST> y;
+                Ring<AB> sums;
                 bool first, last;
             } queue[kGroups - 1] = {};
-            int waiting = 0, n = 0, done = 0;
+            int waiting = 0;
+            Ring<XB> x;
+            Ring<ST> y;
+            Ring<kGroups> groups;
+            Ring<AB> sums;
+            int acc_full = 0;
             const auto issue_sums = [&] {
                 const Pending t = queue[0];
 #pragma unroll
                 for (int i = 0; i + 1 < kGroups - 1; ++i) queue[i] = queue[i + 1];
                 --waiting;
-                const int group = t.n % kGroups, stage = t.n % ST;
-                if (t.first && t.item > 0) fine = fine && barrier_wait(&sm.acc_free, (t.item - 1) & 1);
-                if (!KEYS && p.key_words != nullptr) fine = fine && barrier_wait(&sm.y_clean[stage], (t.n / ST) & 1);
-                fine = fine && barrier_wait(&sm.p_full[group], (t.n / kGroups) & 1);
+                const int group = t.group, stage = t.y.at;
+                if (t.first) fine = fine && barrier_wait(&sm.acc_free[t.sums.at], t.sums.parity ^ 1);
+                if (!KEYS && p.key_words != nullptr) fine = fine && barrier_wait(&sm.y_clean[stage], t.y.parity);
+                fine = fine && barrier_wait(&sm.p_full[group], t.turn);
                 fence_after();
                 if (fine) {
                     const uint32_t from = tmem + group * kGroup, za = z0 + stage * (2 * TERMS * kYBytes >> 4);
+                    const uint32_t acc = tmem + Sh::kAcc + t.sums.at * Sh::kSums;
 #pragma unroll
                     for (int k = kPairs - kPairsOf; k < kPairs; ++k) {
                         const bool add = !t.first || k > kPairs - kPairsOf;
@@ -458,24 +474,23 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         for (int j = 0; j < kY; j += 16) {
                             const uint32_t of = right_term(k) * kYBytes + j * kRow;
                             if constexpr (KEYS)
-                                mma_ts<kRow>(tmem + kAcc0, from + (left_term(k) == 2 ? Sh::third(true) : kS + 32 * left_term(k)) + j / 2, za + (TERMS * kYBytes + of >> 4), kSums, add || j > 0);
-                            mma_ts<kRow>(tmem + kAcc1, from + (left_term(k) == 2 ? Sh::third(false) : kT + 32 * left_term(k)) + j / 2, za + (of >> 4), kSums, add || j > 0);
+                                mma_ts<kRow>(acc, from + (left_term(k) == 2 ? Sh::third(true) : kS + 32 * left_term(k)) + j / 2, za + (TERMS * kYBytes + of >> 4), kGradients, add || j > 0);
+                            mma_ts<kRow>(acc + (KEYS ? DP : 0), from + (left_term(k) == 2 ? Sh::third(false) : kT + 32 * left_term(k)) + j / 2, za + (of >> 4), kGradients, add || j > 0);
                         }
                     }
                     commit(&sm.y_free[stage]);
-                    if (t.last) commit(&sm.acc_full[t.item & 3]);
+                    if (t.last) commit(&sm.acc_full[t.acc_full]);
                 }
             };
-            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+            for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
                 const Item it = item_of(p, i, x_tiles, x_rows);
                 const Walk<KEYS> walk(p, it, y_rows);
                 if (walk.count == 0) continue;
-                const int buffer = done % XB;
-                fine = barrier_wait(&sm.x_full[buffer], (done / XB) & 1);
-                for (int j = 0; fine && j < walk.count; ++j, ++n) {
-                    const bool first = j == 0;
-                    const int stage = n % ST, group = n % kGroups;
-                    fine = barrier_wait(&sm.y_full[stage], (n / ST) & 1);
+                const int buffer = x.at;
+                fine = barrier_wait(&sm.x_full[buffer], x.parity);
+                for (int j = 0; fine && j < walk.count; ++j, y.next(), groups.next()) {
+                    const int stage = y.at, group = groups.at;
+                    fine = barrier_wait(&sm.y_full[stage], y.parity);
                     if (fine) {
                         const uint32_t to = tmem + group * kGroup;
                         const uint32_t xa = x0 + buffer * (2 * TERMS * kXBytes >> 4), ya = y0 + stage * (2 * TERMS * kYBytes >> 4);
@@ -495,25 +510,25 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         if (j == walk.count - 1) commit(&sm.x_free[buffer]);
                     }
                     if (waiting == kGroups - 1) issue_sums();
-                    const Pending t = {n, done, first, j == walk.count - 1};
+                    const Pending t = {group, acc_full, groups.parity, y, sums, j == 0, j == walk.count - 1};
                     if (kGroups == 2 || waiting == 0) queue[0] = t; else queue[kGroups - 2] = t;
                     ++waiting;
                 }
-                ++done;
+                x.next(), sums.next(), acc_full = (acc_full + 1) & 3;
             }
             while (fine && waiting > 0) issue_sums();
         } else if (warp == kLast + 3 && !KEYS && p.key_words != nullptr) {
             // rows of k that nobody may see: their dS is 0 and its products have to be
-            int n = 0;
-            for (int64_t i = blockIdx.x; fine && i < items; i += gridDim.x) {
+            Ring<ST> y;
+            for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
                 const Item it = item_of(p, i, x_tiles, x_rows);
                 const Walk<KEYS> walk(p, it, y_rows);
                 const uint32_t *words = key_words_of(p, it.b, it.h);
-                for (int j = 0; fine && j < walk.count; ++j, ++n) {
+                for (int j = 0; fine && j < walk.count; ++j, y.next()) {
                     const uint32_t entry = walk[j];
-                    const int stage = n % ST;
+                    const int stage = y.at;
                     // (whether their scores are formed before or after makes no difference: they are masked)
-                    fine = barrier_wait(&sm.y_full[stage], (n / ST) & 1);
+                    fine = barrier_wait(&sm.y_full[stage], y.parity);
                     if (fine && !(entry >> 31)) {
                         const uint2 see = __ldg(reinterpret_cast<const uint2 *>(words) + entry);
                         constexpr int kChunks = DP / 8;
@@ -568,9 +583,10 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     const int rows = row_tile / p.share * p.share;
     const int x_rows = KEYS ? kX : rows, y_rows = KEYS ? rows : kY;
     const int64_t items = (int64_t)p.B * p.K * p.splits * (((KEYS ? p.S : p.R) + x_rows - 1) / x_rows);
+    if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const unsigned grid = (unsigned)std::min<int64_t>(items, 148);
-    kernel<<<grid, Shape<DP, KEYS, TERMS>::kThreads, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v, items,
-                                                                     x_rows, y_rows);
+    kernel<<<grid, Shape<DP, KEYS, TERMS>::kThreads, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v,
+                                                                     (unsigned)items, x_rows, y_rows);
     return cudaGetLastError();
 }
 

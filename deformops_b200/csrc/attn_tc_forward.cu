@@ -96,12 +96,10 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     const int row_tiles = (p.R + RT * kTileRows - 1) / (RT * kTileRows);
-    int64_t i = blockIdx.x;
-    const int first = (int)(i % row_tiles) * RT * kTileRows;
-    i /= row_tiles;
-    const int part = (int)(i % p.splits);
-    const int64_t bh = i / p.splits;
-    const int b = (int)(bh / p.K), h = (int)(bh % p.K);
+    const unsigned outer = blockIdx.x / row_tiles, of = outer / p.splits;
+    const int first = (int)(blockIdx.x - outer * row_tiles) * RT * kTileRows, part = (int)(outer - of * p.splits);
+    const int64_t bh = of;
+    const int b = (int)(of / p.K), h = (int)(of - b * p.K);
     const uint32_t *words = key_words_of(p, b, h);
     const Tiles<BN> tiles(p, b, h, part);
 
@@ -323,9 +321,10 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
         registers_down<Sh::kFew>();
         if (warp == kLast && elect_one()) {
             int n = 0;
-            for (; fine && n < tiles.count; ++n) {
-                const int stage = n % ST, turn = n / ST, state = (int)(tiles[n] & 0x7fffffff) * BN;
-                if (turn > 0) fine = barrier_wait(&sm.free[stage], (turn - 1) & 1);
+            Ring<ST> ring;
+            for (; fine && n < tiles.count; ++n, ring.next()) {
+                const int stage = ring.at, state = (int)(tiles[n] & 0x7fffffff) * BN;
+                fine = barrier_wait(&sm.free[stage], ring.parity ^ 1);
                 if (!fine) break;
                 barrier_expect(&sm.full[stage], 2 * TERMS * kTile);
 #pragma unroll
@@ -348,13 +347,16 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
             const uint32_t q0 = descriptor(smem_address(sm.q), 16), k0 = descriptor(smem_address(sm.k), 16),
                            v0 = descriptor(smem_address(sm.v), BN * 128);
             int n = 0;
+            Ring<ST> now, then;                // of tiles n and n - KW
             for (int round = 0; fine && n < tiles.count + KW; ++round) {
 #pragma unroll
                 for (int w = 0; w < KW; ++w, ++n) {
-                    const bool scores = n < tiles.count, weights = n >= KW && n - KW < tiles.count;
-                    const int stage = n % ST, last = (n + ST - KW) % ST;
-                    if (scores) fine = fine && barrier_wait(&sm.full[stage], (n / ST) & 1);
-                    if (weights && words != nullptr) fine = fine && barrier_wait(&sm.clean[last], ((n - KW) / ST) & 1);
+                    const bool scores = n < tiles.count, weights = round > 0 && n - KW < tiles.count;
+                    const int stage = now.at, last = then.at;
+                    if (scores) fine = fine && barrier_wait(&sm.full[stage], now.parity);
+                    if (weights && words != nullptr) fine = fine && barrier_wait(&sm.clean[last], then.parity);
+                    now.next();
+                    if (round > 0) then.next();
                     const uint32_t ka = k0 + stage * (TERMS * kTile >> 4), va = v0 + last * (TERMS * kTile >> 4);
 #pragma unroll
                     for (int q = 0; q < RT; ++q) {
@@ -390,10 +392,11 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
             }
         } else if (warp == kLast + 2 && words != nullptr) {
             // rows of v that nobody may see: whatever they hold, their weight is 0 and has to stay it
-            for (int n = 0; fine && n < tiles.count; ++n) {
+            Ring<ST> ring;
+            for (int n = 0; fine && n < tiles.count; ++n, ring.next()) {
                 const uint32_t entry = tiles[n];
-                const int stage = n % ST;
-                fine = barrier_wait(&sm.full[stage], (n / ST) & 1);
+                const int stage = ring.at;
+                fine = barrier_wait(&sm.full[stage], ring.parity);
                 if (fine && !(entry >> 31)) {
                     Words<NW> see;
                     see.load(words, entry);

@@ -72,6 +72,18 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *bar, uint32_t parity) {
     return done != 0;
 }
 
+// Where one walks in a ring of SIZE barriers, and the parity of its round there.  Whoever waits for places to be free
+// waits for the other parity: before the first round that is over.
+template <int SIZE>
+struct Ring {
+    int at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next(int steps = 1) {
+        at += steps;
+        if (at >= SIZE) at -= SIZE, parity ^= 1;
+    }
+};
+
 // plain stores to shared memory, before the asynchronous units read them
 __device__ __forceinline__ void fence_async_shared() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
