@@ -33,7 +33,9 @@ struct Shape {
     static constexpr int XB = DP * TERMS > 96 ? 1 : 2;                                   // tiles X
     // warpgroups that take the tiles Y in turn: as many as tensor memory has room for
     static constexpr int kGroups = TERMS == 3 || DP == 128 ? 2 : 3;
-    static constexpr int kThreads = kGroups * 128 + 128;
+    static constexpr int kThreads = kGroups * 128 + 256;
+    // what a thread may hold: all of the block's at launch, shared out anew
+    static constexpr int kRegisters = kGroups == 3 ? 120 : 192, kFew = 56, kWriting = 64;
     // columns of tensor memory: of a group S and T, in whose places P and dS come (third terms need more), then the sums
     static constexpr uint32_t kS = 0, kT = 64;
     __host__ __device__ static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }
@@ -54,7 +56,7 @@ struct Shared {
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
     uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
-    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[4], acc_free[2];
+    uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[2], acc_free[2];
     uint32_t tmem;
 };
 
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     using namespace tc;
     using Sh = Shape<DP, KEYS, TERMS>;
     using Out = std::conditional_t<TERMS == 3, float, T>;      // of the call's tensors; T is that of the products
-    constexpr int ST = Sh::ST, XB = Sh::XB, kGroups = Sh::kGroups, kLast = 4 * kGroups;
+    constexpr int ST = Sh::ST, XB = Sh::XB, kGroups = Sh::kGroups, kLast = 4 * kGroups, kWriters = kLast + 4;
     constexpr int kPairsOf = TERMS == 3 ? kPairs : 1;
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     constexpr int AB = Sh::AB;
@@ -126,11 +128,10 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             barrier_init(&sm.y_clean[s], 32);
             barrier_init(&sm.row_full[s], 32), barrier_init(&sm.row_free[s], 128);
         }
-        for (int s = 0; s < 4; ++s) barrier_init(&sm.acc_full[s], 1);
-        for (int s = 0; s < 2; ++s) barrier_init(&sm.acc_free[s], 128);
+        for (int s = 0; s < 2; ++s) barrier_init(&sm.acc_full[s], 1), barrier_init(&sm.acc_free[s], 128);
     }
     if (y_rows < kY) {      // rows that no load reaches
-        for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += kGroups * 128 + 128) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += Sh::kThreads) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
         fence_async_shared();
     }
     fence_before();
@@ -141,11 +142,11 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     bool fine = true;
 
     if (warp < kLast) {
-        registers_up<kGroups == 2 ? 224 : 152>();
+        registers_up<Sh::kRegisters>();
         const int group = warp >> 2, row = threadIdx.x & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const uint32_t mine = tmem + group * kGroup + lanes;
+        const uint32_t mine = tmem + group * kGroup + ((uint32_t)(warp & 3) << 21);
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+        const bool own_words = p.row_words != nullptr;
         const auto put = [](float2 x, uint32_t (&to)[TERMS][16], int c) {
             if constexpr (TERMS == 3) {
                 uint32_t t[3];
@@ -157,8 +158,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
         };
         int before = 0, n = group;       // tiles of the items so far; this group's next one
         Ring<ST> y;
-        Ring<4> full;                    // of items with tiles
-        Ring<AB> sums;
         uint32_t turn = 0;               // parity of the group's tiles
         y.next(group);
         for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
@@ -178,7 +177,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 my_delta = -p.delta[it.bh * p.R + x];
                 rw = row_words_of(p, it.b, it.h, x);
             }
-            const bool own_words = p.row_words != nullptr;
             if (rw == nullptr) rw = words;
             uint32_t entry = 0;
             uint2 see = make_uint2(0, 0);
@@ -193,105 +191,106 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             for (; fine && n < before + walk.count; n += kGroups, y.next(kGroups), turn ^= 1) {
                 const int stage = y.at;
                 const uint32_t now = entry;
-                uint2 may = see;
+                const uint2 may = see;
                 if constexpr (!KEYS) fetch(n + kGroups);
                 if constexpr (KEYS) fine = barrier_wait(&sm.row_full[stage], y.parity);
                 fine = barrier_wait(&sm.s_full[group], turn) && fine;
                 if (!fine) break;
                 fence_after();
                 if (!idle) {
-                    uint32_t s[2][32], t[32];
-                    tmem_load32(s[0], mine + kS), tmem_load32(s[1], mine + kS + 32);
-                    tmem_wait_load();
-                    loaded(s[0]), loaded(s[1]);
-                    tmem_load32(t, mine + kT);
-                    float2 w[32];
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const uint32_t *from = &s[c >> 4][(2 * c) & 31];
-                        float4 l = make_float4(my_lse, my_lse, my_lse, my_lse);
-                        if constexpr (KEYS) l = *reinterpret_cast<const float4 *>(&sm.lse[stage][2 * c]);
-                        w[c] = fma2(make_float2(__uint_as_float(from[0]), __uint_as_float(from[1])), scale2, make_float2(l.x, l.y));
-                        w[c + 1] = fma2(make_float2(__uint_as_float(from[2]), __uint_as_float(from[3])), scale2, make_float2(l.z, l.w));
-                        w[c].x = fast_exp2(w[c].x), w[c].y = fast_exp2(w[c].y);
-                        w[c + 1].x = fast_exp2(w[c + 1].x), w[c + 1].y = fast_exp2(w[c + 1].y);
-                    }
+                    uint32_t s[32], t[32];
+                    tmem_load32(s, mine + kS);
                     // which of the 64 may be seen; `some` where not all of the warp's are
                     const bool some = KEYS ? own_words || !__all_sync(0xffffffffu, seen)
                                       : own_words ? !__all_sync(0xffffffffu, (may.x & may.y) == 0xffffffffu) : !(now >> 31);
-                    uint32_t see0 = may.x, see1 = may.y;
+                    uint32_t sees[2] = {may.x, may.y};
                     if (some) {
-                        if constexpr (!KEYS)
-                            if (rw == nullptr) {
-                                see0 = key_word(nullptr, p.S, 2 * (now & 0x7fffffff));
-                                see1 = key_word(nullptr, p.S, 2 * (now & 0x7fffffff) + 1);
-                            }
                         if constexpr (KEYS) {
-                            see0 = see1 = seen ? 0xffffffffu : 0u;
+                            sees[0] = sees[1] = seen ? 0xffffffffu : 0u;
                             if (own_words) {
-                                see0 = see1 = 0;
                                 const uint32_t *of = sm.words[stage][warp & 3];
+                                sees[0] = sees[1] = 0;
 #pragma unroll
                                 for (int c = 0; c < 32; ++c) {
-                                    see0 |= ((of[c] >> lane) & 1u) << c;
-                                    see1 |= ((of[32 + c] >> lane) & 1u) << c;
+                                    sees[0] |= ((of[c] >> lane) & 1u) << c;
+                                    sees[1] |= ((of[32 + c] >> lane) & 1u) << c;
                                 }
                             }
-                        }
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const uint32_t bits = c < 16 ? see0 >> (2 * c) : see1 >> (2 * c - 32);
-                            if (!(bits & 1)) w[c].x = 0.f;
-                            if (!(bits & 2)) w[c].y = 0.f;
+                        } else if (rw == nullptr) {
+                            sees[0] = key_word(nullptr, p.S, 2 * (now & 0x7fffffff));
+                            sees[1] = key_word(nullptr, p.S, 2 * (now & 0x7fffffff) + 1);
                         }
                     }
-                    if constexpr (KEYS) {
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            uint32_t packed[TERMS][16];
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) put(w[16 * half + c], packed, c);
-                            tmem_store16(mine + kS + 16 * half, packed[0]);
-                            if constexpr (TERMS == 3) {
-                                tmem_store16(mine + kS + 32 + 16 * half, packed[1]);
-                                tmem_store16(mine + Sh::third(true) + 16 * half, packed[TERMS - 1]);
-                            }
-                        }
-                    }
-                    // The first half of dS takes the place of a quarter of T that is in registers by then.  With three
-                    // terms its second one would take T's second half: that is kept back.
-                    uint32_t second[16];
+                    // Half by half, loads under the work on what came before.  What is stored takes the place of
+                    // columns that are in registers by then: P that of S's first half, dS that of T's; their second
+                    // terms would take the second halves, and wait for those.
+                    uint32_t second[TERMS == 3 ? 16 : 1], later[TERMS == 3 ? 16 : 1];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        if (half == 1) tmem_load32(t, mine + kT + 32);
                         tmem_wait_load();
-                        loaded(t);
-                        uint32_t packed[TERMS][16];
+                        loaded(s);
+                        tmem_load32(t, mine + kT + 32 * half);
+                        float2 w[16];
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
-                            const int at = 16 * half + c;
-                            float4 d = make_float4(my_delta, my_delta, my_delta, my_delta);
-                            if constexpr (KEYS) d = *reinterpret_cast<const float4 *>(&sm.delta[stage][2 * at]);
-                            float2 x = fmul2(w[at], add2(make_float2(__uint_as_float(t[2 * c]), __uint_as_float(t[2 * c + 1])), make_float2(d.x, d.y)));
-                            float2 y = fmul2(w[at + 1], add2(make_float2(__uint_as_float(t[2 * c + 2]), __uint_as_float(t[2 * c + 3])), make_float2(d.z, d.w)));
-                            if (some) {
-                                // (0 times what an unseen state's v holds)
-                                const uint32_t bits = half == 0 ? see0 >> (2 * c) : see1 >> (2 * c);
-                                if (!(bits & 1)) x.x = 0.f;
-                                if (!(bits & 2)) x.y = 0.f;
-                                if (!(bits & 4)) y.x = 0.f;
-                                if (!(bits & 8)) y.y = 0.f;
-                            }
-                            put(x, packed, c), put(y, packed, c + 1);
+                            float4 l = make_float4(my_lse, my_lse, my_lse, my_lse);
+                            if constexpr (KEYS) l = *reinterpret_cast<const float4 *>(&sm.lse[stage][32 * half + 2 * c]);
+                            w[c] = fma2(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, make_float2(l.x, l.y));
+                            w[c + 1] = fma2(make_float2(__uint_as_float(s[2 * c + 2]), __uint_as_float(s[2 * c + 3])), scale2, make_float2(l.z, l.w));
+                            w[c].x = fast_exp2(w[c].x), w[c].y = fast_exp2(w[c].y);
+                            w[c + 1].x = fast_exp2(w[c + 1].x), w[c + 1].y = fast_exp2(w[c + 1].y);
                         }
+                        if (some) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                if (!((sees[half] >> (2 * c)) & 1)) w[c].x = 0.f;
+                                if (!((sees[half] >> (2 * c)) & 2)) w[c].y = 0.f;
+                            }
+                        }
+                        uint32_t packed[TERMS][16];
+                        if constexpr (KEYS) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) put(w[c], packed, c);
+                            if constexpr (TERMS == 3) {
+                                if (half == 0) {
+#pragma unroll
+                                    for (int c = 0; c < 16; ++c) second[c] = packed[1][c];
+                                } else {
+                                    tmem_store16(mine + kS + 32, second);
+                                    tmem_store16(mine + kS + 48, packed[1]);
+                                }
+                                tmem_store16(mine + Sh::third(true) + 16 * half, packed[TERMS - 1]);
+                            }
+                            tmem_store16(mine + kS + 16 * half, packed[0]);
+                        }
+                        tmem_wait_load();
+                        loaded(t);
+                        if (half == 0) tmem_load32(s, mine + kS + 32);
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) {
+                            float4 d = make_float4(my_delta, my_delta, my_delta, my_delta);
+                            if constexpr (KEYS) d = *reinterpret_cast<const float4 *>(&sm.delta[stage][32 * half + 2 * c]);
+                            w[c] = fmul2(w[c], add2(make_float2(__uint_as_float(t[2 * c]), __uint_as_float(t[2 * c + 1])), make_float2(d.x, d.y)));
+                            w[c + 1] = fmul2(w[c + 1], add2(make_float2(__uint_as_float(t[2 * c + 2]), __uint_as_float(t[2 * c + 3])), make_float2(d.z, d.w)));
+                        }
+                        if (some) {
+                            // (0 times what an unseen state's v holds)
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                if (!((sees[half] >> (2 * c)) & 1)) w[c].x = 0.f;
+                                if (!((sees[half] >> (2 * c)) & 2)) w[c].y = 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) put(w[c], packed, c);
                         tmem_store16(mine + kT + 16 * half, packed[0]);
                         if constexpr (TERMS == 3) {
                             tmem_store16(mine + Sh::third(false) + 16 * half, packed[TERMS - 1]);
                             if (half == 0) {
 #pragma unroll
-                                for (int c = 0; c < 16; ++c) second[c] = packed[1][c];
+                                for (int c = 0; c < 16; ++c) later[c] = packed[1][c];
                             } else {
-                                tmem_store16(mine + kT + 32, second);
+                                tmem_store16(mine + kT + 32, later);
                                 tmem_store16(mine + kT + 48, packed[1]);
                             }
                         }
@@ -302,27 +301,32 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 fence_before();
                 barrier_arrive(&sm.p_full[group]);
             }
-            // The group that had the last tile writes the sums; its next tile is the furthest off, and the others go
-            // on with the next item.  (Four barriers in turn: a group that waits for one of them has to find the
-            // phase before over, and no more than three items are under way.)
-            const bool some = walk.count > 0;
             before += walk.count;
-            const Ring<4> item = full;
-            const Ring<AB> buffer = sums;
-            if (some) full.next(), sums.next();
-            if (some ? n - kGroups != before - 1 : group != 0) continue;
+        }
+    } else if (warp >= kWriters) {
+        // sums to memory, while the next item is worked on
+        registers_down<Sh::kWriting>();
+        const int row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        Ring<AB> sums;
+        for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
+            const Item it = item_of(p, i, x_tiles, x_rows);
+            const Walk<KEYS> walk(p, it, y_rows);
+            const bool some = walk.count > 0;
             if (some) {
-                fine = fine && barrier_wait(&sm.acc_full[item.at], item.parity);
+                fine = barrier_wait(&sm.acc_full[sums.at], sums.parity);
                 fence_after();
             }
-            const int rows = KEYS ? p.S : p.R;
+            const int rows = KEYS ? p.S : p.R, x = it.first + row;
+            const bool valid = row < x_rows && x < rows;
+            const bool idle = (row & ~31) >= x_rows || it.first + (row & ~31) >= rows;
             const int query = x / p.share;
             const int64_t at = KEYS ? (((int64_t)it.b * p.S + x) * p.K + it.h) * p.D
                                     : (((int64_t)it.b * p.Q + query) * p.K * p.share + it.h * p.share + (x - query * p.share)) * p.D;
             const int64_t part_at = ((it.part * (int64_t)p.B * p.K + it.bh) * rows + x) * p.D;
 #pragma unroll
             for (int which = KEYS ? 0 : 1; which < 2; ++which) {
-                const uint32_t acc = tmem + lanes + Sh::kAcc + buffer.at * Sh::kSums + (KEYS && which == 1 ? DP : 0);
+                const uint32_t acc = tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + (KEYS && which == 1 ? DP : 0);
                 const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale;
                 Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
                 float *parts = (which == 0 ? p.part2 : p.part) + part_at;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                     for (int c = 0; c < 8; ++c)
                         y[c] = some ? make_float2(__uint_as_float(v[2 * c]) * factor, __uint_as_float(v[2 * c + 1]) * factor)
                                     : make_float2(0.f, 0.f);
-                    if (!mine_valid) continue;
+                    if (!valid) continue;
 #pragma unroll
                     for (int c = 0; c < 8; c += 4) {
                         const int col = d + 2 * c;
@@ -358,11 +362,12 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             }
             if (some) {
                 fence_before();
-                barrier_arrive(&sm.acc_free[buffer.at]);
+                barrier_arrive(&sm.acc_free[sums.at]);
+                sums.next();
             }
         }
     } else {
-        registers_down<56>();
+        registers_down<Sh::kFew>();
         if (warp == kLast && elect_one()) {
             int n = 0, done = 0;
             Ring<XB> x;
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             // Tiles whose products with P and dS are still to be issued, one fewer than there are groups: the scores
             // of a tile take the place of what the oldest one's products have read.
             struct Pending {
-                int group, acc_full;
+                int group;
                 uint32_t turn;
                 Ring<ST> y;
                 Ring<AB> sums;
@@ -453,7 +458,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             Ring<ST> y;
             Ring<kGroups> groups;
             Ring<AB> sums;
-            int acc_full = 0;
             const auto issue_sums = [&] {
                 const Pending t = queue[0];
 #pragma unroll
@@ -479,7 +483,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         }
                     }
                     commit(&sm.y_free[stage]);
-                    if (t.last) commit(&sm.acc_full[t.acc_full]);
+                    if (t.last) commit(&sm.acc_full[t.sums.at]);
                 }
             };
             for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
@@ -510,11 +514,11 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         if (j == walk.count - 1) commit(&sm.x_free[buffer]);
                     }
                     if (waiting == kGroups - 1) issue_sums();
-                    const Pending t = {group, acc_full, groups.parity, y, sums, j == 0, j == walk.count - 1};
+                    const Pending t = {group, groups.parity, y, sums, j == 0, j == walk.count - 1};
                     if (kGroups == 2 || waiting == 0) queue[0] = t; else queue[kGroups - 2] = t;
                     ++waiting;
                 }
-                x.next(), sums.next(), acc_full = (acc_full + 1) & 3;
+                x.next(), sums.next();
             }
             while (fine && waiting > 0) issue_sums();
         } else if (warp == kLast + 3 && !KEYS && p.key_words != nullptr) {
