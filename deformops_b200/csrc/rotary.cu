@@ -2,13 +2,14 @@
 //
 //   (a, b) -> (a cos - b sin, a sin + b cos),   angle = position of the pair's axis * its frequency
 //
-// One pass over x.  A CTA takes a few tokens: first it forms the sine and cosine of every (token, pair),
-// once for all heads, then its threads turn 16-byte vectors of both halves of the pairs.  Angles
-// are formed in 64 bits as turns and reduced to [-1/2, 1/2] before anything is rounded to 32: at
-// position 10^6 a 32-bit angle is 0.03 off.  (float64 multiplies run at half the float32 rate here and
-// there is one for each of G * D / pairs channels.)  The backward pass is the same kernel with the
-// angles' sign turned.
+// One pass over x, bound by its bytes.  A CTA takes a few tokens of a sample: its threads ask for the vectors that
+// they will turn (both halves of the pairs), form the sine and cosine of every (token, pair) once for all heads
+// while those are on their way, and turn them.  Angles are formed in 64 bits as turns and reduced to [-1/2, 1/2]
+// before anything is rounded to 32: at position 10^6 a 32-bit angle is 0.03 off.  (float64 multiplies run at half
+// the float32 rate here and there is one for each of G * D / pairs channels.)  The backward pass is the same
+// kernel with the angles' sign turned.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/msda_b200.h"
 #include "msda_common.cuh"
@@ -19,13 +20,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostPairs = 128;
+constexpr int kInFlight = 2;          // pairs of vectors that a thread asks for at a time
 
 struct RotaryParams {
     const void *x, *positions;
     void *out;
     int64_t xs[3], ps[3];                 // strides of (sample, token, head), (sample, token, axis)
-    int64_t tokens;                       // of all samples
     int N, G, D, pairs, tile;             // tile: tokens of a CTA
+    unsigned tiles;                       // of a sample
     int position_dtype;
     float sign;
     double turns[kMostPairs];             // frequency / 2 pi
@@ -41,82 +43,139 @@ __device__ __forceinline__ double position(const RotaryParams &p, int64_t at) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void turn(T &x, T &y, float2 w) {
-    const float a = VecTraits<T>::to_float(x), b = VecTraits<T>::to_float(y);
-    // (written out, so that every variant of the kernel gives the same bits)
-    x = VecTraits<T>::from_float(__fmaf_rn(a, w.x, __fmul_rn(-b, w.y)));
-    y = VecTraits<T>::from_float(__fmaf_rn(a, w.y, __fmul_rn(b, w.x)));
+// (a, b) turned; written out, so that every variant of the kernel gives the same bits
+__device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
+    const float x = __fmaf_rn(a, c, __fmul_rn(-b, s));
+    b = __fmaf_rn(a, s, __fmul_rn(b, c));
+    a = x;
 }
 
-// VEC elements to a load, 16 bytes or one element; INTERLEAVED: a pair is two neighbours, else the
-// channels i and i + pairs
-template <typename T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-    struct alignas(sizeof(T) * VEC) Vec {
-        T v[VEC];
-    };
-    extern __shared__ float2 table[];     // (tile, pairs) of (cos, sin)
-    const int64_t first = (int64_t)blockIdx.x * p.tile;
-    const int count = (int)min((int64_t)p.tile, p.tokens - first);
-    for (int i = threadIdx.x; i < count * p.pairs; i += kThreads) {
-        const int token = i / p.pairs, pair = i - token * p.pairs;
-        const int64_t b = (first + token) / p.N, n = first + token - b * p.N;
-        double turns = position(p, b * p.ps[0] + n * p.ps[1] + p.axis[pair] * p.ps[2]) * p.turns[pair];
-        turns -= rint(turns);
-        float s, c;
-        sincospif(2.f * (float)turns, &s, &c);
-        table[i] = make_float2(c, s * p.sign);
+// Sine and cosine of so many turns, |turns| <= 1/2.  Results of 16 bits have a half step of 2^-11 and more, where
+// the hardware's approximation (2^-20 within half a turn) costs 6 instructions instead of 50.
+template <typename T>
+__device__ __forceinline__ void sine_cosine(float turns, float &s, float &c) {
+    if constexpr (sizeof(T) == 4) {
+        sincospif(2.f * turns, &s, &c);
+    } else {
+        const float x = 6.283185307f * turns;
+        s = __sinf(x), c = __cosf(x);
     }
-    __syncthreads();
+}
 
-    // a unit: two vectors of pairs (one of interleaved pairs where VEC > 1), or one behind the turned channels
-    constexpr bool kOne = INTERLEAVED && VEC > 1;
-    const int turning = (kOne ? 2 : 1) * p.pairs / VEC;
-    const int units = turning + (p.D - 2 * p.pairs) / VEC;
-    const int per_token = p.G * units;
-    for (int i = threadIdx.x; i < count * per_token; i += kThreads) {
-        const int token = i / per_token, rest = i - token * per_token, head = rest / units, unit = rest - head * units;
-        const int64_t b = (first + token) / p.N, n = first + token - b * p.N;
-        const T *x = static_cast<const T *>(p.x) + b * p.xs[0] + n * p.xs[1] + head * p.xs[2];
-        T *out = static_cast<T *>(p.out) + ((first + token) * p.G + head) * p.D;
-        const float2 *cs = table + token * p.pairs;
-        if (unit >= turning) {
-            const int c = 2 * p.pairs + (unit - turning) * VEC;
-            *reinterpret_cast<Vec *>(out + c) = *reinterpret_cast<const Vec *>(x + c);
-        } else if constexpr (kOne) {
-            Vec v = *reinterpret_cast<const Vec *>(x + unit * VEC);
+// WIDE: 16-byte vectors, else single elements; INTERLEAVED: a pair is two neighbours, else the channels i and
+// i + pairs.  The table has the cosines of a token's pairs, then their sines.
+template <typename T, bool WIDE, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+    constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
+    using Raw = std::conditional_t<WIDE, uint4, T>;
+    // a unit: two vectors of pairs (one of interleaved pairs where it is wide), or one behind the turned channels
+    constexpr bool kOne = INTERLEAVED && WIDE;
+    constexpr int kUnits = kOne ? 2 * kInFlight : kInFlight;
+    extern __shared__ __align__(16) float table[];
+    const unsigned b = blockIdx.x / p.tiles;
+    const int first = (int)(blockIdx.x - b * p.tiles) * p.tile, count = min(p.tile, p.N - first);
+    const int turning = (kOne ? 2 : 1) * p.pairs / VEC, units = turning + (p.D - 2 * p.pairs) / VEC;
+    const int per_token = p.G * units, all = count * per_token;
+    // this thread's next unit, and how far the one after that is
+    int token = threadIdx.x / per_token, head = (threadIdx.x - token * per_token) / units;
+    int unit = threadIdx.x - token * per_token - head * units;
+    const int tokens = kThreads / per_token, heads = (kThreads - tokens * per_token) / units;
+    const int step = kThreads - tokens * per_token - heads * units;
+    const T *const x = static_cast<const T *>(p.x) + b * p.xs[0] + first * p.xs[1];
+    T *const out = static_cast<T *>(p.out) + ((int64_t)b * p.N + first) * p.G * p.D;
+    const int other = INTERLEAVED ? 1 : p.pairs;           // from a pair's first vector to its second
+    bool formed = false;
+    for (int i = threadIdx.x; i - (int)threadIdx.x < all; i += kUnits * kThreads) {
+        Raw v[kUnits], u[kOne ? 1 : kUnits];
+        int at[kUnits], cs[kUnits];       // in out; in the table, or less than 0: nothing to turn
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) turn(v.v[j], v.v[j + 1], cs[(unit * VEC + j) / 2]);
-            *reinterpret_cast<Vec *>(out + unit * VEC) = v;
-        } else {
-            const int c0 = INTERLEAVED ? 2 * unit : unit * VEC, c1 = INTERLEAVED ? 2 * unit + 1 : p.pairs + unit * VEC;
-            Vec v = *reinterpret_cast<const Vec *>(x + c0), u = *reinterpret_cast<const Vec *>(x + c1);
+        for (int k = 0; k < kUnits; ++k) {
+            const bool turns = unit < turning;
+            const int c = !turns ? 2 * p.pairs + (unit - turning) * VEC : INTERLEAVED && !WIDE ? 2 * unit : unit * VEC;
+            at[k] = i + k * kThreads < all ? (token * p.G + head) * p.D + c : -1;
+            cs[k] = turns ? token * 2 * p.pairs + (kOne ? unit * VEC / 2 : unit * VEC) : -1;
+            if (at[k] >= 0) {
+                const T *from = x + token * p.xs[1] + head * p.xs[2] + c;
+                v[k] = *reinterpret_cast<const Raw *>(from);
+                if constexpr (!kOne) {
+                    if (turns) u[k] = *reinterpret_cast<const Raw *>(from + other);
+                }
+            }
+            token += tokens, head += heads, unit += step;
+            if (unit >= units) unit -= units, ++head;
+            if (head >= p.G) head -= p.G, ++token;
+        }
+        if (!formed) {
+            int of = threadIdx.x / max(p.pairs, 1), pair = threadIdx.x - of * p.pairs;
+            const int steps = kThreads / max(p.pairs, 1), rest = kThreads - steps * p.pairs;
+            const int64_t from = b * p.ps[0] + first * p.ps[1];
+            for (int j = threadIdx.x; j < count * p.pairs; j += kThreads) {
+                double turns = position(p, from + of * p.ps[1] + p.axis[pair] * p.ps[2]) * p.turns[pair];
+                turns -= rint(turns);
+                float s, c;
+                sine_cosine<T>((float)turns, s, c);
+                table[of * 2 * p.pairs + pair] = c;
+                table[of * 2 * p.pairs + p.pairs + pair] = s * p.sign;
+                of += steps, pair += rest;
+                if (pair >= p.pairs) pair -= p.pairs, ++of;
+            }
+            __syncthreads();
+            formed = true;
+        }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) turn(v.v[j], u.v[j], cs[unit * VEC + j]);
-            *reinterpret_cast<Vec *>(out + c0) = v;
-            *reinterpret_cast<Vec *>(out + c1) = u;
+        for (int k = 0; k < kUnits; ++k) {
+            if (at[k] < 0) continue;
+            if (cs[k] >= 0) {
+                const float *c = table + cs[k], *s = c + p.pairs;
+                if constexpr (!WIDE) {
+                    float y = VecTraits<T>::to_float(v[k]), z = VecTraits<T>::to_float(u[k]);
+                    turn(y, z, *c, *s);
+                    v[k] = VecTraits<T>::from_float(y);
+                    out[at[k] + other] = VecTraits<T>::from_float(z);
+                } else if constexpr (INTERLEAVED) {
+                    float2 y[VEC / 2];
+                    VecTraits<T>::unpack(v[k], y);
+#pragma unroll
+                    for (int j = 0; j < VEC / 2; j += 2) {
+                        const float2 c2 = *reinterpret_cast<const float2 *>(c + j), s2 = *reinterpret_cast<const float2 *>(s + j);
+                        turn(y[j].x, y[j].y, c2.x, s2.x);
+                        turn(y[j + 1].x, y[j + 1].y, c2.y, s2.y);
+                    }
+                    v[k] = VecTraits<T>::pack(y);
+                } else {
+                    float2 y[VEC / 2], z[VEC / 2];
+                    VecTraits<T>::unpack(v[k], y);
+                    VecTraits<T>::unpack(u[k], z);
+#pragma unroll
+                    for (int j = 0; j < VEC / 2; j += 2) {
+                        const float4 c4 = *reinterpret_cast<const float4 *>(c + 2 * j), s4 = *reinterpret_cast<const float4 *>(s + 2 * j);
+                        turn(y[j].x, z[j].x, c4.x, s4.x), turn(y[j].y, z[j].y, c4.y, s4.y);
+                        turn(y[j + 1].x, z[j + 1].x, c4.z, s4.z), turn(y[j + 1].y, z[j + 1].y, c4.w, s4.w);
+                    }
+                    v[k] = VecTraits<T>::pack(y);
+                    *reinterpret_cast<uint4 *>(out + at[k] + other) = VecTraits<T>::pack(z);
+                }
+            }
+            *reinterpret_cast<Raw *>(out + at[k]) = v[k];
         }
     }
 }
 
-template <typename T, int VEC, bool INTERLEAVED>
-cudaError_t launch(const RotaryParams &p, cudaStream_t stream) {
-    const int64_t grid = (p.tokens + p.tile - 1) / p.tile;
-    if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    rotary_kernel<T, VEC, INTERLEAVED><<<(unsigned)grid, kThreads, p.tile * p.pairs * sizeof(float2), stream>>>(p);
+template <typename T, bool WIDE, bool INTERLEAVED>
+cudaError_t launch(const RotaryParams &p, unsigned grid, cudaStream_t stream) {
+    rotary_kernel<T, WIDE, INTERLEAVED><<<grid, kThreads, p.tile * p.pairs * 2 * sizeof(float), stream>>>(p);
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_typed(const RotaryParams &p, bool interleaved, cudaStream_t stream) {
+cudaError_t launch_typed(const RotaryParams &p, bool interleaved, unsigned grid, cudaStream_t stream) {
     // 16-byte vectors where every one of them is aligned and belongs to one kind of unit
     constexpr int kVec = 16 / sizeof(T);
     const bool wide = p.D % kVec == 0 && (interleaved ? 2 * p.pairs : p.pairs) % kVec == 0 && p.xs[0] % kVec == 0 &&
                       p.xs[1] % kVec == 0 && p.xs[2] % kVec == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 &&
                       reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-    if (interleaved) return wide ? launch<T, kVec, true>(p, stream) : launch<T, 1, true>(p, stream);
-    return wide ? launch<T, kVec, false>(p, stream) : launch<T, 1, false>(p, stream);
+    if (interleaved) return wide ? launch<T, true, true>(p, grid, stream) : launch<T, false, true>(p, grid, stream);
+    return wide ? launch<T, true, false>(p, grid, stream) : launch<T, false, false>(p, grid, stream);
 }
 
 int refuse(int status, const char *message) { return set_last_error(status, message); }
@@ -147,7 +206,7 @@ extern "C" int msda_b200_rotary(const void *x, const int64_t *x_strides, const v
     RotaryParams p{};
     p.x = x, p.positions = positions, p.out = out;
     for (int i = 0; i < 3; ++i) p.xs[i] = x_strides[i], p.ps[i] = position_strides[i];
-    p.tokens = B * N, p.N = (int)N, p.G = (int)G, p.D = (int)D, p.pairs = (int)pairs;
+    p.N = (int)N, p.G = (int)G, p.D = (int)D, p.pairs = (int)pairs;
     p.position_dtype = position_dtype;
     p.sign = inverse ? -1.f : 1.f;
     for (int i = 0; i < pairs; ++i) {
@@ -156,18 +215,22 @@ extern "C" int msda_b200_rotary(const void *x, const int64_t *x_strides, const v
         p.turns[i] = frequencies[i] * 0.15915494309189535;      // 1 / (2 pi)
         p.axis[i] = (uint8_t)axis_of_pair[i];
     }
-    // about four vectors to a thread, as long as every SM gets some tokens; the table within 32 KB
+    // as many tokens to a CTA as its threads ask for at a time, as long as every SM gets some; the table within 32 KB
     const int64_t bytes = G * D * (dtype == MSDA_B200_F32 ? 4 : 2);
-    int64_t tile = std::max<int64_t>(1, 4 * kThreads * 16 / std::max<int64_t>(bytes, 1));
-    tile = std::min(tile, std::max<int64_t>(1, p.tokens / (148 * 4)));
+    int64_t tile = std::max<int64_t>(1, 2 * kInFlight * kThreads * 16 / bytes);
+    tile = std::min(tile, std::max<int64_t>(1, B * N / (148 * 4)));
     if (pairs > 0) tile = std::min<int64_t>(tile, 4096 / pairs);
-    p.tile = (int)std::max<int64_t>(1, tile);
+    tile = std::max<int64_t>(1, std::min(tile, N));
+    p.tile = (int)tile;
+    p.tiles = (unsigned)((N + tile - 1) / tile);
+    const int64_t grid = B * ((N + tile - 1) / tile);
+    if (grid > 0x7fffffff) return refuse(MSDA_B200_UNSUPPORTED, "rotary: too many tokens");
     const DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return refuse(MSDA_B200_CUDA_ERROR, cudaGetErrorString(guard.err));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = dtype == MSDA_B200_F32 ? launch_typed<float>(p, interleaved != 0, s)
-                          : dtype == MSDA_B200_F16 ? launch_typed<__half>(p, interleaved != 0, s)
-                                                   : launch_typed<__nv_bfloat16>(p, interleaved != 0, s);
+    const cudaError_t e = dtype == MSDA_B200_F32 ? launch_typed<float>(p, interleaved != 0, (unsigned)grid, s)
+                          : dtype == MSDA_B200_F16 ? launch_typed<__half>(p, interleaved != 0, (unsigned)grid, s)
+                                                   : launch_typed<__nv_bfloat16>(p, interleaved != 0, (unsigned)grid, s);
     if (e != cudaSuccess) return refuse(MSDA_B200_CUDA_ERROR, cudaGetErrorString(e));
     count_launches(1, 0);
     return MSDA_B200_OK;
