@@ -4,10 +4,11 @@
 //
 // One pass over x, bound by its bytes.  A CTA takes a few tokens of a sample: its threads ask for the vectors that
 // they will turn (both halves of the pairs), form the sine and cosine of every (token, pair) once for all heads
-// while those are on their way, and turn them.  Angles are formed in 64 bits as turns and reduced to [-1/2, 1/2]
-// before anything is rounded to 32: at position 10^6 a 32-bit angle is 0.03 off.  (float64 multiplies run at half
-// the float32 rate here and there is one for each of G * D / pairs channels.)  The backward pass is the same
-// kernel with the angles' sign turned.
+// while those are on their way, and turn them.  Angles are turns in more than 32 bits, reduced to [-1/2, 1/2] before
+// anything is rounded: at position 10^6 a 32-bit angle is 0.03 off.  float32 positions take a frequency of two
+// floats and the rounding error of the product that a fused multiply-add gives (2^-48 of the turns), others float64.
+// The frequencies go to shared memory first: lanes that index kernel parameters differently are served one by one.
+// The backward pass is the same kernel with the angles' sign turned.
 #include <algorithm>
 #include <type_traits>
 
@@ -18,7 +19,7 @@ namespace msda_b200 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMostPairs = 128;
 constexpr int kInFlight = 2;          // pairs of vectors that a thread asks for at a time
 
@@ -36,7 +37,6 @@ struct RotaryParams {
 
 __device__ __forceinline__ double position(const RotaryParams &p, int64_t at) {
     switch (p.position_dtype) {
-        case MSDA_B200_F32: return __ldg(static_cast<const float *>(p.positions) + at);
         case MSDA_B200_F64: return __ldg(static_cast<const double *>(p.positions) + at);
         case MSDA_B200_I32: return __ldg(static_cast<const int *>(p.positions) + at);
         default: return (double)__ldg(static_cast<const long long *>(p.positions) + at);
@@ -65,13 +65,16 @@ __device__ __forceinline__ void sine_cosine(float turns, float &s, float &c) {
 // WIDE: 16-byte vectors, else single elements; INTERLEAVED: a pair is two neighbours, else the channels i and
 // i + pairs.  The table has the cosines of a token's pairs, then their sines.
 template <typename T, bool WIDE, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_constant__ RotaryParams p) {
     constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
     using Raw = std::conditional_t<WIDE, uint4, T>;
     // a unit: two vectors of pairs (one of interleaved pairs where it is wide), or one behind the turned channels
     constexpr bool kOne = INTERLEAVED && WIDE;
     constexpr int kUnits = kOne ? 2 * kInFlight : kInFlight;
     extern __shared__ __align__(16) float table[];
+    __shared__ double frequency[kMostPairs];
+    __shared__ float2 split[kMostPairs];
+    __shared__ int axis[kMostPairs];
     const unsigned b = blockIdx.x / p.tiles;
     const int first = (int)(blockIdx.x - b * p.tiles) * p.tile, count = min(p.tile, p.N - first);
     const int turning = (kOne ? 2 : 1) * p.pairs / VEC, units = turning + (p.D - 2 * p.pairs) / VEC;
@@ -84,6 +87,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const T *const x = static_cast<const T *>(p.x) + b * p.xs[0] + first * p.xs[1];
     T *const out = static_cast<T *>(p.out) + ((int64_t)b * p.N + first) * p.G * p.D;
     const int other = INTERLEAVED ? 1 : p.pairs;           // from a pair's first vector to its second
+    for (int j = threadIdx.x; j < p.pairs; j += kThreads) {
+        const double f = p.turns[j];
+        frequency[j] = f;
+        split[j] = make_float2((float)f, (float)(f - (float)f));
+        axis[j] = p.axis[j];
+    }
     bool formed = false;
     for (int i = threadIdx.x; i - (int)threadIdx.x < all; i += kUnits * kThreads) {
         Raw v[kUnits], u[kOne ? 1 : kUnits];
@@ -106,14 +115,22 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
             if (head >= p.G) head -= p.G, ++token;
         }
         if (!formed) {
+            __syncthreads();
             int of = threadIdx.x / max(p.pairs, 1), pair = threadIdx.x - of * p.pairs;
             const int steps = kThreads / max(p.pairs, 1), rest = kThreads - steps * p.pairs;
             const int64_t from = b * p.ps[0] + first * p.ps[1];
             for (int j = threadIdx.x; j < count * p.pairs; j += kThreads) {
-                double turns = position(p, from + of * p.ps[1] + p.axis[pair] * p.ps[2]) * p.turns[pair];
-                turns -= rint(turns);
-                float s, c;
-                sine_cosine<T>((float)turns, s, c);
+                const int64_t place = from + of * p.ps[1] + axis[pair] * p.ps[2];
+                float turns, s, c;
+                if (p.position_dtype == MSDA_B200_F32) {
+                    const float at = __ldg(static_cast<const float *>(p.positions) + place), most = __fmul_rn(at, split[pair].x);
+                    const float rest = __fmaf_rn(at, split[pair].y, __fmaf_rn(at, split[pair].x, -most));
+                    turns = (most - rintf(most)) + rest;
+                } else {
+                    const double all = position(p, place) * frequency[pair];
+                    turns = (float)(all - rint(all));
+                }
+                sine_cosine<T>(turns, s, c);
                 table[of * 2 * p.pairs + pair] = c;
                 table[of * 2 * p.pairs + p.pairs + pair] = s * p.sign;
                 of += steps, pair += rest;
