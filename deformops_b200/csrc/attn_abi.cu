@@ -51,21 +51,25 @@ AttentionSplit even_split(int64_t items, int64_t tiles, int extra, int64_t most)
 // Float32 sums on the tensor cores are cut off, not rounded, at every product that is added: with at most 32
 // tiles (2048 states or rows) to a part, and parts added with rounding, that stays near 2^-20.
 constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 32;
+constexpr int64_t kFewRows = 16;
 
 bool on_tensor_cores(const msda_b200_attention &c) { return c.dtype != MSDA_B200_F32 || c.head_dim <= 64; }
 
 Pass forward_pass(const msda_b200_attention &c) {
     const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
     Pass pass{};
-    if (on_tensor_cores(c) && rows > 16) {
+    if (on_tensor_cores(c) && rows > kFewRows) {
         pass.row_tiles = 13 * ((rows + 127) / 128) > 20 * ((rows + 255) / 256) ? 2 : 1;
         const int64_t held = 128 * pass.row_tiles, tile = c.head_dim > 64 ? 128 : 64;
         pass.split = even_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 8,
                                 c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
-    } else {
+    } else if (rows > kFewRows) {
         const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
-        const int64_t held = rows <= 16 ? 16 : 64;
-        pass.split = attention_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 148 * 4, 4);
+        pass.split = attention_split(bk * ((rows + 63) / 64), (c.states + tile - 1) / tile, 148 * 4, 4);
+    } else {
+        // a stretch has some blocks for each of its four warps
+        const FewShape few = attention_few_shape(c.dtype, c.head_dim);
+        pass.split = attention_split(bk, (c.states + few.block - 1) / few.block, 148 * few.resident, 16);
     }
     const int64_t parts = pass.split.splits * bk * rows;
     pass.bytes = pass.split.splits > 1 ? round16(parts * 4) + parts * c.head_dim * 4 : 0;
@@ -248,6 +252,7 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     p.v_terms = static_cast<char *>(p.k_terms) + term_bytes(*call, call->states, call->kv_heads);
     const int terms = call->dtype == MSDA_B200_F32 && pass.row_tiles > 0 ? 2 : 0;
     cudaError_t e = cudaErrorNotSupported;
+    if (p.R <= kFewRows) e = launch_attention_few(p, call->dtype, s);
     if (pass.row_tiles > 0) {
         e = launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
         if (e == cudaErrorNotSupported && p.D > 64) p.tiles *= 2;      // the other kernel's tiles have 64 states

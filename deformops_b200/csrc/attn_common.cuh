@@ -149,6 +149,12 @@ cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cu
 // 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to a CTA, stretches of whole tiles of 64 states (128 where D > 64).  cudaErrorNotSupported (and
 // nothing launched) where k or v cannot be described to TMA.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
+// at most 16 rows to a key head; stretches of p.tiles blocks
+struct FewShape {
+    int block, resident;      // states of a block; CTAs to an SM
+};
+FewShape attention_few_shape(int dtype, int64_t D);
+cudaError_t launch_attention_few(const AttentionParams &p, int dtype, cudaStream_t stream);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 

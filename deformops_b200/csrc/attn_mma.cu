@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "attn_common.cuh"
+#include "warp_mma.cuh"
 
 namespace msda_b200 {
 
@@ -52,40 +53,6 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void *p)
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(smem_address(p)));
-}
-
-template <typename T>
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same_v<T, __half>)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                     "{%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-
-// x = hi + lo, hi rounded to 11 bits (half away from zero); of lo the matrix instruction takes the first 11
-__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-    lo = __float_as_uint(x - __uint_as_float(hi));
-}
-
-__device__ __forceinline__ void mma_tf32x3(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4],
-                                           const uint32_t (&bh)[2], const uint32_t (&bl)[2]) {
-    mma_tf32(c, al, bh);
-    mma_tf32(c, ah, bl);
-    mma_tf32(c, ah, bh);
 }
 
 // acc (16 x 8N) = A B^T: A the warp's 16 rows, B 8N rows, DP columns each
@@ -240,16 +207,15 @@ __device__ __forceinline__ int next_tile(const uint32_t *words, int S, int t, in
     return end;
 }
 
-// WR warps side by side over 16 rows each, the other way 4 / WR warps over parts of every tile
-template <typename T, int DP, int WR>
+// four warps, 16 rows each
+template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr int BN = kTile<T, DP>, KG = 4 / WR, N = BN / KG / 8, ROWS = 16 * WR, P = kPitch<T, DP>;
+    constexpr int BN = kTile<T, DP>, N = BN / 8, ROWS = 64, P = kPitch<T, DP>;
     extern __shared__ __align__(16) unsigned char smem[];
     T *const sq = reinterpret_cast<T *>(smem);
     T *const sk = sq + ROWS * P;                       // two stages of k and v
     T *const sv = sk + 2 * BN * P;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int wr = warp % WR, wk = warp / WR;
 
     const int row_tiles = (p.R + ROWS - 1) / ROWS;
     int64_t i = blockIdx.x;
@@ -275,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const _
     float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
-    const int r0 = first + wr * 16 + g;
+    const int r0 = first + warp * 16 + g;
     const uint32_t *rw[2] = {r0 < p.R ? row_words_of(p, b, h, r0) : nullptr,
                              r0 + 8 < p.R ? row_words_of(p, b, h, r0 + 8) : nullptr};
 
@@ -290,11 +256,11 @@ __global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const _
         __syncthreads();
 
         float s[N][4];
-        product_nt<T, DP, N>(s, sq + wr * 16 * P, sk + (stage * BN + wk * N * 8) * P);
+        product_nt<T, DP, N>(s, sq + warp * 16 * P, sk + stage * BN * P);
         float top[2] = {m[0], m[1]}, keep[2];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int state = tile * BN + (wk * N + n) * 8;
+            const int state = tile * BN + n * 8;
             const uint32_t common = key_word(words, p.S, state >> 5);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -324,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const _
                 }
             l[half] = l[half] * keep[half] + sum;
         }
-        product_nn<T, DP, N, true>(o, s, sv + (stage * BN + wk * N * 8) * P, keep);
+        product_nn<T, DP, N, true>(o, s, sv + stage * BN * P, keep);
         __syncthreads();
         tile = next;
     }
@@ -334,46 +300,6 @@ __global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const _
     for (int half = 0; half < 2; ++half) {
         l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
         l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-    }
-    if constexpr (KG > 1) {
-        // the warps' parts meet in the first warp of each row group
-        __syncthreads();
-        float *const sm = reinterpret_cast<float *>(smem);            // (4, 16) maxima, sums, then (4, 16, DP)
-        float *const sl = sm + 64, *const so = sl + 64;
-        if (t == 0) {
-            sm[warp * 16 + g] = m[0], sm[warp * 16 + g + 8] = m[1];
-            sl[warp * 16 + g] = l[0], sl[warp * 16 + g + 8] = l[1];
-        }
-#pragma unroll
-        for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                so[(warp * 16 + g + 8 * (e >> 1)) * DP + d * 8 + 2 * t + (e & 1)] = o[d][e];
-        __syncthreads();
-        if (wk != 0) return;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int row = g + 8 * half;
-            float top = m[half];
-            for (int w = 1; w < KG; ++w) top = fmaxf(top, sm[(w * WR + wr) * 16 + row]);
-            const float base = top == -INFINITY ? 0.f : top;
-            l[half] *= fast_exp2(m[half] - base);
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) o[d][2 * half + e] *= fast_exp2(m[half] - base);
-            for (int w = 1; w < KG; ++w) {
-                const int from = (w * WR + wr) * 16 + row;
-                const float keep = fast_exp2(sm[from] - base);
-                l[half] += keep * sl[from];
-#pragma unroll
-                for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        o[d][2 * half + e] += keep * so[from * DP + d * 8 + 2 * t + e];
-            }
-            m[half] = top;
-        }
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -569,13 +495,11 @@ cudaError_t launch(Kernel kernel, int64_t grid, size_t smem, cudaStream_t stream
     return cudaGetLastError();
 }
 
-template <typename T, int DP, int WR>
+template <typename T, int DP>
 cudaError_t forward(const AttentionParams &p, cudaStream_t stream) {
-    constexpr int rows = 16 * WR;
-    constexpr size_t tiles = (size_t)(rows + 4 * kTile<T, DP>) * kPitch<T, DP> * sizeof(T);
-    constexpr size_t join = (128 + 64 * DP) * sizeof(float);
-    const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + rows - 1) / rows);
-    return launch(attention_forward_mma_kernel<T, DP, WR>, grid, WR < 4 ? std::max(tiles, join) : tiles, stream, p);
+    constexpr size_t smem = (size_t)(64 + 4 * kTile<T, DP>) * kPitch<T, DP> * sizeof(T);
+    const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + 63) / 64);
+    return launch(attention_forward_mma_kernel<T, DP>, grid, smem, stream, p);
 }
 
 template <typename T, int DP, bool KEYS>
@@ -588,18 +512,13 @@ cudaError_t backward(const AttentionParams &p, cudaStream_t stream) {
 }
 
 template <typename T, int DP>
-cudaError_t forward_rows(const AttentionParams &p, cudaStream_t stream) {
-    return p.R <= 16 ? forward<T, DP, 1>(p, stream) : forward<T, DP, 4>(p, stream);
-}
-template <typename T, int DP>
 cudaError_t backward_side(const AttentionParams &p, bool keys, cudaStream_t stream) {
     return keys ? backward<T, DP, true>(p, stream) : backward<T, DP, false>(p, stream);
 }
 
 template <typename T>
 cudaError_t forward_typed(const AttentionParams &p, cudaStream_t stream) {
-    return p.D <= 32 ? forward_rows<T, 32>(p, stream)
-           : p.D <= 64 ? forward_rows<T, 64>(p, stream) : forward_rows<T, 128>(p, stream);
+    return p.D <= 32 ? forward<T, 32>(p, stream) : p.D <= 64 ? forward<T, 64>(p, stream) : forward<T, 128>(p, stream);
 }
 template <typename T>
 cudaError_t backward_typed(const AttentionParams &p, bool keys, cudaStream_t stream) {
