@@ -68,7 +68,7 @@ Pass forward_pass(const msda_b200_attention &c) {
         pass.split = attention_split(bk * ((rows + 63) / 64), (c.states + tile - 1) / tile, 148 * 4, 4);
     } else {
         // a stretch has some blocks for each of its four warps
-        const FewShape few = attention_few_shape(c.dtype, c.head_dim);
+        const FewShape few = attention_few_shape(c.dtype, c.head_dim, rows);
         pass.split = attention_split(bk, (c.states + few.block - 1) / few.block, 148 * few.resident, 16);
     }
     const int64_t parts = pass.split.splits * bk * rows;

@@ -153,7 +153,7 @@ cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int
 struct FewShape {
     int block, resident;      // states of a block; CTAs to an SM
 };
-FewShape attention_few_shape(int dtype, int64_t D);
+FewShape attention_few_shape(int dtype, int64_t D, int64_t rows);
 cudaError_t launch_attention_few(const AttentionParams &p, int dtype, cudaStream_t stream);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);

@@ -8,6 +8,9 @@
 //   O        B = v: lane (g, t) has channels 8 g .. 8 g + 7 of states 2 t, 2 t + 1, 2 t + 8 and 2 t + 9, two states
 //            packed to a register; column g of product i is channel 8 g + i
 //
+// With at most eight rows (EIGHT) the second product is O^T = v^T p^T, the channels 8 g + 2 i and 8 g + 2 i + 1 as
+// rows g and g + 8 of product i: half the products and half the registers for O, so more warps.
+//
 // (float32: four channels to 16 bytes, two terms of tf32, products of 8 instead of 16.)  Every warp takes blocks
 // of its CTA's stretch of states with a running maximum and sum of its own; the warps, and the stretches
 // (attn_aux.cu), are joined at the end.
@@ -28,8 +31,8 @@ template <typename T, int DP>
 constexpr int kBlock = sizeof(T) == 4 ? (DP == 128 ? 8 : 16) : DP == 32 ? 32 : 16;
 
 // CTAs to an SM, as registers allow
-template <typename T, int DP>
-constexpr int kResident = DP == 128 ? 2 : sizeof(T) == 4 && DP == 64 ? 3 : 4;
+template <typename T, int DP, bool EIGHT>
+constexpr int kResident = DP == 128 ? (EIGHT && sizeof(T) == 2 ? 3 : 2) : sizeof(T) == 4 && DP == 64 ? (EIGHT ? 4 : 3) : EIGHT ? 5 : 4;
 
 template <typename T, int DP>
 struct Few {
@@ -53,8 +56,8 @@ __device__ __forceinline__ void load_lane(uint32_t (&r)[N], const void *p, bool 
     }
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kernel(const __grid_constant__ AttentionParams p) {
+template <typename T, int DP, bool EIGHT>
+__global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_few_kernel(const __grid_constant__ AttentionParams p) {
     using F = Few<T, DP>;
     constexpr int KB = F::KB, NT = F::NT, KC = F::KC, VC = F::VC, CH = F::kChannels;
     __shared__ float s_max[kWarps][16], s_sum[kWarps][16];
@@ -65,12 +68,13 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
     const T *k = static_cast<const T *>(p.k) + b * p.ks[0] + h * p.ks[2];
     const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + h * p.vs[2];
     const uint32_t *words = key_words_of(p, b, h);
-    const bool two = p.R > 8;                                      // rows g + 8 exist
+    constexpr int kHalves = EIGHT ? 1 : 2;                         // rows g, and g + 8
+    constexpr int CO = EIGHT ? CH / 2 : CH;                        // products of a span of channels
 
-    uint32_t q[2][KC][4];
-    const uint32_t *rw[2];
+    uint32_t q[kHalves][KC][4];
+    const uint32_t *rw[kHalves];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < kHalves; ++half) {
         const int r = g + 8 * half;
         const T *from = static_cast<const T *>(p.q) + (r < p.R ? row_offset(p.qs, p.share, b, h, r) : 0);
 #pragma unroll
@@ -81,11 +85,11 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
         rw[half] = r < p.R ? row_words_of(p, b, h, r) : nullptr;
     }
 
-    float o[VC][CH][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[VC][CO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < VC; ++c)
 #pragma unroll
-        for (int i = 0; i < CH; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
+        for (int i = 0; i < CO; ++i) o[c][i][0] = o[c][i][1] = o[c][i][2] = o[c][i][3] = 0.f;
 
     const int end = (int)min((int64_t)p.S, (int64_t)(part + 1) * p.tiles * KB);
     for (int first = part * p.tiles * KB + warp * KB; first < end; first += kWarps * KB) {
@@ -115,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
             for (int c = 0; c < KC; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    const uint32_t a[4] = {q[0][c][i], q[1][c][i], q[0][c][i + 1], q[1][c][i + 1]};
+                    const uint32_t a[4] = {q[0][c][i], EIGHT ? 0u : q[kHalves - 1][c][i], q[0][c][i + 1], EIGHT ? 0u : q[kHalves - 1][c][i + 1]};
                     if constexpr (F::kWide) {
                         uint32_t ah[4], al[4], bh2[2], bl[2];
 #pragma unroll
@@ -130,8 +134,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
         }
         float keep[2] = {1.f, 1.f};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (half == 1 && !two) continue;
+        for (int half = 0; half < kHalves; ++half) {
             uint32_t bits = seen;
             if (rw[half] != nullptr) bits = __ldg(rw[half] + (first >> 5)) >> (first & 31);
             float top = m[half];
@@ -158,41 +161,57 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
                 }
             l[half] = l[half] * keep[half] + sum;
         }
-        if (!two) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][2] = s[n][3] = 0.f;
+        if constexpr (EIGHT) {
+            // (the lanes of row r are 4 r .. 4 r + 3; O has rows 2 t and 2 t + 1 here)
+            const float mine = keep[0];
+            keep[0] = __shfl_sync(0xffffffffu, mine, 8 * t), keep[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
         }
 #pragma unroll
         for (int c = 0; c < VC; ++c)
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
+            for (int i = 0; i < CO; ++i) {
                 if constexpr (F::kWide) {
                     // (from zero, and added with rounding: a matrix instruction cuts its sums off)
                     float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         uint32_t ah[4], al[4], bh2[2], bl[2];
-                        split_tf32(s[n][0], ah[0], al[0]), split_tf32(s[n][2], ah[1], al[1]);
-                        split_tf32(s[n][1], ah[2], al[2]), split_tf32(s[n][3], ah[3], al[3]);
-                        split_tf32(__uint_as_float(fv[2 * n][c][i]), bh2[0], bl[0]);
-                        split_tf32(__uint_as_float(fv[2 * n + 1][c][i]), bh2[1], bl[1]);
+                        if constexpr (EIGHT) {
+                            split_tf32(__uint_as_float(fv[2 * n][c][2 * i]), ah[0], al[0]);
+                            split_tf32(__uint_as_float(fv[2 * n][c][2 * i + 1]), ah[1], al[1]);
+                            split_tf32(__uint_as_float(fv[2 * n + 1][c][2 * i]), ah[2], al[2]);
+                            split_tf32(__uint_as_float(fv[2 * n + 1][c][2 * i + 1]), ah[3], al[3]);
+                            split_tf32(s[n][0], bh2[0], bl[0]), split_tf32(s[n][1], bh2[1], bl[1]);
+                        } else {
+                            split_tf32(s[n][0], ah[0], al[0]), split_tf32(s[n][2], ah[1], al[1]);
+                            split_tf32(s[n][1], ah[2], al[2]), split_tf32(s[n][3], ah[3], al[3]);
+                            split_tf32(__uint_as_float(fv[2 * n][c][i]), bh2[0], bl[0]);
+                            split_tf32(__uint_as_float(fv[2 * n + 1][c][i]), bh2[1], bl[1]);
+                        }
                         mma_tf32x3(add, ah, al, bh2, bl);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[c][i][e] = fmaf(o[c][i][e], keep[e >> 1], add[e]);
+                    for (int e = 0; e < 4; ++e) o[c][i][e] = fmaf(o[c][i][e], keep[EIGHT ? e & 1 : e >> 1], add[e]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[c][i][e] *= keep[e >> 1];
+                    for (int e = 0; e < 4; ++e) o[c][i][e] *= keep[EIGHT ? e & 1 : e >> 1];
 #pragma unroll
                     for (int n = 0; n < NT; n += 2) {
-                        const uint32_t a[4] = {VecTraits<T>::pack2(make_float2(s[n][0], s[n][1])),
-                                               VecTraits<T>::pack2(make_float2(s[n][2], s[n][3])),
-                                               VecTraits<T>::pack2(make_float2(s[n + 1][0], s[n + 1][1])),
-                                               VecTraits<T>::pack2(make_float2(s[n + 1][2], s[n + 1][3]))};
-                        // channel i of two neighbouring states
-                        constexpr uint32_t kPick[2] = {0x5410, 0x7632};
-                        mma16<T>(o[c][i], a, __byte_perm(fv[2 * n][c][i >> 1], fv[2 * n + 1][c][i >> 1], kPick[i & 1]),
-                                 __byte_perm(fv[2 * n + 2][c][i >> 1], fv[2 * n + 3][c][i >> 1], kPick[i & 1]));
+                        // a channel of two neighbouring states: the lower or the upper halves of two registers
+                        const auto pair = [&](int state, int channel) {
+                            return __byte_perm(fv[state][c][channel >> 1], fv[state + 1][c][channel >> 1], channel & 1 ? 0x7632 : 0x5410);
+                        };
+                        if constexpr (EIGHT) {
+                            const uint32_t a[4] = {pair(2 * n, 2 * i), pair(2 * n, 2 * i + 1), pair(2 * n + 2, 2 * i), pair(2 * n + 2, 2 * i + 1)};
+                            mma16<T>(o[c][i], a, VecTraits<T>::pack2(make_float2(s[n][0], s[n][1])),
+                                     VecTraits<T>::pack2(make_float2(s[n + 1][0], s[n + 1][1])));
+                        } else {
+                            const uint32_t a[4] = {VecTraits<T>::pack2(make_float2(s[n][0], s[n][1])),
+                                                   VecTraits<T>::pack2(make_float2(s[n][2], s[n][3])),
+                                                   VecTraits<T>::pack2(make_float2(s[n + 1][0], s[n + 1][1])),
+                                                   VecTraits<T>::pack2(make_float2(s[n + 1][2], s[n + 1][3]))};
+                            mma16<T>(o[c][i], a, pair(2 * n, i), pair(2 * n + 2, i));
+                        }
                     }
                 }
             }
@@ -200,20 +219,22 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
 
     // the warps' parts: a thread to a channel of a row
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < kHalves; ++half) {
         const int r = g + 8 * half;
         l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
         l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        if (r >= p.R) continue;
-        if (t == 0) s_max[warp][r] = m[half], s_sum[warp][r] = l[half];
-        float *to = s_out + (warp * p.R + r) * DP;
-#pragma unroll
-        for (int c = 0; c < VC; ++c)
-#pragma unroll
-            for (int i = 0; i < CH; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) to[c * F::kSpan + (2 * t + e) * CH + i] = o[c][i][2 * half + e];
+        if (t == 0 && r < p.R) s_max[warp][r] = m[half], s_sum[warp][r] = l[half];
     }
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+        for (int i = 0; i < CO; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = EIGHT ? 2 * t + (e & 1) : g + 8 * (e >> 1);
+                const int d = c * F::kSpan + (EIGHT ? g * CH + 2 * i + (e >> 1) : (2 * t + (e & 1)) * CH + i);
+                if (r < p.R) s_out[(warp * p.R + r) * DP + d] = o[c][i][e];
+            }
     __syncthreads();
     const int64_t rows = (int64_t)p.B * p.K * p.R;
     for (int i = threadIdx.x; i < p.R * p.D; i += kThreads) {
@@ -244,10 +265,10 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP>) attention_few_kern
     }
 }
 
-template <typename T, int DP>
-cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
-    const auto kernel = attention_few_kernel<T, DP>;
-    constexpr int most = kWarps * 16 * DP * sizeof(float);
+template <typename T, int DP, bool EIGHT>
+cudaError_t launch_rows(const AttentionParams &p, cudaStream_t stream) {
+    const auto kernel = attention_few_kernel<T, DP, EIGHT>;
+    constexpr int most = kWarps * (EIGHT ? 8 : 16) * DP * sizeof(float);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)p.B * p.K * p.splits;
@@ -256,19 +277,29 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+template <typename T, int DP>
+cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
+    return p.R <= 8 ? launch_rows<T, DP, true>(p, stream) : launch_rows<T, DP, false>(p, stream);
+}
+
 template <typename T>
 cudaError_t launch_typed(const AttentionParams &p, cudaStream_t stream) {
     return p.D <= 32 ? launch<T, 32>(p, stream) : p.D <= 64 ? launch<T, 64>(p, stream) : launch<T, 128>(p, stream);
 }
 
+template <typename T, int DP>
+FewShape shape(int64_t rows) {
+    return {kBlock<T, DP>, rows <= 8 ? kResident<T, DP, true> : kResident<T, DP, false>};
+}
+template <typename T>
+FewShape shape_typed(int64_t D, int64_t rows) {
+    return D <= 32 ? shape<T, 32>(rows) : D <= 64 ? shape<T, 64>(rows) : shape<T, 128>(rows);
+}
+
 }  // namespace
 
-FewShape attention_few_shape(int dtype, int64_t D) {
-    if (dtype == 0)
-        return D <= 32 ? FewShape{kBlock<float, 32>, kResident<float, 32>}
-               : D <= 64 ? FewShape{kBlock<float, 64>, kResident<float, 64>} : FewShape{kBlock<float, 128>, kResident<float, 128>};
-    return D <= 32 ? FewShape{kBlock<__half, 32>, kResident<__half, 32>}
-           : D <= 64 ? FewShape{kBlock<__half, 64>, kResident<__half, 64>} : FewShape{kBlock<__half, 128>, kResident<__half, 128>};
+FewShape attention_few_shape(int dtype, int64_t D, int64_t rows) {
+    return dtype == 0 ? shape_typed<float>(D, rows) : shape_typed<__half>(D, rows);
 }
 
 cudaError_t launch_attention_few(const AttentionParams &p, int dtype, cudaStream_t stream) {
