@@ -250,7 +250,7 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     p.part = p.part_lse + round16((int64_t)p.splits * p.B * p.K * p.R * 4) / 4;
     p.k_terms = static_cast<char *>(workspace) + round16(pass.bytes);
     p.v_terms = static_cast<char *>(p.k_terms) + term_bytes(*call, call->states, call->kv_heads);
-    const int terms = call->dtype == MSDA_B200_F32 && pass.row_tiles > 0 ? 2 : 0;
+    const int terms = call->dtype == MSDA_B200_F32 && pass.row_tiles > 0 ? 1 : 0;
     cudaError_t e = cudaErrorNotSupported;
     if (p.R <= kFewRows) e = launch_attention_few(p, call->dtype, s);
     if (pass.row_tiles > 0) {
@@ -308,23 +308,24 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
         p.k_terms = terms, p.v_terms = terms + state_terms, p.q_terms = terms + 2 * state_terms;
         p.g_terms = terms + 2 * state_terms + row_terms;
         const int H = (int)call->heads;
-        if (e == cudaSuccess) e = launch_attention_terms(p.k, p.ks, p.B, p.S, p.K, p.D, p.k_terms, s);
-        if (e == cudaSuccess) e = launch_attention_terms(p.v, p.vs, p.B, p.S, p.K, p.D, p.v_terms, s);
-        if (e == cudaSuccess) e = launch_attention_terms(p.q, p.qs, p.B, p.Q, H, p.D, p.q_terms, s);
-        if (e == cudaSuccess) e = launch_attention_terms(p.grad_out, gs, p.B, p.Q, H, p.D, p.g_terms, s);
-        launches += 4;
+        const TermsParams all = {{{p.k, p.k_terms, {p.ks[0], p.ks[1], p.ks[2]}, p.S, p.K},
+                                  {p.v, p.v_terms, {p.vs[0], p.vs[1], p.vs[2]}, p.S, p.K},
+                                  {p.q, p.q_terms, {p.qs[0], p.qs[1], p.qs[2]}, p.Q, H},
+                                  {p.grad_out, p.g_terms, {gs[0], gs[1], gs[2]}, p.Q, H}},
+                                 4, p.B, p.D};
+        if (e == cudaSuccess) e = launch_attention_terms(all, s);
+        ++launches;
     }
     if (e == cudaSuccess) {
         p.part2 = p.part + (int64_t)keys.split.splits * p.B * p.K * p.S * p.D;
         e = launch_backward(p, keys, call->dtype, true, s);
-        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part, p.dk, true, call->dtype, s);
-        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part2, p.dv, true, call->dtype, s);
-        launches += p.splits > 1 ? 2 : 0;
+        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, true, call->dtype, s);
+        launches += p.splits > 1;
     }
     if (e == cudaSuccess) {
         e = launch_backward(p, rows, call->dtype, false, s);
-        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, p.part, p.dq, false, call->dtype, s);
-        launches += p.splits > 1 ? 1 : 0;
+        if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, false, call->dtype, s);
+        launches += p.splits > 1;
     }
     if (e == cudaSuccess) count_launches(launches, 0);
     return status_of(e);

@@ -56,23 +56,62 @@ __device__ __forceinline__ uint32_t pack_word(const uint8_t *hidden, int64_t str
     return __ballot_sync(0xffffffffu, state < S && __ldg(hidden + state * stride) == 0);
 }
 
+// Words first .. first + 31 of a mask row, one to a lane.  States that are neighbours are read 16 bytes to a lane from
+// the last 16-byte boundary on, and the bytes that were asked for are moved into place on the way (rows of odd
+// length have no alignment); others a byte to a lane.
+__device__ __forceinline__ uint32_t pack_words(const uint8_t *hidden, int64_t stride, int first, int W, int S) {
+    const int lane = threadIdx.x & 31;
+    uint32_t word = 0;
+    if (stride != 1) {
+        for (int i = 0; i < 32 && first + i < W; ++i) {
+            const uint32_t x = pack_word(hidden, stride, (first + i) * 32 + lane, S);
+            if (i == lane) word = x;
+        }
+        return word;
+    }
+    // lane i: the bytes of 32 states, from three aligned vectors
+    const int state = (first + lane) * 32, left = S - state;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(hidden + state);
+    const uint4 *from = reinterpret_cast<const uint4 *>(at & ~(uintptr_t)15);
+    const int off = (int)(at & 15);
+    uint32_t bits[2] = {0, 0};
+#pragma unroll
+    for (int v = 0; v < 3; ++v) {
+        // (a vector with one byte that exists lies within the allocation's 16-byte granule)
+        if (left > 0 && 16 * v - off < min(left, 32)) {
+            const uint4 x = __ldg(from + v);
+            const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+            uint32_t seen = 0;                                               // of 16 bytes
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                // each byte 0 or not: its lowest bit to bit 4 i + byte
+                seen |= ((__vcmpeq4(in[i], 0) & 0x08040201u) * 0x01010101u >> 24) << (4 * i);
+            if (v < 2)
+                bits[0] |= seen << (16 * v);
+            else
+                bits[1] = seen;
+        }
+    }
+    word = __funnelshift_r(bits[0], bits[1], off);
+    return left >= 32 ? word : left <= 0 ? 0u : word & ((1u << left) - 1);
+}
+
 // padding alone: a CTA to a sample packs it and lists its tiles
 __global__ void __launch_bounds__(1024) attention_padding_kernel(const __grid_constant__ MaskParams p) {
+    grid_launch_dependents();
     const int lane = threadIdx.x & 31, b = blockIdx.x;
-    const uint8_t *padding = p.padding + b * p.ps[0];
     uint32_t *words = p.key_words + (int64_t)b * p.W;
-    for (int w = threadIdx.x >> 5; w < p.W; w += 32) {
-        const uint32_t word = pack_word(padding, p.ps[1], w * 32 + lane, p.S);
-        if (lane == 0) words[w] = word;
+    for (int first = threadIdx.x & ~31; first < p.W; first += 1024) {
+        const uint32_t word = pack_words(p.padding + b * p.ps[0], p.ps[1], first, p.W, p.S);
+        if (first + lane < p.W) words[first + lane] = word;
     }
     __syncthreads();
     list_both(words, p.S, p.lists + b * list_words(p.S));
 }
 
-// A warp packs 1024 states of one mask row at a time.  Rows whose states are neighbours are read 16 bytes to a
-// lane from the last 16-byte boundary on, and the bytes that were asked for are moved into place on the way (rows
-// of odd length have no alignment); others a byte to a lane.
+// a warp to 1024 states of a mask row at a time
 __global__ void __launch_bounds__(kThreads) attention_mask_kernel(const __grid_constant__ MaskParams p) {
+    grid_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int groups = (p.W + 31) / 32;
     const int64_t rows = (int64_t)p.B * p.H * p.Q, tasks = rows * groups;
@@ -81,47 +120,8 @@ __global__ void __launch_bounds__(kThreads) attention_mask_kernel(const __grid_c
         const int64_t row = task / groups;
         const int first = (int)(task - row * groups) * 32;                 // word
         const int64_t bh = row / p.Q, query = row - bh * p.Q, b = bh / p.H;
-        const uint8_t *mask = p.mask + b * p.ms[0] + (bh - b * p.H) * p.ms[1] + query * p.ms[2];
-        uint32_t word = 0;
-        if (p.ms[3] == 1) {
-            // lane i: bytes of states first * 32 + 32 i .. + 31, from three aligned vectors
-            const int state = (first + lane) * 32;
-            const uintptr_t at = reinterpret_cast<uintptr_t>(mask + state);
-            const uint4 *from = reinterpret_cast<const uint4 *>(at & ~(uintptr_t)15);
-            const int off = (int)(at & 15), left = p.S - state;            // bytes that exist
-            uint32_t bits[2] = {0, 0};
-#pragma unroll
-            for (int v = 0; v < 3; ++v) {
-                // (a vector with one byte that exists is within the allocation's 16-byte granule)
-                if (left > 0 && 16 * v - off < min(left, 32)) {
-                    const uint4 x = __ldg(from + v);
-                    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-                    uint32_t seen = 0;                                       // of 16 bytes
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        // each byte 0 or not: its lowest bit to bit 4 i + byte
-                        seen |= ((__vcmpeq4(in[i], 0) & 0x08040201u) * 0x01010101u >> 24) << (4 * i);
-                    if (v < 2)
-                        bits[0] |= seen << (16 * v);
-                    else
-                        bits[1] = seen;
-                }
-            }
-            word = __funnelshift_r(bits[0], bits[1], off);
-            if (left < 32) word = left <= 0 ? 0u : word & ((1u << left) - 1);
-        } else {
-            for (int i = 0; i < 32 && first + i < p.W; ++i) {
-                const uint32_t x = pack_word(mask, p.ms[3], (first + i) * 32 + lane, p.S);
-                if (i == lane) word = x;
-            }
-        }
-        if (p.padding != nullptr) {
-            const uint8_t *padding = p.padding + b * p.ps[0];
-            for (int i = 0; i < 32 && first + i < p.W; ++i) {
-                const uint32_t x = pack_word(padding, p.ps[1], (first + i) * 32 + lane, p.S);
-                if (i == lane) word &= x;
-            }
-        }
+        uint32_t word = pack_words(p.mask + b * p.ms[0] + (bh - b * p.H) * p.ms[1] + query * p.ms[2], p.ms[3], first, p.W, p.S);
+        if (p.padding != nullptr) word &= pack_words(p.padding + b * p.ps[0], p.ps[1], first, p.W, p.S);
         if (first + lane < p.W) p.row_words[row * p.W + first + lane] = word;
     }
 }
@@ -129,6 +129,8 @@ __global__ void __launch_bounds__(kThreads) attention_mask_kernel(const __grid_c
 // key words: the or of all rows of a sample (or of the heads that share a key head)
 __global__ void __launch_bounds__(1024) attention_mask_any_kernel(const __grid_constant__ MaskParams p) {
     __shared__ uint32_t any[32][33];
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
     const int blocks = (p.W + 31) / 32;
     const int bk = blockIdx.x / blocks, w = (blockIdx.x - bk * blocks) * 32 + lane;
@@ -144,56 +146,76 @@ __global__ void __launch_bounds__(1024) attention_mask_any_kernel(const __grid_c
 }
 
 __global__ void __launch_bounds__(1024) attention_list_kernel(const __grid_constant__ MaskParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     list_both(p.key_words + (int64_t)blockIdx.x * p.W, p.S, p.lists + blockIdx.x * list_words(p.S));
 }
 
-// a thread to eight channels, zeros behind the last one
-__global__ void __launch_bounds__(kThreads) attention_terms_kernel(const float *x, int64_t s0, int64_t s1, int64_t s2, int tokens,
-                                                                   int heads, int D, int64_t rows, uint4 *terms) {
-    const int chunks = (D + 7) / 8;
-    const int64_t all = rows * chunks;
+// a thread to eight channels, zeros behind the last one; blockIdx.y: the tensor
+__global__ void __launch_bounds__(kThreads) attention_terms_kernel(const __grid_constant__ TermsParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const TermsParams::Tensor &t = p.of[blockIdx.y];
+    const unsigned chunks = (p.D + 7) / 8;
+    const int64_t all = (int64_t)p.B * t.tokens * t.heads * chunks;
+    uint4 *terms = static_cast<uint4 *>(t.terms);
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t row = i / chunks, token = row / heads, b = token / tokens;
+        const int64_t row = i / chunks, token = row / t.heads, b = token / t.tokens;
         const int c = (int)(i - row * chunks) * 8;
-        const float *from = x + b * s0 + (token - b * tokens) * s1 + (row - token * heads) * s2 + c;
+        const float *from = static_cast<const float *>(t.x) + b * t.strides[0] + (token - b * t.tokens) * t.strides[1] +
+                            (row - token * t.heads) * t.strides[2] + c;
         const float4 lo = __ldg(reinterpret_cast<const float4 *>(from));
-        const float4 hi = c + 4 < D ? __ldg(reinterpret_cast<const float4 *>(from + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        uint32_t t[4][3];
-        split_terms(make_float2(lo.x, lo.y), t[0]), split_terms(make_float2(lo.z, lo.w), t[1]);
-        split_terms(make_float2(hi.x, hi.y), t[2]), split_terms(make_float2(hi.z, hi.w), t[3]);
+        const float4 hi = c + 4 < p.D ? __ldg(reinterpret_cast<const float4 *>(from + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t w[4][3];
+        split_terms(make_float2(lo.x, lo.y), w[0]), split_terms(make_float2(lo.z, lo.w), w[1]);
+        split_terms(make_float2(hi.x, hi.y), w[2]), split_terms(make_float2(hi.z, hi.w), w[3]);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) terms[k * all + i] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+        for (int k = 0; k < 3; ++k) terms[k * all + i] = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
     }
 }
 
-// eight lanes to a row
+// eight lanes to a row, rows in the order of `out`
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr int kVec = VecTraits<T>::kVec;
+    constexpr int kVec = VecTraits<T>::kVec, kRows = 4;
+    grid_launch_dependents();
     const int lane = threadIdx.x & 7;
-    const int64_t rows = (int64_t)p.B * p.K * p.R;
-    const int64_t first = (int64_t)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3);
-    float sum = 0.f;
-    if (first < rows) {
-        const int64_t bh = first / p.R;
-        const int r = (int)(first - bh * p.R), query = r / p.share, b = (int)(bh / p.K), h = (int)(bh - (int64_t)b * p.K);
-        const int64_t at = (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
-        for (int c = lane * kVec; c < p.D; c += 8 * kVec) {
-            float2 x[kVec / 2], y[kVec / 2];
-            VecTraits<T>::unpack(ldg16(static_cast<const T *>(p.out) + at + c), x);
-            VecTraits<T>::unpack(ldg16(static_cast<const T *>(p.grad_out) + at + c), y);
+    const unsigned rows = (unsigned)p.B * p.Q * p.K * p.share;
+    const unsigned first = blockIdx.x * (kThreads / 8 * kRows) + (threadIdx.x >> 3);
+    float sum[kRows] = {};
+    for (int c = lane * kVec; c < p.D; c += 8 * kVec) {
+        uint4 x[kRows], y[kRows];
 #pragma unroll
-            for (int i = 0; i < kVec / 2; ++i) sum += x[i].x * y[i].x + x[i].y * y[i].y;
+        for (int k = 0; k < kRows; ++k) {
+            const unsigned row = first + k * (kThreads / 8);
+            const int64_t at = (int64_t)row * p.D + c;
+            x[k] = row < rows ? ldg16(static_cast<const T *>(p.out) + at) : make_uint4(0, 0, 0, 0);
+            y[k] = row < rows ? ldg16(static_cast<const T *>(p.grad_out) + at) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            float2 u[kVec / 2], v[kVec / 2];
+            VecTraits<T>::unpack(x[k], u);
+            VecTraits<T>::unpack(y[k], v);
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) sum[k] += u[i].x * v[i].x + u[i].y * v[i].y;
         }
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0 && first < rows) p.delta[first] = sum;
+    for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+        const unsigned row = first + k * (kThreads / 8), token = row / (p.K * p.share), head = row - token * p.K * p.share;
+        const unsigned b = token / p.Q, h = head / p.share;
+        if (lane == 0 && row < rows)
+            p.delta[((int64_t)b * p.K + h) * p.R + (int64_t)(token - b * p.Q) * p.share + (head - h * p.share)] = sum[k];
+    }
 }
 
 // o = sum of 2^(L_i - L) o_i, a thread to four channels of a row
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionParams p) {
+    grid_dependency_wait();
     const int lanes = p.D / 4;
     const int64_t rows = (int64_t)p.B * p.K * p.R;
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -231,6 +253,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) attention_join_many_kernel(const __grid_constant__ AttentionParams p) {
     __shared__ float tops[4], weights[128];
     __shared__ float4 sums[128];
+    grid_dependency_wait();
     const int64_t rows = (int64_t)p.B * p.K * p.R, row = blockIdx.x;
     const int lanes = p.D / 4, groups = 128 / lanes, group = threadIdx.x / lanes, c = (threadIdx.x - group * lanes) * 4;
     float top = -INFINITY;
@@ -270,10 +293,13 @@ __global__ void __launch_bounds__(128) attention_join_many_kernel(const __grid_c
     if (c == 0) p.lse[row] = sum == 0.f ? INFINITY : base + log2f(sum);
 }
 
-// gradients: the parts' sum, in the order of the parts
+// gradients: the parts' sum, in the order of the parts; blockIdx.y: dk (or dq), dv
 template <typename T, bool KEYS>
-__global__ void __launch_bounds__(kThreads) attention_sum_kernel(const __grid_constant__ AttentionParams p,
-                                                                 const float *part, T *out) {
+__global__ void __launch_bounds__(kThreads) attention_sum_kernel(const __grid_constant__ AttentionParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const float *part = blockIdx.y == 0 ? p.part : p.part2;
+    T *out = static_cast<T *>(!KEYS ? p.dq : blockIdx.y == 0 ? p.dk : p.dv);
     const int lanes = p.D / 4, X = KEYS ? p.S : p.R;
     const int64_t rows = (int64_t)p.B * p.K * X;
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -301,29 +327,22 @@ unsigned blocks_for(int64_t threads) {
 }
 
 template <typename T>
-cudaError_t sum_typed(const AttentionParams &p, const float *part, void *out, bool keys, cudaStream_t stream) {
-    const unsigned grid = blocks_for((int64_t)p.B * p.K * (keys ? p.S : p.R) * (p.D / 4));
-    if (keys)
-        attention_sum_kernel<T, true><<<grid, kThreads, 0, stream>>>(p, part, static_cast<T *>(out));
-    else
-        attention_sum_kernel<T, false><<<grid, kThreads, 0, stream>>>(p, part, static_cast<T *>(out));
-    return cudaGetLastError();
+cudaError_t sum_typed(const AttentionParams &p, bool keys, cudaStream_t stream) {
+    const dim3 grid(blocks_for((int64_t)p.B * p.K * (keys ? p.S : p.R) * (p.D / 4)), keys ? 2 : 1);
+    return launch_dependent(keys ? attention_sum_kernel<T, true> : attention_sum_kernel<T, false>, grid, kThreads, 0, stream, p);
 }
 
 template <typename T>
 cudaError_t join_typed(const AttentionParams &p, cudaStream_t stream) {
     const int64_t rows = (int64_t)p.B * p.K * p.R;
-    if (p.splits >= kManyParts && rows < 148 * 64) {
-        attention_join_many_kernel<T><<<(unsigned)rows, 128, 0, stream>>>(p);
-        return cudaGetLastError();
-    }
-    attention_join_kernel<T><<<blocks_for((int64_t)p.B * p.K * p.R * (p.D / 4)), kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    if (p.splits >= kManyParts && rows < 148 * 64)
+        return launch_dependent(attention_join_many_kernel<T>, dim3((unsigned)rows), 128, 0, stream, p);
+    return launch_dependent(attention_join_kernel<T>, dim3(blocks_for(rows * (p.D / 4))), kThreads, 0, stream, p);
 }
 
 template <typename T>
 cudaError_t delta_typed(const AttentionParams &p, cudaStream_t stream) {
-    attention_delta_kernel<T><<<blocks_for((int64_t)p.B * p.K * p.R * 8), kThreads, 0, stream>>>(p);
+    attention_delta_kernel<T><<<blocks_for((int64_t)p.B * p.K * p.R * 2), kThreads, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
@@ -337,18 +356,18 @@ cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream) {
     const int64_t tasks = (int64_t)p.B * p.H * p.Q * ((p.W + 31) / 32);
     const int64_t grid = std::min<int64_t>((tasks + kThreads / 32 - 1) / (kThreads / 32), 148 * 64);
     attention_mask_kernel<<<(unsigned)grid, kThreads, 0, stream>>>(p);
-    attention_mask_any_kernel<<<(unsigned)(p.B * p.KW * ((p.W + 31) / 32)), 1024, 0, stream>>>(p);
-    attention_list_kernel<<<(unsigned)(p.B * p.KW), 1024, 0, stream>>>(p);
-    return cudaGetLastError();
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess)
+        e = launch_dependent(attention_mask_any_kernel, dim3((unsigned)(p.B * p.KW * ((p.W + 31) / 32))), 1024, 0, stream, p);
+    if (e == cudaSuccess) e = launch_dependent(attention_list_kernel, dim3((unsigned)(p.B * p.KW)), 1024, 0, stream, p);
+    return e;
 }
 
-cudaError_t launch_attention_terms(const void *x, const int64_t (&strides)[3], int B, int tokens, int heads, int D, void *terms,
-                                   cudaStream_t stream) {
-    const int64_t rows = (int64_t)B * tokens * heads;
-    const int64_t grid = std::min<int64_t>((rows * ((D + 7) / 8) + kThreads - 1) / kThreads, 148 * 32);
-    attention_terms_kernel<<<(unsigned)grid, kThreads, 0, stream>>>(static_cast<const float *>(x), strides[0], strides[1], strides[2],
-                                                                     tokens, heads, D, rows, static_cast<uint4 *>(terms));
-    return cudaGetLastError();
+cudaError_t launch_attention_terms(const TermsParams &p, cudaStream_t stream) {
+    int64_t most = 0;
+    for (int i = 0; i < p.tensors; ++i) most = std::max(most, (int64_t)p.B * p.of[i].tokens * p.of[i].heads * ((p.D + 7) / 8));
+    const int64_t grid = std::min<int64_t>((most + kThreads - 1) / kThreads, 148 * 32);
+    return launch_dependent(attention_terms_kernel, dim3((unsigned)grid, p.tensors), kThreads, 0, stream, p);
 }
 
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream) {
@@ -359,11 +378,9 @@ cudaError_t launch_attention_join(const AttentionParams &p, int dtype, cudaStrea
     return dtype == 0 ? join_typed<float>(p, stream)
            : dtype == 1 ? join_typed<__half>(p, stream) : join_typed<__nv_bfloat16>(p, stream);
 }
-cudaError_t launch_attention_sum(const AttentionParams &p, const float *part, void *out, bool keys, int dtype,
-                                 cudaStream_t stream) {
-    return dtype == 0 ? sum_typed<float>(p, part, out, keys, stream)
-           : dtype == 1 ? sum_typed<__half>(p, part, out, keys, stream)
-                        : sum_typed<__nv_bfloat16>(p, part, out, keys, stream);
+cudaError_t launch_attention_sum(const AttentionParams &p, bool keys, int dtype, cudaStream_t stream) {
+    return dtype == 0 ? sum_typed<float>(p, keys, stream)
+           : dtype == 1 ? sum_typed<__half>(p, keys, stream) : sum_typed<__nv_bfloat16>(p, keys, stream);
 }
 
 }  // namespace msda_b200

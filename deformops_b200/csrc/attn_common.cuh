@@ -145,9 +145,28 @@ __device__ __forceinline__ float2 add2(const float2 a, const float2 b) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------
+// A launch that may become resident while the kernel before it drains; it begins with grid_dependency_wait().  For
+// the small kernels of a call, each of which would wait for the one before to leave the GPU.
+template <typename... Formal, typename... Actual>
+inline cudaError_t launch_dependent(void (*kernel)(Formal...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                                    const Actual &...actual) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(actual)...);
+}
+
 cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream);
-// 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to a CTA, stretches of whole tiles of 64 states (128 where D > 64).  cudaErrorNotSupported (and
-// nothing launched) where k or v cannot be described to TMA.
+// 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to an item, stretches of
+// whole tiles of 64 states (128 where D > 64).  cudaErrorNotSupported (and nothing launched) where an operand cannot
+// be described to TMA.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
 // at most 16 rows to a key head; stretches of p.tiles blocks
 struct FewShape {
@@ -158,14 +177,21 @@ cudaError_t launch_attention_few(const AttentionParams &p, int dtype, cudaStream
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 
-// the terms of a (B, tokens, heads, D) float32 tensor with these strides
-cudaError_t launch_attention_terms(const void *x, const int64_t (&strides)[3], int B, int tokens, int heads, int D, void *terms,
-                                   cudaStream_t stream);
+// the terms of (B, tokens, heads, D) float32 tensors
+struct TermsParams {
+    struct Tensor {
+        const void *x;
+        void *terms;
+        int64_t strides[3];
+        int tokens, heads;
+    } of[4];
+    int tensors, B, D;
+};
+cudaError_t launch_attention_terms(const TermsParams &p, cudaStream_t stream);
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream);
 // parts of a split pass to the result: outputs and sums (forward), or the sum of gradients
 cudaError_t launch_attention_join(const AttentionParams &p, int dtype, cudaStream_t stream);
-cudaError_t launch_attention_sum(const AttentionParams &p, const float *part, void *out, bool keys, int dtype,
-                                 cudaStream_t stream);
+cudaError_t launch_attention_sum(const AttentionParams &p, bool keys, int dtype, cudaStream_t stream);
 struct MaskParams {
     const uint8_t *padding, *mask;        // true: not to be seen; either may be null
     int64_t ps[2], ms[4];                 // strides of (sample, state), (sample, head, query, state)

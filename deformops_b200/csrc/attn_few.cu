@@ -63,6 +63,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_f
     __shared__ float s_max[kWarps][16], s_sum[kWarps][16];
     extern __shared__ float s_out[];                               // (warps, rows, DP)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    grid_launch_dependents();
+    grid_dependency_wait();            // (of the masks that this call has packed)
     const unsigned bh = blockIdx.x / p.splits;
     const int part = (int)(blockIdx.x - bh * p.splits), b = (int)(bh / p.K), h = (int)(bh - b * p.K);
     const T *k = static_cast<const T *>(p.k) + b * p.ks[0] + h * p.ks[2];
@@ -273,8 +275,7 @@ cudaError_t launch_rows(const AttentionParams &p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)p.B * p.K * p.splits;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    kernel<<<(unsigned)grid, kThreads, kWarps * p.R * DP * sizeof(float), stream>>>(p);
-    return cudaGetLastError();
+    return launch_dependent(kernel, dim3((unsigned)grid), kThreads, kWarps * p.R * DP * sizeof(float), stream, p);
 }
 
 template <typename T, int DP>

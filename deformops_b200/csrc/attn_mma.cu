@@ -217,6 +217,8 @@ __global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const _
     T *const sv = sk + 2 * BN * P;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int row_tiles = (p.R + ROWS - 1) / ROWS;
     int64_t i = blockIdx.x;
     const int first = (int)(i % row_tiles) * ROWS;
@@ -347,6 +349,8 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
     uint32_t *const s_words = reinterpret_cast<uint32_t *>(s_delta + 2 * BN);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int x_tiles = ((KEYS ? p.S : p.R) + BX - 1) / BX;
     int64_t i = blockIdx.x;
     const int first = (int)(i % x_tiles) * BX;
@@ -491,8 +495,7 @@ cudaError_t launch(Kernel kernel, int64_t grid, size_t smem, cudaStream_t stream
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)grid, kThreads, smem, stream>>>(p);
-    return cudaGetLastError();
+    return launch_dependent(kernel, dim3((unsigned)grid), kThreads, smem, stream, p);
 }
 
 template <typename T, int DP>

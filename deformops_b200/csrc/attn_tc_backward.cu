@@ -134,6 +134,8 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
         for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += Sh::kThreads) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
         fence_async_shared();
     }
+    grid_launch_dependents();
+    grid_dependency_wait();            // (of what this call has launched before)
     fence_before();
     __syncthreads();
     fence_after();
@@ -589,9 +591,8 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     const int64_t items = (int64_t)p.B * p.K * p.splits * (((KEYS ? p.S : p.R) + x_rows - 1) / x_rows);
     if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const unsigned grid = (unsigned)std::min<int64_t>(items, 148);
-    kernel<<<grid, Shape<DP, KEYS, TERMS>::kThreads, smem, stream>>>(p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k, KEYS ? g : v,
-                                                                     (unsigned)items, x_rows, y_rows);
-    return cudaGetLastError();
+    return launch_dependent(kernel, dim3(grid), Shape<DP, KEYS, TERMS>::kThreads, smem, stream, p, KEYS ? k : q, KEYS ? v : g, KEYS ? q : k,
+                            KEYS ? g : v, (unsigned)items, x_rows, y_rows);
 }
 
 template <typename T>

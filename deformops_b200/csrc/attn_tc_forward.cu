@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
     const int64_t bh = of;
     const int b = (int)(of / p.K), h = (int)(of - b * p.K);
     const uint32_t *words = key_words_of(p, b, h);
-    const Tiles<BN> tiles(p, b, h, part);
 
     if (warp == kLast) tmem_alloc(&sm.tmem, 512);
     if (threadIdx.x == 0) {
@@ -111,6 +110,9 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
         for (int g = 0; g < Sh::kGroups; ++g)
             barrier_init(&sm.s_full[g], 1), barrier_init(&sm.p_full[g], 128), barrier_init(&sm.o_full[g], 1);
     }
+    grid_launch_dependents();
+    grid_dependency_wait();            // (of what this call has launched before: masks, terms)
+    const Tiles<BN> tiles(p, b, h, part);
     if (warp < 4 * RT) {
         // a thread to a row of q
         const int r = first + threadIdx.x;
@@ -433,8 +435,9 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
         if (!tc::make_map<T, DP>(km, p.k_terms, dense, 3 * p.B, p.S, p.K, 1, (int)D8, Sh::BN) ||
             !tc::make_map<T, DP>(vm, p.v_terms, dense, 3 * p.B, p.S, p.K, 1, (int)D8, Sh::BN))
             return cudaErrorNotSupported;
-        cudaError_t e = launch_attention_terms(p.k, p.ks, p.B, p.S, p.K, p.D, p.k_terms, stream);
-        if (e == cudaSuccess) e = launch_attention_terms(p.v, p.vs, p.B, p.S, p.K, p.D, p.v_terms, stream);
+        TermsParams terms = {{{p.k, p.k_terms, {p.ks[0], p.ks[1], p.ks[2]}, p.S, p.K}, {p.v, p.v_terms, {p.vs[0], p.vs[1], p.vs[2]}, p.S, p.K}},
+                             2, p.B, p.D};
+        const cudaError_t e = launch_attention_terms(terms, stream);
         if (e != cudaSuccess) return e;
     } else if (!tc::make_map<T, DP>(km, p.k, p.ks, p.B, p.S, p.K, 1, p.D, Sh::BN) ||
                !tc::make_map<T, DP>(vm, p.v, p.vs, p.B, p.S, p.K, 1, p.D, Sh::BN)) {
@@ -447,8 +450,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + RT * kTileRows - 1) / (RT * kTileRows));
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    kernel<<<(unsigned)grid, Sh::kThreads, smem, stream>>>(p, km, vm);
-    return cudaGetLastError();
+    return launch_dependent(kernel, dim3((unsigned)grid), Sh::kThreads, smem, stream, p, km, vm);
 }
 
 template <typename T>
