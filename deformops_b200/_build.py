@@ -25,7 +25,7 @@ LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libmsda_b200.so"
 SOURCES = ["msda_forward.cu", "msda_backward.cu", "msda_abi.cu", "msda_static_scratch.cu",
            "msda_f64.cu", "msda_sorted.cu", "msda_linear.cu", "attn_abi.cu", "attn_aux.cu", "attn_few.cu",
-           "attn_mma.cu", "attn_tc_backward.cu", "attn_tc_forward.cu", "rotary.cu"]
+           "attn_mma.cu", "attn_tc_backward.cu", "attn_tc_forward.cu", "attn_tc_wide.cu", "rotary.cu"]
 HEADERS = [CSRC / "msda_common.cuh", CSRC / "msda_sorted.cuh", CSRC / "attn_common.cuh", CSRC / "tensor_core.cuh", CSRC / "warp_mma.cuh",
            PKG.parent / "include" / "msda_b200.h"]
 #: bench-only microbenchmarks of the hardware floors (csrc/floors/bench_floors.cu); never

@@ -53,19 +53,16 @@ AttentionSplit even_split(int64_t items, int64_t tiles, int extra, int64_t most)
 constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 32;
 constexpr int64_t kFewRows = 16;
 
-bool on_tensor_cores(const msda_b200_attention &c) { return c.dtype != MSDA_B200_F32 || c.head_dim <= 64; }
+bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 && c.head_dim > 64; }
 
 Pass forward_pass(const msda_b200_attention &c) {
     const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
     Pass pass{};
-    if (on_tensor_cores(c) && rows > kFewRows) {
-        pass.row_tiles = 13 * ((rows + 127) / 128) > 20 * ((rows + 255) / 256) ? 2 : 1;
-        const int64_t held = 128 * pass.row_tiles, tile = c.head_dim > 64 ? 128 : 64;
+    if (rows > kFewRows) {
+        pass.row_tiles = !wide_float(c) && 13 * ((rows + 127) / 128) > 20 * ((rows + 255) / 256) ? 2 : 1;
+        const int64_t held = 128 * pass.row_tiles, tile = c.head_dim > 64 && !wide_float(c) ? 128 : 64;
         pass.split = even_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 8,
                                 c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
-    } else if (rows > kFewRows) {
-        const int tile = c.dtype == MSDA_B200_F32 && c.head_dim > 64 ? 32 : 64;
-        pass.split = attention_split(bk * ((rows + 63) / 64), (c.states + tile - 1) / tile, 148 * 4, 4);
     } else {
         // a stretch has some blocks for each of its four warps
         const FewShape few = attention_few_shape(c.dtype, c.head_dim, rows);
@@ -80,9 +77,9 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
     const int64_t share = c.heads / c.kv_heads, rows = c.queries * share, bk = c.batch * c.kv_heads;
     const int64_t held = keys ? c.states : rows, walked = keys ? rows : c.states;
     Pass pass{};
-    if (on_tensor_cores(c) && share <= 64) {
+    if (share <= 64) {
         pass.row_tiles = 1;
-        const int64_t x_rows = keys ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
+        const int64_t x_rows = keys || wide_float(c) ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
         pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, 6,
                                 c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
     } else {
@@ -97,7 +94,8 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
 cudaError_t launch_backward(AttentionParams &p, const Pass &pass, int dtype, bool keys, cudaStream_t stream) {
     p.splits = pass.split.splits, p.tiles = pass.split.tiles;
     if (pass.row_tiles > 0) {
-        const cudaError_t e = launch_attention_backward_tc(p, dtype, keys, stream);
+        const cudaError_t e = dtype == MSDA_B200_F32 && p.D > 64 ? launch_attention_backward_wide(p, keys, stream)
+                                                                 : launch_attention_backward_tc(p, dtype, keys, stream);
         if (e != cudaErrorNotSupported) return e;
         if (p.D > 64) p.tiles *= 2;
     }
@@ -254,7 +252,7 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     cudaError_t e = cudaErrorNotSupported;
     if (p.R <= kFewRows) e = launch_attention_few(p, call->dtype, s);
     if (pass.row_tiles > 0) {
-        e = launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
+        e = wide_float(*call) ? launch_attention_forward_wide(p, s) : launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
         if (e == cudaErrorNotSupported && p.D > 64) p.tiles *= 2;      // the other kernel's tiles have 64 states
     }
     if (e == cudaErrorNotSupported) e = launch_attention_forward_mma(p, call->dtype, s);
@@ -320,7 +318,7 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
         p.part2 = p.part + (int64_t)keys.split.splits * p.B * p.K * p.S * p.D;
         e = launch_backward(p, keys, call->dtype, true, s);
         if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, true, call->dtype, s);
-        launches += p.splits > 1;
+        launches += (p.splits > 1) + (wide_float(*call) && keys.row_tiles > 0);
     }
     if (e == cudaSuccess) {
         e = launch_backward(p, rows, call->dtype, false, s);

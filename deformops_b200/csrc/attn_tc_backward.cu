@@ -567,7 +567,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     tc::TensorMap q, g, k, v;
     if constexpr (TERMS == 3) {
         const int64_t D8 = (p.D + 7) / 8 * 8, heads = (int64_t)p.K * p.share;
-        const int64_t rows[3] = {p.Q * heads * D8, heads * D8, D8}, states[3] = {p.S * p.K * D8, p.K * D8, D8};
+        const int64_t rows[3] = {p.Q * heads * D8, heads * D8, D8}, states[3] = {(int64_t)p.S * p.K * D8, p.K * D8, D8};
         if (!tc::make_map<T, DP>(q, p.q_terms, rows, 3 * p.B, p.Q, p.K, p.share, (int)D8, row_tile) ||
             !tc::make_map<T, DP>(g, p.g_terms, rows, 3 * p.B, p.Q, p.K, p.share, (int)D8, row_tile) ||
             !tc::make_map<T, DP>(k, p.k_terms, states, 3 * p.B, p.S, p.K, 1, (int)D8, state_tile) ||

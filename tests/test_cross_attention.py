@@ -131,6 +131,9 @@ SIZES = [  # B, Q, S, G, K, D, masks
     (2, 1000, 16, 2, 2, 64, "heads"), (1, 257, 513, 4, 2, 128, "padding"), (2, 33, 127, 2, 2, 16, "none"),
     (1, 640, 640, 3, 3, 64, ""), (1, 200, 130, 16, 4, 128, "queries"), (1, 2, 5000, 2, 2, 32, "padding"),
     (10, 40, 1000, 16, 16, 128, ""), (3, 130, 700, 60, 60, 128, ""), (10, 40, 1000, 16, 16, 64, ""), (5, 128, 128, 1, 1, 128, ""), (1, 70, 4099, 1, 1, 56, "padding"),
+    # shared heads that do not divide a tile, or fill more than one; lists of many tiles
+    (1, 50, 200, 6, 2, 128, "heads"), (2, 45, 333, 12, 2, 32, "padding queries"), (1, 9, 150, 70, 1, 64, "queries"), (1, 2, 140, 130, 1, 128, ""),
+    (1, 3, 4000, 4, 1, 128, "heads"), (1, 4, 3001, 2, 1, 64, "heads"), (1, 20, 70001, 1, 1, 16, "padding"), (2, 300, 2200, 2, 1, 72, "padding queries"),
 ]
 
 
@@ -222,6 +225,20 @@ def test_strides(dtype, Q):
     out = cross_attention(q, leaf.expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1))
     (grad,) = torch.autograd.grad(out, leaf, do)
     assert torch.allclose(grad.double(), full[2].double().sum(0, keepdim=True), atol=4 * torch.finfo(dtype).eps * full[2].abs().max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("D", [32, 128])
+@pytest.mark.parametrize("Q", [2, 70])
+def test_one_state_or_one_head_for_all(dtype, Q, D):
+    """Expanded operands: their strides are 0, and their gradients sums."""
+    q, k, v, do = make(2, Q, 200, 4, 4, D, dtype)
+    for of in ((slice(None), slice(0, 1)), (slice(0, 1),), (slice(None), slice(None), slice(0, 1))):
+        a, b = k[of].expand_as(k), v[of].expand_as(v)
+        check(run(q, a, b, do), formula(q, a, b, do))
+        c = q[of].expand_as(q)
+        check(run(c, k, v, do), formula(c, k, v, do))
 
 
 @pytest.mark.gpu
