@@ -31,19 +31,27 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 struct Pass {
     AttentionSplit split;
     int64_t bytes;       // parts
-    int row_tiles;       // tiles of 128 rows that a CTA of the tensor-core kernel holds, 0 for the other
+    bool tensor_cores;
+    int row_tiles;       // forward: tiles of 128 rows that a CTA holds, 0 for a small one
 };
 
-// Splits of a pass whose CTAs (148 of them) take items in turn: the number that ends soonest, where an item
-// costs its tiles and `extra` more; items of at most `most` tiles.
-AttentionSplit even_split(int64_t items, int64_t tiles, int extra, int64_t most) {
+// What a pass takes, in twentieths of a tile of 256 rows: an SM takes `at_once` items together, each of them a share
+// of the time of all, which has its tiles, a beginning and an end, and parts to write and read where it is split.
+struct Cost {
+    int64_t tile, item, join, at_once;
+};
+
+// The number of splits that ends soonest, with items of at most `most` tiles.
+AttentionSplit even_split(int64_t items, int64_t tiles, const Cost &cost, int64_t most, int64_t *best_cost = nullptr) {
     const int64_t fewest = std::max<int64_t>(1, (tiles + most - 1) / most);
-    int64_t best = fewest, best_cost = INT64_MAX;
-    for (int64_t s = fewest; s <= std::max<int64_t>(fewest, std::min<int64_t>(tiles / 2, 148)); ++s) {
-        const int64_t each = (tiles + s - 1) / s, cost = (items * s + 147) / 148 * (each + extra);
-        if (cost < best_cost) best = s, best_cost = cost;
-        if (items * s > 148 * 8) break;
+    int64_t best = fewest, lowest = INT64_MAX;
+    for (int64_t s = fewest; s <= std::max<int64_t>(fewest, std::min<int64_t>(tiles / 2, 148 * cost.at_once)); ++s) {
+        const int64_t each = (tiles + s - 1) / s, turns = std::max(cost.at_once, (items * s + 147) / 148);
+        const int64_t all = turns * (each * cost.tile + cost.item + (s > 1 ? cost.join : 0)) + (s > 1 ? 80 : 0);
+        if (all < lowest) best = s, lowest = all;
+        if (items * s > 148 * 8 * cost.at_once) break;
     }
+    if (best_cost != nullptr) *best_cost = lowest;
     const int64_t each = std::max<int64_t>(1, (tiles + best - 1) / best);
     return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
 }
@@ -55,14 +63,35 @@ constexpr int64_t kFewRows = 16;
 
 bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 && c.head_dim > 64; }
 
+// The forward pass has three forms of CTA: two tiles of 128 rows; one, with twice the groups to it; or, where a
+// pass is short, small ones of 128 rows, several to an SM, that begin and end in one another's shadow.  The costs
+// are fits of times (0.7 us for 20 with up to 64 channels, 2 us with 128).  bf16, 4096 rows of 32 heads of 64: small ones
+// 20.7 us over 77 states and 205 over 4096, big ones 31.3 and 265 (in two parts; 214 in one); 1 x 16 384 x 16 heads
+// over 4096: big 361 us, small 399; 64 heads of 100 rows over 17 821 states: one tile to a CTA 61 us, small 84.
+void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
+    const int64_t most = c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles, bk = c.batch * c.kv_heads;
+    const bool half = c.dtype != MSDA_B200_F32, wide = wide_float(c), deep = c.head_dim > 64 && !wide;
+    const int64_t tiles = (c.states + 63) / 64, big = deep ? (c.states + 127) / 128 : tiles, one = (rows + 127) / 128, two = (rows + 255) / 256;
+    int64_t lowest;
+    pass.row_tiles = 1;
+    pass.split = even_split(bk * one, big, {deep ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most, &lowest);
+    if (wide) return;
+    const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost) {
+        int64_t all;
+        const AttentionSplit split = even_split(items, of, cost, most, &all);
+        if (all < lowest) lowest = all, pass.split = split, pass.row_tiles = row_tiles;
+    };
+    take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1});
+    if (deep) take(0, bk * one, tiles, {7, 40, 30, 2});
+    else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {13, 50, 30, 3});
+}
+
 Pass forward_pass(const msda_b200_attention &c) {
     const int64_t rows = c.queries * (c.heads / c.kv_heads), bk = c.batch * c.kv_heads;
     Pass pass{};
     if (rows > kFewRows) {
-        pass.row_tiles = !wide_float(c) && 13 * ((rows + 127) / 128) > 20 * ((rows + 255) / 256) ? 2 : 1;
-        const int64_t held = 128 * pass.row_tiles, tile = c.head_dim > 64 && !wide_float(c) ? 128 : 64;
-        pass.split = even_split(bk * ((rows + held - 1) / held), (c.states + tile - 1) / tile, 8,
-                                c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
+        pass.tensor_cores = true;
+        plan_forward(c, rows, pass);
     } else {
         // a stretch has some blocks for each of its four warps
         const FewShape few = attention_few_shape(c.dtype, c.head_dim, rows);
@@ -78,9 +107,9 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
     const int64_t held = keys ? c.states : rows, walked = keys ? rows : c.states;
     Pass pass{};
     if (share <= 64) {
-        pass.row_tiles = 1;
+        pass.tensor_cores = true;
         const int64_t x_rows = keys || wide_float(c) ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
-        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, 6,
+        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, {20, 120, 60, 1},
                                 c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
     } else {
         const int tile = c.head_dim > 64 ? 32 : 64;
@@ -93,7 +122,7 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
 // a pass on the tensor cores, or on the other kernel (whose tiles have 64 rows, or 32) where they cannot take it
 cudaError_t launch_backward(AttentionParams &p, const Pass &pass, int dtype, bool keys, cudaStream_t stream) {
     p.splits = pass.split.splits, p.tiles = pass.split.tiles;
-    if (pass.row_tiles > 0) {
+    if (pass.tensor_cores) {
         const cudaError_t e = dtype == MSDA_B200_F32 && p.D > 64 ? launch_attention_backward_wide(p, keys, stream)
                                                                  : launch_attention_backward_tc(p, dtype, keys, stream);
         if (e != cudaErrorNotSupported) return e;
@@ -107,13 +136,13 @@ int64_t term_bytes(const msda_b200_attention &c, int64_t tokens, int64_t heads) 
     return 6 * c.batch * tokens * heads * ((c.head_dim + 7) / 8 * 8);
 }
 int64_t forward_bytes(const msda_b200_attention &c, const Pass &pass) {
-    const bool terms = c.dtype == MSDA_B200_F32 && pass.row_tiles > 0;
+    const bool terms = c.dtype == MSDA_B200_F32 && pass.tensor_cores;
     return round16(pass.bytes) + (terms ? 2 * term_bytes(c, c.states, c.kv_heads) : 0);
 }
 int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
 
 int64_t backward_bytes(const msda_b200_attention &c, const Pass &keys, const Pass &rows) {
-    const bool terms = c.dtype == MSDA_B200_F32 && keys.row_tiles > 0;
+    const bool terms = c.dtype == MSDA_B200_F32 && keys.tensor_cores;
     return delta_bytes(c) + round16(std::max(keys.bytes, rows.bytes)) +
            (terms ? 2 * term_bytes(c, c.states, c.kv_heads) + 2 * term_bytes(c, c.queries, c.heads) : 0);
 }
@@ -248,12 +277,12 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     p.part = p.part_lse + round16((int64_t)p.splits * p.B * p.K * p.R * 4) / 4;
     p.k_terms = static_cast<char *>(workspace) + round16(pass.bytes);
     p.v_terms = static_cast<char *>(p.k_terms) + term_bytes(*call, call->states, call->kv_heads);
-    const int terms = call->dtype == MSDA_B200_F32 && pass.row_tiles > 0 ? 1 : 0;
+    const int terms = call->dtype == MSDA_B200_F32 && pass.tensor_cores ? 1 : 0;
     cudaError_t e = cudaErrorNotSupported;
     if (p.R <= kFewRows) e = launch_attention_few(p, call->dtype, s);
-    if (pass.row_tiles > 0) {
+    if (pass.tensor_cores) {
         e = wide_float(*call) ? launch_attention_forward_wide(p, s) : launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
-        if (e == cudaErrorNotSupported && p.D > 64) p.tiles *= 2;      // the other kernel's tiles have 64 states
+        if (e == cudaErrorNotSupported && p.D > 64 && pass.row_tiles > 0) p.tiles *= 2;      // the other kernel's tiles have 64 states
     }
     if (e == cudaErrorNotSupported) e = launch_attention_forward_mma(p, call->dtype, s);
     if (e == cudaSuccess && p.splits > 1) e = launch_attention_join(p, call->dtype, s);
@@ -299,7 +328,7 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
     p.part = p.delta + delta_bytes(*call) / 4;
     int launches = 3;
     cudaError_t e = launch_attention_delta(p, call->dtype, s);
-    if (call->dtype == MSDA_B200_F32 && keys.row_tiles > 0) {
+    if (call->dtype == MSDA_B200_F32 && keys.tensor_cores) {
         const int64_t gs[3] = {call->queries * call->heads * call->head_dim, call->heads * call->head_dim, call->head_dim};
         char *terms = reinterpret_cast<char *>(p.part) + round16(std::max(keys.bytes, rows.bytes));
         const int64_t state_terms = term_bytes(*call, call->states, call->kv_heads), row_terms = term_bytes(*call, call->queries, call->heads);
@@ -318,7 +347,7 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
         p.part2 = p.part + (int64_t)keys.split.splits * p.B * p.K * p.S * p.D;
         e = launch_backward(p, keys, call->dtype, true, s);
         if (e == cudaSuccess && p.splits > 1) e = launch_attention_sum(p, true, call->dtype, s);
-        launches += (p.splits > 1) + (wide_float(*call) && keys.row_tiles > 0);
+        launches += (p.splits > 1) + (wide_float(*call) && keys.tensor_cores);
     }
     if (e == cudaSuccess) {
         e = launch_backward(p, rows, call->dtype, false, s);

@@ -164,9 +164,9 @@ inline cudaError_t launch_dependent(void (*kernel)(Formal...), dim3 grid, unsign
 }
 
 cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream);
-// 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to an item, stretches of
-// whole tiles of 64 states (128 of 16 bits where D > 64).  cudaErrorNotSupported (and nothing launched) where an operand cannot
-// be described to TMA.
+// 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to a CTA (0: a small
+// CTA of 128 rows), stretches of whole tiles of 64 states (128 of 16 bits where D > 64, but for small CTAs).
+// cudaErrorNotSupported (and nothing launched) where an operand cannot be described to TMA.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
 // float32 of 65 to 128 channels, the same way (backward: of a pass over the held states both gradients)
 cudaError_t launch_attention_forward_wide(const AttentionParams &p, cudaStream_t stream);

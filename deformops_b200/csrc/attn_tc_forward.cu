@@ -11,7 +11,10 @@
 // KW groups share a row tile and take the state tiles in turn, each with a maximum, sum and O of its
 // own; at the end the parts are weighted and added.  The work is bound by latencies of a group's cycle
 // (scores, loads, exponentials, stores, product), so as many groups as tensor memory holds run at once:
-// four with BN = 64 up to 64 channels, two with BN = 128 above.
+// four with BN = 64 up to 64 channels, two with BN = 128 above.  Short passes are bound by the beginning and end of a
+// CTA and take one group, 128 rows and a share of the SM: three CTAs to it, two above 64 channels (four of up to 64
+// channels fit, with fewer registers: 19.0 us against 17.0 for 4 x 4096 rows of 8 heads over 64 states, and 30.7
+// with big CTAs).
 //
 // The running maximum is only raised when a row would leave exp2's range of 2^8 above it: then the
 // row's sums in tensor memory are scaled, which is rare after the first tiles, and exact in between (a
@@ -30,14 +33,18 @@ constexpr int kTileRows = 128;
 
 template <int DP, int RT, int KW, int TERMS>
 struct Shape {
-    static constexpr int BN = DP == 128 ? 128 : 64;            // states of a tile
-    static constexpr int ST = DP == 128 || DP * TERMS > 128 ? KW + 1 : TERMS == 3 ? 6 : 8;     // tiles of k and v in flight
+    static constexpr bool kSmall = RT * KW == 1;               // several CTAs to an SM
+    static constexpr int BN = DP == 128 && !kSmall ? 128 : 64; // states of a tile
+    static constexpr int ST = kSmall ? 2 : DP == 128 || DP * TERMS > 128 ? KW + 1 : TERMS == 3 ? 6 : 8;     // tiles of k and v in flight
     static constexpr int kGroups = RT * KW;
     static constexpr int kThreads = kGroups * 128 + 128;
     // columns of tensor memory of a group: S, in whose place P comes (a third term needs more), O
     static constexpr uint32_t kWeights = BN / 2, kO = std::max<uint32_t>(BN, TERMS * kWeights), kColumns = kO + DP;
+    static constexpr int kAllocated = !kSmall ? 512 : kColumns <= 128 ? 128 : 256;
+    static constexpr int kCtas = !kSmall ? 1 : std::min<int>(3, 512 / kAllocated);
     // what a thread may hold: all of the block's at launch, less what the last four warps need
-    static constexpr int kRegisters = kGroups == 4 ? 104 : 224, kFew = kGroups == 4 ? 64 : 56;
+    static constexpr int kRegisters = kSmall ? (kCtas == 3 ? 128 : 200) : kGroups == 4 ? 104 : 224;
+    static constexpr int kFew = kSmall ? (kCtas == 3 ? 32 : 56) : kGroups == 4 ? 64 : 56;
     static_assert(kGroups * kColumns <= 512);
     static_assert(ST > KW);                                    // a tile is freed KW tiles after its scores
 };
@@ -80,7 +87,7 @@ struct Words {
 };
 
 template <typename T, int DP, int RT, int KW, int TERMS>
-__global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, RT, KW, TERMS>::kCtas)
     attention_forward_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ tc::TensorMap km,
                                 const __grid_constant__ tc::TensorMap vm) {
     using namespace tc;
@@ -102,17 +109,31 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
     const int b = (int)(of / p.K), h = (int)(of - b * p.K);
     const uint32_t *words = key_words_of(p, b, h);
 
-    if (warp == kLast) tmem_alloc(&sm.tmem, 512);
-    if (threadIdx.x == 0) {
+    if (warp == kLast + 1) tmem_alloc(&sm.tmem, Sh::kAllocated);
+    if (warp == kLast && elect_one()) {
         for (int s = 0; s < ST; ++s) {
             barrier_init(&sm.full[s], 1), barrier_init(&sm.free[s], 1), barrier_init(&sm.clean[s], 32);
         }
         for (int g = 0; g < Sh::kGroups; ++g)
             barrier_init(&sm.s_full[g], 1), barrier_init(&sm.p_full[g], 128), barrier_init(&sm.o_full[g], 1);
+        fence_async_shared();
     }
+    __syncwarp();
     grid_launch_dependents();
     grid_dependency_wait();            // (of what this call has launched before: masks, terms)
     const Tiles<BN> tiles(p, b, h, part);
+    const auto load = [&](int n, int stage) {
+        const int state = (int)(tiles[n] & 0x7fffffff) * BN;
+        barrier_expect(&sm.full[stage], 2 * TERMS * kTile);
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) {
+            load_rows<DP, BN>(sm.k[stage][i], km, &sm.full[stage], b + i * p.B, h, state);
+            load_rows<DP, BN>(sm.v[stage][i], vm, &sm.full[stage], b + i * p.B, h, state);
+        }
+    };
+    // the first tiles are on their way while the rows of q come
+    if (warp == kLast && elect_one())
+        for (int n = 0; n < ST && n < tiles.count; ++n) load(n, n);
     if (warp < 4 * RT) {
         // a thread to a row of q
         const int r = first + threadIdx.x;
@@ -322,18 +343,13 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
     } else {
         registers_down<Sh::kFew>();
         if (warp == kLast && elect_one()) {
-            int n = 0;
+            int n = min(ST, tiles.count);
             Ring<ST> ring;
+            ring.next(n);
             for (; fine && n < tiles.count; ++n, ring.next()) {
-                const int stage = ring.at, state = (int)(tiles[n] & 0x7fffffff) * BN;
-                fine = barrier_wait(&sm.free[stage], ring.parity ^ 1);
+                fine = barrier_wait(&sm.free[ring.at], ring.parity ^ 1);
                 if (!fine) break;
-                barrier_expect(&sm.full[stage], 2 * TERMS * kTile);
-#pragma unroll
-                for (int i = 0; i < TERMS; ++i) {
-                    load_rows<DP, BN>(sm.k[stage][i], km, &sm.full[stage], b + i * p.B, h, state);
-                    load_rows<DP, BN>(sm.v[stage][i], vm, &sm.full[stage], b + i * p.B, h, state);
-                }
+                load(n, ring.at);
             }
             // nothing may still be on its way when the CTA ends
             for (int s = 0; s < ST && !fine; ++s) {
@@ -419,10 +435,10 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, 1)
         }
     }
     __syncthreads();
-    if (warp == kLast) {
+    if (warp == kLast + 1) {
         __syncwarp();
         fence_after();
-        tmem_free(tmem, 512);
+        tmem_free(tmem, Sh::kAllocated);
     }
 }
 
@@ -445,7 +461,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
     }
     const auto kernel = attention_forward_tc_kernel<T, DP, RT, KW, TERMS>;
     constexpr size_t smem = sizeof(Shared<DP, RT, KW, TERMS>);
-    static_assert(smem <= 227 * 1024);
+    static_assert((smem + 1024) * Sh::kCtas <= 228 * 1024);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + RT * kTileRows - 1) / (RT * kTileRows));
@@ -455,6 +471,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_typed(const AttentionParams &p, int row_tiles, cudaStream_t stream) {
+    if (row_tiles == 0) return p.D <= 32 ? launch<T, 32, 1, 1>(p, stream) : p.D <= 64 ? launch<T, 64, 1, 1>(p, stream) : launch<T, 128, 1, 1>(p, stream);
     if (p.D <= 32) return row_tiles == 1 ? launch<T, 32, 1, 4>(p, stream) : launch<T, 32, 2, 2>(p, stream);
     if (p.D <= 64) return row_tiles == 1 ? launch<T, 64, 1, 4>(p, stream) : launch<T, 64, 2, 2>(p, stream);
     return row_tiles == 1 ? launch<T, 128, 1, 2>(p, stream) : launch<T, 128, 2, 1>(p, stream);
@@ -462,6 +479,7 @@ cudaError_t launch_typed(const AttentionParams &p, int row_tiles, cudaStream_t s
 
 cudaError_t launch_float(const AttentionParams &p, int row_tiles, cudaStream_t stream) {
     using T = __nv_bfloat16;
+    if (row_tiles == 0) return launch<T, 32, 1, 1, 3>(p, stream);
     if (p.D <= 32) return row_tiles == 1 ? launch<T, 32, 1, 4, 3>(p, stream) : launch<T, 32, 2, 2, 3>(p, stream);
     return row_tiles == 1 ? launch<T, 64, 1, 2, 3>(p, stream) : launch<T, 64, 2, 1, 3>(p, stream);
 }
