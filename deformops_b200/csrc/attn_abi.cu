@@ -41,19 +41,41 @@ struct Cost {
     int64_t tile, item, join, at_once;
 };
 
-// The number of splits that ends soonest, with items of at most `most` tiles.
-AttentionSplit even_split(int64_t items, int64_t tiles, const Cost &cost, int64_t most, int64_t *best_cost = nullptr) {
-    const int64_t fewest = std::max<int64_t>(1, (tiles + most - 1) / most);
+// Of `fewest` to `most` stretches of `tiles` tiles the number that cost(stretches, tiles of each) has lowest: all small
+// numbers, a few of the larger ones, and `full`, with which the GPU is just full.
+template <typename F>
+AttentionSplit best_split(int64_t tiles, int64_t fewest, int64_t most, int64_t full, const F &cost, int64_t *best_cost = nullptr) {
     int64_t best = fewest, lowest = INT64_MAX;
-    for (int64_t s = fewest; s <= std::max<int64_t>(fewest, std::min<int64_t>(tiles / 2, 148 * cost.at_once)); ++s) {
-        const int64_t each = (tiles + s - 1) / s, turns = std::max(cost.at_once, (items * s + 147) / 148);
-        const int64_t all = turns * (each * cost.tile + cost.item + (s > 1 ? cost.join : 0)) + (s > 1 ? 80 : 0);
+    const auto consider = [&](int64_t s) {
+        const int64_t all = cost(s, (tiles + s - 1) / s);
         if (all < lowest) best = s, lowest = all;
-        if (items * s > 148 * 8 * cost.at_once) break;
-    }
+    };
+    for (int64_t s = fewest; s <= std::max(fewest, most); s += 1 + s / 16) consider(s);
+    if (full > fewest && full <= most) consider(full);
     if (best_cost != nullptr) *best_cost = lowest;
     const int64_t each = std::max<int64_t>(1, (tiles + best - 1) / best);
     return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
+}
+
+// the number of splits that ends soonest, with items of at most `most` tiles
+AttentionSplit even_split(int64_t items, int64_t tiles, const Cost &cost, int64_t most, int64_t *best_cost = nullptr) {
+    const int64_t at_once = 148 * cost.at_once;
+    return best_split(tiles, std::max<int64_t>(1, (tiles + most - 1) / most), std::min({tiles / 2, at_once, at_once * 8 / items + 1}), at_once / items,
+                      [&](int64_t s, int64_t each) {
+                          return std::max(cost.at_once, (items * s + 147) / 148) * (each * cost.tile + cost.item + (s > 1 ? cost.join : 0)) +
+                                 (s > 1 ? 80 : 0);
+                      },
+                      best_cost);
+}
+
+// The same where `slots` CTAs of four warps run at a time, whatever else does: a stretch takes its blocks and about 8
+// more, parts 16 and some to join.  Four parts for 512 (sample, head)s of 4000 states of 64 channels are 89 us where one
+// is 97 (only 512 of 740 slots have work), for 512 of 8000 of 128 channels 353 us and 464 (444 slots); 18 for 8 of
+// 1500 states 6.2 us, one 15.2; one for 8 of 77 states 3.3 us, two 5.0.
+AttentionSplit few_split(int64_t items, int64_t blocks, int64_t slots) {
+    return best_split(blocks, 1, std::min(blocks / 4, slots * 8 / items + 1), slots / items, [&](int64_t s, int64_t each) {
+        return (items * s + slots - 1) / slots * (each + 8) + (s > 1 ? 16 + s / 4 : 0);
+    });
 }
 
 // Float32 sums on the tensor cores are cut off, not rounded, at every product that is added: with at most 32
@@ -68,13 +90,14 @@ bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 
 // are fits of times (0.7 us for 20 with up to 64 channels, 2 us with 128).  bf16, 4096 rows of 32 heads of 64: small ones
 // 20.7 us over 77 states and 205 over 4096, big ones 31.3 and 265 (in two parts; 214 in one); 1 x 16 384 x 16 heads
 // over 4096: big 361 us, small 399; 64 heads of 100 rows over 17 821 states: one tile to a CTA 61 us, small 84.
+// float32, 8 heads of 32 for 8 x 640 rows over 4096: small 174 us, big 197.
 void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
     const int64_t most = c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles, bk = c.batch * c.kv_heads;
     const bool half = c.dtype != MSDA_B200_F32, wide = wide_float(c), deep = c.head_dim > 64 && !wide;
     const int64_t tiles = (c.states + 63) / 64, big = deep ? (c.states + 127) / 128 : tiles, one = (rows + 127) / 128, two = (rows + 255) / 256;
     int64_t lowest;
     pass.row_tiles = 1;
-    pass.split = even_split(bk * one, big, {deep ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most, &lowest);
+    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most, &lowest);
     if (wide) return;
     const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost) {
         int64_t all;
@@ -83,7 +106,7 @@ void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
     };
     take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1});
     if (deep) take(0, bk * one, tiles, {7, 40, 30, 2});
-    else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {13, 50, 30, 3});
+    else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {half ? 13 : 11, 50, 30, 3});
 }
 
 Pass forward_pass(const msda_b200_attention &c) {
@@ -93,9 +116,8 @@ Pass forward_pass(const msda_b200_attention &c) {
         pass.tensor_cores = true;
         plan_forward(c, rows, pass);
     } else {
-        // a stretch has some blocks for each of its four warps
         const FewShape few = attention_few_shape(c.dtype, c.head_dim, rows);
-        pass.split = attention_split(bk, (c.states + few.block - 1) / few.block, 148 * few.resident, 16);
+        pass.split = few_split(bk, (c.states + few.block - 1) / few.block, 148 * few.resident);
     }
     const int64_t parts = pass.split.splits * bk * rows;
     pass.bytes = pass.split.splits > 1 ? round16(parts * 4) + parts * c.head_dim * 4 : 0;
