@@ -78,9 +78,10 @@ AttentionSplit few_split(int64_t items, int64_t blocks, int64_t slots) {
     });
 }
 
-// Float32 sums on the tensor cores are cut off, not rounded, at every product that is added: with at most 32
-// tiles (2048 states or rows) to a part, and parts added with rounding, that stays near 2^-20.
-constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 32;
+// Float32 sums on the tensor cores are cut off, not rounded, at every product that is added to them: 2^-25.7 of the sum
+// each, 24 times a tile with the six products of terms.  Sums over 32 tiles were 1.4e-5 off (normal inputs, relative);
+// of at most 8 tiles (512 states or rows), the parts added with rounding, they are 3e-6.
+constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 8;
 constexpr int64_t kFewRows = 16;
 
 bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 && c.head_dim > 64; }
@@ -92,21 +93,23 @@ bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 
 // over 4096: big 361 us, small 399; 64 heads of 100 rows over 17 821 states: one tile to a CTA 61 us, small 84.
 // float32, 8 heads of 32 for 8 x 640 rows over 4096: small 174 us, big 197.
 void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
-    const int64_t most = c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles, bk = c.batch * c.kv_heads;
+    const int64_t bk = c.batch * c.kv_heads;
     const bool half = c.dtype != MSDA_B200_F32, wide = wide_float(c), deep = c.head_dim > 64 && !wide;
     const int64_t tiles = (c.states + 63) / 64, big = deep ? (c.states + 127) / 128 : tiles, one = (rows + 127) / 128, two = (rows + 255) / 256;
+    // `groups` with sums of their own share a part
+    const auto most = [&](int groups) { return half ? kMostTiles : kMostFloatTiles * groups; };
     int64_t lowest;
     pass.row_tiles = 1;
-    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most, &lowest);
+    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most(wide ? 1 : c.head_dim <= 32 ? 4 : 2), &lowest);
     if (wide) return;
-    const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost) {
+    const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost, int groups) {
         int64_t all;
-        const AttentionSplit split = even_split(items, of, cost, most, &all);
+        const AttentionSplit split = even_split(items, of, cost, most(groups), &all);
         if (all < lowest) lowest = all, pass.split = split, pass.row_tiles = row_tiles;
     };
-    take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1});
-    if (deep) take(0, bk * one, tiles, {7, 40, 30, 2});
-    else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {half ? 13 : 11, 50, 30, 3});
+    take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1}, c.head_dim <= 32 ? 2 : 1);
+    if (deep) take(0, bk * one, tiles, {7, 40, 30, 2}, 1);
+    else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {half ? 13 : 11, 50, 30, 3}, 1);
 }
 
 Pass forward_pass(const msda_b200_attention &c) {
