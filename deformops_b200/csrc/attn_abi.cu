@@ -97,17 +97,17 @@ void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
     const bool half = c.dtype != MSDA_B200_F32, wide = wide_float(c), deep = c.head_dim > 64 && !wide;
     const int64_t tiles = (c.states + 63) / 64, big = deep ? (c.states + 127) / 128 : tiles, one = (rows + 127) / 128, two = (rows + 255) / 256;
     // `groups` with sums of their own share a part
-    const auto most = [&](int groups) { return half ? kMostTiles : kMostFloatTiles * groups; };
+    const auto most = [&](int groups) { return half || (c.head_dim > 32 && !wide) ? kMostTiles : kMostFloatTiles * groups; };
     int64_t lowest;
     pass.row_tiles = 1;
-    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most(wide ? 1 : c.head_dim <= 32 ? 4 : 2), &lowest);
+    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most(wide ? 1 : 4), &lowest);
     if (wide) return;
     const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost, int groups) {
         int64_t all;
         const AttentionSplit split = even_split(items, of, cost, most(groups), &all);
         if (all < lowest) lowest = all, pass.split = split, pass.row_tiles = row_tiles;
     };
-    take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1}, c.head_dim <= 32 ? 2 : 1);
+    take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1}, 2);
     if (deep) take(0, bk * one, tiles, {7, 40, 30, 2}, 1);
     else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {half ? 13 : 11, 50, 30, 3}, 1);
 }
@@ -135,7 +135,7 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
         pass.tensor_cores = true;
         const int64_t x_rows = keys || wide_float(c) ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
         pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, {20, 120, 60, 1},
-                                c.dtype == MSDA_B200_F32 ? kMostFloatTiles : kMostTiles);
+                                wide_float(c) ? kMostFloatTiles : kMostTiles);
     } else {
         const int tile = c.head_dim > 64 ? 32 : 64;
         pass.split = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);

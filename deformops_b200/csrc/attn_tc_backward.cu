@@ -35,7 +35,11 @@ struct Shape {
     static constexpr int kGroups = TERMS == 3 || DP == 128 ? 2 : 3;
     static constexpr int kThreads = kGroups * 128 + 256;
     // what a thread may hold: all of the block's at launch, shared out anew
-    static constexpr int kRegisters = kGroups == 3 ? 120 : 192, kFew = 56, kWriting = 64;
+    static constexpr int kWriting = TERMS == 1 ? 64 : KEYS && DP == 64 ? 168 : 104;
+    static constexpr int kRegisters = kGroups == 3 ? 120 : kWriting == 64 ? 192 : kWriting == 104 ? 176 : 144, kFew = 56;
+    // tiles after which the writers take the sums on: those of the tensor cores are cut off, not rounded, at every
+    // product that is added (2^-25.7 of the sum each, 24 times a tile with terms)
+    static constexpr int kRun = TERMS == 1 ? 1 << 30 : 8;
     // columns of tensor memory: of a group S and T, in whose places P and dS come (third terms need more), then the sums
     static constexpr uint32_t kS = 0, kT = 64;
     __host__ __device__ static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }
@@ -307,18 +311,13 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
         }
     } else if (warp >= kWriters) {
         // sums to memory, while the next item is worked on
-        registers_down<Sh::kWriting>();
+        if constexpr (Sh::kWriting > 128) registers_up<Sh::kWriting>(); else registers_down<Sh::kWriting>();
         const int row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         Ring<AB> sums;
         for (unsigned i = blockIdx.x; fine && i < items; i += gridDim.x) {
             const Item it = item_of(p, i, x_tiles, x_rows);
             const Walk<KEYS> walk(p, it, y_rows);
-            const bool some = walk.count > 0;
-            if (some) {
-                fine = barrier_wait(&sm.acc_full[sums.at], sums.parity);
-                fence_after();
-            }
             const int rows = KEYS ? p.S : p.R, x = it.first + row;
             const bool valid = row < x_rows && x < rows;
             const bool idle = (row & ~31) >= x_rows || it.first + (row & ~31) >= rows;
@@ -326,25 +325,60 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             const int64_t at = KEYS ? (((int64_t)it.b * p.S + x) * p.K + it.h) * p.D
                                     : (((int64_t)it.b * p.Q + query) * p.K * p.share + it.h * p.share + (x - query * p.share)) * p.D;
             const int64_t part_at = ((it.part * (int64_t)p.B * p.K + it.bh) * rows + x) * p.D;
+            constexpr int kOf = TERMS == 3 ? (int)Sh::kSums : 2;
+            [[maybe_unused]] float sum[kOf];          // float32: of the runs so far
+#pragma unroll
+            for (int c = 0; c < kOf; ++c) sum[c] = 0.f;
+            if constexpr (TERMS == 3) {
+                for (int j = 0; j < walk.count; j += Sh::kRun, sums.next()) {
+                    fine = fine && barrier_wait(&sm.acc_full[sums.at], sums.parity);
+                    fence_after();
+                    if (!idle) {
+#pragma unroll
+                        for (int d = 0; d < (int)Sh::kSums; d += 16) {
+                            uint32_t v[16];
+                            tmem_load16(v, tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + d);
+                            tmem_wait_load();
+                            loaded(v);
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) sum[d + c] += __uint_as_float(v[c]);
+                        }
+                    }
+                    fence_before();
+                    barrier_arrive(&sm.acc_free[sums.at]);
+                }
+            } else if (walk.count > 0) {
+                fine = barrier_wait(&sm.acc_full[sums.at], sums.parity);
+                fence_after();
+            }
 #pragma unroll
             for (int which = KEYS ? 0 : 1; which < 2; ++which) {
-                const uint32_t acc = tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + (KEYS && which == 1 ? DP : 0);
+                constexpr int kSecond = KEYS ? DP : 0;
+                const uint32_t acc = tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + (which == 1 ? kSecond : 0);
                 const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale;
                 Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
                 float *parts = (which == 0 ? p.part2 : p.part) + part_at;
 #pragma unroll
                 for (int d = 0; d < DP; d += 16) {
-                    uint32_t v[16];
-                    if (some && !idle) {
-                        tmem_load16(v, acc + d);
-                        tmem_wait_load();
-                        loaded(v);
-                    }
                     float2 y[8];
+                    if constexpr (TERMS == 3) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        y[c] = some ? make_float2(__uint_as_float(v[2 * c]) * factor, __uint_as_float(v[2 * c + 1]) * factor)
-                                    : make_float2(0.f, 0.f);
+                        for (int c = 0; c < 8; ++c) {
+                            const int of = (which == 1 ? kSecond : 0) + d + 2 * c;
+                            y[c] = make_float2(sum[of] * factor, sum[of + 1] * factor);
+                        }
+                    } else {
+                        uint32_t v[16];
+                        if (walk.count > 0 && !idle) {
+                            tmem_load16(v, acc + d);
+                            tmem_wait_load();
+                            loaded(v);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            y[c] = walk.count > 0 ? make_float2(__uint_as_float(v[2 * c]) * factor, __uint_as_float(v[2 * c + 1]) * factor)
+                                                  : make_float2(0.f, 0.f);
+                    }
                     if (!valid) continue;
 #pragma unroll
                     for (int c = 0; c < 8; c += 4) {
@@ -362,7 +396,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                     }
                 }
             }
-            if (some) {
+            if (TERMS == 1 && walk.count > 0) {
                 fence_before();
                 barrier_arrive(&sm.acc_free[sums.at]);
                 sums.next();
@@ -516,11 +550,12 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         if (j == walk.count - 1) commit(&sm.x_free[buffer]);
                     }
                     if (waiting == kGroups - 1) issue_sums();
-                    const Pending t = {group, groups.parity, y, sums, j == 0, j == walk.count - 1};
+                    const Pending t = {group, groups.parity, y, sums, j % Sh::kRun == 0, (j + 1) % Sh::kRun == 0 || j == walk.count - 1};
                     if (kGroups == 2 || waiting == 0) queue[0] = t; else queue[kGroups - 2] = t;
                     ++waiting;
+                    if (t.last) sums.next();
                 }
-                x.next(), sums.next();
+                x.next();
             }
             while (fine && waiting > 0) issue_sums();
         } else if (warp == kLast + 3 && !KEYS && p.key_words != nullptr) {

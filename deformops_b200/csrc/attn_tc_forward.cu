@@ -45,6 +45,11 @@ struct Shape {
     // what a thread may hold: all of the block's at launch, less what the last four warps need
     static constexpr int kRegisters = kSmall ? (kCtas == 3 ? 128 : 200) : kGroups == 4 ? 104 : 224;
     static constexpr int kFew = kSmall ? (kCtas == 3 ? 32 : 56) : kGroups == 4 ? 64 : 56;
+    // Tiles after which a group takes its sums on in registers: those of the tensor cores are cut off, not rounded, at
+    // every product that is added (2^-25.7 of the sum each, 24 times a tile with terms).  Up to 32 channels there are
+    // no registers for it, and parts are short instead.
+    static constexpr bool kRuns = TERMS == 3 && DP == 64;
+    static constexpr int kRun = kRuns ? 8 : 1 << 30;
     static_assert(kGroups * kColumns <= 512);
     static_assert(ST > KW);                                    // a tile is freed KW tiles after its scores
 };
@@ -179,6 +184,20 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
         if (rw == nullptr) rw = words;
         float m = -INFINITY, l = 0.f;
         int done = 0;
+        [[maybe_unused]] float sums[Sh::kRuns ? DP : 1] = {};      // of the runs so far
+        const auto take_on = [&] {
+            if constexpr (Sh::kRuns) {
+#pragma unroll
+                for (int d = 0; d < DP; d += 16) {
+                    uint32_t o[16];
+                    tmem_load16(o, mine + kO + d);
+                    tmem_wait_load();
+                    loaded(o);
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) sums[d + c] += __uint_as_float(o[c]);
+                }
+            }
+        };
         const bool own_words = p.row_words != nullptr;
         uint32_t entry = way < tiles.count ? tiles[way] : 0;
         Words<NW> see{};
@@ -195,6 +214,8 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
             if (!fine) break;
             fence_after();
             if (!idle) {
+                const bool starts = done % Sh::kRun == 0;          // a run; what was summed before lies there still
+                if (starts && done > 0) take_on();
                 uint32_t s[NW][32];
 #pragma unroll
                 for (int j = 0; j < NW; ++j) tmem_load32(s[j], mine + 32 * j);
@@ -224,7 +245,11 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
                     const float keep = to == -INFINITY ? 1.f : fast_exp2(m - to);
                     m = to;
                     l *= keep;
-                    if (done > 0) {        // (that the scores are there says that the product before is done)
+                    if constexpr (Sh::kRuns) {
+#pragma unroll
+                        for (int d = 0; d < DP; ++d) sums[d] *= keep;
+                    }
+                    if (!starts) {         // (that the scores are there says that the product before is done)
 #pragma unroll
                         for (int d = 0; d < DP; d += 16) {
                             uint32_t o[16];
@@ -271,6 +296,19 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
         if (done > 0) {
             fine = fine && barrier_wait(&sm.o_full[group], 0);
             fence_after();
+        }
+        if constexpr (Sh::kRuns) {
+            if (done > Sh::kRun && !idle) {
+                take_on();
+#pragma unroll
+                for (int d = 0; d < DP; d += 16) {
+                    uint32_t o[16];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(sums[d + c]);
+                    tmem_store16(mine + kO + d, o);
+                }
+                tmem_wait_store();
+            }
         }
         if (!fine) l = NAN;
         float factor[KW], lse;
@@ -389,7 +427,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
 #pragma unroll
                                 for (int j = 0; j < BN; j += 16)
                                     mma_ts<kRow>(at + kO, at + left_term(i) * kP + j / 2, va + (right_term(i) * kTile + j * kRow >> 4), kOut,
-                                                 round > 1 || j > 0 || i > kPairs - kPairsOf);
+                                                 (round - 1) % Sh::kRun != 0 || j > 0 || i > kPairs - kPairsOf);
                             }
                             if (q == RT - 1) commit(&sm.free[last]);
                             if (!scores) commit(&sm.o_full[group]);
