@@ -78,9 +78,9 @@ AttentionSplit few_split(int64_t items, int64_t blocks, int64_t slots) {
     });
 }
 
-// Float32 sums on the tensor cores are cut off, not rounded, at every product that is added to them: 2^-25.7 of the sum
-// each, 24 times a tile with the six products of terms.  Sums over 32 tiles were 1.4e-5 off (normal inputs, relative);
-// of at most 8 tiles (512 states or rows), the parts added with rounding, they are 3e-6.
+// Float32 sums on the tensor cores are cut off, not rounded, at every product that is added to them.  The kernels take
+// them on in registers after a few tiles, but for the forward pass up to 32 channels, which has none to spare: there a
+// group has at most eight tiles of a part (over 32 the result was 1.1e-5 off, relative; over eight it is 3e-6).
 constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 8;
 constexpr int64_t kFewRows = 16;
 
@@ -97,10 +97,10 @@ void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
     const bool half = c.dtype != MSDA_B200_F32, wide = wide_float(c), deep = c.head_dim > 64 && !wide;
     const int64_t tiles = (c.states + 63) / 64, big = deep ? (c.states + 127) / 128 : tiles, one = (rows + 127) / 128, two = (rows + 255) / 256;
     // `groups` with sums of their own share a part
-    const auto most = [&](int groups) { return half || (c.head_dim > 32 && !wide) ? kMostTiles : kMostFloatTiles * groups; };
+    const auto most = [&](int groups) { return half || c.head_dim > 32 ? kMostTiles : kMostFloatTiles * groups; };
     int64_t lowest;
     pass.row_tiles = 1;
-    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most(wide ? 1 : 4), &lowest);
+    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most(4), &lowest);
     if (wide) return;
     const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost, int groups) {
         int64_t all;
@@ -134,8 +134,7 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
     if (share <= 64) {
         pass.tensor_cores = true;
         const int64_t x_rows = keys || wide_float(c) ? 128 : 128 / share * share, y_rows = keys ? 64 / share * share : 64;
-        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, {20, 120, 60, 1},
-                                wide_float(c) ? kMostFloatTiles : kMostTiles);
+        pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, {20, 120, 60, 1}, kMostTiles);
     } else {
         const int tile = c.head_dim > 64 ? 32 : 64;
         pass.split = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);

@@ -38,8 +38,9 @@ struct Shape {
     static constexpr int kWriting = TERMS == 1 ? 64 : KEYS && DP == 64 ? 168 : 104;
     static constexpr int kRegisters = kGroups == 3 ? 120 : kWriting == 64 ? 192 : kWriting == 104 ? 176 : 144, kFew = 56;
     // tiles after which the writers take the sums on: those of the tensor cores are cut off, not rounded, at every
-    // product that is added (2^-25.7 of the sum each, 24 times a tile with terms)
-    static constexpr int kRun = TERMS == 1 ? 1 << 30 : 8;
+    // product that is added (2^-25.7 of the sum each, 24 times a tile with terms): over 32 tiles gradients were 1.4e-5
+    // off, with runs of eight 3.3e-6, of four 1.6e-6, in the same time
+    static constexpr int kRun = TERMS == 1 ? 1 << 30 : 4;
     // columns of tensor memory: of a group S and T, in whose places P and dS come (third terms need more), then the sums
     static constexpr uint32_t kS = 0, kT = 64;
     __host__ __device__ static constexpr uint32_t third(bool p) { return KEYS && !p ? 160 : 128; }

@@ -49,7 +49,7 @@ struct Shape {
     // every product that is added (2^-25.7 of the sum each, 24 times a tile with terms).  Up to 32 channels there are
     // no registers for it, and parts are short instead.
     static constexpr bool kRuns = TERMS == 3 && DP == 64;
-    static constexpr int kRun = kRuns ? 8 : 1 << 30;
+    static constexpr int kRun = kRuns ? 4 : 1 << 30;
     static_assert(kGroups * kColumns <= 512);
     static_assert(ST > KW);                                    // a tile is freed KW tiles after its scores
 };

@@ -21,7 +21,7 @@
 // FORWARD and VALUES have the scores of the next tile formed while one warpgroup, a thread to a row, works on this
 // one's: bound by the tensor cores, 96 products of 32 cycles a tile.  KEYS and ROWS have no columns left for that; two
 // warpgroups share the columns of a tile, and the tensor cores wait for them.  2 x 2048 queries over 4096 states, 16
-// heads on 4 of 128 channels: 591 us forward and 2444 us backward (1395 and 1350 TFLOP/s of bf16 products); products of
+// heads on 4 of 128 channels: 573 us forward and 2642 us backward (1440 and 1250 TFLOP/s of bf16 products); products of
 // tf32 terms by warps took 20 ms for both.
 #include "attn_common.cuh"
 #include "tensor_core.cuh"
@@ -33,13 +33,19 @@ namespace {
 enum Mode { FORWARD, VALUES, KEYS, ROWS };
 
 constexpr int kX = 128, kY = 64, kD = 128, kTile = kY * kD * 2;        // (bytes of a term of a walked tile)
+// Tiles after which the sums are taken on in registers: those of the tensor cores are cut off, not rounded, at every
+// product that is added (2^-25.7 of the sum each, 24 times a tile).  Normal inputs over 2048 states: 1.4e-5 off without,
+// 3.3e-6 with runs of eight tiles, 1.6e-6 with four; a run costs a reading of the sums, 1 % of its time.
+constexpr int kRun = 4;
 constexpr uint32_t kSums = 192, kScores = 320, kBuffer = 96, kSecond = 448;
 
 template <Mode M>
 struct Shape {
     static constexpr bool kOne = M == FORWARD || M == VALUES;          // one product of scores, two tiles under way
     static constexpr bool kHoldsRows = M == FORWARD || M == ROWS;
-    static constexpr int kGroups = kOne ? 1 : 2, kThreads = 128 * kGroups + 128, kZ = kOne ? 2 : 1;
+    static constexpr int kGroups = kOne ? 1 : 2, kThreads = 128 * kGroups + 256, kZ = kOne ? 2 : 1;
+    // what a thread may hold: all of the block's at launch, shared out anew
+    static constexpr int kRegisters = kOne ? 200 : 144, kSumming = kOne ? 200 : 144, kFew = kOne ? 104 : 80;
 };
 
 template <Mode M>
@@ -47,7 +53,8 @@ struct Shared {
     alignas(1024) unsigned char y[2][3][kTile];
     alignas(1024) unsigned char z[Shape<M>::kZ][3][kTile];
     alignas(1024) unsigned char x[Shape<M>::kOne ? 1 : 2][Shape<M>::kOne ? 16 : kX * kD * 2];      // second and third term of X1
-    uint64_t y_full[2], y_free[2], z_full[2], z_free[2], clean[2], s_full[2], p_full[2], done, finished, drained;
+    float m[2][kX], l[kX];              // FORWARD: the maximum that a run's sums go by; the sum of all weights
+    uint64_t y_full[2], y_free[2], z_full[2], z_free[2], clean[2], s_full[2], p_full[2], done, run_full, run_free, m_full[2], l_full, drained;
     uint32_t tmem;
 };
 
@@ -75,7 +82,8 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
             barrier_init(&sm.y_full[s], 1), barrier_init(&sm.y_free[s], 1), barrier_init(&sm.z_full[s], 1), barrier_init(&sm.z_free[s], 1);
             barrier_init(&sm.clean[s], 32), barrier_init(&sm.s_full[s], 1), barrier_init(&sm.p_full[s], 128 * kGroups);
         }
-        barrier_init(&sm.done, 1), barrier_init(&sm.finished, 1), barrier_init(&sm.drained, 1);
+        barrier_init(&sm.done, 1), barrier_init(&sm.run_full, 1), barrier_init(&sm.run_free, 128);
+        barrier_init(&sm.m_full[0], 128), barrier_init(&sm.m_full[1], 128), barrier_init(&sm.l_full, 128), barrier_init(&sm.drained, 1);
     }
     if (y_rows < kY) {      // rows that no load reaches
         constexpr int kY16 = sizeof(sm.y) / 16, kZ16 = sizeof(sm.z) / 16;
@@ -150,6 +158,7 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
     bool fine = true;
 
     if (warp < kLast) {
+        registers_up<Sh::kRegisters>();
         const bool valid = x < held, idle = first + (row & ~31) >= held;       // (a whole warp behind the last row)
         const bool own_words = p.row_words != nullptr;
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
@@ -247,7 +256,7 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
                         const float keep = to == -INFINITY ? 1.f : fast_exp2(m - to);
                         m = to;
                         l *= keep;
-                        if (n > 0) {
+                        if (n % kRun != 0) {       // (else the sums begin anew)
                             fine = barrier_wait(&sm.done, (n - 1) & 1);
                             fence_after();
 #pragma unroll
@@ -297,156 +306,192 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
                 tmem_wait_store();
             }
             if (kOne && n > 0) fine = barrier_wait(&sm.done, (n - 1) & 1) && fine;       // (every phase is waited for)
+            if (M == FORWARD && (n % kRun == kRun - 1 || n == count - 1)) {
+                const int run = n / kRun & 1;      // (what it held two runs before is read: the run before has begun)
+                sm.m[run][row] = m;
+                barrier_arrive(&sm.m_full[run]);
+            }
             fence_before();
             barrier_arrive(&sm.p_full[buffer]);
         }
-        if (count > 0) {
-            fine = fine && barrier_wait(&sm.finished, 0);
-            fence_after();
-        }
-        float factor = M == VALUES ? 1.f : p.scale;
-        const int64_t at = (int64_t)bh * held + x, all = (int64_t)p.B * p.K * held;
         if constexpr (M == FORWARD) {
             if (!fine) l = NAN;
-            factor = l == 0.f ? 0.f : 1.f / l;
             const float lse = l == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m + log2f(l);
-            if (valid) (p.splits > 1 ? p.part_lse + part * all : p.lse)[at] = lse;
+            if (valid) (p.splits > 1 ? p.part_lse + part * ((int64_t)p.B * p.K * held) : p.lse)[(int64_t)bh * held + x] = lse;
+            sm.l[row] = l;
+            barrier_arrive(&sm.l_full);
+        }
+    } else if (warp >= kLast + 4) {
+        // the sums, a thread to a row
+        registers_up<Sh::kSumming>();
+        const bool valid = x < held, idle = first + (row & ~31) >= held;
+        float sum[kD], m = -INFINITY;
+#pragma unroll
+        for (int d = 0; d < kD; ++d) sum[d] = 0.f;
+        for (int n = 0, run = 0; fine && n < count; n += kRun, ++run) {
+            float keep = 1.f;
+            if constexpr (M == FORWARD) {
+                fine = barrier_wait(&sm.m_full[run & 1], (run >> 1) & 1);
+                const float to = sm.m[run & 1][row];
+                keep = to == -INFINITY ? 1.f : fast_exp2(m - to);
+                m = to;
+            }
+            fine = barrier_wait(&sm.run_full, run & 1) && fine;
+            if (!fine) break;
+            fence_after();
+            if (!idle) {
+#pragma unroll
+                for (int d = 0; d < kD; d += 16) {
+                    uint32_t o[16];
+                    tmem_load16(o, mine + kSums + d);
+                    tmem_wait_load();
+                    loaded(o);
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        sum[d + c] = M == FORWARD ? fmaf(sum[d + c], keep, __uint_as_float(o[c])) : sum[d + c] + __uint_as_float(o[c]);
+                }
+            }
+            fence_before();
+            barrier_arrive(&sm.run_free);
+        }
+        float factor = M == VALUES ? 1.f : p.scale;
+        if constexpr (M == FORWARD) {
+            fine = barrier_wait(&sm.l_full, 0) && fine;
+            const float l = sm.l[row];
+            factor = l == 0.f ? 0.f : 1.f / l;
         }
         if (!fine) factor = NAN;
         float *to = static_cast<float *>(M == FORWARD ? p.out : M == VALUES ? p.dv : M == KEYS ? p.dk : p.dq);
         if (p.splits > 1) {
-            to = (M == VALUES ? p.part2 : p.part) + (part * all + at) * p.D;
+            to = (M == VALUES ? p.part2 : p.part) + (part * ((int64_t)p.B * p.K * held) + (int64_t)bh * held + x) * p.D;
         } else if constexpr (kHoldsRows) {
             const int query = x / p.share;
             to += (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (x - query * p.share)) * p.D;
         } else {
             to += (((int64_t)b * p.S + x) * p.K + h) * p.D;
         }
-        if (!idle) {
+        if (valid) {
 #pragma unroll
-            for (int i = 0; i < kD / kGroups; i += 16) {
-                const int d = group * (kD / kGroups) + i;
-                uint32_t o[16];
-                tmem_load16(o, mine + kSums + d);
-                tmem_wait_load();
-                loaded(o);
-                if (!valid) continue;
-#pragma unroll
-                for (int c = 0; c < 16; c += 4) {
-                    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);        // (sums that nothing was added to are not there)
-                    if (count > 0 && factor != 0.f)
-                        f = make_float4(__uint_as_float(o[c]) * factor, __uint_as_float(o[c + 1]) * factor,
-                                        __uint_as_float(o[c + 2]) * factor, __uint_as_float(o[c + 3]) * factor);
-                    if (d + c < p.D) *reinterpret_cast<float4 *>(to + d + c) = f;
-                }
+            for (int d = 0; d < kD; d += 4) {
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (factor != 0.f) f = make_float4(sum[d] * factor, sum[d + 1] * factor, sum[d + 2] * factor, sum[d + 3] * factor);
+                if (d < p.D) *reinterpret_cast<float4 *>(to + d) = f;
             }
         }
-        fence_before();
-    } else if (warp == kLast && elect_one()) {
-        // loads, in the order in which their places get free: Y is one tile ahead
-        int ny = 0, nz = 0;
-        const auto load = [&](bool second, int &n) {
-            const bool two = !second || kZ == 2;
-            const int stage = two ? n & 1 : 0;
-            const uint32_t turn = two ? (n >> 1) & 1 : n & 1;
-            fine = fine && barrier_wait(second ? &sm.z_free[stage] : &sm.y_free[stage], turn ^ 1);
-            if (!fine) return;
-            uint64_t *full = second ? &sm.z_full[stage] : &sm.y_full[stage];
-            const int at = (int)(tile_at(n) & 0x7fffffff) * y_rows;
-            barrier_expect(full, 3 * y_rows * kD * 2);
-            for (int i = 0; i < 3; ++i)
-                load_rows<kD, kY>(second ? sm.z[stage][i] : sm.y[stage][i], second ? zm : ym, full, b + i * p.B, h, at);
-            ++n;
-        };
-        if (count > 0) load(false, ny);
-        while (fine && nz < count) {
-            if (kOne && ny < count) load(false, ny);
-            if (fine) load(true, nz);
-            if (!kOne && fine && ny < count) load(false, ny);
-        }
-        if (!fine) {     // nothing may still be on its way when the CTA ends
-            for (int s = 0; s < 2; ++s)
-                if (ny > s) barrier_wait(&sm.y_full[s], ((ny - s + 1) / 2 - 1) & 1);
-            for (int s = 0; s < kZ; ++s)
-                if (nz > s) barrier_wait(&sm.z_full[s], ((nz - s + kZ - 1) / kZ - 1) & 1);
-        }
-    } else if (warp == kLast + 1 && elect_one()) {
-        constexpr uint32_t kOf = instruction(true, kX, kY, false, false), kAdd = instruction(true, kX, kD, false, true);
-        constexpr int kTerm = kTile >> 4, kHeld = kX * kD * 2 >> 4;
-        const uint32_t y0 = descriptor(smem_address(sm.y), 16), z0 = descriptor(smem_address(sm.z), 16), x0 = descriptor(smem_address(sm.x), 16);
-        const uint32_t sums_of = descriptor(kOne ? smem_address(sm.z) : smem_address(sm.y), kY * 128);
-        const auto scores = [&](int n) {
-            fine = fine && barrier_wait(&sm.y_full[n & 1], (n >> 1) & 1);
-            if (!fine) return;
-            const uint32_t to = tmem + kScores + (kOne ? (n & 1) * kBuffer : 0), ya = y0 + (n & 1) * 3 * kTerm;
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i)
-#pragma unroll
-                for (int d = 0; d < kD; d += 16)
-                    mma_ts<128>(to, tmem + 64 * left_term(i) + d / 2, ya + right_term(i) * kTerm + ((d & 64) * kY * 2 + (d & 63) * 2 >> 4), kOf,
-                                i > 0 || d > 0);
-            if constexpr (kOne) {
-                commit(&sm.y_free[n & 1]);
-            } else {
-                fine = barrier_wait(&sm.z_full[0], n & 1);
+    } else {
+        registers_down<Sh::kFew>();
+        if (warp == kLast && elect_one()) {
+            // loads, in the order in which their places get free: Y is one tile ahead
+            int ny = 0, nz = 0;
+            const auto load = [&](bool second, int &n) {
+                const bool two = !second || kZ == 2;
+                const int stage = two ? n & 1 : 0;
+                const uint32_t turn = two ? (n >> 1) & 1 : n & 1;
+                fine = fine && barrier_wait(second ? &sm.z_free[stage] : &sm.y_free[stage], turn ^ 1);
                 if (!fine) return;
-#pragma unroll
+                uint64_t *full = second ? &sm.z_full[stage] : &sm.y_full[stage];
+                const int at = (int)(tile_at(n) & 0x7fffffff) * y_rows;
+                barrier_expect(full, 3 * y_rows * kD * 2);
+                for (int i = 0; i < 3; ++i)
+                    load_rows<kD, kY>(second ? sm.z[stage][i] : sm.y[stage][i], second ? zm : ym, full, b + i * p.B, h, at);
+                ++n;
+            };
+            if (count > 0) load(false, ny);
+            while (fine && nz < count) {
+                if (kOne && ny < count) load(false, ny);
+                if (fine) load(true, nz);
+                if (!kOne && fine && ny < count) load(false, ny);
+            }
+            if (!fine) {     // nothing may still be on its way when the CTA ends
+                for (int s = 0; s < 2; ++s)
+                    if (ny > s) barrier_wait(&sm.y_full[s], ((ny - s + 1) / 2 - 1) & 1);
+                for (int s = 0; s < kZ; ++s)
+                    if (nz > s) barrier_wait(&sm.z_full[s], ((nz - s + kZ - 1) / kZ - 1) & 1);
+            }
+        } else if (warp == kLast + 1 && elect_one()) {
+            constexpr uint32_t kOf = instruction(true, kX, kY, false, false), kAdd = instruction(true, kX, kD, false, true);
+            constexpr int kTerm = kTile >> 4, kHeld = kX * kD * 2 >> 4;
+            const uint32_t y0 = descriptor(smem_address(sm.y), 16), z0 = descriptor(smem_address(sm.z), 16), x0 = descriptor(smem_address(sm.x), 16);
+            const uint32_t sums_of = descriptor(kOne ? smem_address(sm.z) : smem_address(sm.y), kY * 128);
+            const auto scores = [&](int n) {
+                fine = fine && barrier_wait(&sm.y_full[n & 1], (n >> 1) & 1);
+                if (!fine) return;
+                const uint32_t to = tmem + kScores + (kOne ? (n & 1) * kBuffer : 0), ya = y0 + (n & 1) * 3 * kTerm;
+    #pragma unroll
                 for (int i = 0; i < kPairs; ++i)
-#pragma unroll
-                    for (int d = 0; d < kD; d += 16) {
-                        const uint32_t za = z0 + right_term(i) * kTerm + ((d & 64) * kY * 2 + (d & 63) * 2 >> 4);
-                        if (left_term(i) == 0)
-                            mma_ts<128>(to + 64, tmem + kSecond + d / 2, za, kOf, i > 0 || d > 0);
-                        else
-                            mma<128>(to + 64, x0 + (left_term(i) - 1) * kHeld + ((d & 64) * kX * 2 + (d & 63) * 2 >> 4), za, kOf, i > 0 || d > 0);
-                    }
-                commit(&sm.z_free[0]);
-            }
-            commit(&sm.s_full[n & 1]);
-        };
-        const auto sums = [&](int n) {
-            if (kOne) fine = fine && barrier_wait(&sm.z_full[n & 1], (n >> 1) & 1);
-            if (kHoldsRows && words != nullptr) fine = fine && barrier_wait(&sm.clean[n & 1], (n >> 1) & 1);
-            fine = fine && barrier_wait(&sm.p_full[n & 1], (n >> 1) & 1);
-            if (!fine) return;
-            fence_after();
-            const uint32_t from = tmem + kScores + (kOne ? (n & 1) * kBuffer : 0), of = sums_of + (n & 1) * 3 * kTerm;
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i)
-#pragma unroll
-                for (int j = 0; j < kY; j += 16)
-                    mma_ts<128>(tmem + kSums, from + 32 * left_term(i) + j / 2, of + right_term(i) * kTerm + (j * 128 >> 4), kAdd,
-                                n > 0 || i > 0 || j > 0);
-            commit(kOne ? &sm.z_free[n & 1] : &sm.y_free[n & 1]);
-            commit(&sm.done);
-        };
-        constexpr int kAhead = kOne ? 2 : 1;          // tiles whose scores are there before the first sums
-        for (int n = 0; fine && n < count + kAhead; ++n) {
-            if (n >= kAhead) sums(n - kAhead);
-            if (fine && n < count) scores(n);
-        }
-        commit(fine ? &sm.finished : &sm.drained);
-        if (!fine) barrier_wait(&sm.drained, 0);      // (else the groups wait for all that was issued)
-    } else if (warp == kLast + 2 && kHoldsRows && words != nullptr) {
-        // rows of v (of k) that nobody may see: whatever they hold, their weight is 0 and has to stay it
-        for (int n = 0; fine && n < count; ++n) {
-            const uint32_t entry = tile_at(n);
-            fine = barrier_wait(kOne ? &sm.z_full[n & 1] : &sm.y_full[n & 1], (n >> 1) & 1);
-            if (fine && !(entry >> 31)) {
-                const uint2 see = __ldg(reinterpret_cast<const uint2 *>(words) + entry);
-                constexpr int kChunks = kD / 8;
-                for (int c = lane; c < kY * kChunks; c += 32) {
-                    const int r = c / kChunks;
-                    if (!(((r < 32 ? see.x : see.y) >> (r & 31)) & 1)) {
-#pragma unroll
-                        for (int i = 0; i < 3; ++i)
-                            *reinterpret_cast<uint4 *>((kOne ? sm.z[n & (kZ - 1)][i] : sm.y[n & 1][i]) + swizzled<kD, kY>(r, c % kChunks)) =
-                                make_uint4(0, 0, 0, 0);
-                    }
+    #pragma unroll
+                    for (int d = 0; d < kD; d += 16)
+                        mma_ts<128>(to, tmem + 64 * left_term(i) + d / 2, ya + right_term(i) * kTerm + ((d & 64) * kY * 2 + (d & 63) * 2 >> 4), kOf,
+                                    i > 0 || d > 0);
+                if constexpr (kOne) {
+                    commit(&sm.y_free[n & 1]);
+                } else {
+                    fine = barrier_wait(&sm.z_full[0], n & 1);
+                    if (!fine) return;
+    #pragma unroll
+                    for (int i = 0; i < kPairs; ++i)
+    #pragma unroll
+                        for (int d = 0; d < kD; d += 16) {
+                            const uint32_t za = z0 + right_term(i) * kTerm + ((d & 64) * kY * 2 + (d & 63) * 2 >> 4);
+                            if (left_term(i) == 0)
+                                mma_ts<128>(to + 64, tmem + kSecond + d / 2, za, kOf, i > 0 || d > 0);
+                            else
+                                mma<128>(to + 64, x0 + (left_term(i) - 1) * kHeld + ((d & 64) * kX * 2 + (d & 63) * 2 >> 4), za, kOf, i > 0 || d > 0);
+                        }
+                    commit(&sm.z_free[0]);
                 }
-                fence_async_shared();
+                commit(&sm.s_full[n & 1]);
+            };
+            const auto sums = [&](int n) {
+                if (kOne) fine = fine && barrier_wait(&sm.z_full[n & 1], (n >> 1) & 1);
+                if (kHoldsRows && words != nullptr) fine = fine && barrier_wait(&sm.clean[n & 1], (n >> 1) & 1);
+                fine = fine && barrier_wait(&sm.p_full[n & 1], (n >> 1) & 1);
+                if (!fine) return;
+                fence_after();
+                const int run = n / kRun;
+                if (n % kRun == 0) fine = barrier_wait(&sm.run_free, (run & 1) ^ 1);
+                if (!fine) return;
+                const uint32_t from = tmem + kScores + (kOne ? (n & 1) * kBuffer : 0), of = sums_of + (n & 1) * 3 * kTerm;
+    #pragma unroll
+                for (int i = 0; i < kPairs; ++i)
+    #pragma unroll
+                    for (int j = 0; j < kY; j += 16)
+                        mma_ts<128>(tmem + kSums, from + 32 * left_term(i) + j / 2, of + right_term(i) * kTerm + (j * 128 >> 4), kAdd,
+                                    n % kRun != 0 || i > 0 || j > 0);
+                commit(kOne ? &sm.z_free[n & 1] : &sm.y_free[n & 1]);
+                commit(&sm.done);
+                if (n % kRun == kRun - 1 || n == count - 1) commit(&sm.run_full);
+            };
+            constexpr int kAhead = kOne ? 2 : 1;          // tiles whose scores are there before the first sums
+            for (int n = 0; fine && n < count + kAhead; ++n) {
+                if (n >= kAhead) sums(n - kAhead);
+                if (fine && n < count) scores(n);
             }
-            barrier_arrive(&sm.clean[n & 1]);
+            if (!fine) {          // (else the last run is waited for)
+                commit(&sm.drained);
+                barrier_wait(&sm.drained, 0);
+            }
+        } else if (warp == kLast + 2 && kHoldsRows && words != nullptr) {
+            // rows of v (of k) that nobody may see: whatever they hold, their weight is 0 and has to stay it
+            for (int n = 0; fine && n < count; ++n) {
+                const uint32_t entry = tile_at(n);
+                fine = barrier_wait(kOne ? &sm.z_full[n & 1] : &sm.y_full[n & 1], (n >> 1) & 1);
+                if (fine && !(entry >> 31)) {
+                    const uint2 see = __ldg(reinterpret_cast<const uint2 *>(words) + entry);
+                    constexpr int kChunks = kD / 8;
+                    for (int c = lane; c < kY * kChunks; c += 32) {
+                        const int r = c / kChunks;
+                        if (!(((r < 32 ? see.x : see.y) >> (r & 31)) & 1)) {
+    #pragma unroll
+                            for (int i = 0; i < 3; ++i)
+                                *reinterpret_cast<uint4 *>((kOne ? sm.z[n & (kZ - 1)][i] : sm.y[n & 1][i]) + swizzled<kD, kY>(r, c % kChunks)) =
+                                    make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    fence_async_shared();
+                }
+                barrier_arrive(&sm.clean[n & 1]);
+            }
         }
     }
     __syncthreads();
