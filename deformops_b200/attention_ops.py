@@ -44,11 +44,14 @@ def _strides(t: Tensor) -> list[int]:
     return [0 if n <= 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
 
 
-def _readable(t: Tensor) -> Tensor:
-    """``t`` as the kernels read it: dense last axis, everything else in whole 16-byte vectors."""
+def _readable(t: Tensor, share: int = 1) -> Tensor:
+    """``t`` as the kernels read it: dense last axis, everything else in whole 16-byte vectors, every token (and, where
+    ``share`` heads of it meet one key head, every head) at a place of its own."""
     vec = 16 // t.element_size()
+    strides = _strides(t)
     if (t.stride(3) == 1 or t.shape[3] <= 1) and t.data_ptr() % 16 == 0 and all(
-            s >= 0 and s % vec == 0 for s in _strides(t)):
+            s >= 0 and s % vec == 0 for s in strides) and not (
+            (strides[1] == 0 and t.shape[1] > 1) or (strides[2] == 0 and share > 1)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -109,7 +112,7 @@ def _forward_cuda(query, key, value, key_padding_mask, attention_mask, scale):
     lse = torch.empty((B, key.shape[2], Q, G // key.shape[2]), dtype=torch.float32, device=query.device)
     shim = load_library()
     packed = _pack(shim, query, key, key_padding_mask, attention_mask)
-    query, key, value = map(_readable, (query, key, value))
+    query, key, value = _readable(query, query.shape[2] // key.shape[2]), _readable(key), _readable(value)
     call = _call(query, key, value, packed, _mask_heads(attention_mask), scale)
     workspace = _workspace(shim, call, False, query)
     st = shim.attention_forward(ctypes.byref(call), _ptr(query), _ptr(key), _ptr(value), _ptr(out), _ptr(lse),
@@ -126,7 +129,7 @@ def _backward_cuda(query, key, value, packed, mask_heads, out, grad_output, lse,
         raise RuntimeError("grad_output must be contiguous and have the query's dtype")
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key, value)]
     shim = load_library()
-    query, key, value = map(_readable, (query, key, value))
+    query, key, value = _readable(query, query.shape[2] // key.shape[2]), _readable(key), _readable(value)
     out, grad_output = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (out.contiguous(), grad_output))
     call = _call(query, key, value, packed, mask_heads, scale)
     workspace = _workspace(shim, call, True, query)

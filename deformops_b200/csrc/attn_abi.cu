@@ -9,15 +9,12 @@
 
 namespace msda_b200 {
 
-AttentionSplit attention_split(int64_t ctas, int64_t tiles, int64_t ctas_at_once, int fewest_tiles) {
-    int64_t splits = 1;
-    if (ctas > 0 && ctas < ctas_at_once) splits = std::min(ctas_at_once / ctas, tiles / std::max(fewest_tiles, 1));
-    splits = std::max<int64_t>(1, splits);
-    const int64_t each = std::max<int64_t>(1, (tiles + splits - 1) / splits);
-    return {(int)std::max<int64_t>(1, (tiles + each - 1) / each), (int)each};
-}
-
 namespace {
+
+// how a pass over the tiles of the long axis is split: stretches, tiles of each
+struct AttentionSplit {
+    int splits, tiles;
+};
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -137,22 +134,17 @@ Pass backward_pass(const msda_b200_attention &c, bool keys) {
         pass.split = even_split(bk * ((held + x_rows - 1) / x_rows), (walked + y_rows - 1) / y_rows, {20, 120, 60, 1}, kMostTiles);
     } else {
         const int tile = c.head_dim > 64 ? 32 : 64;
-        pass.split = attention_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3, 4);
+        pass.split = few_split(bk * ((held + 63) / 64), (walked + tile - 1) / tile, 148 * 3);
     }
     pass.bytes = pass.split.splits > 1 ? (keys ? 2 : 1) * pass.split.splits * bk * held * c.head_dim * 4 : 0;
     return pass;
 }
 
-// a pass on the tensor cores, or on the other kernel (whose tiles have 64 rows, or 32) where they cannot take it
 cudaError_t launch_backward(AttentionParams &p, const Pass &pass, int dtype, bool keys, cudaStream_t stream) {
     p.splits = pass.split.splits, p.tiles = pass.split.tiles;
-    if (pass.tensor_cores) {
-        const cudaError_t e = dtype == MSDA_B200_F32 && p.D > 64 ? launch_attention_backward_wide(p, keys, stream)
-                                                                 : launch_attention_backward_tc(p, dtype, keys, stream);
-        if (e != cudaErrorNotSupported) return e;
-        if (p.D > 64) p.tiles *= 2;
-    }
-    return launch_attention_backward_mma(p, dtype, keys, stream);
+    if (!pass.tensor_cores) return launch_attention_backward_mma(p, dtype, keys, stream);
+    return dtype == MSDA_B200_F32 && p.D > 64 ? launch_attention_backward_wide(p, keys, stream)
+                                              : launch_attention_backward_tc(p, dtype, keys, stream);
 }
 
 // the terms of `tokens` x `heads` float32 rows, where a pass needs them
@@ -195,6 +187,9 @@ int check(const msda_b200_attention *c) {
         for (int i = 0; i < 3; ++i)
             if (s[i] < 0 || s[i] % vec != 0)
                 return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: strides must be whole 16-byte vectors");
+    if ((c->queries > 1 && c->query_strides[1] == 0) || (c->states > 1 && (c->key_strides[1] == 0 || c->value_strides[1] == 0)) ||
+        (c->heads > c->kv_heads && c->query_strides[2] == 0))
+        return refuse(MSDA_B200_UNSUPPORTED, "attention: tokens, and query heads that share a key head, need strides of their own");
     return MSDA_B200_OK;
 }
 
@@ -302,13 +297,9 @@ int msda_b200_attention_forward(const msda_b200_attention *call, const void *que
     p.k_terms = static_cast<char *>(workspace) + round16(pass.bytes);
     p.v_terms = static_cast<char *>(p.k_terms) + term_bytes(*call, call->states, call->kv_heads);
     const int terms = call->dtype == MSDA_B200_F32 && pass.tensor_cores ? 1 : 0;
-    cudaError_t e = cudaErrorNotSupported;
-    if (p.R <= kFewRows) e = launch_attention_few(p, call->dtype, s);
-    if (pass.tensor_cores) {
-        e = wide_float(*call) ? launch_attention_forward_wide(p, s) : launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
-        if (e == cudaErrorNotSupported && p.D > 64 && pass.row_tiles > 0) p.tiles *= 2;      // the other kernel's tiles have 64 states
-    }
-    if (e == cudaErrorNotSupported) e = launch_attention_forward_mma(p, call->dtype, s);
+    cudaError_t e = !pass.tensor_cores ? launch_attention_few(p, call->dtype, s)
+                    : wide_float(*call) ? launch_attention_forward_wide(p, s)
+                                        : launch_attention_forward_tc(p, call->dtype, pass.row_tiles, s);
     if (e == cudaSuccess && p.splits > 1) e = launch_attention_join(p, call->dtype, s);
     if (e == cudaSuccess) count_launches((p.splits > 1 ? 2 : 1) + terms, 0);
     return status_of(e);

@@ -163,10 +163,10 @@ inline cudaError_t launch_dependent(void (*kernel)(Formal...), dim3 grid, unsign
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(actual)...);
 }
 
-cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream);
 // 16-bit types, and float32 of up to 64 channels with its terms; row_tiles of 128 rows to a CTA (0: a small
 // CTA of 128 rows), stretches of whole tiles of 64 states (128 of 16 bits where D > 64, but for small CTAs).
-// cudaErrorNotSupported (and nothing launched) where an operand cannot be described to TMA.
+// cudaErrorNotSupported (and nothing launched) where an operand cannot be described to TMA.  Backward: at most 64 query
+// heads to a key head.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, int dtype, int row_tiles, cudaStream_t stream);
 // float32 of 65 to 128 channels, the same way (backward: of a pass over the held states both gradients)
 cudaError_t launch_attention_forward_wide(const AttentionParams &p, cudaStream_t stream);
@@ -178,6 +178,7 @@ struct FewShape {
 FewShape attention_few_shape(int dtype, int64_t D, int64_t rows);
 cudaError_t launch_attention_few(const AttentionParams &p, int dtype, cudaStream_t stream);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
+// the same for more of them
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream);
 
 // the terms of (B, tokens, heads, D) float32 tensors
@@ -202,11 +203,5 @@ struct MaskParams {
     uint32_t *key_words, *row_words, *lists;
 };
 cudaError_t launch_attention_mask(const MaskParams &p, cudaStream_t stream);
-
-// how a pass over `tiles` tiles of the long axis is split, given the CTAs that one stretch has
-struct AttentionSplit {
-    int splits, tiles;      // stretches, tiles of each
-};
-AttentionSplit attention_split(int64_t ctas, int64_t tiles, int64_t ctas_at_once, int fewest_tiles);
 
 }  // namespace msda_b200

@@ -1,18 +1,15 @@
-// Cross attention with warp-level matrix instructions: every type, every size.
+// Cross attention backward with warp-level matrix instructions, for more than 64 query heads to a key head: whole tokens
+// of so many rows fill no tile of the kernel of attn_tc_backward.cu.  2 x 64 queries of 130 heads over 4096 states
+// of one head of 64, float32: 1.7 ms.
 //
-// Forward: one pass over the states with the running maximum and sum of the softmax, scores and
-// weights in registers.  Backward: one kernel template in two forms.  "keys" holds 64 states and
-// walks the rows (dk, dv), the other holds 64 rows and walks the states (dq); the weights are formed
-// again in both, so that every gradient is summed by one warp in a fixed order: no atomics, the same
-// bits on every run.
+// One kernel template in two forms.  "keys" holds 64 states and walks the rows (dk, dv), the other holds 64 rows and
+// walks the states (dq); the weights are formed again in both, so that every gradient is summed by one warp in a
+// fixed order: no atomics, the same bits on every run.
 //
 // float32 operands go through the tensor cores as two terms of tf32 (x = hi + lo, 11 bits each);
 // lo * hi + hi * lo + hi * hi leaves 2^-21 of a product, sums are float32.  16-bit operands take
 // m16n8k16; the weights, and ds, are rounded to the type there (half a step each, the step of the
 // result's own rounding) and everything else stays float32.
-//
-// Where the states are many and the rows few, the states are split over CTAs and the parts joined
-// (attn_join.cu).
 #include <algorithm>
 #include <type_traits>
 
@@ -140,11 +137,9 @@ __device__ __forceinline__ void add_product_nn(float (&acc)[DP / 8][4], const fl
 
 // The same with sums kept apart for float32: a matrix instruction cuts its sum off where it should round,
 // always towards zero, which over the thousands of instructions of a long axis adds up (17 821 states: 1.6e-5 of
-// the result, against 1e-6 so).  A tile's product starts from zero and is added with rounding; with KEEP the rows
-// of acc are scaled first, as the running maximum asks.
-template <typename T, int DP, int N, bool KEEP>
-__device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float (&w)[N][4], const T *b,
-                                           const float (&keep)[2]) {
+// the result, against 1e-6 so).  A tile's product starts from zero and is added with rounding.
+template <typename T, int DP, int N>
+__device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float (&w)[N][4], const T *b) {
     if constexpr (sizeof(T) == 4) {
         float tile[DP / 8][4];
 #pragma unroll
@@ -153,15 +148,8 @@ __device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float 
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                acc[d][e] = KEEP ? fmaf(acc[d][e], keep[e >> 1], tile[d][e]) : acc[d][e] + tile[d][e];
+            for (int e = 0; e < 4; ++e) acc[d][e] += tile[d][e];
     } else {
-        if constexpr (KEEP) {
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[d][e] *= keep[e >> 1];
-        }
         add_product_nn<T, DP, N>(acc, w, b);
     }
 }
@@ -191,9 +179,6 @@ __device__ __forceinline__ void load_rows(T *to, const T *base, const int64_t (&
     }
 }
 
-template <typename T, int DP>
-constexpr int kTile = sizeof(T) == 4 && DP == 128 ? 32 : 64;      // rows of a walked tile
-
 // the first tile of `tiles` (each WORDS mask words) from t on in which some state may be seen
 template <int WORDS>
 __device__ __forceinline__ int next_tile(const uint32_t *words, int S, int t, int end) {
@@ -205,133 +190,6 @@ __device__ __forceinline__ int next_tile(const uint32_t *words, int S, int t, in
         if (any) return t;
     }
     return end;
-}
-
-// four warps, 16 rows each
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attention_forward_mma_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr int BN = kTile<T, DP>, N = BN / 8, ROWS = 64, P = kPitch<T, DP>;
-    extern __shared__ __align__(16) unsigned char smem[];
-    T *const sq = reinterpret_cast<T *>(smem);
-    T *const sk = sq + ROWS * P;                       // two stages of k and v
-    T *const sv = sk + 2 * BN * P;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const int row_tiles = (p.R + ROWS - 1) / ROWS;
-    int64_t i = blockIdx.x;
-    const int first = (int)(i % row_tiles) * ROWS;
-    i /= row_tiles;
-    const int part = (int)(i % p.splits);
-    const int64_t bh = i / p.splits;
-    const int b = (int)(bh / p.K), h = (int)(bh % p.K);
-    const T *k = static_cast<const T *>(p.k) + b * p.ks[0] + h * p.ks[2];
-    const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + h * p.vs[2];
-    const uint32_t *words = key_words_of(p, b, h);
-    const int all_tiles = (p.S + BN - 1) / BN;
-    const int end = min(all_tiles, (part + 1) * p.tiles);
-
-    int tile = next_tile<BN / 32>(words, p.S, part * p.tiles, end);
-    load_rows<T, DP, ROWS>(sq, static_cast<const T *>(p.q), p.qs, p, b, h, first);
-    if (tile < end) {
-        load_states<T, DP, BN>(sk, k, p.ks[1], tile * BN, p.S, p.D, words);
-        load_states<T, DP, BN>(sv, v, p.vs[1], tile * BN, p.S, p.D, words);
-    }
-    cp_async_commit();
-
-    float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
-    const int r0 = first + warp * 16 + g;
-    const uint32_t *rw[2] = {r0 < p.R ? row_words_of(p, b, h, r0) : nullptr,
-                             r0 + 8 < p.R ? row_words_of(p, b, h, r0 + 8) : nullptr};
-
-    for (int stage = 0; tile < end; stage ^= 1) {
-        const int next = next_tile<BN / 32>(words, p.S, tile + 1, end);
-        if (next < end) {
-            load_states<T, DP, BN>(sk + (stage ^ 1) * BN * P, k, p.ks[1], next * BN, p.S, p.D, words);
-            load_states<T, DP, BN>(sv + (stage ^ 1) * BN * P, v, p.vs[1], next * BN, p.S, p.D, words);
-        }
-        cp_async_commit();
-        cp_async_wait<1>();
-        __syncthreads();
-
-        float s[N][4];
-        product_nt<T, DP, N>(s, sq + warp * 16 * P, sk + stage * BN * P);
-        float top[2] = {m[0], m[1]}, keep[2];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int state = tile * BN + n * 8;
-            const uint32_t common = key_word(words, p.S, state >> 5);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t bits = (rw[half] != nullptr ? __ldg(rw[half] + (state >> 5)) : common) >> ((state & 31) + 2 * t);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float &x = s[n][2 * half + e];
-                    x = (bits >> e) & 1 ? x * p.scale_log2 : -INFINITY;
-                    top[half] = fmaxf(top[half], x);
-                }
-            }
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-            top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-            const float base = top[half] == -INFINITY ? 0.f : top[half];     // nothing seen so far
-            keep[half] = fast_exp2(m[half] - base);
-            m[half] = top[half];
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s[n][2 * half + e] = fast_exp2(s[n][2 * half + e] - base);
-                    sum += s[n][2 * half + e];
-                }
-            l[half] = l[half] * keep[half] + sum;
-        }
-        product_nn<T, DP, N, true>(o, s, sv + stage * BN * P, keep);
-        __syncthreads();
-        tile = next;
-    }
-    cp_async_wait<0>();
-
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int r = r0 + 8 * half;
-        if (r >= p.R) continue;
-        const float inverse = l[half] > 0.f || l[half] != l[half] ? 1.f / l[half] : 0.f;
-        // (a part that saw nothing has no weight when the parts are joined)
-        const float lse = l[half] == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m[half] + log2f(l[half]);
-        const int64_t at = bh * p.R + r;
-        if (p.splits > 1) {
-            float *to = p.part + (part * (int64_t)p.B * p.K * p.R + at) * p.D;
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-                if (d * 8 + 2 * t < p.D)
-                    *reinterpret_cast<float2 *>(to + d * 8 + 2 * t) =
-                        make_float2(o[d][2 * half] * inverse, o[d][2 * half + 1] * inverse);
-            if (t == 0) p.part_lse[part * (int64_t)p.B * p.K * p.R + at] = lse;
-        } else {
-            const int query = r / p.share;
-            T *to = static_cast<T *>(p.out) +
-                    (((int64_t)b * p.Q + query) * p.K * p.share + h * p.share + (r - query * p.share)) * p.D;
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-                if (d * 8 + 2 * t < p.D) {
-                    to[d * 8 + 2 * t] = VecTraits<T>::from_float(o[d][2 * half] * inverse);
-                    to[d * 8 + 2 * t + 1] = VecTraits<T>::from_float(o[d][2 * half + 1] * inverse);
-                }
-            if (t == 0) p.lse[at] = lse;
-        }
-    }
 }
 
 // KEYS: holds 64 states, walks the rows, sums dv = p^T do and dk = ds^T q.  Otherwise holds 64 rows,
@@ -453,8 +311,8 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
                     s[n][j] = may ? fast_exp2(s[n][j] * p.scale_log2 - row_lse) : 0.f;
                     ds[n][j] = may ? s[n][j] * (ds[n][j] - row_delta) : 0.f;
                 }
-        if constexpr (KEYS) product_nn<T, DP, N, false>(a0, s, y1 + stage * BN * P, delta);
-        product_nn<T, DP, N, false>(a1, ds, y0 + stage * BN * P, delta);
+        if constexpr (KEYS) product_nn<T, DP, N>(a0, s, y1 + stage * BN * P);
+        product_nn<T, DP, N>(a1, ds, y0 + stage * BN * P);
         __syncthreads();
         tile = next;
     }
@@ -498,13 +356,6 @@ cudaError_t launch(Kernel kernel, int64_t grid, size_t smem, cudaStream_t stream
     return launch_dependent(kernel, dim3((unsigned)grid), kThreads, smem, stream, p);
 }
 
-template <typename T, int DP>
-cudaError_t forward(const AttentionParams &p, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)(64 + 4 * kTile<T, DP>) * kPitch<T, DP> * sizeof(T);
-    const int64_t grid = (int64_t)p.B * p.K * p.splits * ((p.R + 63) / 64);
-    return launch(attention_forward_mma_kernel<T, DP>, grid, smem, stream, p);
-}
-
 template <typename T, int DP, bool KEYS>
 cudaError_t backward(const AttentionParams &p, cudaStream_t stream) {
     constexpr int BN = DP == 128 ? 32 : 64;
@@ -520,21 +371,12 @@ cudaError_t backward_side(const AttentionParams &p, bool keys, cudaStream_t stre
 }
 
 template <typename T>
-cudaError_t forward_typed(const AttentionParams &p, cudaStream_t stream) {
-    return p.D <= 32 ? forward<T, 32>(p, stream) : p.D <= 64 ? forward<T, 64>(p, stream) : forward<T, 128>(p, stream);
-}
-template <typename T>
 cudaError_t backward_typed(const AttentionParams &p, bool keys, cudaStream_t stream) {
     return p.D <= 32 ? backward_side<T, 32>(p, keys, stream)
            : p.D <= 64 ? backward_side<T, 64>(p, keys, stream) : backward_side<T, 128>(p, keys, stream);
 }
 
 }  // namespace
-
-cudaError_t launch_attention_forward_mma(const AttentionParams &p, int dtype, cudaStream_t stream) {
-    return dtype == 0 ? forward_typed<float>(p, stream)
-           : dtype == 1 ? forward_typed<__half>(p, stream) : forward_typed<__nv_bfloat16>(p, stream);
-}
 
 cudaError_t launch_attention_backward_mma(const AttentionParams &p, int dtype, bool keys, cudaStream_t stream) {
     return dtype == 0 ? backward_typed<float>(p, keys, stream)

@@ -273,13 +273,15 @@ void set_strides(const Tensor &t, int64_t (&to)[3]) {
     for (int i = 0; i < 3; ++i) to[i] = t.size(i) <= 1 ? 0 : t.stride(i);
 }
 
-// as the kernels read it: dense last axis, everything else in whole 16-byte vectors
-Tensor readable(const Tensor &t) {
+// as the kernels read it: dense last axis, everything else in whole 16-byte vectors, every token (and, where `share`
+// heads of it meet one key head, every head) at a place of its own
+Tensor readable(const Tensor &t, int64_t share = 1) {
     const int64_t vec = 16 / (int64_t)t.element_size();
     int64_t strides[3];
     set_strides(t, strides);
     bool fine = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     for (const int64_t s : strides) fine = fine && s >= 0 && s % vec == 0;
+    fine = fine && (strides[1] != 0 || t.size(1) <= 1) && (strides[2] != 0 || share <= 1);
     return fine ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -325,7 +327,7 @@ Tensor pack_mask(const Tensor &q, const Tensor &k, const Tensor &padding, const 
 std::pair<Tensor, Tensor> run_attention(const Tensor &q_in, const Tensor &k_in, const Tensor &v_in, const Tensor &packed,
                                         int64_t mask_heads, double scale) {
     const at::Device device = q_in.device();
-    const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
+    const Tensor q = readable(q_in, q_in.size(2) / k_in.size(2)), k = readable(k_in), v = readable(v_in);
     const msda_b200_attention c = attention_call(q, k, v, packed, mask_heads, scale);
     Tensor out = empty({c.batch, c.queries, c.heads * c.head_dim}, q.scalar_type(), device);
     Tensor lse = empty({c.batch, c.kv_heads, c.queries, c.heads / c.kv_heads}, at::kFloat, device);
@@ -343,7 +345,7 @@ variable_list run_attention_backward(const variable_list &saved, const Tensor &g
     RECORD_FUNCTION("deformops_b200::cross_attention_backward", std::vector<c10::IValue>());
     const at::Device device = saved[0].device();
     const c10::cuda::CUDAGuard on_device(device);
-    const Tensor q = readable(saved[0]), k = readable(saved[1]), v = readable(saved[2]);
+    const Tensor q = readable(saved[0], saved[0].size(2) / saved[1].size(2)), k = readable(saved[1]), v = readable(saved[2]);
     const Tensor &packed = saved[3], out = aligned(saved[4]), &lse = saved[5];
     const Tensor grad_out = aligned(grad_in.to(q.scalar_type()).contiguous());
     const msda_b200_attention c = attention_call(q, k, v, packed, mask_heads, scale);

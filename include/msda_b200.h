@@ -239,7 +239,8 @@ int msda_b200_launch_geometry(int64_t B, int64_t G, int64_t D, int64_t Q, int64_
  * over the states j that the mask lets query q see; h = g / (heads / kv_heads).  A query that may see
  * nothing has zeros, and no gradients.
  *   query (batch, queries, heads, head_dim), key and value (batch, states, kv_heads, head_dim): last
- *   axis dense, the other strides (in elements) given, whole 16-byte vectors; pointers 16-byte
+ *   axis dense, the other strides (in elements) given, whole 16-byte vectors (0 for samples and heads that
+ *   are all the same, but not for tokens nor for query heads that share a key head); pointers 16-byte
  *   aligned.  out and grad_out (batch, queries, heads * head_dim), grad_query like a dense query,
  *   grad_key and grad_value like a dense key.  lse (batch, kv_heads, queries, heads / kv_heads) float32: base-2
  *   logarithm of the softmax's sum, written by the forward call for the backward one.

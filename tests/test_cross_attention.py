@@ -393,6 +393,8 @@ def test_statuses_of_the_c_interface():
     assert call(head_dim=36) == -2 and call(head_dim=136) == -2 and call(states=1 << 31) == -2
     assert call(query_strides=three(512, 127, 32)) == -1 and "strides" in shim.last_error()
     assert call(key_strides=three(-8, 64, 32)) == -1
+    assert call(key_strides=three(576, 0, 32)) == -2 and call(query_strides=three(512, 128, 0)) == -2
+    assert call(query_strides=three(512, 0, 32)) == -2 and "of their own" in shim.last_error()
     assert call(queries=0) == 0 and call(batch=0) == 0
     assert shim.attention_forward(None, *[None] * 6, 0, -1, None) == -1
     # 129 states: 8 words, lists of 3 and 2 tiles with their counts (in whole 16 bytes)
