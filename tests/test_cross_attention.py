@@ -303,6 +303,88 @@ def test_captured_and_replayed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, D", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float32, 96)], ids=str)
+def test_a_captured_run_of_calls(dtype, D):
+    """Rotations, a pass over many rows and one over single tokens, one behind the other in one graph."""
+    from deformops_b200.registry import rotary
+
+    q, k, v, do = make(2, 150, 700, 4, 2, D, dtype)
+    padding = masks("padding", 2, 150, 700, 4)["key_padding_mask"]
+    places = torch.rand(700, 2, device="cuda") * 50
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        turned = rotary(k, places)
+        out = cross_attention(rotary(q, places[:150]), turned, v, key_padding_mask=padding)
+        token = cross_attention(out.view(2, 150, 4, D)[:, :1], turned, v)
+        return [out, token, *torch.autograd.grad([out, token], leaves, [do, do[:, :1]])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got))
+    with torch.no_grad():
+        for t in leaves:
+            t.mul_(-0.75)
+    torch.cuda.synchronize()
+    # the two, at once on two streams: no workspace is shared
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for stream, (graph, _) in zip(streams, graphs):
+        with torch.cuda.stream(stream):
+            graph.replay(), graph.replay()
+    torch.cuda.synchronize()
+    want = step()
+    for _, got in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Q", [2, 40])
+def test_offsets_past_32_bits(Q):
+    """A cache whose tokens lie 2^20 elements apart: the last ones behind 2^31."""
+    S, step = 2500, 1 << 20
+    q, k, v, do = make(1, Q, S, 2, 1, 64, torch.bfloat16)
+    cache = torch.empty(S * step, dtype=torch.bfloat16, device="cuda")
+    far = [cache.as_strided((1, S, 1, 64), (0, step, 0, 1), at) for at in (0, 64)]
+    for to, of in zip(far, (k, v)):
+        to.copy_(of)
+    check(run(q, *far, do), formula(q, k, v, do))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, D", [(torch.float16, 32), (torch.float16, 128), (torch.float32, 32), (torch.float32, 64),
+                                      (torch.float32, 128)], ids=str)
+@pytest.mark.parametrize("Q", [5, 200])
+def test_rows_do_not_meet(dtype, D, Q):
+    """A query that holds NaN has a result of NaN, and no other query has another result for it."""
+    q, k, v, _ = make(2, Q, 150, 4, 2, D, dtype)
+    want = cross_attention(q, k, v)
+    q[1, 2, 3, 0] = math.nan
+    got = cross_attention(q, k, v).view(2, Q, 4, D)
+    assert got[1, 2, 3].isnan().all()
+    got[1, 2, 3] = want.view_as(got)[1, 2, 3]
+    assert torch.equal(got.view_as(want), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_sums_in_float32(D):
+    """Sums on the tensor cores are cut off at every addition, by 2^-25.7 of the sum at most on average: 24 additions a
+    tile, four tiles to a sum, are 1.8e-6 of the result; scores and products with terms add a third of that."""
+    q, k, v, do = make(2, 700, 4096, 2, 2, D, torch.float32)
+    got, want = run(q, k, v, do), formula(q, k, v, do)
+    for x, (y, _) in zip(got, want):
+        assert (x.detach().double() - y).norm() <= 2.5e-6 * y.norm()
+
+
+@pytest.mark.gpu
 def test_calls_on_two_streams_at_once():
     sets = [make(2, 64, 2000, 4, 4, 64, torch.float16, seed=s) for s in range(2)]
     want = [run(*s) for s in sets]
