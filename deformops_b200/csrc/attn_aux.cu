@@ -1,6 +1,7 @@
 // Cross attention: masks to bits, rowsum(do o), and the joining of split passes.  All of them read
 // their input once and are bound by that, or by their launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.cuh"
 
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_
     const int lane = threadIdx.x & 7;
     const unsigned rows = (unsigned)p.B * p.Q * p.K * p.share;
     const unsigned first = blockIdx.x * (kThreads / 8 * kRows) + (threadIdx.x >> 3);
-    float sum[kRows] = {};
+    float sum[kRows] = {}, most = 0.f;
     for (int c = lane * kVec; c < p.D; c += 8 * kVec) {
         uint4 x[kRows], y[kRows];
 #pragma unroll
@@ -198,7 +199,10 @@ __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_
             VecTraits<T>::unpack(x[k], u);
             VecTraits<T>::unpack(y[k], v);
 #pragma unroll
-            for (int i = 0; i < kVec / 2; ++i) sum[k] += u[i].x * v[i].x + u[i].y * v[i].y;
+            for (int i = 0; i < kVec / 2; ++i) {
+                sum[k] += u[i].x * v[i].x + u[i].y * v[i].y;
+                if constexpr (std::is_same_v<T, __half>) most = fmaxf(most, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+            }
         }
     }
 #pragma unroll
@@ -209,6 +213,16 @@ __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_
         const unsigned b = token / p.Q, h = head / p.share;
         if (lane == 0 && row < rows)
             p.delta[((int64_t)b * p.K + h) * p.R + (int64_t)(token - b * p.Q) * p.share + (head - h * p.share)] = sum[k];
+    }
+    if constexpr (std::is_same_v<T, __half>) {
+        __shared__ uint32_t warps[kThreads / 32];
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = bits;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            const uint32_t all = __reduce_max_sync(0xffffffffu, warps[threadIdx.x % (kThreads / 32)]);
+            if (threadIdx.x == 0) p.largest[blockIdx.x] = all;
+        }
     }
 }
 
@@ -342,7 +356,7 @@ cudaError_t join_typed(const AttentionParams &p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t delta_typed(const AttentionParams &p, cudaStream_t stream) {
-    attention_delta_kernel<T><<<blocks_for((int64_t)p.B * p.K * p.R * 2), kThreads, 0, stream>>>(p);
+    attention_delta_kernel<T><<<(unsigned)attention_delta_blocks((int64_t)p.B * p.K * p.R), kThreads, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
@@ -369,6 +383,8 @@ cudaError_t launch_attention_terms(const TermsParams &p, cudaStream_t stream) {
     const int64_t grid = std::min<int64_t>((most + kThreads - 1) / kThreads, 148 * 32);
     return launch_dependent(attention_terms_kernel, dim3((unsigned)grid, p.tensors), kThreads, 0, stream, p);
 }
+
+int64_t attention_delta_blocks(int64_t rows) { return (rows * 2 + kThreads - 1) / kThreads; }
 
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream) {
     return dtype == 0 ? delta_typed<float>(p, stream)

@@ -209,6 +209,8 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
 
     grid_launch_dependents();
     grid_dependency_wait();
+    __shared__ uint32_t largest[kThreads / 32];
+    const float grow = gradient_scale<T, kThreads>(p, largest);
     const int x_tiles = ((KEYS ? p.S : p.R) + BX - 1) / BX;
     int64_t i = blockIdx.x;
     const int first = (int)(i % x_tiles) * BX;
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
                         row_lse = lse[half], row_delta = delta[half];
                     }
                     s[n][j] = may ? fast_exp2(s[n][j] * p.scale_log2 - row_lse) : 0.f;
-                    ds[n][j] = may ? s[n][j] * (ds[n][j] - row_delta) : 0.f;
+                    ds[n][j] = may ? s[n][j] * ((ds[n][j] - row_delta) * grow) : 0.f;
                 }
         if constexpr (KEYS) product_nn<T, DP, N>(a0, s, y1 + stage * BN * P);
         product_nn<T, DP, N>(a1, ds, y0 + stage * BN * P);
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
             if (c >= p.D) continue;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float grad = a1[d][2 * half + e] * p.scale;
+                const float grad = a1[d][2 * half + e] * (p.scale / grow);
                 if (p.splits > 1) {
                     p.part[(part * rows + at) * p.D + c + e] = grad;
                     if constexpr (KEYS) p.part2[(part * rows + at) * p.D + c + e] = a0[d][2 * half + e];

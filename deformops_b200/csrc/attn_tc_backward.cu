@@ -60,6 +60,7 @@ struct Shared {
     alignas(16) float lse[KEYS ? ST : 1][kY];                   // of the walked rows, both with the sign turned
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
+    uint32_t largest[Sh::kThreads / 32];
     uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
     uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[2], acc_free[2];
     uint32_t tmem;
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    const float grow = gradient_scale<T, Sh::kThreads>(p, sm.largest);
     const unsigned x_tiles = ((KEYS ? p.S : p.R) + x_rows - 1) / x_rows;
     bool fine = true;
 
@@ -162,6 +164,11 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             } else {
                 to[0][c] = VecTraits<T>::pack2(x);
             }
+        };
+        // (T - delta), float16: scaled
+        const auto less = [&](float2 t, float2 d) {
+            if constexpr (std::is_same_v<T, __half>) return fma2(t, make_float2(grow, grow), d);
+            return add2(t, d);
         };
         int before = 0, n = group;       // tiles of the items so far; this group's next one
         Ring<ST> y;
@@ -181,7 +188,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 seen = mine_valid && ((key_word(words, p.S, x >> 5) >> (x & 31)) & 1);
             } else if (mine_valid) {
                 my_lse = -p.lse[it.bh * p.R + x];
-                my_delta = -p.delta[it.bh * p.R + x];
+                my_delta = -p.delta[it.bh * p.R + x] * grow;
                 rw = row_words_of(p, it.b, it.h, x);
             }
             if (rw == nullptr) rw = words;
@@ -277,8 +284,8 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         for (int c = 0; c < 16; c += 2) {
                             float4 d = make_float4(my_delta, my_delta, my_delta, my_delta);
                             if constexpr (KEYS) d = *reinterpret_cast<const float4 *>(&sm.delta[stage][32 * half + 2 * c]);
-                            w[c] = fmul2(w[c], add2(make_float2(__uint_as_float(t[2 * c]), __uint_as_float(t[2 * c + 1])), make_float2(d.x, d.y)));
-                            w[c + 1] = fmul2(w[c + 1], add2(make_float2(__uint_as_float(t[2 * c + 2]), __uint_as_float(t[2 * c + 3])), make_float2(d.z, d.w)));
+                            w[c] = fmul2(w[c], less(make_float2(__uint_as_float(t[2 * c]), __uint_as_float(t[2 * c + 1])), make_float2(d.x, d.y)));
+                            w[c + 1] = fmul2(w[c + 1], less(make_float2(__uint_as_float(t[2 * c + 2]), __uint_as_float(t[2 * c + 3])), make_float2(d.z, d.w)));
                         }
                         if (some) {
                             // (0 times what an unseen state's v holds)
@@ -356,7 +363,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             for (int which = KEYS ? 0 : 1; which < 2; ++which) {
                 constexpr int kSecond = KEYS ? DP : 0;
                 const uint32_t acc = tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + (which == 1 ? kSecond : 0);
-                const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale;
+                const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale / grow;
                 Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
                 float *parts = (which == 0 ? p.part2 : p.part) + part_at;
 #pragma unroll
@@ -456,7 +463,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         const int col = lane + 32 * c, r = tile * y_rows + col;
                         const bool valid = col < y_rows && r < p.R;
                         lse[c] = valid ? -p.lse[it.bh * p.R + r] : -INFINITY;
-                        delta[c] = valid ? -p.delta[it.bh * p.R + r] : 0.f;
+                        delta[c] = valid ? -p.delta[it.bh * p.R + r] * grow : 0.f;
                         if (p.row_words != nullptr)
                             see[c] = valid ? __ldg(reinterpret_cast<const uint4 *>(row_words_of(p, it.b, it.h, r) + it.first / 32))
                                            : make_uint4(0, 0, 0, 0);

@@ -385,6 +385,18 @@ def test_long_sums_in_float32(D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shift", [-12, 8])
+@pytest.mark.parametrize("heads, D", [((4, 4), 32), ((2, 1), 128), ((70, 1), 64)], ids=str)
+def test_small_and_large_gradients_in_float16(heads, D, shift):
+    """A weight times a gradient is often below 2^-14, where float16 loses bits.  Results are off by their own rounding, half of
+    2^-24 at least, and by six half steps: dS, the weights, o (by way of delta) and what these add up to."""
+    q, k, v, do = make(1, 40 if heads[0] == 70 else 150, 1000, *heads, D, torch.float16)
+    do = (do * 2.0 ** shift).to(torch.float16)
+    for x, (y, _) in zip(run(q, k, v, do), formula(q, k, v, do)):
+        assert (x.double() - y).norm() <= y.numel() ** 0.5 * 2.0 ** -25 + 6 * 2.0 ** -11 * y.norm()
+
+
+@pytest.mark.gpu
 def test_calls_on_two_streams_at_once():
     sets = [make(2, 64, 2000, 4, 4, 64, torch.float16, seed=s) for s in range(2)]
     want = [run(*s) for s in sets]
