@@ -14,6 +14,9 @@
 // (float32: four channels to 16 bytes, two terms of tf32, products of 8 instead of 16.)  Every warp takes blocks
 // of its CTA's stretch of states with a running maximum and sum of its own; the warps, and the stretches
 // (attn_aux.cu), are joined at the end.
+//
+// bf16: 512 caches of 4000 states of 64 channels 89 us (5.9 TB/s), 512 of 8000 of 128 340 us (6.2 TB/s), 128 of 1500 of 128
+// 23 us (4.2 TB/s, and 3 to join three parts).
 #include <algorithm>
 #include <type_traits>
 

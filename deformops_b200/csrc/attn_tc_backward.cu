@@ -12,9 +12,14 @@
 // Either way a thread owns a row of S and T (a lane of tensor memory), P and dS go back to tensor
 // memory in 16 bits as left operands, and the walked tile serves both products from one copy in shared
 // memory (rows along k, then rows along the other axis).  The weights are formed twice, in both
-// forms, so that every gradient is summed by one CTA in one order: no atomics.  Two warpgroups take
+// forms, so that every gradient is summed by one CTA in one order: no atomics.  Two or three warpgroups take
 // the Y tiles in turn, each with scores of its own; a CTA goes on to the next X tile while the sums of
-// the last one are written.
+// the last one are written by a warpgroup of their own.
+//
+// Bound by the cycle of a warpgroup (scores, exponentials, weights back) where heads are small, by that and the tensor
+// cores in turn where they are large.  4 x 300 queries over 17 821 states, 8 heads of 32, bf16: 141 us with states
+// held and 109 with rows held (exponential unit 36 and 41 %, issue slots 47 %, tensor cores 16 and 18 %; half of the
+// exponentials left out: 15 % less); 2 x 2048 over 4096, 16 heads on 4 of 128: 270 and 225 us (tensor cores 63 and 57 %).
 #include <algorithm>
 #include <type_traits>
 

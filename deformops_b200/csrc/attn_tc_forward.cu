@@ -19,6 +19,9 @@
 // The running maximum is only raised when a row would leave exp2's range of 2^8 above it: then the
 // row's sums in tensor memory are scaled, which is rare after the first tiles, and exact in between (a
 // weight of up to 2^8 rounds like one of 1).
+//
+// 4 x 300 queries over 17 821 states, 8 heads of 32, bf16: 98 us (exponential unit and issue slots 48 %, tensor cores
+// 14 %); 2 x 2048 over 4096, 16 heads on 4 of 128: 130 us, 1050 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
