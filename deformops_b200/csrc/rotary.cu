@@ -10,8 +10,9 @@
 // The frequencies go to shared memory first: lanes that index kernel parameters differently are served one by one.
 // The backward pass is the same kernel with the angles' sign turned.
 //
-// 4 x 21 504 tokens of 8 heads of 32, bf16: 19 us (4.6 TB/s; instruction issue 76 %); 2 x 16 384
-// of 16 heads of 128, float16, 50 us (5.4 TB/s); 2 x 17 821 of 8 heads of 32, float32, 15 us (4.9 TB/s).
+// 4 x 21 504 tokens of 8 heads of 32, bf16: 17.5 us (5.0 TB/s; 19.3 with divisions and without packed arithmetic, when
+// instructions filled 76 % of the issue slots); 2 x 16 384 of 16 heads of 128, float16, 48 us (5.6 TB/s); 2 x 17 821 of 8
+// heads of 32, float32, 14 us (5.3 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -32,6 +33,12 @@ struct RotaryParams {
     int64_t xs[3], ps[3];                 // strides of (sample, token, head), (sample, token, axis)
     int N, G, D, pairs, tile;             // tile: tokens of a CTA
     unsigned tiles;                       // of a sample
+    // How a CTA's threads go through its tokens' units (vectors, or pairs of them) and pairs.  Divisions are the host's:
+    // a thread has two units, and would spend a third of its instructions on them.
+    int units, turning, per_token;        // units of a head, those that turn, units of a token
+    int tokens, heads, step;              // from a thread's unit to its next one
+    int pair_tokens, pair_step;           // the same of pairs
+    float per_token_inverse, units_inverse, pairs_inverse;
     int position_dtype;
     float sign;
     double turns[kMostPairs];             // frequency / 2 pi
@@ -46,11 +53,21 @@ __device__ __forceinline__ double position(const RotaryParams &p, int64_t at) {
     }
 }
 
+// t / n of a thread's number t, given 1 / n: t + 1/2 is 1/2 away from every multiple of n, a rounding 2^-17 at most
+__device__ __forceinline__ int over(int t, float inverse) { return (int)(((float)t + 0.5f) * inverse); }
+
 // (a, b) turned; written out, so that every variant of the kernel gives the same bits
 __device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
     const float x = __fmaf_rn(a, c, __fmul_rn(-b, s));
     b = __fmaf_rn(a, s, __fmul_rn(b, c));
     a = x;
+}
+
+// the same of two pairs
+__device__ __forceinline__ void turn2(float2 &a, float2 &b, float2 c, float2 s) {
+    float2 x = fmul2(b, make_float2(-s.x, -s.y)), y = fmul2(b, c);
+    ffma2(x, a, c), ffma2(y, a, s);
+    a = x, b = y;
 }
 
 // Sine and cosine of so many turns, |turns| <= 1/2.  Results of 16 bits have a half step of 2^-11 and more, where
@@ -80,13 +97,10 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
     __shared__ int axis[kMostPairs];
     const unsigned b = blockIdx.x / p.tiles;
     const int first = (int)(blockIdx.x - b * p.tiles) * p.tile, count = min(p.tile, p.N - first);
-    const int turning = (kOne ? 2 : 1) * p.pairs / VEC, units = turning + (p.D - 2 * p.pairs) / VEC;
-    const int per_token = p.G * units, all = count * per_token;
+    const int turning = p.turning, units = p.units, per_token = p.per_token, all = count * per_token;
     // this thread's next unit, and how far the one after that is
-    int token = threadIdx.x / per_token, head = (threadIdx.x - token * per_token) / units;
+    int token = over(threadIdx.x, p.per_token_inverse), head = over(threadIdx.x - token * per_token, p.units_inverse);
     int unit = threadIdx.x - token * per_token - head * units;
-    const int tokens = kThreads / per_token, heads = (kThreads - tokens * per_token) / units;
-    const int step = kThreads - tokens * per_token - heads * units;
     const T *const x = static_cast<const T *>(p.x) + b * p.xs[0] + first * p.xs[1];
     T *const out = static_cast<T *>(p.out) + ((int64_t)b * p.N + first) * p.G * p.D;
     const int other = INTERLEAVED ? 1 : p.pairs;           // from a pair's first vector to its second
@@ -113,14 +127,13 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
                     if (turns) u[k] = *reinterpret_cast<const Raw *>(from + other);
                 }
             }
-            token += tokens, head += heads, unit += step;
+            token += p.tokens, head += p.heads, unit += p.step;
             if (unit >= units) unit -= units, ++head;
             if (head >= p.G) head -= p.G, ++token;
         }
         if (!formed) {
             __syncthreads();
-            int of = threadIdx.x / max(p.pairs, 1), pair = threadIdx.x - of * p.pairs;
-            const int steps = kThreads / max(p.pairs, 1), rest = kThreads - steps * p.pairs;
+            int of = over(threadIdx.x, p.pairs_inverse), pair = threadIdx.x - of * p.pairs;
             const int64_t from = b * p.ps[0] + first * p.ps[1];
             for (int j = threadIdx.x; j < count * p.pairs; j += kThreads) {
                 const int64_t place = from + of * p.ps[1] + axis[pair] * p.ps[2];
@@ -136,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
                 sine_cosine<T>(turns, s, c);
                 table[of * 2 * p.pairs + pair] = c;
                 table[of * 2 * p.pairs + p.pairs + pair] = s * p.sign;
-                of += steps, pair += rest;
+                of += p.pair_tokens, pair += p.pair_step;
                 if (pair >= p.pairs) pair -= p.pairs, ++of;
             }
             __syncthreads();
@@ -169,8 +182,8 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
 #pragma unroll
                     for (int j = 0; j < VEC / 2; j += 2) {
                         const float4 c4 = *reinterpret_cast<const float4 *>(c + 2 * j), s4 = *reinterpret_cast<const float4 *>(s + 2 * j);
-                        turn(y[j].x, z[j].x, c4.x, s4.x), turn(y[j].y, z[j].y, c4.y, s4.y);
-                        turn(y[j + 1].x, z[j + 1].x, c4.z, s4.z), turn(y[j + 1].y, z[j + 1].y, c4.w, s4.w);
+                        turn2(y[j], z[j], make_float2(c4.x, c4.y), make_float2(s4.x, s4.y));
+                        turn2(y[j + 1], z[j + 1], make_float2(c4.z, c4.w), make_float2(s4.z, s4.w));
                     }
                     v[k] = VecTraits<T>::pack(y);
                     *reinterpret_cast<uint4 *>(out + at[k] + other) = VecTraits<T>::pack(z);
@@ -182,7 +195,15 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
 }
 
 template <typename T, bool WIDE, bool INTERLEAVED>
-cudaError_t launch(const RotaryParams &p, unsigned grid, cudaStream_t stream) {
+cudaError_t launch(RotaryParams p, unsigned grid, cudaStream_t stream) {
+    constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
+    p.turning = (INTERLEAVED && WIDE ? 2 : 1) * p.pairs / VEC;
+    p.units = p.turning + (p.D - 2 * p.pairs) / VEC;
+    p.per_token = p.G * p.units;
+    p.tokens = kThreads / p.per_token, p.heads = kThreads % p.per_token / p.units, p.step = kThreads % p.per_token % p.units;
+    const int pairs = std::max(p.pairs, 1);
+    p.pair_tokens = kThreads / pairs, p.pair_step = kThreads % pairs;
+    p.per_token_inverse = 1.f / p.per_token, p.units_inverse = 1.f / p.units, p.pairs_inverse = 1.f / pairs;
     rotary_kernel<T, WIDE, INTERLEAVED><<<grid, kThreads, p.tile * p.pairs * 2 * sizeof(float), stream>>>(p);
     return cudaGetLastError();
 }
