@@ -21,6 +21,7 @@
 // held and 109 with rows held (exponential unit 36 and 41 %, issue slots 47 %, tensor cores 16 and 18 %; half of the
 // exponentials left out: 15 % less); 2 x 2048 over 4096, 16 heads on 4 of 128: 270 and 225 us (tensor cores 63 and 57 %).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "attn_common.cuh"
@@ -630,6 +631,10 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
             return cudaErrorNotSupported;
     }
     const auto kernel = attention_backward_tc_kernel<T, DP, KEYS, TERMS>;
+    using Sh = Shape<DP, KEYS, TERMS>;
+    static std::atomic<bool> fits{false};
+    if (!fits) fits = tc::registers_suffice(kernel, Sh::kThreads, 128 * (Sh::kGroups * Sh::kRegisters + Sh::kFew + Sh::kWriting));
+    if (!fits) return cudaErrorInvalidConfiguration;
     constexpr size_t smem = sizeof(Shared<DP, KEYS, TERMS>);
     static_assert(smem <= 227 * 1024);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

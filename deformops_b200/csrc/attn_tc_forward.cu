@@ -23,6 +23,7 @@
 // 4 x 300 queries over 17 821 states, 8 heads of 32, bf16: 98 us (exponential unit and issue slots 48 %, tensor cores
 // 14 %); 2 x 2048 over 4096, 16 heads on 4 of 128: 130 us, 1050 TFLOP/s.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "attn_common.cuh"
@@ -501,6 +502,9 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t stream) {
         return cudaErrorNotSupported;
     }
     const auto kernel = attention_forward_tc_kernel<T, DP, RT, KW, TERMS>;
+    static std::atomic<bool> fits{false};
+    if (!fits) fits = tc::registers_suffice(kernel, Sh::kThreads, 128 * (Sh::kGroups * Sh::kRegisters + Sh::kFew));
+    if (!fits) return cudaErrorInvalidConfiguration;
     constexpr size_t smem = sizeof(Shared<DP, RT, KW, TERMS>);
     static_assert((smem + 1024) * Sh::kCtas <= 228 * 1024);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

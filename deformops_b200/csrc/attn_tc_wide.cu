@@ -23,6 +23,8 @@
 // warpgroups share the columns of a tile, and the tensor cores wait for them.  2 x 2048 queries over 4096 states, 16
 // heads on 4 of 128 channels: 573 us forward and 2642 us backward (1440 and 1250 TFLOP/s of bf16 products); products of
 // tf32 terms by warps took 20 ms for both.
+#include <atomic>
+
 #include "attn_common.cuh"
 #include "tensor_core.cuh"
 
@@ -505,6 +507,10 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
 template <Mode M>
 cudaError_t launch(const AttentionParams &p, const tc::TensorMap &y, const tc::TensorMap &z, cudaStream_t stream) {
     const auto kernel = attention_wide_kernel<M>;
+    using Sh = Shape<M>;
+    static std::atomic<bool> fits{false};
+    if (!fits) fits = tc::registers_suffice(kernel, Sh::kThreads, 128 * (Sh::kGroups * Sh::kRegisters + Sh::kFew + Sh::kSumming));
+    if (!fits) return cudaErrorInvalidConfiguration;
     constexpr size_t smem = sizeof(Shared<M>);
     static_assert(smem <= 227 * 1024);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -305,6 +305,13 @@ template <int N>
 __device__ __forceinline__ void registers_down() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+// Whether a block has the registers that its warps share out among them: they are those that the compiler gave it at
+// launch, and an increase beyond them would wait for good.  Asked once for each kernel.
+template <typename Kernel>
+bool registers_suffice(Kernel kernel, int threads, int shared_out) {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs * threads >= shared_out;
+}
 
 }  // namespace tc
 }  // namespace msda_b200
