@@ -146,7 +146,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
         for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += Sh::kThreads) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);
         fence_async_shared();
     }
-    grid_launch_dependents();
     grid_dependency_wait();            // (of what this call has launched before)
     fence_before();
     __syncthreads();

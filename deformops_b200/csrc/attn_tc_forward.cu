@@ -128,7 +128,6 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
         fence_async_shared();
     }
     __syncwarp();
-    grid_launch_dependents();
     grid_dependency_wait();            // (of what this call has launched before: masks, terms)
     const Tiles<BN> tiles(p, b, h, part);
     const auto load = [&](int n, int stage) {

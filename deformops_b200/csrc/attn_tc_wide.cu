@@ -93,7 +93,6 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
             (i < kY16 ? reinterpret_cast<uint4 *>(sm.y)[i] : reinterpret_cast<uint4 *>(sm.z)[i - kY16]) = make_uint4(0, 0, 0, 0);
         fence_async_shared();
     }
-    grid_launch_dependents();
     grid_dependency_wait();            // (of what this call has launched before: masks, terms, delta)
     fence_before();
     __syncthreads();

@@ -97,10 +97,14 @@ __device__ __forceinline__ void tma_load(void *to, const CUtensorMap *map, uint6
 }
 
 // ---- tensor memory --------------------------------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t *to, uint32_t columns) {       // one whole warp
+// One whole warp.  Only then may the kernel behind this one begin (grid_launch_dependents): a CTA has said so as soon as one
+// of its threads has, and a CTA of that kernel which took these columns first would hold them until this kernel ends,
+// which could not end without them.
+__device__ __forceinline__ void tmem_alloc(uint32_t *to, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(to)), "r"(columns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {         // one whole warp
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
