@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             barrier_init(&sm.row_full[s], 32), barrier_init(&sm.row_free[s], 128);
         }
         for (int s = 0; s < 2; ++s) barrier_init(&sm.acc_full[s], 1), barrier_init(&sm.acc_free[s], 128);
+        fence_async_shared();
     }
     if (y_rows < kY) {      // rows that no load reaches
         for (int i = threadIdx.x; i < (int)sizeof(sm.y) / 16; i += Sh::kThreads) reinterpret_cast<uint4 *>(sm.y)[i] = make_uint4(0, 0, 0, 0);

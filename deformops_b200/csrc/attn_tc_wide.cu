@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
         }
         barrier_init(&sm.done, 1), barrier_init(&sm.run_full, 1), barrier_init(&sm.run_free, 128);
         barrier_init(&sm.m_full[0], 128), barrier_init(&sm.m_full[1], 128), barrier_init(&sm.l_full, 128), barrier_init(&sm.drained, 1);
+        fence_async_shared();
     }
     if (y_rows < kY) {      // rows that no load reaches
         constexpr int kY16 = sizeof(sm.y) / 16, kZ16 = sizeof(sm.z) / 16;

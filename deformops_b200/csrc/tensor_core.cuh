@@ -84,7 +84,8 @@ struct Ring {
     }
 };
 
-// plain stores to shared memory, before the asynchronous units read them
+// plain stores to shared memory, before the asynchronous units read them (of barriers that were just made too: loads and
+// products arrive on them)
 __device__ __forceinline__ void fence_async_shared() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }

@@ -29,3 +29,16 @@ def test_dependents_begin_after_tensor_memory_is_taken(path):
     assert "tmem_alloc(" in text and "launch_dependents" not in text
     alloc = re.search(r"void tmem_alloc\(.*?\n}", code(CSRC / "tensor_core.cuh"), re.S).group(0)
     assert alloc.index("tcgen05.alloc") < alloc.index("griddepcontrol.launch_dependents")
+
+
+@pytest.mark.parametrize("path", KERNELS, ids=lambda p: p.name)
+def test_barriers_are_there_for_the_asynchronous_units(path):
+    """Loads and products arrive on barriers through another path than the plain stores that made them: whoever makes them
+    fences in the same block, after the last one."""
+    text = code(path)
+    at = text.rindex("barrier_init(")
+    depth, end = 0, at
+    while depth >= 0:       # the end of the block that the last barrier is made in
+        depth += {"{": 1, "}": -1}.get(text[end], 0)
+        end += 1
+    assert "fence_async_shared();" in text[at:end]
