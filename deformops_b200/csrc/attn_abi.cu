@@ -155,15 +155,16 @@ int64_t forward_bytes(const msda_b200_attention &c, const Pass &pass) {
     const bool terms = c.dtype == MSDA_B200_F32 && pass.tensor_cores;
     return round16(pass.bytes) + (terms ? 2 * term_bytes(c, c.states, c.kv_heads) : 0);
 }
-// rowsum(do o), and behind it the largest |do|
+// rowsum(do o), and behind it what float16 is scaled by: norms of the rows and of the states, bounds
 int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
-int64_t largest_bytes(const msda_b200_attention &c) {
-    return c.dtype == MSDA_B200_F16 ? round16(attention_delta_blocks(c.batch * c.heads * c.queries) * 4) : 0;
+int64_t state_norm_bytes(const msda_b200_attention &c) { return round16(c.batch * c.kv_heads * c.states * 4); }
+int64_t scaling_bytes(const msda_b200_attention &c) {
+    return c.dtype == MSDA_B200_F16 ? delta_bytes(c) + state_norm_bytes(c) + c.batch * c.kv_heads * 16 : 0;
 }
 
 int64_t backward_bytes(const msda_b200_attention &c, const Pass &keys, const Pass &rows) {
     const bool terms = c.dtype == MSDA_B200_F32 && keys.tensor_cores;
-    return delta_bytes(c) + largest_bytes(c) + round16(std::max(keys.bytes, rows.bytes)) +
+    return delta_bytes(c) + scaling_bytes(c) + round16(std::max(keys.bytes, rows.bytes)) +
            (terms ? 2 * term_bytes(c, c.states, c.kv_heads) + 2 * term_bytes(c, c.queries, c.heads) : 0);
 }
 
@@ -344,10 +345,11 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
     p.out = const_cast<void *>(out), p.grad_out = grad_out, p.lse = const_cast<float *>(lse);
     p.dq = grad_query, p.dk = grad_key, p.dv = grad_value;
     p.delta = static_cast<float *>(workspace);
-    p.largest = reinterpret_cast<uint32_t *>(p.delta + delta_bytes(*call) / 4);
-    p.largest_of = (int)attention_delta_blocks((int64_t)p.B * p.K * p.R);
-    p.part = p.delta + (delta_bytes(*call) + largest_bytes(*call)) / 4;
-    int launches = 3;
+    p.row_norms = p.delta + delta_bytes(*call) / 4;
+    p.state_norms = p.row_norms + delta_bytes(*call) / 4;
+    p.bounds = reinterpret_cast<float4 *>(p.state_norms + state_norm_bytes(*call) / 4);
+    p.part = p.delta + (delta_bytes(*call) + scaling_bytes(*call)) / 4;
+    int launches = call->dtype == MSDA_B200_F16 ? 4 : 3;
     cudaError_t e = launch_attention_delta(p, call->dtype, s);
     if (call->dtype == MSDA_B200_F32 && keys.tensor_cores) {
         const int64_t gs[3] = {call->queries * call->heads * call->head_dim, call->heads * call->head_dim, call->head_dim};

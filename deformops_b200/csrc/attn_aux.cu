@@ -176,15 +176,67 @@ __global__ void __launch_bounds__(kThreads) attention_terms_kernel(const __grid_
     }
 }
 
-// eight lanes to a row, rows in the order of `out`
+constexpr int kRowsAtOnce = 4, kDeltaRows = kThreads / 8 * kRowsAtOnce;
+
+// Norms of v's rows, LANES lanes to one, rows in the order of dense states, a CTA to kStateRows of a sample.  What unseen
+// states hold is read with the rest, so as not to wait for the mask, and not used.
+template <int LANES>
+constexpr int kStateRows = kThreads / LANES * kRowsAtOnce;
+template <typename T, int LANES>
+__device__ __forceinline__ void state_norms(const AttentionParams &p, unsigned block) {
+    constexpr int kVec = VecTraits<T>::kVec, kStep = kThreads / LANES;
+    const int64_t all = (int64_t)p.S * p.K;
+    const unsigned blocks = (unsigned)((all + kStateRows<LANES> - 1) / kStateRows<LANES>);
+    const int b = (int)(block / blocks), lane = threadIdx.x & (LANES - 1);
+    const int64_t row = (int64_t)(block - b * blocks) * kStateRows<LANES> + threadIdx.x / LANES;
+    int state = all >> 32 != 0 ? (int)(row / p.K) : (int)((unsigned)row / p.K), h = (int)(row - (int64_t)state * p.K);
+    const int states = kStep / p.K, heads = kStep - states * p.K;
+    uint4 x[kRowsAtOnce];
+    float sum[kRowsAtOnce] = {};
+    int64_t at[kRowsAtOnce];
+    const T *from[kRowsAtOnce];
+    bool seen[kRowsAtOnce];
+#pragma unroll
+    for (int k = 0; k < kRowsAtOnce; ++k) {
+        const bool there = row + k * kStep < all;
+        at[k] = there ? ((int64_t)b * p.K + h) * p.S + state : -1;
+        from[k] = there ? static_cast<const T *>(p.v) + b * p.vs[0] + state * p.vs[1] + h * p.vs[2] : nullptr;
+        seen[k] = there && ((key_word(key_words_of(p, b, h), p.S, state >> 5) >> (state & 31)) & 1);
+        state += states, h += heads;
+        if (h >= p.K) h -= p.K, ++state;
+    }
+    for (int c = lane * kVec; c < p.D; c += LANES * kVec) {
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) x[k] = from[k] != nullptr ? ldg16(from[k] + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            float2 u[kVec / 2];
+            VecTraits<T>::unpack(x[k], u);
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) sum[k] += u[i].x * u[i].x + u[i].y * u[i].y;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kRowsAtOnce; ++k) {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+        if (lane == 0 && at[k] >= 0) p.state_norms[at[k]] = seen[k] ? sqrtf(sum[k]) : 0.f;
+    }
+}
+
+// eight lanes to a row, rows in the order of `out`; float16: CTAs behind the last row take v's
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr int kVec = VecTraits<T>::kVec, kRows = 4;
+    constexpr int kVec = VecTraits<T>::kVec, kRows = kRowsAtOnce;
     grid_launch_dependents();
     const int lane = threadIdx.x & 7;
     const unsigned rows = (unsigned)p.B * p.Q * p.K * p.share;
-    const unsigned first = blockIdx.x * (kThreads / 8 * kRows) + (threadIdx.x >> 3);
-    float sum[kRows] = {}, most = 0.f;
+    if constexpr (kScaled<T>) {
+        const unsigned blocks = (rows + kDeltaRows - 1) / kDeltaRows;
+        if (blockIdx.x >= blocks) return p.D <= 32 ? state_norms<T, 4>(p, blockIdx.x - blocks) : state_norms<T, 8>(p, blockIdx.x - blocks);
+    }
+    const unsigned first = blockIdx.x * kDeltaRows + (threadIdx.x >> 3);
+    float sum[kRows] = {}, square[kRows] = {};
     for (int c = lane * kVec; c < p.D; c += 8 * kVec) {
         uint4 x[kRows], y[kRows];
 #pragma unroll
@@ -202,29 +254,56 @@ __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < kVec / 2; ++i) {
                 sum[k] += u[i].x * v[i].x + u[i].y * v[i].y;
-                if constexpr (std::is_same_v<T, __half>) most = fmaxf(most, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+                if constexpr (kScaled<T>) square[k] += v[i].x * v[i].x + v[i].y * v[i].y;
             }
         }
     }
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+        for (int o = 4; o > 0; o >>= 1) {
+            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+            if constexpr (kScaled<T>) square[k] += __shfl_xor_sync(0xffffffffu, square[k], o);
+        }
         const unsigned row = first + k * (kThreads / 8), token = row / (p.K * p.share), head = row - token * p.K * p.share;
         const unsigned b = token / p.Q, h = head / p.share;
-        if (lane == 0 && row < rows)
-            p.delta[((int64_t)b * p.K + h) * p.R + (int64_t)(token - b * p.Q) * p.share + (head - h * p.share)] = sum[k];
-    }
-    if constexpr (std::is_same_v<T, __half>) {
-        __shared__ uint32_t warps[kThreads / 32];
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = bits;
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            const uint32_t all = __reduce_max_sync(0xffffffffu, warps[threadIdx.x % (kThreads / 32)]);
-            if (threadIdx.x == 0) p.largest[blockIdx.x] = all;
+        const int64_t at = ((int64_t)b * p.K + h) * p.R + (int64_t)(token - b * p.Q) * p.share + (head - h * p.share);
+        if (lane == 0 && row < rows) {
+            p.delta[at] = sum[k];
+            if constexpr (kScaled<T>) p.row_norms[at] = p.lse[at] == INFINITY ? 0.f : sqrtf(square[k]);
         }
     }
+}
+
+// the largest norms and |delta| of a (sample, key head), by one CTA; what is not finite does not count
+__global__ void __launch_bounds__(1024) attention_bounds_kernel(const __grid_constant__ AttentionParams p) {
+    __shared__ uint32_t warps[3][32];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int64_t bh = blockIdx.x;
+    const auto finite = [](float x) {
+        const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
+        return bits < 0x7f800000u ? bits : 0u;
+    };
+    uint32_t most[3] = {0, 0, 0};
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.R; i += 1024) {
+        most[0] = max(most[0], finite(p.row_norms[bh * p.R + i]));
+        most[1] = max(most[1], finite(p.delta[bh * p.R + i]));
+    }
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.S; i += 1024) most[2] = max(most[2], finite(p.state_norms[bh * p.S + i]));
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        most[k] = __reduce_max_sync(0xffffffffu, most[k]);
+        if ((threadIdx.x & 31) == 0) warps[k][threadIdx.x >> 5] = most[k];
+    }
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) most[k] = __reduce_max_sync(0xffffffffu, warps[k][threadIdx.x]);
+    if (threadIdx.x == 0)
+        p.bounds[bh] = make_float4(__uint_as_float(most[0]), __uint_as_float(most[1]), __uint_as_float(most[2]), 0.f);
 }
 
 // o = sum of 2^(L_i - L) o_i, a thread to four channels of a row
@@ -357,8 +436,14 @@ cudaError_t join_typed(const AttentionParams &p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t delta_typed(const AttentionParams &p, cudaStream_t stream) {
-    attention_delta_kernel<T><<<(unsigned)attention_delta_blocks((int64_t)p.B * p.K * p.R), kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    int64_t blocks = ((int64_t)p.B * p.K * p.R + kDeltaRows - 1) / kDeltaRows;
+    const int64_t each = p.D <= 32 ? kStateRows<4> : kStateRows<8>;
+    if constexpr (kScaled<T>) blocks += p.B * (((int64_t)p.S * p.K + each - 1) / each);
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    attention_delta_kernel<T><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (!kScaled<T> || e != cudaSuccess) return e;
+    return launch_dependent(attention_bounds_kernel, dim3((unsigned)(p.B * p.K)), 1024, 0, stream, p);
 }
 
 }  // namespace
@@ -384,8 +469,6 @@ cudaError_t launch_attention_terms(const TermsParams &p, cudaStream_t stream) {
     const int64_t grid = std::min<int64_t>((most + kThreads - 1) / kThreads, 148 * 32);
     return launch_dependent(attention_terms_kernel, dim3((unsigned)grid, p.tensors), kThreads, 0, stream, p);
 }
-
-int64_t attention_delta_blocks(int64_t rows) { return (rows * 2 + kThreads - 1) / kThreads; }
 
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream) {
     return dtype == 0 ? delta_typed<float>(p, stream)

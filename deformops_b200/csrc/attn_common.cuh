@@ -39,8 +39,10 @@ struct AttentionParams {
     void *out;                             // (B, Q, G * D)
     float *lse;                            // (B, K, R), log2 of the sum of exp2
     float *delta;                          // (B, K, R), rowsum(do o); backward only
-    uint32_t *largest;                     // float16: the largest |do| of every CTA that formed `delta`, as bits
-    int largest_of;                        // how many
+    // float16: norms of do's rows, (B, K, R), 0 for rows that see nothing, and of v's, (B, K, S), 0 for states that nobody
+    // sees; of every (sample, key head) the largest of the first, of |delta| and of the second
+    float *row_norms, *state_norms;
+    float4 *bounds;
     void *dq, *dk, *dv;                    // contiguous (B, Q, G, D), (B, S, K, D)
     // work over the long axis is split into `splits` stretches of `tiles` tiles; with more than one,
     // partial results go to part (splits, B, K, rows, D) and part_lse (splits, B, K, rows)
@@ -66,21 +68,24 @@ __device__ __forceinline__ void split_terms(float2 x, uint32_t (&t)[3]) {
     }
 }
 
-// float16: what dS is multiplied by before it is rounded, and its gradients are divided by: the power of two that brings
-// the largest |do| to 1 .. 2.  A weight is 1 / S or so, and float16 has no normal numbers below 2^-14 (do of 2^-12
-// over 1000 states: dq 1.5 % off without, its own rounding is 0.3 %).  All threads of the CTA.
-template <typename T, int THREADS>
-__device__ __forceinline__ float gradient_scale(const AttentionParams &p, uint32_t (&warps)[THREADS / 32]) {
-    if constexpr (!std::is_same_v<T, __half>) return 1.f;
-    uint32_t most = 0;
-    for (int i = threadIdx.x; i < p.largest_of; i += THREADS) most = max(most, p.largest[i]);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) most = max(most, warps[i]);
-    const uint32_t exponent = most >> 23;
-    return exponent == 0 || exponent == 255 ? 1.f : __uint_as_float((254 - exponent) << 23);
+// float16 has no normal numbers below 2^-14 and none above 65 504.  dS is multiplied by a power of two of the row (of do,
+// or of k and v) that a thread holds, which its sum is divided by: the one that brings a bound of |dP - delta| to
+// 2^14 .. 2^15, so nothing can overflow and what is 2^-29 of the bound has all its bits still.  The bound:
+// |do_r v_j| <= |do_r| |v_j| with 2-norms, rows held with the largest |v| and the row's own delta, states held with the
+// largest |do| and |delta| of the (sample, key head).  Rows of do that hold infinities or NaN do not count for the others.
+// (Rows 2^-10 of the largest over 17 821 states: dq was 12 % off with one factor from the largest |do| of all.)
+template <typename T>
+constexpr bool kScaled = std::is_same_v<T, __half>;
+__device__ __forceinline__ float scale_below(float bound) {
+    const uint32_t exponent = __float_as_uint(bound) >> 23;       // (bound < 2^(exponent - 126))
+    return exponent >= 255 ? 1.f : __uint_as_float((268 - max(exponent, 64u)) << 23);
+}
+__device__ __forceinline__ float row_scale(const AttentionParams &p, int64_t bh, int r) {
+    return scale_below(p.row_norms[bh * p.R + r] * p.bounds[bh].z + fabsf(p.delta[bh * p.R + r]));
+}
+__device__ __forceinline__ float state_scale(const AttentionParams &p, int64_t bh, int state) {
+    const float4 most = p.bounds[bh];
+    return scale_below(most.x * p.state_norms[bh * p.S + state] + most.y);
 }
 
 // ---- which states a tile of 32 * N of them may use --------------------------------------------------
@@ -213,7 +218,6 @@ struct TermsParams {
     int tensors, B, D;
 };
 cudaError_t launch_attention_terms(const TermsParams &p, cudaStream_t stream);
-int64_t attention_delta_blocks(int64_t rows);       // CTAs, each with a place in `largest`
 cudaError_t launch_attention_delta(const AttentionParams &p, int dtype, cudaStream_t stream);
 // parts of a split pass to the result: outputs and sums (forward), or the sum of gradients
 cudaError_t launch_attention_join(const AttentionParams &p, int dtype, cudaStream_t stream);

@@ -209,8 +209,6 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
 
     grid_launch_dependents();
     grid_dependency_wait();
-    __shared__ uint32_t largest[kThreads / 32];
-    const float grow = gradient_scale<T, kThreads>(p, largest);
     const int x_tiles = ((KEYS ? p.S : p.R) + BX - 1) / BX;
     int64_t i = blockIdx.x;
     const int first = (int)(i % x_tiles) * BX;
@@ -260,6 +258,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
 
     const int x_row = first + warp * 16 + g;           // and x_row + 8
     float lse[2] = {INFINITY, INFINITY}, delta[2] = {0.f, 0.f};
+    float grow[2] = {1.f, 1.f}, unscale[2] = {p.scale, p.scale};     // of dS, and back (float16)
     const uint32_t *rw[2] = {nullptr, nullptr};
     bool seen[2] = {false, false};
 #pragma unroll
@@ -271,6 +270,10 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
             lse[half] = p.lse[bh * p.R + r];
             delta[half] = p.delta[bh * p.R + r];
             rw[half] = row_words_of(p, b, h, r);
+        }
+        if (kScaled<T> && r < (KEYS ? p.S : p.R)) {
+            const float by = KEYS ? state_scale(p, bh, r) : row_scale(p, bh, r);
+            grow[half] = by, unscale[half] = p.scale / by;
         }
     }
 
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
                         row_lse = lse[half], row_delta = delta[half];
                     }
                     s[n][j] = may ? fast_exp2(s[n][j] * p.scale_log2 - row_lse) : 0.f;
-                    ds[n][j] = may ? s[n][j] * ((ds[n][j] - row_delta) * grow) : 0.f;
+                    ds[n][j] = may ? s[n][j] * ((ds[n][j] - row_delta) * grow[half]) : 0.f;
                 }
         if constexpr (KEYS) product_nn<T, DP, N>(a0, s, y1 + stage * BN * P);
         product_nn<T, DP, N>(a1, ds, y0 + stage * BN * P);
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
             if (c >= p.D) continue;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float grad = a1[d][2 * half + e] * (p.scale / grow);
+                const float grad = a1[d][2 * half + e] * unscale[half];
                 if (p.splits > 1) {
                     p.part[(part * rows + at) * p.D + c + e] = grad;
                     if constexpr (KEYS) p.part2[(part * rows + at) * p.D + c + e] = a0[d][2 * half + e];

@@ -66,7 +66,6 @@ struct Shared {
     alignas(16) float lse[KEYS ? ST : 1][kY];                   // of the walked rows, both with the sign turned
     alignas(16) float delta[KEYS ? ST : 1][kY];
     alignas(16) uint32_t words[KEYS ? ST : 1][4][kY];           // word w of a row: states 32 w .. of X
-    uint32_t largest[Sh::kThreads / 32];
     uint64_t x_full[2], x_free[2], y_full[ST], y_free[ST], y_clean[ST], row_full[ST], row_free[ST];
     uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], acc_full[2], acc_free[2];
     uint32_t tmem;
@@ -152,7 +151,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-    const float grow = gradient_scale<T, Sh::kThreads>(p, sm.largest);
     const unsigned x_tiles = ((KEYS ? p.S : p.R) + x_rows - 1) / x_rows;
     bool fine = true;
 
@@ -171,11 +169,6 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                 to[0][c] = VecTraits<T>::pack2(x);
             }
         };
-        // (T - delta), float16: scaled
-        const auto less = [&](float2 t, float2 d) {
-            if constexpr (std::is_same_v<T, __half>) return fma2(t, make_float2(grow, grow), d);
-            return add2(t, d);
-        };
         int before = 0, n = group;       // tiles of the items so far; this group's next one
         Ring<ST> y;
         uint32_t turn = 0;               // parity of the group's tiles
@@ -188,16 +181,25 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             const bool mine_valid = row < x_rows && x < (KEYS ? p.S : p.R);
             const bool idle = (row & ~31) >= x_rows || it.first + (row & ~31) >= (KEYS ? p.S : p.R);
             float my_lse = -INFINITY, my_delta = 0.f;
+            [[maybe_unused]] float grow = 1.f;           // float16: what dS is scaled by
             const uint32_t *rw = nullptr;
             bool seen = false;
             if constexpr (KEYS) {
                 seen = mine_valid && ((key_word(words, p.S, x >> 5) >> (x & 31)) & 1);
+                if (kScaled<T> && mine_valid) grow = state_scale(p, it.bh, x);
             } else if (mine_valid) {
                 my_lse = -p.lse[it.bh * p.R + x];
+                if constexpr (kScaled<T>) grow = row_scale(p, it.bh, x);
                 my_delta = -p.delta[it.bh * p.R + x] * grow;
                 rw = row_words_of(p, it.b, it.h, x);
             }
             if (rw == nullptr) rw = words;
+            // T - delta, scaled (rows held: delta is already)
+            const auto less = [&](float2 t, float2 d) {
+                if constexpr (!kScaled<T>) return add2(t, d);
+                else if constexpr (KEYS) return fmul2(add2(t, d), make_float2(grow, grow));
+                else return fma2(t, make_float2(grow, grow), d);
+            };
             uint32_t entry = 0;
             uint2 see = make_uint2(0, 0);
             // the mask of this group's next tile comes while it works on another
@@ -335,6 +337,8 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             const int rows = KEYS ? p.S : p.R, x = it.first + row;
             const bool valid = row < x_rows && x < rows;
             const bool idle = (row & ~31) >= x_rows || it.first + (row & ~31) >= rows;
+            float unscale = p.scale;                  // of dk and dq
+            if (kScaled<T> && valid) unscale /= KEYS ? state_scale(p, it.bh, x) : row_scale(p, it.bh, x);
             const int query = x / p.share;
             const int64_t at = KEYS ? (((int64_t)it.b * p.S + x) * p.K + it.h) * p.D
                                     : (((int64_t)it.b * p.Q + query) * p.K * p.share + it.h * p.share + (x - query * p.share)) * p.D;
@@ -369,7 +373,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             for (int which = KEYS ? 0 : 1; which < 2; ++which) {
                 constexpr int kSecond = KEYS ? DP : 0;
                 const uint32_t acc = tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + (which == 1 ? kSecond : 0);
-                const float factor = !fine ? NAN : which == 0 ? 1.f : p.scale / grow;
+                const float factor = !fine ? NAN : which == 1 ? unscale : 1.f;
                 Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
                 float *parts = (which == 0 ? p.part2 : p.part) + part_at;
 #pragma unroll
@@ -469,7 +473,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                         const int col = lane + 32 * c, r = tile * y_rows + col;
                         const bool valid = col < y_rows && r < p.R;
                         lse[c] = valid ? -p.lse[it.bh * p.R + r] : -INFINITY;
-                        delta[c] = valid ? -p.delta[it.bh * p.R + r] * grow : 0.f;
+                        delta[c] = valid ? -p.delta[it.bh * p.R + r] : 0.f;
                         if (p.row_words != nullptr)
                             see[c] = valid ? __ldg(reinterpret_cast<const uint4 *>(row_words_of(p, it.b, it.h, r) + it.first / 32))
                                            : make_uint4(0, 0, 0, 0);

@@ -494,3 +494,69 @@ def test_statuses_of_the_c_interface():
     # 129 states: 8 words, lists of 3 and 2 tiles with their counts (in whole 16 bytes)
     assert shim.attention_mask_bytes(2, 5, 129, 2, 0) == 2 * (8 + 8) * 4
     assert shim.attention_mask_bytes(2, 5, 129, 2, 4) == 4 * 2 * (2 * 8 + 8 * (2 + 4 * 5))
+
+
+def rows_within(got, want, steps=6):
+    """Row by row (the last axis): half a step of 2^-24 for what is small, and so many half steps of the row's norm."""
+    off, size = (got.double() - want).norm(dim=-1), want.norm(dim=-1)
+    worst = (off / (want.shape[-1] ** 0.5 * 2.0 ** -25 + steps * 2.0 ** -11 * size)).max().item()
+    assert worst <= 1.0, f"{worst:.2f} of the bound off"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1000, 4096])
+@pytest.mark.parametrize("heads, D", [((4, 4), 32), ((4, 2), 64), ((2, 1), 128), ((70, 1), 64)], ids=str)
+def test_rows_of_unlike_gradients_in_float16(heads, D, S):
+    """Gradients 2^12 apart: between samples, heads and rows, and for states that only the small rows see.  Every row of
+    dq, dk and dv is off by its own rounding and by that of dS, of the weights and of o: six half steps hold them, as where
+    all rows are alike.  Small rows keep their bits: what is 2^-29 of the bound that dS is scaled by is normal, and theirs
+    is 2^-12 of it, times 1 / S, times 2^-4 for a product of vectors that are not parallel."""
+    G, K = heads
+    B, Q = 3, 40 if G == 70 else 150
+    q, k, v, do = make(B, Q, S, G, K, D, torch.float16)
+    by = torch.full((B, Q, G), 2.0 ** 9, device="cuda")
+    by[0, ::2] *= 2.0 ** -12
+    by[1] *= 2.0 ** -12
+    by[2, :, : G // K] *= 2.0 ** -12                        # of one key head
+    do = (do.view(B, Q, G, D) * by.unsqueeze(-1)).to(torch.float16).view(B, Q, G * D)
+    mask = torch.zeros(B, Q, S, dtype=torch.bool, device="cuda")
+    mask[0, 1::2, 3 * S // 4:] = True
+    got = run(q, k, v, do, attention_mask=mask)[1:]
+    for x, (y, _) in zip(got, formula(q, k, v, do, mask=mask)[1:]):
+        rows_within(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(4, 2), (70, 1)], ids=str)
+def test_gradients_of_other_samples_and_heads_do_not_matter(heads):
+    G, K = heads
+    q, k, v, do = make(3, 60, 500, G, K, 32, torch.float16)
+    want = run(q, k, v, do)
+    louder = do.view(3, 60, G, 32).clone()
+    louder[1] *= 2.0 ** 10
+    louder[2, :, : G // K] *= 2.0 ** 12
+    louder[2, 5, 0, 3] = math.inf
+    got = run(q, k, v, louder.view_as(do))
+    for x, y in zip(got[1:], want[1:]):
+        assert torch.equal(x[0], y[0])
+        assert torch.equal(x[2, :, x.shape[2] // K:], y[2, :, y.shape[2] // K:])
+    # of the head with the infinity: the other rows' dq
+    finite = louder.clone()
+    finite[2, 5, 0, 3] = 1.0
+    dq = run(q, k, v, finite.view_as(do))[1]
+    dq[2, 5, 0] = got[1][2, 5, 0]
+    assert torch.equal(got[1].nan_to_num(), dq.nan_to_num()) and got[1][2, 5, 0].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size, least, most", [(800.0, -10, -10), (8000.0, -14, -12), (1.0, -22, -20), (2.0 ** -12, 0, 8)], ids=str)
+@pytest.mark.parametrize("heads", [(2, 2), (70, 1)], ids=str)
+def test_values_of_any_size_in_float16(heads, size, least, most):
+    """dS is as large as |do| |v|: states whose v is the same in all channels, and gradients that are too."""
+    q, k, v, do = make(1, 30, 8, *heads, 128, torch.float16)
+    v = (v[..., :1] * size).expand_as(v).contiguous()
+    by = 2.0 ** torch.linspace(least, most, 30, device="cuda").round().view(1, 30, 1)
+    do = by.expand_as(do).to(torch.float16).contiguous()
+    got, want = run(q, k, v, do), formula(q, k, v, do)
+    assert all(torch.isfinite(t).all() for t in got)
+    check(got, want)
