@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
             load_rows<T, DP, BN>(y1 + stage * BN * P, static_cast<const T *>(p.grad_out), gs, p, b, h, tile * BN);
             for (int c = threadIdx.x; c < BN; c += kThreads) {
                 const int r = tile * BN + c;
-                s_lse[stage * BN + c] = r < p.R ? p.lse[bh * p.R + r] : INFINITY;
+                s_lse[stage * BN + c] = r < p.R ? p.lse[bh * p.R + r] - (kScaled<T> ? kWeightExponent : 0.f) : INFINITY;
                 s_delta[stage * BN + c] = r < p.R ? p.delta[bh * p.R + r] : 0.f;
                 if (p.row_words != nullptr)
 #pragma unroll
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
         }
         if (kScaled<T> && r < (KEYS ? p.S : p.R)) {
             const float by = KEYS ? state_scale(p, bh, r) : row_scale(p, bh, r);
-            grow[half] = by, unscale[half] = p.scale / by;
+            grow[half] = KEYS ? by * (1.f / kWeightScale) : by, unscale[half] = p.scale / by;
         }
     }
 
@@ -339,13 +339,14 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float grad = a1[d][2 * half + e] * unscale[half];
+                float grad_value = 0.f;
+                if constexpr (KEYS) grad_value = a0[d][2 * half + e] * (kScaled<T> ? 1.f / kWeightScale : 1.f);
                 if (p.splits > 1) {
                     p.part[(part * rows + at) * p.D + c + e] = grad;
-                    if constexpr (KEYS) p.part2[(part * rows + at) * p.D + c + e] = a0[d][2 * half + e];
+                    if constexpr (KEYS) p.part2[(part * rows + at) * p.D + c + e] = grad_value;
                 } else {
                     static_cast<T *>(KEYS ? p.dk : p.dq)[final_at + c + e] = VecTraits<T>::from_float(grad);
-                    if constexpr (KEYS)
-                        static_cast<T *>(p.dv)[final_at + c + e] = VecTraits<T>::from_float(a0[d][2 * half + e]);
+                    if constexpr (KEYS) static_cast<T *>(p.dv)[final_at + c + e] = VecTraits<T>::from_float(grad_value);
                 }
             }
         }

@@ -181,12 +181,12 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             const bool mine_valid = row < x_rows && x < (KEYS ? p.S : p.R);
             const bool idle = (row & ~31) >= x_rows || it.first + (row & ~31) >= (KEYS ? p.S : p.R);
             float my_lse = -INFINITY, my_delta = 0.f;
-            [[maybe_unused]] float grow = 1.f;           // float16: what dS is scaled by
+            [[maybe_unused]] float grow = 1.f;           // float16: what dS is scaled by, less what P is by
             const uint32_t *rw = nullptr;
             bool seen = false;
             if constexpr (KEYS) {
                 seen = mine_valid && ((key_word(words, p.S, x >> 5) >> (x & 31)) & 1);
-                if (kScaled<T> && mine_valid) grow = state_scale(p, it.bh, x);
+                if (kScaled<T> && mine_valid) grow = state_scale(p, it.bh, x) * (1.f / kWeightScale);
             } else if (mine_valid) {
                 my_lse = -p.lse[it.bh * p.R + x];
                 if constexpr (kScaled<T>) grow = row_scale(p, it.bh, x);
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
             for (int which = KEYS ? 0 : 1; which < 2; ++which) {
                 constexpr int kSecond = KEYS ? DP : 0;
                 const uint32_t acc = tmem + lanes + Sh::kAcc + sums.at * Sh::kSums + (which == 1 ? kSecond : 0);
-                const float factor = !fine ? NAN : which == 1 ? unscale : 1.f;
+                const float factor = !fine ? NAN : which == 1 ? unscale : kScaled<T> ? 1.f / kWeightScale : 1.f;
                 Out *out = static_cast<Out *>(KEYS ? (which == 0 ? p.dv : p.dk) : p.dq) + at;
                 float *parts = (which == 0 ? p.part2 : p.part) + part_at;
 #pragma unroll
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(Shape<DP, KEYS, TERMS>::kThreads, 1)
                     for (int c = 0; c < 2; ++c) {
                         const int col = lane + 32 * c, r = tile * y_rows + col;
                         const bool valid = col < y_rows && r < p.R;
-                        lse[c] = valid ? -p.lse[it.bh * p.R + r] : -INFINITY;
+                        lse[c] = valid ? (kScaled<T> ? kWeightExponent : 0.f) - p.lse[it.bh * p.R + r] : -INFINITY;
                         delta[c] = valid ? -p.delta[it.bh * p.R + r] : 0.f;
                         if (p.row_words != nullptr)
                             see[c] = valid ? __ldg(reinterpret_cast<const uint4 *>(row_words_of(p, it.b, it.h, r) + it.first / 32))

@@ -560,3 +560,14 @@ def test_values_of_any_size_in_float16(heads, size, least, most):
     got, want = run(q, k, v, do), formula(q, k, v, do)
     assert all(torch.isfinite(t).all() for t in got)
     check(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, Q", [((1, 1), 40), ((70, 1), 1)], ids=str)
+def test_small_weights_in_float16(heads, Q):
+    """Over 2^20 states a weight is 2^-20, where a step of float16 is 2^-24."""
+    q, k, v, do = make(1, Q, 1 << 20, *heads, 16, torch.float16)
+    do = do * 2.0 ** 12
+    got, want = run(q, k, v, do), formula(q, k, v, do)
+    for x, (y, _) in zip(got[1:], want[1:]):
+        assert (x.double() - y).norm() <= y.numel() ** 0.5 * 2.0 ** -25 + 6 * 2.0 ** -11 * y.norm()
