@@ -76,8 +76,8 @@ AttentionSplit few_split(int64_t items, int64_t blocks, int64_t slots) {
 }
 
 // Float32 sums on the tensor cores are cut off, not rounded, at every product that is added to them.  The kernels take
-// them on in registers after a few tiles, but for the forward pass up to 32 channels, which has none to spare: there a
-// group has at most eight tiles of a part (over 32 the result was 1.1e-5 off, relative; over eight it is 3e-6).
+// them on after a few tiles, but for two forms of the forward pass up to 32 channels (one row tile, small CTAs), whose groups
+// have at most eight (over 32 the result was 1.1e-5 off, relative; over eight it is 3e-6).
 constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 8;
 constexpr int64_t kFewRows = 16;
 
@@ -88,23 +88,26 @@ bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 
 // are fits of times (0.7 us for 20 with up to 64 channels, 2 us with 128).  bf16, 4096 rows of 32 heads of 64: small ones
 // 20.7 us over 77 states and 205 over 4096, big ones 31.3 and 265 (in two parts; 214 in one); 1 x 16 384 x 16 heads
 // over 4096: big 361 us, small 399; 64 heads of 100 rows over 17 821 states: one tile to a CTA 61 us, small 84.
-// float32, 8 heads of 32 for 8 x 640 rows over 4096: small 174 us, big 197.
+// float32, heads of 32: 2 x 8 heads of 300 rows over 17 821 states, one tile to a CTA 130 us, two 143; 4 heads of 8192 rows over
+// 4096, two 105 us (137 in four short parts).
 void plan_forward(const msda_b200_attention &c, int64_t rows, Pass &pass) {
     const int64_t bk = c.batch * c.kv_heads;
     const bool half = c.dtype != MSDA_B200_F32, wide = wide_float(c), deep = c.head_dim > 64 && !wide;
     const int64_t tiles = (c.states + 63) / 64, big = deep ? (c.states + 127) / 128 : tiles, one = (rows + 127) / 128, two = (rows + 255) / 256;
-    // `groups` with sums of their own share a part
-    const auto most = [&](int groups) { return half || c.head_dim > 32 ? kMostTiles : kMostFloatTiles * groups; };
-    int64_t lowest;
-    pass.row_tiles = 1;
-    pass.split = even_split(bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, most(4), &lowest);
-    if (wide) return;
+    const bool runs = half || c.head_dim > 32;
+    int64_t lowest = INT64_MAX;
+    // `groups` with sums of their own share a part.  Parts that are short for the sums' sake have theirs in the workspace:
+    // no more of them than eight rounds of CTAs would make of the rows anyway.
     const auto take = [&](int row_tiles, int64_t items, int64_t of, const Cost &cost, int groups) {
+        const int64_t most = runs || row_tiles == 2 ? kMostTiles : kMostFloatTiles * groups, fewest = (of + most - 1) / most;
+        if (fewest > 1 && fewest * items > 148 * 8 * cost.at_once) return;
         int64_t all;
-        const AttentionSplit split = even_split(items, of, cost, most(groups), &all);
+        const AttentionSplit split = even_split(items, of, cost, most, &all);
         if (all < lowest) lowest = all, pass.split = split, pass.row_tiles = row_tiles;
     };
-    take(2, bk * two, big, {20, deep ? 80 : half ? 190 : 125, 60, 1}, 2);
+    take(1, bk * one, big, {deep || !half ? 13 : 11, deep ? 50 : half ? 150 : 100, 30, 1}, 4);
+    if (wide) return;
+    take(2, bk * two, big, {runs ? 20 : 22, deep ? 80 : half ? 190 : 125, 60, 1}, 2);
     if (deep) take(0, bk * one, tiles, {7, 40, 30, 2}, 1);
     else if (half || c.head_dim <= 32) take(0, bk * one, tiles, {half ? 13 : 11, 50, 30, 3}, 1);
 }

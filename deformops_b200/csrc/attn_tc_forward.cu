@@ -39,7 +39,8 @@ template <int DP, int RT, int KW, int TERMS>
 struct Shape {
     static constexpr bool kSmall = RT * KW == 1;               // several CTAs to an SM
     static constexpr int BN = DP == 128 && !kSmall ? 128 : 64; // states of a tile
-    static constexpr int ST = kSmall ? 2 : DP == 128 || DP * TERMS > 128 ? KW + 1 : TERMS == 3 ? 6 : 8;     // tiles of k and v in flight
+    // tiles of k and v in flight
+    static constexpr int ST = kSmall ? 2 : DP == 128 || DP * TERMS > 128 ? KW + 1 : TERMS == 3 ? (RT == 1 ? 6 : 4) : 8;
     static constexpr int kGroups = RT * KW;
     static constexpr int kThreads = kGroups * 128 + 128;
     // columns of tensor memory of a group: S, in whose place P comes (a third term needs more), O
@@ -50,9 +51,10 @@ struct Shape {
     static constexpr int kRegisters = kSmall ? (kCtas == 3 ? 128 : 200) : kGroups == 4 ? 104 : 224;
     static constexpr int kFew = kSmall ? (kCtas == 3 ? 32 : 56) : kGroups == 4 ? 64 : 56;
     // Tiles after which a group takes its sums on in registers: those of the tensor cores are cut off, not rounded, at
-    // every product that is added (2^-25.7 of the sum each, 24 times a tile with terms).  Up to 32 channels there are
-    // no registers for it, and parts are short instead.
-    static constexpr bool kRuns = TERMS == 3 && DP == 64;
+    // every product that is added (2^-25.7 of the sum each, 24 times a tile with terms).  Four groups (up to 32 channels)
+    // have no registers for it: those of two row tiles keep them in shared memory; those of one, which would have room for
+    // five tiles in flight then and be 1.4 times slower, and small CTAs take few tiles instead.
+    static constexpr bool kRuns = TERMS == 3 && (DP == 64 || RT == 2), kShared = kRuns && DP == 32;
     static constexpr int kRun = kRuns ? 4 : 1 << 30;
     static_assert(kGroups * kColumns <= 512);
     static_assert(ST > KW);                                    // a tile is freed KW tiles after its scores
@@ -65,6 +67,7 @@ struct Shared {
     alignas(1024) unsigned char k[Sh::ST][TERMS][Sh::BN * DP * 2];
     alignas(1024) unsigned char v[Sh::ST][TERMS][Sh::BN * DP * 2];
     float m[Sh::kGroups][kTileRows], l[Sh::kGroups][kTileRows];
+    float sums[Sh::kShared ? Sh::kGroups : 1][Sh::kShared ? DP : 1][kTileRows];      // of the runs so far
     uint64_t full[Sh::ST], clean[Sh::ST], free[Sh::ST];        // of a stage: its k and v
     uint64_t s_full[Sh::kGroups], p_full[Sh::kGroups], o_full[Sh::kGroups];
     uint32_t tmem;
@@ -187,8 +190,8 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
         if (rw == nullptr) rw = words;
         float m = -INFINITY, l = 0.f;
         int done = 0;
-        [[maybe_unused]] float sums[Sh::kRuns ? DP : 1] = {};      // of the runs so far
-        const auto take_on = [&] {
+        [[maybe_unused]] float sums[Sh::kRuns && !Sh::kShared ? DP : 1] = {};      // of the runs so far
+        const auto take_on = [&](bool first_run) {
             if constexpr (Sh::kRuns) {
 #pragma unroll
                 for (int d = 0; d < DP; d += 16) {
@@ -197,7 +200,14 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
                     tmem_wait_load();
                     loaded(o);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) sums[d + c] += __uint_as_float(o[c]);
+                    for (int c = 0; c < 16; ++c) {
+                        if constexpr (Sh::kShared) {
+                            float &sum = sm.sums[group][d + c][row];
+                            sum = __uint_as_float(o[c]) + (first_run ? 0.f : sum);
+                        } else {
+                            sums[d + c] += __uint_as_float(o[c]);
+                        }
+                    }
                 }
             }
         };
@@ -218,7 +228,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
             fence_after();
             if (!idle) {
                 const bool starts = done % Sh::kRun == 0;          // a run; what was summed before lies there still
-                if (starts && done > 0) take_on();
+                if (starts && done > 0) take_on(done == Sh::kRun);
                 uint32_t s[NW][32];
 #pragma unroll
                 for (int j = 0; j < NW; ++j) tmem_load32(s[j], mine + 32 * j);
@@ -248,7 +258,12 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
                     const float keep = to == -INFINITY ? 1.f : fast_exp2(m - to);
                     m = to;
                     l *= keep;
-                    if constexpr (Sh::kRuns) {
+                    if constexpr (Sh::kShared) {
+                        if (done >= Sh::kRun) {
+#pragma unroll 8
+                            for (int d = 0; d < DP; ++d) sm.sums[group][d][row] *= keep;
+                        }
+                    } else if constexpr (Sh::kRuns) {
 #pragma unroll
                         for (int d = 0; d < DP; ++d) sums[d] *= keep;
                     }
@@ -302,12 +317,15 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
         }
         if constexpr (Sh::kRuns) {
             if (done > Sh::kRun && !idle) {
-                take_on();
+                take_on(false);
 #pragma unroll
                 for (int d = 0; d < DP; d += 16) {
                     uint32_t o[16];
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(sums[d + c]);
+                    for (int c = 0; c < 16; ++c) {
+                        if constexpr (Sh::kShared) o[c] = __float_as_uint(sm.sums[group][d + c][row]);
+                        else o[c] = __float_as_uint(sums[d + c]);
+                    }
                     tmem_store16(mine + kO + d, o);
                 }
                 tmem_wait_store();

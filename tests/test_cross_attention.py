@@ -571,3 +571,34 @@ def test_small_weights_in_float16(heads, Q):
     got, want = run(q, k, v, do), formula(q, k, v, do)
     for x, (y, _) in zip(got[1:], want[1:]):
         assert (x.double() - y).norm() <= y.numel() ** 0.5 * 2.0 ** -25 + 6 * 2.0 ** -11 * y.norm()
+
+
+@pytest.mark.parametrize("Q, S", [(300, 17821), (640, 4096), (9000, 20000), (1 << 16, 1 << 16), (1 << 18, 1 << 18), (1 << 10, 1 << 22), (1 << 20, 1 << 12), (17, 1 << 24)])
+@pytest.mark.parametrize("B, D", [(1, 32), (8, 16)])
+def test_workspace_is_no_larger_than_the_tensors(Q, S, B, D):
+    """float32, forward: three terms of 2 bytes of k and v (in vectors of eight channels), and parts: as many as eight CTAs
+    of 256 rows (24 of 128) to each of 148 SMs have rows, and one more result.  Never a product of rows and states."""
+    import ctypes
+
+    from deformops_b200._loader import AttentionCall, load_library
+
+    G = 8
+    three = ctypes.c_int64 * 3
+    states = three(S * G * D, G * D, D)
+    call = AttentionCall(batch=B, queries=Q, states=S, heads=G, kv_heads=G, head_dim=D, query_strides=three(Q * G * D, G * D, D),
+                         key_strides=states, value_strides=states, mask=None, mask_heads=0, dtype=0, scale=0.1)
+    rows, terms = B * G * Q, 2 * 6 * B * S * G * D
+    most = terms + 4 * (D + 1) * (rows + 148 * 24 * 128) + 64
+    assert 0 < load_library().attention_workspace_bytes(ctypes.byref(call), 0) <= most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(8, 640, 4096, 8, 8, 32), (8, 100, 17821, 8, 8, 32), (2, 300, 17821, 2, 1, 16), (1, 8192, 4096, 2, 2, 32), (1, 600, 4500, 6, 6, 32),
+                                  (4, 2000, 512, 8, 8, 32), (2, 200, 1344, 8, 8, 24)], ids=str)
+def test_long_sums_in_float32_up_to_32_channels(size):
+    """As with more channels, 1.8e-6 for sums of four tiles and a third of that for scores and terms; small CTAs have sums of up to
+    eight, 3.6e-6.  Gradients have sums of four."""
+    q, k, v, do = make(*size, torch.float32)
+    got, want = run(q, k, v, do), formula(q, k, v, do)
+    for x, (y, _), most in zip(got, want, (4.2e-6, 2.5e-6, 2.5e-6, 2.5e-6)):
+        assert (x.detach().double() - y).norm() <= most * y.norm()
