@@ -5,8 +5,9 @@
 // One pass over x, bound by its bytes.  A CTA takes a few tokens of a sample: its threads ask for the vectors that
 // they will turn (both halves of the pairs), form the sine and cosine of every (token, pair) once for all heads
 // while those are on their way, and turn them.  Angles are turns in more than 32 bits, reduced to [-1/2, 1/2] before
-// anything is rounded: at position 10^6 a 32-bit angle is 0.03 off.  float32 positions take a frequency of two
-// floats and the rounding error of the product that a fused multiply-add gives (2^-48 of the turns), others float64.
+// anything is rounded: at position 10^6 a 32-bit angle is 0.03 off.  float32 positions of less than 2^20 turns take a
+// frequency of two floats and the rounding error of the product that a fused multiply-add gives (2^-48 of the turns),
+// all others float64.  (Rounding to whole turns by two additions: with rint and the branch this costs 20.5 us, below.)
 // The frequencies go to shared memory first: lanes that index kernel parameters differently are served one by one.
 // The backward pass is the same kernel with the angles' sign turned.
 //
@@ -26,6 +27,7 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kMostPairs = 128;
 constexpr int kInFlight = 2;          // pairs of vectors that a thread asks for at a time
+constexpr float kFarTurns = 1048576.f;
 
 struct RotaryParams {
     const void *x, *positions;
@@ -55,6 +57,14 @@ __device__ __forceinline__ double position(const RotaryParams &p, int64_t at) {
 
 // t / n of a thread's number t, given 1 / n: t + 1/2 is 1/2 away from every multiple of n, a rounding 2^-17 at most
 __device__ __forceinline__ int over(int t, float inverse) { return (int)(((float)t + 0.5f) * inverse); }
+
+// the whole number that is nearest to x, |x| < 2^22
+__device__ __forceinline__ float nearest(float x) { return __fadd_rn(__fadd_rn(x, 12582912.f), -12582912.f); }
+
+__device__ __forceinline__ float far_turns(double at, double frequency) {
+    const double all = at * frequency;
+    return (float)(all - rint(all));
+}
 
 // (a, b) turned; written out, so that every variant of the kernel gives the same bits
 __device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
@@ -141,10 +151,11 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
                 if (p.position_dtype == MSDA_B200_F32) {
                     const float at = __ldg(static_cast<const float *>(p.positions) + place), most = __fmul_rn(at, split[pair].x);
                     const float rest = __fmaf_rn(at, split[pair].y, __fmaf_rn(at, split[pair].x, -most));
-                    turns = (most - rintf(most)) + rest;
+                    turns = (most - nearest(most)) + rest;
+                    turns -= nearest(turns);
+                    if (!(fabsf(most) < kFarTurns)) turns = far_turns(at, frequency[pair]);
                 } else {
-                    const double all = position(p, place) * frequency[pair];
-                    turns = (float)(all - rint(all));
+                    turns = far_turns(position(p, place), frequency[pair]);
                 }
                 sine_cosine<T>(turns, s, c);
                 table[of * 2 * p.pairs + pair] = c;

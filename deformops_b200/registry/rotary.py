@@ -67,7 +67,7 @@ def rotary(x: Tensor, positions: Tensor, *, sections: Sequence[int] | None = Non
     ``2 P`` that turn, or with ``interleaved`` the neighbours ``(2 i, 2 i + 1)``.
 
     Positions are float32, float64, int32 or int64, of any size and sign (angles are formed in 64
-    bits), and take no gradient.  The result is dense and has the type of ``x`` (float32, float16, bfloat16).
+    bits; those of float32 positions to 2^-28 of a turn up to 2^20 turns), and take no gradient.  The result is dense and has the type of ``x`` (float32, float16, bfloat16).
     """
     heads_dim = x.shape[3] if x.dim() == 4 else 0
     if sections is None:

@@ -289,7 +289,8 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
  * pass).  x: last axis dense, strides of (sample, token, head) in elements; positions (B, N, axes) of
  * f32, f64, i32 or i64 with strides of all three axes; out dense.  Any alignment of whole elements.
  * `frequencies` and `axis_of_pair` are HOST arrays of `pairs` (at most 128) entries, read during the call.
- * Angles are formed in 64 bits.  No counterpart in the reference.
+ * Angles are formed in 64 bits, of f32 positions up to 2^20 turns in two f32 (2^-28 of a turn).  No counterpart in the
+ * reference.
  */
 int msda_b200_rotary(const void *x, const int64_t *x_strides, const void *positions, const int64_t *position_strides,
                      int position_dtype, void *out, int64_t B, int64_t N, int64_t G, int64_t D, int64_t axes,

@@ -225,3 +225,24 @@ def test_layer_refuses_sizes():
         with pytest.raises(ValueError):
             RotaryCrossAttn(64, **options)
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("kind", [torch.float32, torch.float64], ids=str)
+def test_far_float_positions(dtype, kind):
+    """A product in 64 bits is 2^-53 of its turns off, and the frequency as much: pi 2^-51 of the largest position in all, and the
+    reduced angle 2^-22 as near the origin."""
+    x = torch.randn(1, 12, 2, 64, device="cuda").to(dtype)
+    far = torch.tensor([3e5, 6.5e6, 6.6e6, 1e8, -2.5e8, 1e9, 2.0 ** 31, -1e10, 12345678901.0, 1e11, 1e12, -1e12], device="cuda", dtype=kind)
+    want = turned(x, far.view(-1, 1), (32,))
+    off = (rotary(x, far.view(-1, 1)).double() - want).abs()
+    size = x.double().abs()
+    size = (size[..., :32] + size[..., 32:]).repeat(1, 1, 1, 2)
+    limit = bound(x, want, (32,), False) + size * (far.double().abs() * 2.0 ** -51 * 3.15).view(1, -1, 1, 1)
+    assert (off <= limit).all()
+    # whatever they are, the pairs keep their lengths
+    huge = torch.tensor([1e15, -1e20, 3e38], device="cuda", dtype=kind).view(-1, 1)
+    out = rotary(x[:, :3], huge).double()
+    length = lambda t: (t[..., :32] ** 2 + t[..., 32:] ** 2).sqrt()  # noqa: E731
+    assert ((length(out) / length(x[:, :3].double()) - 1).abs() <= 2 * torch.finfo(dtype).eps + 2.0 ** -20).all()
