@@ -68,7 +68,7 @@ class Shim:
         self.lib = ctypes.CDLL(path)
         missing = [s for s in self.SYMBOLS if not hasattr(self.lib, s)]
         if missing:
-            raise KernelUnavailableError(f"{path} does not export {missing}")
+            raise KernelUnavailableError(f"{path} does not export {missing}: rebuild it")
         self.lib.msda_b200_abi_version.restype = _int
         self.lib.msda_b200_abi_version.argtypes = []
         self.lib.msda_b200_last_error.restype = ctypes.c_char_p

@@ -415,3 +415,17 @@ def test_quotients_next_to_rounding_boundaries():
                     assert rounded(Fraction(float(remainder)) * Fraction(float(rcp)) + Fraction(float(q))) == x / size
                     seen += 1
     assert seen > 500
+
+
+def test_a_library_of_an_older_build_says_so(tmp_path):
+    """One without the newest functions is refused when it is loaded, and told from a broken one."""
+    from deformops_b200 import KernelUnavailableError
+    from deformops_b200._loader import Shim
+
+    source, library = tmp_path / "older.c", tmp_path / "older.so"
+    functions = [name for name in _declared_functions() if "attention" not in name and "rotary" not in name]
+    source.write_text("int msda_b200_abi_version(void) { return 5; }\n"
+                      + "".join(f"void {name}(void) {{}}\n" for name in functions if name != "msda_b200_abi_version"))
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(library), str(source)], check=True)
+    with pytest.raises(KernelUnavailableError, match="msda_b200_rotary.*rebuild it"):
+        Shim(str(library))
