@@ -80,6 +80,7 @@ AttentionSplit few_split(int64_t items, int64_t blocks, int64_t slots) {
 // have at most eight (over 32 the result was 1.1e-5 off, relative; over eight it is 3e-6).
 constexpr int64_t kMostTiles = 1 << 30, kMostFloatTiles = 8;
 constexpr int64_t kFewRows = 16;
+constexpr float kLog2e = 1.4426950408889634f;
 
 bool wide_float(const msda_b200_attention &c) { return c.dtype == MSDA_B200_F32 && c.head_dim > 64; }
 
@@ -186,8 +187,8 @@ int check(const msda_b200_attention *c) {
     if (c->batch > kMost || c->heads > kMost || c->batch * c->heads > 1 << 20 || c->queries > kMost ||
         c->states > kMost || c->queries * (c->heads / c->kv_heads) > kMost)
         return refuse(MSDA_B200_UNSUPPORTED, "attention: more than 2^30 rows or states, or 2^20 heads of all samples");
-    if (!(c->scale > 0.f) || std::isinf(c->scale))
-        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: scale must be positive and finite");
+    if (!(c->scale > 0.f) || std::isinf(c->scale * kLog2e))
+        return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: scale must be positive and finite, times log2(e) too");
     if (c->mask_heads != 0 && c->mask_heads != 1 && c->mask_heads != c->heads)
         return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: mask_heads must be 0, 1 or heads");
     if (!aligned16(c->mask)) return refuse(MSDA_B200_INVALID_ARGUMENT, "attention: misaligned mask");
@@ -208,7 +209,7 @@ AttentionParams params(const msda_b200_attention &c, const void *q, const void *
     p.B = (int)c.batch, p.K = (int)c.kv_heads, p.share = (int)(c.heads / c.kv_heads), p.Q = (int)c.queries;
     p.S = (int)c.states, p.R = p.Q * p.share, p.D = (int)c.head_dim;
     p.scale = c.scale;
-    p.scale_log2 = c.scale * 1.4426950408889634f;
+    p.scale_log2 = c.scale * kLog2e;
     p.W = (int)mask_words(c.states);
     if (c.mask != nullptr) {
         p.lists = static_cast<const uint32_t *>(c.mask);

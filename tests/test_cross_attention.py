@@ -602,3 +602,17 @@ def test_long_sums_in_float32_up_to_32_channels(size):
     got, want = run(q, k, v, do), formula(q, k, v, do)
     for x, (y, _), most in zip(got, want, (4.2e-6, 2.5e-6, 2.5e-6, 2.5e-6)):
         assert (x.detach().double() - y).norm() <= most * y.norm()
+
+
+def test_scales_that_overflow_are_refused():
+    """Scores are formed in base 2: a scale whose product with log2(e) is no number any more would make NaN of them."""
+    import ctypes
+
+    from deformops_b200._loader import AttentionCall, load_library
+
+    three = ctypes.c_int64 * 3
+    for scale, bytes_needed in ((2.0 ** 127, True), (3e38, False), (math.inf, False)):
+        call = AttentionCall(batch=1, queries=40, states=9, heads=1, kv_heads=1, head_dim=32, query_strides=three(1280, 32, 32),
+                             key_strides=three(288, 32, 32), value_strides=three(288, 32, 32), mask=None, mask_heads=0, dtype=0,
+                             scale=scale)
+        assert (load_library().attention_workspace_bytes(ctypes.byref(call), 0) > 0) == bytes_needed
