@@ -74,6 +74,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_f
     const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + h * p.vs[2];
     const uint32_t *words = key_words_of(p, b, h);
     constexpr int kHalves = EIGHT ? 1 : 2;                         // rows g, and g + 8
+    // float16: exponent of what the weights, 1 at most, are multiplied by, and their sum with them (small ones keep their bits)
+    constexpr float kUp = kScaled<T> ? kWeightExponent : 0.f;
     constexpr int CO = EIGHT ? CH / 2 : CH;                        // products of a span of channels
 
     uint32_t q[kHalves][KC][4];
@@ -153,8 +155,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_f
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float base = top == -INFINITY ? 0.f : top;           // nothing seen so far
-            keep[half] = fast_exp2(m[half] - base);
+            const float most = top == -INFINITY ? 0.f : top, base = most - kUp;           // (nothing seen so far)
+            keep[half] = fast_exp2(m[half] - most);
             m[half] = top;
             float sum = 0.f;
 #pragma unroll
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_f
             x += weight * s_out[(w * p.R + r) * DP + d];
         }
         x = total == 0.f ? 0.f : x / total;
-        const float lse = total == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : top + log2f(total);
+        const float lse = total == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : top - kUp + log2f(total);
         const int64_t at = (int64_t)bh * p.R + r;
         const int query = r / p.share;
         if (p.splits > 1) {

@@ -18,7 +18,8 @@
 //
 // The running maximum is only raised when a row would leave exp2's range of 2^8 above it: then the
 // row's sums in tensor memory are scaled, which is rare after the first tiles, and exact in between (a
-// weight of up to 2^8 rounds like one of 1).
+// weight of up to 2^8 rounds like one of 1).  float16 has no normal numbers below 2^-14: its weights are 2^7 times as large,
+// 2^15 at most, and so is the sum that they are divided by (thousands of weights of 2^-21 beside one of 1 had 4 bits).
 //
 // 4 x 300 queries over 17 821 states, 8 heads of 32, bf16: 98 us (exponential unit and issue slots 48 %, tensor cores
 // 14 %); 2 x 2048 over 4096, 16 heads on 4 of 128: 130 us, 1050 TFLOP/s.
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
     constexpr int kPairsOf = TERMS == 3 ? kPairs : 1, kTile = BN * DP * 2;
     constexpr int kLast = Sh::kGroups * 4;                     // first of the last four warps
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    constexpr float kUp = kScaled<T> ? 7.f : 0.f;              // exponent of what the weights are multiplied by
     extern __shared__ __align__(1024) unsigned char raw[];
     auto &sm = *reinterpret_cast<Shared<DP, RT, KW, TERMS> *>(raw);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m;
+                const float base = m == -INFINITY ? 0.f : m - kUp;
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), less2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(l, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -350,10 +352,10 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
             }
 #pragma unroll
             for (int w = 0; w < KW; ++w) factor[w] = total == 0.f ? 0.f : factor[w] / total;
-            lse = total == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : best + log2f(total);
+            lse = total == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : best - kUp + log2f(total);
         } else {
             factor[0] = l == 0.f ? 0.f : 1.f / l;
-            lse = l == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m + log2f(l);
+            lse = l == 0.f ? (p.splits > 1 ? -INFINITY : INFINITY) : m - kUp + log2f(l);
         }
         const int64_t at = bh * p.R + r, rows = (int64_t)p.B * p.K * p.R;
         const int query = r / p.share;

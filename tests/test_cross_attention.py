@@ -616,3 +616,20 @@ def test_scales_that_overflow_are_refused():
                              key_strides=three(288, 32, 32), value_strides=three(288, 32, 32), mask=None, mask_heads=0, dtype=0,
                              scale=scale)
         assert (load_library().attention_workspace_bytes(ctypes.byref(call), 0) > 0) == bytes_needed
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, Q, D, S", [(40, 1, 32, 30), (40, 12, 128, 14), (40, 1, 32, 20000), (40, 40, 32, 20000), (40, 300, 64, 20000), (20, 200, 128, 6000), (40, 200, 64, 60)], ids=str)
+def test_one_large_score_among_small_ones_in_float16(B, Q, D, S):
+    """Every row sees one state of weight 1 whose values are 0, and others whose weights, all alike, are 10 1/2 steps of 2^-24: what is
+    left of the result is theirs.  Weights and result are rounded, half a step each; sums in 32 bits and the score another."""
+    gap = -math.log(10.5 * 2.0 ** -24)
+    q, k, v, _ = make(B, Q, S, 4, 4, D, torch.float16)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 4.0
+    k[:, 7, :, 0] = 4.0
+    v[:, 7] = 0
+    v = v.abs()
+    out = cross_attention(q, k, v, scale=gap / 16)
+    want = formula(q, k, v, out, scale=gap / 16)[0][0]
+    assert (out.double() - want).norm() <= want.numel() ** 0.5 * 2.0 ** -25 + 3 * 2.0 ** -11 * want.norm()
