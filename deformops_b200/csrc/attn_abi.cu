@@ -67,7 +67,7 @@ AttentionSplit even_split(int64_t items, int64_t tiles, const Cost &cost, int64_
 
 // The same where `slots` CTAs of four warps run at a time, whatever else does: a stretch takes its blocks and about 8
 // more, parts 16 and some to join.  Four parts for 512 (sample, head)s of 4000 states of 64 channels are 89 us where one
-// is 97 (only 512 of 740 slots have work), for 512 of 8000 of 128 channels 353 us and 464 (444 slots); 18 for 8 of
+// is 97 (only 512 of 740 slots have work), for 512 of 8000 of 128 channels 340 us and 464 (444 slots); 18 for 8 of
 // 1500 states 6.2 us, one 15.2; one for 8 of 77 states 3.3 us, two 5.0.
 AttentionSplit few_split(int64_t items, int64_t blocks, int64_t slots) {
     return best_split(blocks, 1, std::min(blocks / 4, slots * 8 / items + 1), slots / items, [&](int64_t s, int64_t each) {

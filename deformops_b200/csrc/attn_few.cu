@@ -11,12 +11,14 @@
 // With at most eight rows (EIGHT) the second product is O^T = v^T p^T, the channels 8 g + 2 i and 8 g + 2 i + 1 as
 // rows g and g + 8 of product i: half the products and half the registers for O, so more warps.
 //
-// (float32: four channels to 16 bytes, two terms of tf32, products of 8 instead of 16.)  Every warp takes blocks
+// (float32: four channels to 16 bytes, two terms of tf32, products of 8 instead of 16.  What is left out is 2^-21 of a
+// product, eight times as much as by the kernels of many rows: third terms would double the products.
+// 16 bits: weights are rounded to the type, as there.)  Every warp takes blocks
 // of its CTA's stretch of states with a running maximum and sum of its own; the warps, and the stretches
 // (attn_aux.cu), are joined at the end.
 //
 // bf16: 512 caches of 4000 states of 64 channels 89 us (5.9 TB/s), 512 of 8000 of 128 340 us (6.2 TB/s), 128 of 1500 of 128
-// 23 us (4.2 TB/s, and 3 to join three parts).
+// 23 us (4.2 TB/s, and 3 to join three parts).  float32: 216 us (4.9 TB/s), 1226 (3.4 TB/s) and 76 in all.
 #include <algorithm>
 #include <type_traits>
 
@@ -45,7 +47,7 @@ struct Few {
     // channels of a lane of v, and of all of them; a thread has kLane 32-bit registers of one state
     static constexpr int kChannels = kWide ? 4 : DP == 32 ? 4 : 8, kSpan = 8 * kChannels, VC = DP / kSpan;
     static constexpr int kLane = kWide ? 4 : kChannels / 2;
-    static constexpr int kStates = kWide ? KB / 4 : KB / 4;       // states of v of a thread
+    static constexpr int kStates = KB / 4;                        // states of v of a thread
 };
 
 template <int N>

@@ -1,6 +1,6 @@
 // Cross attention backward with warp-level matrix instructions, for more than 64 query heads to a key head: whole tokens
 // of so many rows fill no tile of the kernel of attn_tc_backward.cu.  2 x 64 queries of 130 heads over 4096 states
-// of one head of 64, float32: 1.7 ms.
+// of one head of 64: float32 1.7 ms (0.16 of products at what the GPU sustains), bf16 0.76.
 //
 // One kernel template in two forms.  "keys" holds 64 states and walks the rows (dk, dv), the other holds 64 rows and
 // walks the states (dq); the weights are formed again in both, so that every gradient is summed by one warp in a
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads) attention_backward_mma_kernel(const 
     }
 }
 
-// more than 48 KB have to be asked for; once per kernel and device, since a capture may not be told
+// more than 48 KB have to be asked for: with every call, captured ones too, since devices do not share it
 template <typename Kernel>
 cudaError_t launch(Kernel kernel, int64_t grid, size_t smem, cudaStream_t stream, const AttentionParams &p) {
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;

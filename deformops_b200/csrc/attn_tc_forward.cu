@@ -21,8 +21,11 @@
 // weight of up to 2^8 rounds like one of 1).  float16 has no normal numbers below 2^-14: its weights are 2^7 times as large,
 // 2^15 at most, and so is the sum that they are divided by (thousands of weights of 2^-21 beside one of 1 had 4 bits).
 //
+// 16-bit types: weights are rounded to the type, which a product's operands have to share.  Half a step each, independent of
+// one another, is about what rounding the result costs once more: bf16 2.1e-3 off, a plain form rounded once 1.7e-3.
+//
 // 4 x 300 queries over 17 821 states, 8 heads of 32, bf16: 98 us (exponential unit and issue slots 48 %, tensor cores
-// 14 %); 2 x 2048 over 4096, 16 heads on 4 of 128: 130 us, 1050 TFLOP/s.
+// 14 %); 2 x 2048 over 4096, 16 heads on 4 of 128: 145 us a call among others, 950 TFLOP/s (160 alone, under a profiler).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -418,8 +421,8 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
                 if (turns > 0) barrier_wait(&sm.full[s], (turns - 1) & 1);
             }
         } else if (warp == kLast + 1 && elect_one()) {
-            constexpr uint32_t kScores = instruction(kBf16, kTileRows, BN, false, false);
-            constexpr uint32_t kOut = instruction(kBf16, kTileRows, DP, false, true);
+            constexpr uint32_t kScores = instruction(kBf16, kTileRows, BN, false);
+            constexpr uint32_t kOut = instruction(kBf16, kTileRows, DP, true);
             constexpr int kRow = kRowBytes<DP>;
             // The n-th tile is the groups' n % KW and their n / KW-th.  Its scores take the place of the weights of
             // their tile before, so the product with those is issued first: products are done in order.

@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(Shape<M>::kThreads, 1)
                     if (nz > s) barrier_wait(&sm.z_full[s], ((nz - s + kZ - 1) / kZ - 1) & 1);
             }
         } else if (warp == kLast + 1 && elect_one()) {
-            constexpr uint32_t kOf = instruction(true, kX, kY, false, false), kAdd = instruction(true, kX, kD, false, true);
+            constexpr uint32_t kOf = instruction(true, kX, kY, false), kAdd = instruction(true, kX, kD, true);
             constexpr int kTerm = kTile >> 4, kHeld = kX * kD * 2 >> 4;
             const uint32_t y0 = descriptor(smem_address(sm.y), 16), z0 = descriptor(smem_address(sm.z), 16), x0 = descriptor(smem_address(sm.x), 16);
             const uint32_t sums_of = descriptor(kOne ? smem_address(sm.z) : smem_address(sm.y), kY * 128);

@@ -144,17 +144,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-        "%30,%31,%32};" ::"r"(at),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // loaded registers may be used from here on (the compiler has to be told: nothing else ties them to the wait)
 __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
@@ -189,8 +178,8 @@ template <int ROW_BYTES>
 constexpr uint32_t kDescriptorHigh = (8 * ROW_BYTES >> 4) | 1u << 14 | (ROW_BYTES == 128 ? 2u : 4u) << 29;
 __device__ __forceinline__ uint32_t descriptor(uint32_t at, uint32_t leading) { return at >> 4 | leading >> 4 << 16; }
 // float32 sums of two 16-bit types alike; b_rows: B's rows run along k
-__host__ __device__ constexpr uint32_t instruction(bool bf16, int m, int n, bool a_rows, bool b_rows) {
-    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_rows ? 1u << 15 : 0u) | (b_rows ? 1u << 16 : 0u) |
+__host__ __device__ constexpr uint32_t instruction(bool bf16, int m, int n, bool b_rows) {
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_rows ? 1u << 16 : 0u) |
            (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 // Issued by one thread, which has to be one that elect_one() chose: then the compiler knows that there is one,
