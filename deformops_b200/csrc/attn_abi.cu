@@ -162,8 +162,11 @@ int64_t forward_bytes(const msda_b200_attention &c, const Pass &pass) {
 // rowsum(do o), and behind it what float16 is scaled by: norms of the rows and of the states, bounds
 int64_t delta_bytes(const msda_b200_attention &c) { return round16(c.batch * c.heads * c.queries * 4); }
 int64_t state_norm_bytes(const msda_b200_attention &c) { return round16(c.batch * c.kv_heads * c.states * 4); }
+int64_t bound_ctas(const msda_b200_attention &c) {
+    return std::min<int64_t>(8, (std::max(c.queries * (c.heads / c.kv_heads), c.states) + 16383) / 16384);
+}
 int64_t scaling_bytes(const msda_b200_attention &c) {
-    return c.dtype == MSDA_B200_F16 ? delta_bytes(c) + state_norm_bytes(c) + c.batch * c.kv_heads * 16 : 0;
+    return c.dtype == MSDA_B200_F16 ? delta_bytes(c) + state_norm_bytes(c) + c.batch * c.kv_heads * (1 + bound_ctas(c)) * 16 : 0;
 }
 
 int64_t backward_bytes(const msda_b200_attention &c, const Pass &keys, const Pass &rows) {
@@ -352,8 +355,10 @@ int msda_b200_attention_backward(const msda_b200_attention *call, const void *qu
     p.row_norms = p.delta + delta_bytes(*call) / 4;
     p.state_norms = p.row_norms + delta_bytes(*call) / 4;
     p.bounds = reinterpret_cast<float4 *>(p.state_norms + state_norm_bytes(*call) / 4);
+    p.bound_parts = p.bounds + call->batch * call->kv_heads;
+    p.bound_ctas = (int)bound_ctas(*call);
     p.part = p.delta + (delta_bytes(*call) + scaling_bytes(*call)) / 4;
-    int launches = call->dtype == MSDA_B200_F16 ? 4 : 3;
+    int launches = call->dtype != MSDA_B200_F16 ? 3 : p.bound_ctas > 1 ? 5 : 4;
     cudaError_t e = launch_attention_delta(p, call->dtype, s);
     if (call->dtype == MSDA_B200_F32 && keys.tensor_cores) {
         const int64_t gs[3] = {call->queries * call->heads * call->head_dim, call->heads * call->head_dim, call->head_dim};

@@ -276,24 +276,26 @@ __global__ void __launch_bounds__(kThreads) attention_delta_kernel(const __grid_
     }
 }
 
-// the largest norms and |delta| of a (sample, key head), by one CTA; what is not finite does not count
+// The largest norms and |delta| of a (sample, key head), by one CTA to 16 384 rows or states and eight at most, whose results the
+// next kernel joins (262 144 rows of one head by one CTA: 30 us); what is not finite does not count.
 __global__ void __launch_bounds__(1024) attention_bounds_kernel(const __grid_constant__ AttentionParams p) {
     __shared__ uint32_t warps[3][32];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int64_t bh = blockIdx.x;
+    const int64_t bh = blockIdx.x / p.bound_ctas;
+    const int first = (int)(blockIdx.x - bh * p.bound_ctas) * 1024 + threadIdx.x, step = 1024 * p.bound_ctas;
     const auto finite = [](float x) {
         const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
         return bits < 0x7f800000u ? bits : 0u;
     };
     uint32_t most[3] = {0, 0, 0};
 #pragma unroll 4
-    for (int i = threadIdx.x; i < p.R; i += 1024) {
+    for (int i = first; i < p.R; i += step) {
         most[0] = max(most[0], finite(p.row_norms[bh * p.R + i]));
         most[1] = max(most[1], finite(p.delta[bh * p.R + i]));
     }
 #pragma unroll 8
-    for (int i = threadIdx.x; i < p.S; i += 1024) most[2] = max(most[2], finite(p.state_norms[bh * p.S + i]));
+    for (int i = first; i < p.S; i += step) most[2] = max(most[2], finite(p.state_norms[bh * p.S + i]));
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         most[k] = __reduce_max_sync(0xffffffffu, most[k]);
@@ -304,7 +306,22 @@ __global__ void __launch_bounds__(1024) attention_bounds_kernel(const __grid_con
 #pragma unroll
     for (int k = 0; k < 3; ++k) most[k] = __reduce_max_sync(0xffffffffu, warps[k][threadIdx.x]);
     if (threadIdx.x == 0)
-        p.bounds[bh] = make_float4(__uint_as_float(most[0]), __uint_as_float(most[1]), __uint_as_float(most[2]), 0.f);
+        (p.bound_ctas > 1 ? p.bound_parts : p.bounds)[blockIdx.x] =
+            make_float4(__uint_as_float(most[0]), __uint_as_float(most[1]), __uint_as_float(most[2]), 0.f);
+}
+
+// a thread to a (sample, key head)
+__global__ void __launch_bounds__(32) attention_bounds_join_kernel(const __grid_constant__ AttentionParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int64_t bh = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    if (bh >= (int64_t)p.B * p.K) return;
+    float4 most = p.bound_parts[bh * p.bound_ctas];
+    for (int i = 1; i < p.bound_ctas; ++i) {
+        const float4 x = p.bound_parts[bh * p.bound_ctas + i];
+        most.x = fmaxf(most.x, x.x), most.y = fmaxf(most.y, x.y), most.z = fmaxf(most.z, x.z);
+    }
+    p.bounds[bh] = most;
 }
 
 // o = sum of 2^(L_i - L) o_i, a thread to four channels of a row
@@ -442,9 +459,14 @@ cudaError_t delta_typed(const AttentionParams &p, cudaStream_t stream) {
     if constexpr (kScaled<T>) blocks += p.B * (((int64_t)p.S * p.K + each - 1) / each);
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     attention_delta_kernel<T><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    const cudaError_t e = cudaGetLastError();
-    if (!kScaled<T> || e != cudaSuccess) return e;
-    return launch_dependent(attention_bounds_kernel, dim3((unsigned)(p.B * p.K)), 1024, 0, stream, p);
+    cudaError_t e = cudaGetLastError();
+    if constexpr (kScaled<T>) {
+        if (e == cudaSuccess)
+            e = launch_dependent(attention_bounds_kernel, dim3((unsigned)(p.B * p.K * p.bound_ctas)), 1024, 0, stream, p);
+        if (e == cudaSuccess && p.bound_ctas > 1)
+            e = launch_dependent(attention_bounds_join_kernel, dim3((unsigned)((p.B * p.K + 31) / 32)), 32, 0, stream, p);
+    }
+    return e;
 }
 
 }  // namespace

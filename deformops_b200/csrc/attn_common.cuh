@@ -42,7 +42,8 @@ struct AttentionParams {
     // float16: norms of do's rows, (B, K, R), 0 for rows that see nothing, and of v's, (B, K, S), 0 for states that nobody
     // sees; of every (sample, key head) the largest of the first, of |delta| and of the second
     float *row_norms, *state_norms;
-    float4 *bounds;
+    float4 *bounds, *bound_parts;          // and those of up to eight CTAs each, behind one another, where there are some
+    int bound_ctas;
     void *dq, *dk, *dv;                    // contiguous (B, Q, G, D), (B, S, K, D)
     // work over the long axis is split into `splits` stretches of `tiles` tiles; with more than one,
     // partial results go to part (splits, B, K, rows, D) and part_lse (splits, B, K, rows)

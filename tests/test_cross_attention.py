@@ -633,3 +633,21 @@ def test_one_large_score_among_small_ones_in_float16(B, Q, D, S):
     out = cross_attention(q, k, v, scale=gap / 16)
     want = formula(q, k, v, out, scale=gap / 16)[0][0]
     assert (out.double() - want).norm() <= want.numel() ** 0.5 * 2.0 ** -25 + 3 * 2.0 ** -11 * want.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Q, S", [(40000, 60), (200, 40000), (140000, 20)])
+def test_bounds_of_long_axes_in_float16(Q, S):
+    """The largest row or state is found wherever it is: were it not, the products with it would overflow."""
+    q, k, v, do = make(2, Q, S, 2, 2, 32, torch.float16)
+    for at in (0, Q // 2 + 3, Q - 1):
+        do[1, at] *= 2.0 ** 11
+    v[0, S - 1] *= 2.0 ** 11
+    v[1, S // 3] *= 2.0 ** 11
+    got, want = run(q, k, v, do), formula(q, k, v, do)
+    # gradients past the largest number of the type (2^11 times 2^11 times the rest) are infinities, and nothing else is
+    past = [(y.abs() - bound) > 65520 for y, bound in want]
+    near = [(y.abs() + bound) > 65504 for y, bound in want]
+    for x, over, may, (y, _) in zip(got, past, near, want):
+        assert torch.equal(x[over].double(), y[over].sign() * math.inf) and torch.isfinite(x[~may]).all()
+    check([x.masked_fill(may, 0.0) for x, may in zip(got, near)], [(y.masked_fill(may, 0.0), b) for (y, b), may in zip(want, near)])
