@@ -70,18 +70,19 @@ __device__ __forceinline__ void split_terms(float2 x, uint32_t (&t)[3]) {
 }
 
 // float16 has no normal numbers below 2^-14 and none above 65 504.  Weights, 1 / S or so where the softmax is flat, are
-// multiplied by 2^15 before they are rounded for dv, which is divided by it.  dS is multiplied by a power of two of the row
+// multiplied by 2^8 before they are rounded for dv, which is divided by it.  dS is multiplied by a power of two of the row
 // (of do, or of k and v) that a thread holds, which its sum is divided by: the one that brings a bound of |dP - delta| to
-// 2^14 .. 2^15, so nothing can overflow and what is 2^-29 of the bound has all its bits still.  The bound:
+// 2^12 .. 2^13, so nothing can overflow and what is 2^-27 of the bound has all its bits still.  (Room is left for weights
+// above 1: scores of 10^7 have an L that is rounded by more than 1, in base 2.)  The bound:
 // |do_r v_j| <= |do_r| |v_j| with 2-norms, rows held with the largest |v| and the row's own delta, states held with the
 // largest |do| and |delta| of the (sample, key head).  Rows of do that hold infinities or NaN do not count for the others.
 // (Rows 2^-10 of the largest over 17 821 states: dq was 12 % off with one factor from the largest |do| of all.)
 template <typename T>
 constexpr bool kScaled = std::is_same_v<T, __half>;
-constexpr float kWeightScale = 32768.f, kWeightExponent = 15.f;
+constexpr float kWeightScale = 256.f, kWeightExponent = 8.f;
 __device__ __forceinline__ float scale_below(float bound) {
     const uint32_t exponent = __float_as_uint(bound) >> 23;       // (bound < 2^(exponent - 126))
-    return exponent >= 255 ? 1.f : __uint_as_float((268 - max(exponent, 64u)) << 23);
+    return exponent >= 255 ? 1.f : __uint_as_float((266 - max(exponent, 64u)) << 23);
 }
 __device__ __forceinline__ float row_scale(const AttentionParams &p, int64_t bh, int r) {
     return scale_below(p.row_norms[bh * p.R + r] * p.bounds[bh].z + fabsf(p.delta[bh * p.R + r]));

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_f
     const uint32_t *words = key_words_of(p, b, h);
     constexpr int kHalves = EIGHT ? 1 : 2;                         // rows g, and g + 8
     // float16: exponent of what the weights, 1 at most, are multiplied by, and their sum with them (small ones keep their bits)
-    constexpr float kUp = kScaled<T> ? kWeightExponent : 0.f;
+    constexpr float kUp = kScaled<T> ? 15.f : 0.f;
     constexpr int CO = EIGHT ? CH / 2 : CH;                        // products of a span of channels
 
     uint32_t q[kHalves][KC][4];
@@ -157,15 +157,15 @@ __global__ void __launch_bounds__(kThreads, kResident<T, DP, EIGHT>) attention_f
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float most = top == -INFINITY ? 0.f : top, base = most - kUp;           // (nothing seen so far)
-            keep[half] = fast_exp2(m[half] - most);
+            const float base = top == -INFINITY ? 0.f : top;           // nothing seen so far
+            keep[half] = fast_exp2(m[half] - base);
             m[half] = top;
             float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    s[n][2 * half + e] = fast_exp2(s[n][2 * half + e] - base);
+                    s[n][2 * half + e] = fast_exp2(s[n][2 * half + e] - base + kUp);       // (less than base first: exact)
                     sum += s[n][2 * half + e];
                 }
             l[half] = l[half] * keep[half] + sum;

@@ -16,10 +16,11 @@
 // channels fit, with fewer registers: 19.0 us against 17.0 for 4 x 4096 rows of 8 heads over 64 states, and 30.7
 // with big CTAs).
 //
-// The running maximum is only raised when a row would leave exp2's range of 2^8 above it: then the
+// The running maximum is only raised when a row would leave a range of 2^8 (float16: 2^4) above it: then the
 // row's sums in tensor memory are scaled, which is rare after the first tiles, and exact in between (a
 // weight of up to 2^8 rounds like one of 1).  float16 has no normal numbers below 2^-14: its weights are 2^7 times as large,
-// 2^15 at most, and so is the sum that they are divided by (thousands of weights of 2^-21 beside one of 1 had 4 bits).
+// and so is the sum that they are divided by (thousands of weights of 2^-21 beside one of 1 had 4 bits).  They are 2^11 at
+// most, and 2^15 where scores are so large, 2^26, that a maximum is rounded by 2.
 //
 // 16-bit types: weights are rounded to the type, which a product's operands have to share.  Half a step each, independent of
 // one another, is about what rounding the result costs once more: bf16 2.1e-3 off, a plain form rounded once 1.7e-3.
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
     constexpr int kLast = Sh::kGroups * 4;                     // first of the last four warps
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     constexpr float kUp = kScaled<T> ? 7.f : 0.f;              // exponent of what the weights are multiplied by
+    constexpr float kAbove = kScaled<T> ? 4.f : 8.f;           // how far they may be above the maximum
     extern __shared__ __align__(1024) unsigned char raw[];
     auto &sm = *reinterpret_cast<Shared<DP, RT, KW, TERMS> *>(raw);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(Shape<DP, RT, KW, TERMS>::kThreads, Shape<DP, 
                     for (int c = 1; c < kRun; ++c) top[j] = fmaxf(top[j], __uint_as_float(s[(j * kRun + c) / 32][(j * kRun + c) % 32]));
                 }
                 const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-                const bool raise = best > m + 8.f || (m == -INFINITY && best > m);
+                const bool raise = best > m + kAbove || (m == -INFINITY && best > m);
                 if (__any_sync(0xffffffffu, raise)) {
                     const float to = raise ? best : m;
                     const float keep = to == -INFINITY ? 1.f : fast_exp2(m - to);

@@ -49,7 +49,8 @@ def cross_attention(query: Tensor, key: Tensor, value: Tensor, *, key_padding_ma
     ``key_padding_mask (B,S)`` for all queries, ``attention_mask`` ``(Q,S)``, ``(B,Q,S)`` or
     ``(B,1|G,Q,S)`` for each.  A query that may see nothing gets zeros, and so do its gradients;
     states that no query may see may hold anything, NaN as well (states that some query
-    may see must be finite).  Strides are free; what the kernels cannot read in 16-byte vectors is
+    may see must be finite).  Scores, times ``scale``, are float32: of 10^6 they leave weights a few per cent
+    off in the backward pass, and above 10^7 results and gradients need not be finite.  Strides are free; what the kernels cannot read in 16-byte vectors is
     copied, and so are tokens expanded from one.
 
     Gradients flow to query, key and value, once.  The same call gives the same bits every time.

@@ -509,8 +509,9 @@ def rows_within(got, want, steps=6):
 def test_rows_of_unlike_gradients_in_float16(heads, D, S):
     """Gradients 2^12 apart: between samples, heads and rows, and for states that only the small rows see.  Every row of
     dq, dk and dv is off by its own rounding and by that of dS, of the weights and of o: six half steps hold them, as where
-    all rows are alike.  Small rows keep their bits: what is 2^-29 of the bound that dS is scaled by is normal, and theirs
-    is 2^-12 of it, times 1 / S, times 2^-4 for a product of vectors that are not parallel."""
+    all rows are alike.  Small rows keep their bits: what is 2^-27 of the bound that dS is scaled by is normal, and theirs
+    is 2^-12 of it, times 1 / S, times 2^-4 for a product of vectors that are not parallel (one bit short over 4096
+    states, which makes one half step two)."""
     G, K = heads
     B, Q = 3, 40 if G == 70 else 150
     q, k, v, do = make(B, Q, S, G, K, D, torch.float16)
@@ -651,3 +652,18 @@ def test_bounds_of_long_axes_in_float16(Q, S):
     for x, over, may, (y, _) in zip(got, past, near, want):
         assert torch.equal(x[over].double(), y[over].sign() * math.inf) and torch.isfinite(x[~may]).all()
     check([x.masked_fill(may, 0.0) for x, may in zip(got, near)], [(y.masked_fill(may, 0.0), b) for (y, b), may in zip(want, near)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads, Q", [((2, 1), 70), ((70, 1), 3), ((2, 2), 5)], ids=str)
+@pytest.mark.parametrize("size", [300.0, 600.0])
+def test_scores_of_tens_of_millions(dtype, heads, Q, size):
+    """Of 1.2 and 4.6 x 10^7, in base 2 times 1.44 and up to 2^26: their float32 is rounded by 4 at most, so weights say little in a
+    backward pass, but nothing overflows, and results are means of the values."""
+    q, k, v, do = make(1, Q, 200, *heads, 128, dtype)
+    q, k = (t.sign() * size for t in (q, k))
+    k[:, 3] = q[:, 0, :1]
+    out, *grads = run(q, k, v, do, scale=1.0)
+    assert torch.isfinite(out).all() and out.abs().max() <= 1.01 * v.abs().max()
+    assert all(torch.isfinite(t).all() for t in grads)
