@@ -76,7 +76,7 @@ __device__ __forceinline__ void split_terms(float2 x, uint32_t (&t)[3]) {
 // above 1: scores of 10^7 have an L that is rounded by more than 1, in base 2.)  The bound:
 // |do_r v_j| <= |do_r| |v_j| with 2-norms, rows held with the largest |v| and the row's own delta, states held with the
 // largest |do| and |delta| of the (sample, key head).  Rows of do that hold infinities or NaN do not count for the others.
-// (Rows 2^-10 of the largest over 17 821 states: dq was 12 % off with one factor from the largest |do| of all.)
+// (Rows 2^-10 of the largest over 17 821 states: dq was 6.5 % off with one factor from the largest |do| of all.)
 template <typename T>
 constexpr bool kScaled = std::is_same_v<T, __half>;
 constexpr float kWeightScale = 256.f, kWeightExponent = 8.f;
